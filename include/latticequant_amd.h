@@ -594,6 +594,43 @@ int lq_resident_attention_noalloc(const lq_resident *k, const lq_resident *v, in
                                   int group, const uint16_t *d_tail_k, const uint16_t *d_tail_v, int64_t t_tail,
                                   uint16_t *d_out, hipStream_t s);
 
+/* ------------------------------------------------- drafted trees, beams -- */
+
+/* Rows of 128 values of (sequence b, head h, token t) at
+ * p + b * stride_b + h * stride_h + t * stride_t (elements of 2 bytes; p 16-byte
+ * aligned, strides multiples of 8). */
+typedef struct {
+    void *p;
+    int64_t stride_b, stride_h, stride_t;
+} lq_rows;
+
+#define LQ_TREE_MAX_NODES 256   /* drafted nodes per sequence */
+
+/* Workspace (bytes) of lq_resident_tree_attention.  Needs no initialisation; the
+ * bytes are in use until the call's work on the stream is done. */
+int64_t lq_tree_attn_workspace(int64_t n_seq, int64_t heads, int64_t n_nodes, int group, int64_t t_prefix,
+                               int64_t tail_cap);
+
+/* Attention of n_nodes drafted tokens of each of n_seq sequences over the first
+ * t_prefix tokens of resident heads (sequence * heads + kv head; heads =
+ * k->n_heads / n_seq), the sequence's tail and the drafts themselves, none of which
+ * is in the cache yet.  Node i of sequence b sees
+ *   prefix tokens t >= d_start[b], tail tokens t < d_tail_len[b] (both nullable: 0
+ *   and tail_cap; the tail's token t counts as t_prefix + t towards d_start), itself
+ *   and its ancestors: parents[b][i] is an earlier node of the sequence, or -1 (a
+ *   root).  Any other parent marks padding: such a node and its descendants see
+ *   nothing, are seen by nothing, and their rows of out are zero.
+ * q, out: query head kvh * group + g, token = node; group 1..16, n_nodes 1..256;
+ * dtype LQ_F16 or LQ_BF16 of q, the drafts, the tail and out (products are fp16:
+ * bf16 values outside fp16's range become infinities).  Scale 1 / sqrt(128).
+ * Tokens that a row does not see do not reach it, whatever their values.
+ * Deterministic. */
+int lq_resident_tree_attention(const lq_resident *k, const lq_resident *v, int64_t t_prefix, const lq_rows *q,
+                               const lq_rows *draft_k, const lq_rows *draft_v, const int32_t *d_parents,
+                               int64_t n_seq, int64_t n_nodes, int group, const lq_rows *tail_k, const lq_rows *tail_v,
+                               int64_t tail_cap, const int32_t *d_tail_len, const int32_t *d_start, int dtype,
+                               void *d_work, const lq_rows *out, hipStream_t s);
+
 #ifdef __cplusplus
 }
 #endif

@@ -94,6 +94,9 @@ _SIGS = {
     "lq_resident_attn_workspace": ([_I64, _INT, _I64, _I64], _I64),
     "lq_resident_attention": ([_P, _P, _I64, _P, _INT, _P, _P, _I64, _P, _P, _P], _INT),
     "lq_resident_attention_noalloc": ([_P, _P, _I64, _P, _INT, _P, _P, _I64, _P, _P], _INT),
+    "lq_tree_attn_workspace": ([_I64, _I64, _I64, _INT, _I64, _I64], _I64),
+    "lq_resident_tree_attention": ([_P, _P, _I64] + [_P] * 4 + [_I64, _I64, _INT, _P, _P, _I64, _P, _P, _INT] + [_P] * 3,
+                                   _INT),
 }
 
 
@@ -114,7 +117,13 @@ class Resident(ctypes.Structure):
                 ("status", _P), ("n_heads", _I64), ("cap_blocks", _I64), ("exc_cap", _I64)]
 
 
+class Rows(ctypes.Structure):
+    """lq_rows: rows of 128 2-byte values addressed by (sequence, head, token)."""
+    _fields_ = [("p", _P), ("stride_b", _I64), ("stride_h", _I64), ("stride_t", _I64)]
+
+
 LQ_RES_ST_EXC_OVERFLOW = 1
+LQ_TREE_MAX_NODES = 256
 
 
 def exported_symbols():

@@ -1,0 +1,143 @@
+"""Drafted tokens over a resident compressed cache.
+
+A drafter proposes a few tokens per sequence, as a chain or as a tree: node 0 is
+the newest token (its K / V are not in the cache yet), every other node continues
+an earlier one.  One pass of the model scores all of them:
+
+* ``resident_tree_attention`` attends every node to the resident prefix, the
+  fp16 / bf16 tail and the node's own ancestors.  Several query tokens would
+  otherwise read a prefix dequantised to memory (``ResidentKVCache.materialise``,
+  the read path of the reference's cache, llm/compressed_kv_cache.py:384-395).
+
+None of it waits for the device; lengths, trees and counts stay there.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from .. import _lib as L
+from .resident import HD, RB, ResidentKV
+
+MAX_NODES = L.LQ_TREE_MAX_NODES
+_DTYPES = (torch.float16, torch.bfloat16)
+
+
+def _rows(t: torch.Tensor):
+    """(tensor, its lq_rows): t (B, H, T, 128) as it lies where the kernels can read
+    16 bytes at a time, else a contiguous copy."""
+    if t.stride(3) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
+        t = t.contiguous()
+    return t, L.Rows(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+
+def _ints(t, shape, name: str, dev) -> torch.Tensor:
+    """Whole numbers of the given shape as a contiguous int32 tensor on dev."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be an int32 or int64 tensor")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    return t.to(device=dev, dtype=torch.int32).contiguous()
+
+
+def _parents(parents, B: int, N: int, dev) -> torch.Tensor:
+    if isinstance(parents, torch.Tensor) and parents.dim() == 1:
+        parents = parents[None].expand(B, -1)
+    p = _ints(parents, (B, N), "parents", dev)
+    if L.debug_checks():
+        bad = (p >= torch.arange(N, device=dev, dtype=torch.int32)).any()
+        if bool(bad):
+            raise ValueError("a node's parent must be an earlier node of its sequence, -1 (root) or -2 (padding)")
+    return p
+
+
+def tree_attn_workspace(n_heads: int, group: int, n_nodes: int, t_prefix: int, tail_cap: int,
+                        device=None) -> torch.Tensor:
+    """Workspace of resident_tree_attention over n_heads resident heads (all
+    sequences' kv heads), n_nodes nodes per sequence; uninitialised."""
+    n = L.load().lq_tree_attn_workspace(1, n_heads, n_nodes, group, t_prefix, tail_cap)
+    if n < 0:
+        raise ValueError("bad tree attention geometry")
+    return torch.empty(int(n), dtype=torch.uint8, device=device)
+
+
+def resident_tree_attention(k: ResidentKV, v: ResidentKV, q: torch.Tensor, draft_k: torch.Tensor,
+                            draft_v: torch.Tensor, parents: torch.Tensor, tail_k: Optional[torch.Tensor] = None,
+                            tail_v: Optional[torch.Tensor] = None, tail_len: Optional[torch.Tensor] = None,
+                            start: Optional[torch.Tensor] = None, work: Optional[torch.Tensor] = None,
+                            out: Optional[torch.Tensor] = None, t_prefix: Optional[int] = None) -> torch.Tensor:
+    """Attention of N drafted nodes per sequence: softmax(q K^T / sqrt(128)) V, each
+    node over the cache, itself and its ancestors.
+
+    q: (B, Hq, N, 128) fp16 or bf16, Hq = group * H_kv (group 1..16, N 1..256);
+    draft_k / draft_v: (B, H_kv, N, 128) of q's type, the nodes' own K / V;
+    parents: (B, N) or (N,) whole numbers: an earlier node, -1 for a root, -2 for
+    padding (padding and its descendants see nothing; their rows are zero).
+    k / v: resident prefixes of B * H_kv heads, read up to t_prefix tokens (a multiple
+    of 16, all of them by default); tail_k / tail_v: (B, H_kv, cap, 128) of q's type,
+    of which sequence b has the first tail_len[b] (all cap without tail_len); start[b]:
+    the first prefix / tail token that sequence b sees (left padding).
+    Any strides with a contiguous last dimension are read in place.  work:
+    tree_attn_workspace, used until the call's work on the stream is done; out: where
+    to write, of q's shape and type.  Returns (B, Hq, N, 128).  The products are
+    fp16: bf16 values beyond its range become infinities.  The same inputs give the
+    same bits."""
+    lib = L.lib()
+    dev = k.a.device
+    if q.dim() != 4 or q.shape[3] != HD or q.dtype not in _DTYPES:
+        raise ValueError("q must be (B, Hq, N, 128) fp16 or bf16")
+    B, Hq, N, _ = q.shape
+    if k.n_heads != v.n_heads or k.n_tokens != v.n_tokens or k.a.device != v.a.device:
+        raise ValueError("K and V resident prefixes must have the same geometry and device")
+    if B < 1 or k.n_heads % B:
+        raise ValueError("the resident prefix must hold B * H_kv heads")
+    Hkv = k.n_heads // B
+    if Hq < 1 or Hq % Hkv or Hq // Hkv > 16:
+        raise ValueError("query heads must be 1..16 times the kv heads")
+    if not 1 <= N <= MAX_NODES:
+        raise ValueError(f"1..{MAX_NODES} nodes per sequence")
+    tp = k.n_tokens if t_prefix is None else int(t_prefix)
+    if tp < 0 or tp > k.n_tokens or tp % RB:
+        raise ValueError("t_prefix must be a multiple of 16 within the resident prefix")
+    if (tail_k is None) != (tail_v is None):
+        raise ValueError("tail K and V go together")
+    given = [q, draft_k, draft_v] + ([tail_k, tail_v] if tail_k is not None else [])
+    if any(t.dtype != q.dtype or t.device != dev for t in given):
+        raise ValueError("q, the drafts and the tail must be of one type, on the resident prefix's device")
+    if draft_k.shape != (B, Hkv, N, HD) or draft_v.shape != draft_k.shape:
+        raise ValueError("draft K / V must be (B, H_kv, N, 128)")
+    cap = 0
+    if tail_k is not None:
+        if tail_k.dim() != 4 or tail_k.shape != tail_v.shape or tail_k.shape[:2] != (B, Hkv) or tail_k.shape[3] != HD:
+            raise ValueError("tail K / V must be (B, H_kv, cap, 128)")
+        cap = int(tail_k.shape[2])
+    elif tail_len is not None:
+        raise ValueError("tail_len without a tail")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif (out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(3) != 1 or
+          any(s % 8 or (s == 0 and n > 1) for s, n in zip(out.stride()[:3], out.shape)) or out.data_ptr() % 16):
+        raise ValueError("out must be like q, its rows 16-byte aligned and apart")
+    need = lib.lq_tree_attn_workspace(B, Hkv, N, Hq // Hkv, tp, cap)
+    if need < 0:
+        raise ValueError("bad tree attention geometry")
+    with torch.cuda.device(dev):
+        if work is None:
+            work = torch.empty(int(need), dtype=torch.uint8, device=dev)
+        elif work.device != dev or not work.is_contiguous() or work.numel() * work.element_size() < need:
+            raise ValueError("attention workspace too small, or on another device")
+        par = _parents(parents, B, N, dev)
+        tl = None if tail_len is None else _ints(tail_len, (B,), "tail_len", dev)
+        st = None if start is None else _ints(start, (B,), "start", dev)
+        keep, rows = zip(*(_rows(t) for t in given))
+        refs = [ctypes.addressof(r) for r in rows] + [None, None]
+        ks, vs = k.struct(), v.struct()
+        ro = L.Rows(out.data_ptr(), out.stride(0), out.stride(1), out.stride(2))
+        L.check(lib.lq_resident_tree_attention(ctypes.addressof(ks), ctypes.addressof(vs), tp, refs[0], refs[1],
+                                               refs[2], par.data_ptr(), B, N, Hq // Hkv, refs[3] if cap else None,
+                                               refs[4] if cap else None, cap, L.ptr(tl), L.ptr(st),
+                                               L.dtype_code(q.dtype), work.data_ptr(), ctypes.addressof(ro),
+                                               L.stream_ptr(dev)), "lq_resident_tree_attention")
+    return out
