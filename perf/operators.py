@@ -416,7 +416,7 @@ def run(state):
         return st["planes"]
     out = []
     for r in st["res"]:
-        n = r.select(st["index"], blocks=st["blocks"])
+        n = r.select(st["index"], st["case"]["batch"], blocks=st["blocks"])
         out.append({**{p: getattr(n, p) for p in PLANES}, "exc": n.exceptions().reshape(-1)})
     return out
 
