@@ -631,6 +631,63 @@ int lq_resident_tree_attention(const lq_resident *k, const lq_resident *v, int64
                                int64_t tail_cap, const int32_t *d_tail_len, const int32_t *d_start, int dtype,
                                void *d_work, const lq_rows *out, hipStream_t s);
 
+/* Workspace (bytes) of lq_accept_drafts with logits; uninitialised. */
+int64_t lq_accept_workspace(int64_t n_seq, int64_t n_nodes, int64_t vocab);
+
+/* Acceptance of drafted trees.  A node's choice is the place of its largest logit
+ * (the lowest of equal ones, NaN above all, as torch.argmax) or, with d_choice, what
+ * d_choice[b][i] says (logits null).  From node 0 the walk goes to the lowest-numbered
+ * child (d_parents[b][j] == node, j > node) whose token d_tokens[b][j] is the node's
+ * choice, until there is none.  d_path[b][0 ..]: the nodes walked, then -1; d_count[b]:
+ * how many; d_next[b]: the last one's choice.  Where node 0 is no root
+ * (d_parents[b][0] != -1) the count is 0 and d_next -1.
+ * Logits (b, i, v) at b * stride_b + i * stride_n + v (elements of dtype, any
+ * alignment of the rows); vocab < 2^31, n_seq * n_nodes <= 65535 with logits. */
+int lq_accept_drafts(const void *d_logits, int dtype, int64_t stride_b, int64_t stride_n, int64_t vocab,
+                     const int64_t *d_choice, const int64_t *d_tokens, const int32_t *d_parents, int64_t n_seq,
+                     int64_t n_nodes, void *d_work, int32_t *d_path, int32_t *d_count, int64_t *d_next, hipStream_t s);
+
+/* Accepted rows behind the tails, n (tail, draft) pairs in one launch per 128:
+ * dst[b, h, d_len[b] + j] = src[b, h, d_path[b][j]] for j < d_count[b];
+ * d_new_len[b] = d_len[b] + d_count[b] (another array than d_len).  Rows of row_bytes
+ * (a multiple of 16) at b, h, t times the strides in bytes, the same for all pairs;
+ * h_dst / h_src / strides are host arrays.  d_path is (n_seq, n_nodes).  Rows past
+ * cap and path entries out of range are left out (d_new_len stops at cap). */
+int lq_append_rows(void *const *h_dst, const void *const *h_src, int64_t n, const int64_t *h_dst_stride,
+                   const int64_t *h_src_stride, int64_t n_seq, int64_t heads, int64_t cap, int64_t n_nodes,
+                   int64_t row_bytes, const int32_t *d_path, const int32_t *d_count, const int32_t *d_len,
+                   int32_t *d_new_len, hipStream_t s);
+
+/* dst[r, h, t] = src[d_index[r], h, t], t < rows, r < n_out, for n pairs laid out as in
+ * lq_append_rows; dst and src apart.  Indices are clamped to 0 .. n_src - 1. */
+int lq_gather_rows(void *const *h_dst, const void *const *h_src, int64_t n, const int64_t *h_dst_stride,
+                   const int64_t *h_src_stride, int64_t n_src, int64_t n_out, int64_t heads, int64_t rows,
+                   int64_t row_bytes, const int32_t *d_index, hipStream_t s);
+
+/* Sequences of n resident prefixes (h_res: host array; K and V of all layers) permuted
+ * in place, without a workspace: blocks blk0 .. blk0 + n_blocks of sequence i become
+ * those of sequence d_index[i] as they were (an index out of range moves nothing).
+ * A sequence is n_heads / n_seq heads; all prefixes have the same n_heads; n_seq <= 128.
+ * Exception entries stay where they are and are shared by the copies. */
+int lq_resident_reorder(const lq_resident *h_res, int64_t n, int64_t n_seq, const int32_t *d_index, int64_t blk0,
+                        int64_t n_blocks, hipStream_t s);
+
+/* Workspace (bytes) of lq_resident_select for heads_out heads of n_blocks blocks. */
+int64_t lq_select_workspace(int64_t heads_out, int64_t n_blocks);
+
+/* A new prefix of chosen sequences and blocks: block j of output sequence r is block
+ * d_blocks[r][j] (null: j) of sequence d_index[r] of src, which has src_blocks blocks in
+ * use per head; dst holds n_out * (src heads per sequence) heads.  Writes dst's
+ * planes with the exception offsets of a list that has the chosen blocks' entries
+ * in block order, and their number to *dst->n_exc; dst->exc is then sized by the
+ * caller and filled by lq_resident_select_exceptions (same arguments).  Indices are
+ * clamped to their ranges. */
+int lq_resident_select(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index, int64_t n_out,
+                       const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst, void *d_work, hipStream_t s);
+int lq_resident_select_exceptions(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index,
+                                  int64_t n_out, const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst,
+                                  hipStream_t s);
+
 #ifdef __cplusplus
 }
 #endif

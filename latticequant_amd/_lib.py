@@ -94,6 +94,14 @@ _SIGS = {
     "lq_resident_attn_workspace": ([_I64, _INT, _I64, _I64], _I64),
     "lq_resident_attention": ([_P, _P, _I64, _P, _INT, _P, _P, _I64, _P, _P, _P], _INT),
     "lq_resident_attention_noalloc": ([_P, _P, _I64, _P, _INT, _P, _P, _I64, _P, _P], _INT),
+    "lq_accept_workspace": ([_I64, _I64, _I64], _I64),
+    "lq_accept_drafts": ([_P, _INT, _I64, _I64, _I64, _P, _P, _P, _I64, _I64] + [_P] * 5, _INT),
+    "lq_append_rows": ([_P, _P, _I64, _P, _P] + [_I64] * 5 + [_P] * 5, _INT),
+    "lq_gather_rows": ([_P, _P, _I64, _P, _P] + [_I64] * 5 + [_P] * 2, _INT),
+    "lq_resident_reorder": ([_P, _I64, _I64, _P, _I64, _I64, _P], _INT),
+    "lq_select_workspace": ([_I64, _I64], _I64),
+    "lq_resident_select": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P], _INT),
+    "lq_resident_select_exceptions": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P], _INT),
     "lq_tree_attn_workspace": ([_I64, _I64, _I64, _INT, _I64, _I64], _I64),
     "lq_resident_tree_attention": ([_P, _P, _I64] + [_P] * 4 + [_I64, _I64, _INT, _P, _P, _I64, _P, _P, _INT] + [_P] * 3,
                                    _INT),

@@ -20,7 +20,7 @@ records merged in the same launch).
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -178,6 +178,82 @@ class ResidentKV:
         self.exc = grown
         self._st = None
 
+    def exceptions(self) -> torch.Tensor:
+        """(n, 8) int16: the exception entries in use (one host read of their number)."""
+        return self.exc[:min(int(self.n_exc.item()), self.exc_cap) * 8].view(-1, 8)
+
+    def reorder(self, index: torch.Tensor, t_from: int = 0) -> None:
+        """reorder_sequences of this prefix alone."""
+        reorder_sequences([self], index, t_from)
+
+    def select(self, index: torch.Tensor, n_seq: int, blocks: Optional[torch.Tensor] = None,
+               cap_tokens: Optional[int] = None) -> "ResidentKV":
+        """A new prefix of chosen sequences, and of chosen blocks of each: fork, drop,
+        evict and compact.  This prefix is n_seq sequences of n_heads / n_seq heads;
+        sequence r of the new one is sequence index[r] (index: (R,) whole numbers) and,
+        with blocks (R, n), holds that sequence's 16-token blocks blocks[r] in the order
+        given, else all of them.  The new prefix has its own exception list, with the
+        entries of the chosen blocks only (their number is read back: one host wait), and
+        room for cap_tokens tokens (those it holds by default).  Indices are clamped to
+        their ranges."""
+        if n_seq < 1 or self.n_heads % n_seq:
+            raise ValueError("n_heads must be a multiple of n_seq")
+        if index.dim() != 1 or index.numel() < 1 or index.dtype not in (torch.int32, torch.int64):
+            raise ValueError("index must be a list of sequences (int32 or int64)")
+        if self.n_tokens % RB:
+            raise ValueError("resident prefix ends inside a block")
+        R, used, dev = index.numel(), self.n_tokens // RB, self.a.device
+        if blocks is not None and (blocks.dim() != 2 or blocks.shape[0] != R or
+                                   blocks.dtype not in (torch.int32, torch.int64)):
+            raise ValueError("blocks must be (R, n) whole numbers")
+        nb = used if blocks is None else blocks.shape[1]
+        cap = max(1, nb, 0 if cap_tokens is None else (int(cap_tokens) + RB - 1) // RB)
+        if nb and not used:
+            raise ValueError("no blocks to choose from")
+        if L.debug_checks() and (bool((index < 0).any()) or bool((index >= n_seq).any()) or
+                                 (blocks is not None and nb and (bool((blocks < 0).any()) or bool((blocks >= used).any())))):
+            raise ValueError("sequence or block out of range")
+        new = ResidentKV._bare(R * (self.n_heads // n_seq), cap, dev)
+        if nb == 0:
+            new.n_exc.zero_()
+            return new
+        lib = L.lib()
+        need = lib.lq_select_workspace(new.n_heads, nb)
+        if need < 0:
+            raise ValueError("too many blocks for one selection")
+        with torch.cuda.device(dev):
+            idx = index.to(device=dev, dtype=torch.int32).contiguous()
+            blk = None if blocks is None else blocks.to(device=dev, dtype=torch.int32).contiguous()
+            work = torch.empty(int(need), dtype=torch.uint8, device=dev)
+            src, dst = self.struct(), new.struct()
+            args = (ctypes.addressof(src), n_seq, used, idx.data_ptr(), R, L.ptr(blk), nb)
+            L.check(lib.lq_resident_select(*args, ctypes.addressof(dst), work.data_ptr(), L.stream_ptr(dev)),
+                    "lq_resident_select")
+            n = int(new.n_exc.item())
+            if n:
+                new.exc = torch.empty(n * 8, dtype=torch.int16, device=dev)
+                new._st = None
+                dst = new.struct()
+                L.check(lib.lq_resident_select_exceptions(*args, ctypes.addressof(dst), L.stream_ptr(dev)),
+                        "lq_resident_select_exceptions")
+        new._exc_known, new.n_tokens = n, nb * RB
+        return new
+
+    @classmethod
+    def _bare(cls, n_heads: int, nb: int, dev) -> "ResidentKV":
+        """nb blocks of room per head, uninitialised, an empty exception list."""
+        r = cls.__new__(cls)
+        r.device, r.n_heads, r.cap_blocks = dev, n_heads, nb
+        for name, per, dt in (("a", 256, torch.int32), ("b", 256, torch.uint8), ("mask", 4, torch.int64),
+                              ("meta", 4, torch.int32), ("scale", RB, torch.float16)):
+            setattr(r, name, torch.empty(n_heads * nb * per, dtype=dt, device=dev))
+        r.n_exc = torch.empty(1, dtype=torch.int32, device=dev)
+        r.status = torch.zeros(1, dtype=torch.int32, device=dev)
+        r.exc = torch.empty(8, dtype=torch.int16, device=dev)
+        r.n_tokens = r._exc_known = r._exc_since = 0
+        r._exc_read = r._st = None
+        return r
+
     def dequant(self, out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
         """(n_heads, n_tokens, 128): lattice point times the stored fp16 scale,
         rounded once (the values _decompress_chunk writes)."""
@@ -200,6 +276,45 @@ def from_chunk(x: torch.Tensor, enc, cap_tokens: Optional[int] = None) -> Reside
     r = ResidentKV(B * H, cap_tokens or T, device=x.device)
     r.append(x, enc.scale32.view(-1)[:B * H], enc.scale16.view(-1)[:B * H])
     return r
+
+
+MAX_REORDER = 128   # sequences of one in-place reorder
+
+
+def reorder_sequences(residents: Sequence[ResidentKV], index: torch.Tensor, t_from: int = 0) -> None:
+    """Permute the sequences of resident prefixes in place (beam search): sequence i
+    becomes sequence index[i] as it was, from token t_from (a multiple of 16) on; what
+    lies before is the same in all sequences (the beams' prompt) and stays.  residents:
+    K and V of all layers (one launch per 64), all of the same heads and tokens, on one
+    device; index: (B,) whole numbers, B <= 128, heads split evenly over B.  A number may
+    stand several times; one out of range leaves its sequence as it is.  No second copy
+    of the cache is made; exception entries are shared by the copies."""
+    if not len(residents):
+        return
+    r0 = residents[0]
+    if index.dim() != 1 or index.dtype not in (torch.int32, torch.int64):
+        raise ValueError("index must be a list of sequences (int32 or int64)")
+    B, dev = index.numel(), r0.a.device
+    if B < 1 or B > MAX_REORDER or r0.n_heads % B:
+        raise ValueError(f"index must name 1..{MAX_REORDER} sequences that the heads divide into evenly "
+                         "(more: ResidentKV.select makes a reordered copy)")
+    if any(r.n_heads != r0.n_heads or r.n_tokens != r0.n_tokens or r.a.device != dev for r in residents):
+        raise ValueError("the prefixes must have the same heads, tokens and device")
+    if len({r.a.data_ptr() for r in residents}) != len(residents):
+        raise ValueError("a prefix stands twice in the list")
+    if t_from < 0 or t_from % RB or t_from > r0.n_tokens or r0.n_tokens % RB:
+        raise ValueError("t_from must be a multiple of 16 within the prefix")
+    nb = (r0.n_tokens - t_from) // RB
+    if nb == 0 or B == 1:
+        return
+    lib = L.lib()
+    with torch.cuda.device(dev):
+        idx = index.to(device=dev, dtype=torch.int32).contiguous()
+        if L.debug_checks() and (bool((idx < 0).any()) or bool((idx >= B).any())):
+            raise ValueError("sequence out of range")
+        table = (L.Resident * len(residents))(*(r.struct() for r in residents))
+        L.check(lib.lq_resident_reorder(ctypes.addressof(table), len(residents), B, idx.data_ptr(), t_from // RB, nb,
+                                        L.stream_ptr(dev)), "lq_resident_reorder")
 
 
 def attn_workspace(n_heads: int, group: int, t_prefix: int, t_tail: int, device=None) -> torch.Tensor:

@@ -8,13 +8,15 @@ an earlier one.  One pass of the model scores all of them:
   fp16 / bf16 tail and the node's own ancestors.  Several query tokens would
   otherwise read a prefix dequantised to memory (``ResidentKVCache.materialise``,
   the read path of the reference's cache, llm/compressed_kv_cache.py:384-395).
+* ``accept_drafts`` finds the path of drafts that the model's own choices confirm;
+* ``append_accepted`` puts those nodes' K / V behind the tails, all layers at once.
 
 None of it waits for the device; lengths, trees and counts stay there.
 """
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -140,4 +142,143 @@ def resident_tree_attention(k: ResidentKV, v: ResidentKV, q: torch.Tensor, draft
                                                refs[4] if cap else None, cap, L.ptr(tl), L.ptr(st),
                                                L.dtype_code(q.dtype), work.data_ptr(), ctypes.addressof(ro),
                                                L.stream_ptr(dev)), "lq_resident_tree_attention")
+    return out
+
+
+def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, logits: Optional[torch.Tensor] = None,
+                  choice: Optional[torch.Tensor] = None, work: Optional[torch.Tensor] = None
+                  ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The drafts of each sequence that the model confirms.
+
+    tokens: (B, N) int64, the drafted tokens (node 0: the newest token); parents:
+    (B, N) or (N,), as in resident_tree_attention; logits: (B, N, V) fp16, bf16 or
+    fp32, the model's at each node, whose argmax (lowest index of equal ones, NaN
+    above all) is the node's choice -- or choice: (B, N) int64, e.g. a sample of each
+    node's distribution.  From node 0 the walk goes to the lowest-numbered child whose
+    token is the node's choice, until there is none.  Returns (path (B, N) int32: the
+    nodes walked, then -1; count (B,) int32: how many, 0 where node 0 is padding;
+    next (B,) int64: the last one's choice, -1 there), on tokens' device."""
+    lib = L.lib()
+    if (logits is None) == (choice is None):
+        raise ValueError("either logits or choice")
+    if tokens.dim() != 2 or tokens.dtype != torch.int64 or not tokens.is_cuda:
+        raise ValueError("tokens must be (B, N) int64 on the GPU")
+    B, N = tokens.shape
+    dev = tokens.device
+    if B < 1 or not 1 <= N <= MAX_NODES:
+        raise ValueError(f"at least one sequence of 1..{MAX_NODES} nodes")
+    vocab = dt = need = 0
+    if logits is not None:
+        if logits.dim() != 3 or logits.shape[:2] != (B, N) or logits.device != dev or logits.shape[2] < 1:
+            raise ValueError("logits must be (B, N, V) on the tokens' device")
+        if logits.dtype not in _DTYPES + (torch.float32,):
+            raise ValueError("logits must be fp16, bf16 or fp32")
+        vocab, dt = logits.shape[2], L.dtype_code(logits.dtype)
+        need = lib.lq_accept_workspace(B, N, vocab)
+        if need < 0:
+            raise ValueError("too many nodes (65535 in all) or too large a vocabulary")
+    elif tuple(choice.shape) != (B, N) or choice.dtype != torch.int64 or choice.device != dev:
+        raise ValueError("choice must be (B, N) int64 on the tokens' device")
+    with torch.cuda.device(dev):
+        if logits is not None:
+            if logits.stride(2) != 1:
+                logits = logits.contiguous()
+            if work is None:
+                work = torch.empty(need, dtype=torch.uint8, device=dev)
+            elif work.device != dev or not work.is_contiguous() or work.numel() * work.element_size() < need:
+                raise ValueError("acceptance workspace too small, or on another device")
+        else:
+            choice = choice.contiguous()
+        par, tok = _parents(parents, B, N, dev), tokens.contiguous()
+        path = torch.empty(B, N, dtype=torch.int32, device=dev)
+        count = torch.empty(B, dtype=torch.int32, device=dev)
+        nxt = torch.empty(B, dtype=torch.int64, device=dev)
+        sb, sn = (0, 0) if logits is None else logits.stride()[:2]
+        L.check(lib.lq_accept_drafts(L.ptr(logits), dt, sb, sn, vocab, L.ptr(choice), tok.data_ptr(), par.data_ptr(),
+                                     B, N, L.ptr(work), path.data_ptr(), count.data_ptr(), nxt.data_ptr(),
+                                     L.stream_ptr(dev)), "lq_accept_drafts")
+    return path, count, nxt
+
+
+def _pairs(dst: Sequence[torch.Tensor], src: Sequence[torch.Tensor], what: str):
+    """Checked (destination, source) lists of row tensors (B, H, rows, width), grouped by
+    layout: [(pointers, pointers, strides, strides, sources kept alive)]."""
+    if not len(dst) or len(dst) != len(src):
+        raise ValueError(f"{what}: as many destinations as sources, one at least")
+    d0, s0 = dst[0], src[0]
+    if d0.dim() != 4 or s0.dim() != 4:
+        raise ValueError(f"{what}: tensors of (B, H, rows, width)")
+    if any(t.shape != d0.shape or t.dtype != d0.dtype or t.device != d0.device for t in dst):
+        raise ValueError(f"{what}: destinations of one shape, type and device")
+    if any(t.shape != s0.shape or t.dtype != d0.dtype or t.device != d0.device for t in src):
+        raise ValueError(f"{what}: sources of one shape, and of the destinations' type and device")
+    el = d0.element_size()
+    if not d0.is_cuda or d0.shape[3] != s0.shape[3] or d0.shape[3] * el % 16 or not 16 <= d0.shape[3] * el <= 4096:
+        raise ValueError(f"{what}: rows on the GPU, of one width, a multiple of 16 bytes")
+
+    def fits(t):
+        return t.stride(3) == 1 and not any(x * el % 16 for x in t.stride()[:3]) and t.data_ptr() % 16 == 0
+    if any(not fits(t) or any(x == 0 and n > 1 for x, n in zip(t.stride(), t.shape)) for t in dst):
+        raise ValueError(f"{what}: destination rows must be contiguous, apart and 16-byte aligned")
+    groups = {}
+    for d, s in zip(dst, src):
+        s = s if fits(s) else s.contiguous()
+        groups.setdefault((d.stride(), s.stride()), []).append((d.data_ptr(), s.data_ptr(), s))
+    out = []
+    for (sd, ss), g in groups.items():
+        n = len(g)
+        out.append((n, (ctypes.c_void_p * n)(*(x[0] for x in g)), (ctypes.c_void_p * n)(*(x[1] for x in g)),
+                    (ctypes.c_int64 * 3)(*(x * el for x in sd[:3])), (ctypes.c_int64 * 3)(*(x * el for x in ss[:3])), g))
+    return out
+
+
+def append_accepted(tails: Sequence[torch.Tensor], drafts: Sequence[torch.Tensor], path: torch.Tensor,
+                    count: torch.Tensor, tail_len: torch.Tensor) -> torch.Tensor:
+    """Accepted drafts into the tails, in place: row tail_len[b] + j of every tail
+    (B, H, cap, width) becomes row path[b][j] of its draft (B, H, N, width), j < count[b];
+    the other rows stay.  tails / drafts: lists (K and V of all layers: one launch per
+    128 of one layout); path (B, N), count and tail_len (B,) as accept_drafts and the
+    tails have them.  Returns the new lengths (B,) int32, tail_len + count.  The caller
+    keeps cap >= tail_len + count: rows past cap are left out (the length stops there)."""
+    lib = L.lib()
+    groups = _pairs(tails, drafts, "append_accepted")
+    B, H, cap, width = tails[0].shape
+    N, dev = drafts[0].shape[2], tails[0].device
+    if drafts[0].shape[:2] != (B, H) or B < 1 or H < 1 or cap < 1 or not 1 <= N <= MAX_NODES:
+        raise ValueError(f"drafts must be (B, H, N, width) of the tails' B and H, N 1..{MAX_NODES}")
+    with torch.cuda.device(dev):
+        pt, ct = _ints(path, (B, N), "path", dev), _ints(count, (B,), "count", dev)
+        ln = _ints(tail_len, (B,), "tail_len", dev)
+        if L.debug_checks() and (bool((ln + ct > cap).any()) or bool((ct > N).any())):
+            raise ValueError("accepted rows do not fit the tails")
+        new = torch.empty(B, dtype=torch.int32, device=dev)
+        for n, d, s, sd, ss, _ in groups:
+            L.check(lib.lq_append_rows(d, s, n, sd, ss, B, H, cap, N, width * tails[0].element_size(), pt.data_ptr(),
+                                       ct.data_ptr(), ln.data_ptr(), new.data_ptr(), L.stream_ptr(dev)),
+                    "lq_append_rows")
+    return new
+
+
+def gather_tails(tails: Sequence[torch.Tensor], index: torch.Tensor) -> list:
+    """New tails of the sequences index[r] of every tail (B, H, T, width): what
+    torch.index_select(tail, 0, index) gives for each, in one launch per 128.  Indices
+    are clamped to 0 .. B - 1."""
+    lib = L.lib()
+    if not len(tails):
+        return []
+    t0 = tails[0]
+    if t0.dim() != 4 or index.dim() != 1 or index.numel() < 1:
+        raise ValueError("tails of (B, H, T, width) and a list of sequences")
+    out = [torch.empty((index.numel(),) + tuple(t.shape[1:]), dtype=t.dtype, device=t.device) for t in tails]
+    if t0.shape[2] == 0 or t0.shape[1] == 0:
+        return out
+    groups = _pairs(out, tails, "gather_tails")
+    B, H, T, width = t0.shape
+    with torch.cuda.device(t0.device):
+        idx = _ints(index, (index.numel(),), "index", t0.device)
+        if B < 1:
+            raise ValueError("no sequences to choose from")
+        for n, d, s, sd, ss, _ in groups:
+            L.check(lib.lq_gather_rows(d, s, n, sd, ss, B, index.numel(), H, T, width * t0.element_size(),
+                                       idx.data_ptr(), L.stream_ptr(t0.device)), "lq_gather_rows")
     return out
