@@ -69,7 +69,7 @@ struct TreeArgs {
     const int32_t* start;
     int64_t tail_cap;
     int heads, group, nodes, rows, rb, nsp, tiles;   // rows = nodes * group; rb: row blocks; tiles: of 32 max(1, C / 2) tokens
-    int np, nt;                                       // prefix and tail tiles (the draft's follow)
+    int np, nt, per;                                  // prefix and tail tiles (the draft's follow); tiles of a split's share
     float* rec;
 };
 
@@ -84,7 +84,8 @@ __device__ __forceinline__ uint32_t range_word(int64_t lo, int64_t hi) {
 struct Sub {
     int kind;        // 0 prefix, 1 tail, 2 draft
     int64_t t;       // first token within its kind
-    uint32_t word;
+    int have;        // tokens from t on that exist, 32 at most
+    uint32_t word;   // those that the sequence sees
 };
 
 template <int S>   // S subtiles per tile
@@ -93,14 +94,17 @@ __device__ __forceinline__ Sub sub_of(const TreeArgs& A, int tile, int u, int64_
     if (tile < A.np) {
         s.kind = 0;
         s.t = ((int64_t)tile * S + u) * 32;
+        s.have = (int)min(A.t_prefix - s.t, (int64_t)32);
         s.word = range_word(start - s.t, A.t_prefix - s.t);
     } else if (tile < A.np + A.nt) {
         s.kind = 1;
         s.t = ((int64_t)(tile - A.np) * S + u) * 32;
+        s.have = (int)min(len - s.t, (int64_t)32);
         s.word = range_word(start - A.t_prefix - s.t, len - s.t);
     } else {
         s.kind = 2;
         s.t = ((int64_t)(tile - A.np - A.nt) * S + u) * 32;
+        s.have = (int)min(A.nodes - s.t, (int64_t)32);
         s.word = range_word(0, A.nodes - s.t);
     }
     return s;
@@ -120,6 +124,8 @@ __device__ __forceinline__ uint4 bf_to_h(const uint4& w) {
     for (int i = 0; i < 4; i++) y[i] = pair_h(__uint_as_float(x[i] << 16), __uint_as_float(x[i] & 0xffff0000u));
     return make_uint4(y[0], y[1], y[2], y[3]);
 }
+
+__device__ __forceinline__ float bf2h2f(uint16_t u) { return h2f(f2h(bf2f(u))); }   // a bf16 value as the products take it
 
 template <bool BF16>
 __device__ __forceinline__ uint4 load_row8(const uint16_t* p) {
@@ -168,10 +174,23 @@ __device__ __forceinline__ T at32(const void* base, uint32_t bytes) {
 
 // Exceptions (vectors outside the 5-bit range): a block's entries lie in record order
 // from its base, so an entry's number is the base plus the set bits of the block's
-// masks before it.  Entries are loaded by all lanes at once (a lane without one reads
-// the list's first) and selected: no lane waits for another's.
-__device__ __forceinline__ uint4 exc_at(const lq_resident& r, bool mine, int64_t e) {
-    return reinterpret_cast<const uint4*>(r.exc)[mine ? e : 0];
+// masks before it.  The first 32 of both blocks are loaded with the tile, one a lane
+// (lanes 0..31 of the first block's, 32..63 of the second's), from the bases and counts
+// of a tile further on: taken when the masks are known, their latency would stand in
+// every tile that has one (with outlier channels all of them: 32768 tokens, 16 rows a
+// head, 5.6 % of K's vectors: 41 us against 32 without any, at first).
+struct Meta {
+    uint32_t base, count;   // of the lane's half
+};
+__device__ __forceinline__ Meta load_meta(const lq_resident& r, int64_t hd, int64_t t, int64_t T, uint32_t lane) {
+    const Blocks B = blocks_of(r, hd, t, T);
+    const uint2 w = at32<uint2>(r.meta + B.rb0 * 4 + 2, ((lane >> 5) & B.d) * 16);
+    return {w.x, w.y};
+}
+__device__ __forceinline__ uint4 load_entry(const lq_resident& r, const Meta& m, uint32_t lane) {
+    const uint32_t e = lane & 31;
+    const int64_t at = (int64_t)m.base + e;
+    return reinterpret_cast<const uint4*>(r.exc)[e < m.count && at < r.exc_cap ? at : 0];
 }
 // an entry's eight values 2c as fp16 pairs of c (halving is exact)
 __device__ __forceinline__ void exc_pairs(const uint4& w, uint32_t p[4]) {
@@ -181,13 +200,6 @@ __device__ __forceinline__ void exc_pairs(const uint4& w, uint32_t p[4]) {
         const h2_t h = {(_Float16)(int16_t)(x[i] & 0xffffu), (_Float16)(int16_t)(x[i] >> 16)};
         p[i] = __builtin_bit_cast(uint32_t, h * (h2_t){(_Float16)0.5f, (_Float16)0.5f});
     }
-}
-__device__ __forceinline__ void exc_select(bool any, bool mine, const uint4& w, uint32_t p[4]) {
-    if (!any) return;   // wave-uniform
-    uint32_t e[4];
-    exc_pairs(w, e);
-#pragma unroll
-    for (int i = 0; i < 4; i++) p[i] = mine ? e[i] : p[i];
 }
 
 // A lane's eight records of 32 tokens, four from rec[0] on and four from rec[1] on (record
@@ -208,10 +220,8 @@ struct Raw {
     uint32_t b[2];
     uint2 s[2];
     uint2 mask[2];   // exceptions of the records' group
-    uint32_t base;   // first exception entry of block lane % 2 (K), of the lane's block (V)
 };
-__device__ __forceinline__ void load_raw(const lq_resident& r, int64_t hd, int64_t t, int64_t T, const Lay& y, uint32_t bhi,
-                                         Raw& d) {
+__device__ __forceinline__ void load_raw(const lq_resident& r, int64_t hd, int64_t t, int64_t T, const Lay& y, Raw& d) {
     const Blocks B = blocks_of(r, hd, t, T);
 #pragma unroll
     for (int j = 0; j < 2; j++) {
@@ -221,41 +231,19 @@ __device__ __forceinline__ void load_raw(const lq_resident& r, int64_t hd, int64
         d.s[j] = at32<uint2>(r.scale + B.rb0 * kRB, (blk * kRB + (y.rec[j] & 15)) * 2);
         d.mask[j] = at32<uint2>(r.mask + B.rb0 * 4, (blk * 4 + (y.rec[j] >> 6)) * 8);
     }
-    d.base = at32<uint32_t>(r.meta + B.rb0 * 4 + 2, (bhi & B.d) * 16);
 }
 
-__device__ __forceinline__ void stage_k(const lq_resident& r, const Raw& d, int lane, char* lds) {
+__device__ __forceinline__ void stage_k(const Raw& d, int lane, char* lds) {
     const int v = lane >> 2, t0 = 4 * (lane & 3);
 #pragma unroll
     for (int x = 0; x < 2; x++) {
         const uint32_t aw[4] = {d.a[x].x, d.a[x].y, d.a[x].z, d.a[x].w};
-        uint4 ex[4];
-        uint32_t own = 0u;
-        bool any[4] = {false, false, false, false};
-        if (__any((d.mask[x].x | d.mask[x].y) != 0u)) {
-            const uint64_t m = ((uint64_t)d.mask[x].y << 32) | d.mask[x].x;
-            const int pc = __builtin_popcountll(m), at = 16 * (v & 3) + t0;
-            uint32_t idx = (uint32_t)__builtin_amdgcn_readlane((int)d.base, x);
-#pragma unroll
-            for (int g = 0; g < 3; g++) idx += (lane >> 4) > g ? __builtin_amdgcn_readlane(pc, 16 * g) : 0;
-            idx += __builtin_popcountll(m & ((1ull << at) - 1ull));
-            own = (uint32_t)(m >> at) & 15u;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int64_t e = (int64_t)idx + __builtin_popcount(own & ((1u << i) - 1u));
-                const bool mine = ((own >> i) & 1u) && e < r.exc_cap;
-                if (!mine) own &= ~(1u << i);
-                any[i] = __any(mine);
-                if (any[i]) ex[i] = exc_at(r, mine, e);
-            }
-        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             uint32_t p[4];
             rec_pairs(aw[i], (d.b[x] >> (8 * i)) & 0xffu, p);
 #pragma unroll
             for (int j = 0; j < 4; j++) p[j] = unbias(p[j]);
-            exc_select(any[i], (own >> i) & 1u, ex[i], p);
             const uint32_t sw = i < 2 ? d.s[x].x : d.s[x].y;
             mul_pairs<4>(p, __builtin_amdgcn_perm(0u, sw, i & 1 ? 0x03020302u : 0x01000100u));
             put_k(lds, 16 * x + t0 + i, v, make_uint4(p[0], p[1], p[2], p[3]));
@@ -263,8 +251,8 @@ __device__ __forceinline__ void stage_k(const lq_resident& r, const Raw& d, int 
     }
 }
 
-// pairs vp[k][i] = dimension 8 n + i of the lane's tokens 2 k, 2 k + 1
-__device__ __forceinline__ void decode_v(const lq_resident& r, const Raw& d, uint32_t word, int lane, uint32_t vp[4][8]) {
+// pairs vp[k][i] = dimension 8 n + i of the lane's tokens 2 k, 2 k + 1, without the scales
+__device__ __forceinline__ void decode_v(const Raw& d, uint32_t vp[4][8]) {
     const uint32_t aw[8] = {d.a[0].x, d.a[0].y, d.a[0].z, d.a[0].w, d.a[1].x, d.a[1].y, d.a[1].z, d.a[1].w};
 #pragma unroll
     for (int k = 0; k < 4; k++) {
@@ -273,45 +261,80 @@ __device__ __forceinline__ void decode_v(const lq_resident& r, const Raw& d, uin
 #pragma unroll
         for (int i = 0; i < 8; i++) vp[k][i] = unbias(vp[k][i]);
     }
-    if (__any((d.mask[0].x | d.mask[0].y) != 0u)) {
-        const int n = lane & 15, k8 = lane >> 4, g = n >> 2;
-        const uint64_t m = ((uint64_t)d.mask[0].y << 32) | d.mask[0].x;
-        const int pc = __builtin_popcountll(m), s0 = 16 * (n & 3) + 8 * (k8 & 1);
-        uint32_t idx = d.base;
-#pragma unroll
-        for (int c = 0; c < 3; c++) {
-            const int lo = __builtin_amdgcn_readlane(pc, 4 * c), hi = __builtin_amdgcn_readlane(pc, 32 + 4 * c);
-            idx += g > c ? ((k8 >> 1) ? hi : lo) : 0;
-        }
-        idx += __builtin_popcountll(m & ((1ull << s0) - 1ull));
-        const uint32_t own = (uint32_t)(m >> s0) & 0xffu;
-#pragma unroll 1
-        for (int q0 = 0; q0 < 8; q0 += 2) {   // the lane's tokens q0, q0 + 1: pair row q0 / 2
-            if (!__any((own >> q0) & 3u)) continue;
-            const int64_t e = (int64_t)idx + __builtin_popcount(own & ((1u << q0) - 1u));
-            const bool m0 = ((own >> q0) & 1u) && e < r.exc_cap;
-            const int64_t e1 = e + ((own >> q0) & 1u);
-            const bool m1 = ((own >> q0) & 2u) && e1 < r.exc_cap;
-            const uint4 x0 = exc_at(r, m0, e), x1 = exc_at(r, m1, e1);
-            uint32_t p0[4], p1[4];
-            exc_pairs(x0, p0);
-            exc_pairs(x1, p1);
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (k != q0 >> 1) continue;   // wave-uniform
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const uint32_t h0 = m0 ? (p0[i >> 1] >> (16 * (i & 1))) & 0xffffu : vp[k][i] & 0xffffu;
-                    const uint32_t h1 = m1 ? (i & 1 ? p1[i >> 1] & 0xffff0000u : p1[i >> 1] << 16) : vp[k][i] & 0xffff0000u;
-                    vp[k][i] = h0 | h1;
-                }
-            }
-        }
-    }
+}
+__device__ __forceinline__ void scale_v(const Raw& d, uint32_t word, int lane, uint32_t vp[4][8]) {
     const uint32_t sw[4] = {d.s[0].x, d.s[0].y, d.s[1].x, d.s[1].y};
 #pragma unroll
     for (int k = 0; k < 4; k++) mul_pairs<8>(vp[k], sw[k]);
     if (word != ~0u) clear_v(word, lane >> 4, vp);
+}
+
+// How many exceptions stand before the lane's four records from rec[j] on in their block:
+// those of the record groups before (popcounts of the other lanes' masks) and in the group.
+__device__ __forceinline__ uint32_t rank_of(bool isk, const Raw& d, const Lay& y, int j, int lane) {
+    const uint64_t m = ((uint64_t)d.mask[j].y << 32) | d.mask[j].x;
+    const int pc = __builtin_popcountll(m), g = (int)(y.rec[j] >> 6);
+    uint32_t n = __builtin_popcountll(m & ((1ull << (y.rec[j] & 63)) - 1ull));
+#pragma unroll
+    for (int c = 0; c < 3; c++) {   // group c: K lane 16 c; V lane 4 c of the first block, 32 + 4 c of the second
+        const int lo = __builtin_amdgcn_readlane(pc, isk ? 16 * c : 4 * c), hi = __builtin_amdgcn_readlane(pc, isk ? 16 * c : 32 + 4 * c);
+        n += g > c ? (lane >> 5 ? hi : lo) : 0;
+    }
+    return n;
+}
+
+__device__ __forceinline__ void wave_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The exceptions of 32 tokens whose records are staged in LDS: a record's lane leaves its
+// place and scale for the lane that holds its entry (place: 64 words of the wave's own),
+// which writes the eight values over the staged ones.  Rounds of 32 entries a block;
+// `ent` has the first.
+__device__ __forceinline__ void patch_lds(bool isk, const lq_resident& r, const Raw& d, const Lay& y, const Meta& m, uint4 ent,
+                                          uint32_t word, int lane, uint32_t* place, char* lds) {
+    if (!__any(((d.mask[0].x | d.mask[0].y) | (d.mask[1].x | d.mask[1].y)) != 0u)) return;
+    uint32_t rank[2], own[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const uint64_t mk = ((uint64_t)d.mask[j].y << 32) | d.mask[j].x;
+        rank[j] = rank_of(isk, d, y, j, lane);
+        own[j] = (uint32_t)(mk >> (y.rec[j] & 63)) & 15u;
+    }
+    const uint32_t most = max(__builtin_amdgcn_readlane((int)m.count, 0), __builtin_amdgcn_readlane((int)m.count, 32));
+#pragma unroll 1
+    for (uint32_t r0 = 0; r0 < most; r0 += 32) {
+        if (r0) ent = load_entry(r, {m.base + r0, m.count > r0 ? m.count - r0 : 0u}, lane);
+        wave_lds_sync();
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t e = rank[j] + __builtin_popcount(own[j] & ((1u << i) - 1u)) - r0;
+                const uint32_t sw = i < 2 ? d.s[j].x : d.s[j].y;
+                if (((own[j] >> i) & 1u) && e < 32u)   // scale, token of the 32, vector
+                    place[32 * y.hi[j] + e] = (i & 1 ? sw & 0xffff0000u : sw << 16) |
+                                              ((16 * y.hi[j] + (y.rec[j] & 15) + i) << 4) | (y.rec[j] >> 4);
+            }
+        wave_lds_sync();
+        const uint32_t e = r0 + (lane & 31);
+        if (e < m.count && (int64_t)m.base + e < r.exc_cap) {
+            const uint32_t got = place[lane], v = got & 15u, tok = (got >> 4) & 31u;
+            uint32_t p[4];
+            exc_pairs(ent, p);
+            mul_pairs<4>(p, __builtin_amdgcn_perm(0u, got, 0x03020302u));
+            if (isk) {
+                put_k(lds, tok, v, make_uint4(p[0], p[1], p[2], p[3]));
+            } else if ((word >> tok) & 1u) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    *reinterpret_cast<uint16_t*>(lds + 32 * kKRow + (16 * i + v) * kVRow + 2 * tok) =
+                        (uint16_t)(i & 1 ? p[i >> 1] >> 16 : p[i >> 1]);
+            }
+        }
+    }
 }
 
 // K for the operands of k_tree_few: a lane has tokens 8 g + 2 i, + 1 (lane % 16 = 4 g + i)
@@ -321,7 +344,6 @@ struct KFew {
     uint32_t b[4];
     uint32_t s;
     uint2 mask;      // lanes 0..7: exceptions of block lane / 4, record group lane % 4
-    uint32_t base;   // first exception entry of the lane's block
 };
 __device__ __forceinline__ void load_few(const lq_resident& r, int64_t hd, int64_t t, int64_t T, uint32_t lane, KFew& d) {
     const Blocks B = blocks_of(r, hd, t, T);
@@ -334,84 +356,127 @@ __device__ __forceinline__ void load_few(const lq_resident& r, int64_t hd, int64
         d.b[c] = at32<uint16_t>(r.b + B.rb0 * 256, rec + 64 * c);
     }
     d.s = at32<uint32_t>(r.scale + B.rb0 * kRB, (blk * kRB + tok) * 2);
-    d.base = at32<uint32_t>(r.meta + B.rb0 * 4 + 2, blk * 16);
     d.mask = at32<uint2>(r.mask + B.rb0 * 4, ((lane >> 2) & B.d) * 32 + (lane & 3) * 8);
 }
 
-// the exception entries of the lane's eight records: bit 2 c + y of own: token y of group c
-struct ExcFew {
-    uint4 e[4][2];
-    uint32_t own, any;
-};
-__device__ __forceinline__ void exc_few(const lq_resident& r, const KFew& d, int lane, ExcFew& ex) {
-    const int row = lane & 15, kg = lane >> 4;
-    const int at = 16 * kg + 8 * ((row >> 2) & 1) + 2 * (row & 3);
-    uint32_t idx = d.base;
-    ex.own = ex.any = 0u;
+// The converted entry (pairs e of the lane that holds it) of the record of rank `rank` in
+// block `blk`, over p, for the lanes that own one.  Entries past the first 32 of a block
+// are loaded here.
+__device__ __forceinline__ void pull_entry(const lq_resident& r, const Meta& m, const uint32_t e[4], bool own, uint32_t blk,
+                                           uint32_t rank, uint32_t p[4]) {
+    if (!__any(own)) return;
+    uint32_t x[4];
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-        const uint32_t l0 = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.x, c), h0 = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.y, c);
-        const uint32_t l1 = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.x, 4 + c), h1 = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.y, 4 + c);
-        if ((l0 | h0 | l1 | h1) == 0u) continue;   // wave-uniform
-        const uint64_t m = row >> 3 ? ((uint64_t)h1 << 32) | l1 : ((uint64_t)h0 << 32) | l0;
-        const int64_t e = (int64_t)idx + __builtin_popcountll(m & ((1ull << at) - 1ull));
-        const uint32_t two = (uint32_t)(m >> at) & 3u;
-        const bool m0 = (two & 1u) && e < r.exc_cap, m1 = (two & 2u) && e + (two & 1u) < r.exc_cap;
-        ex.e[c][0] = exc_at(r, m0, e);
-        ex.e[c][1] = exc_at(r, m1, e + (two & 1u));
-        ex.own |= ((m0 ? 1u : 0u) | (m1 ? 2u : 0u)) << (2 * c);
-        ex.any |= (__any(m0) ? 1u : 0u) << (2 * c) | (__any(m1) ? 2u : 0u) << (2 * c);
-        idx += row >> 3 ? __builtin_popcount(l1) + __builtin_popcount(h1) : __builtin_popcount(l0) + __builtin_popcount(h0);
+    for (int i = 0; i < 4; i++) x[i] = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(4 * (32 * blk + (rank & 31))), (int)e[i]);
+    const uint32_t b0 = (uint32_t)__builtin_amdgcn_readlane((int)m.base, 0), b1 = (uint32_t)__builtin_amdgcn_readlane((int)m.base, 32);
+    const int64_t at = (int64_t)(blk ? b1 : b0) + rank;
+    own = own && at < r.exc_cap;
+    if (__any(own && rank >= 32u)) {
+        uint32_t f[4];
+        exc_pairs(reinterpret_cast<const uint4*>(r.exc)[own ? at : 0], f);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = rank >= 32u ? f[i] : x[i];
     }
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = own ? x[i] : p[i];
 }
 
-template <bool BF16>
-__device__ void rows_k(const Rows& R, int64_t b, int64_t h, int64_t t, uint32_t word, int lane, char* lds) {
-    const uint16_t* p = R.p + b * R.sb + h * R.sh;
+// K's masks of record group c in the lane's block, and how many stand before group c
+struct FewMask {
+    uint64_t m;
+    uint32_t any;   // wave-uniform
+};
+__device__ __forceinline__ FewMask few_mask(const KFew& d, int c, int lane) {
+    const uint32_t l0 = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.x, c), h0 = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.y, c);
+    const uint32_t l1 = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.x, 4 + c), h1 = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.y, 4 + c);
+    return {(lane & 8) ? ((uint64_t)h1 << 32) | l1 : ((uint64_t)h0 << 32) | l0, l0 | h0 | l1 | h1};
+}
+
+// V's exceptions over the pairs of decode_v
+__device__ __forceinline__ void pull_v(const lq_resident& r, const Raw& d, const Lay& y, const Meta& m, uint4 ent, int lane,
+                                       uint32_t vp[4][8]) {
+    if (!__any((d.mask[0].x | d.mask[0].y) != 0u)) return;
+    const uint64_t mk = ((uint64_t)d.mask[0].y << 32) | d.mask[0].x;
+    const uint32_t rank = rank_of(false, d, y, 0, lane), own = (uint32_t)(mk >> (y.rec[0] & 63)) & 0xffu;
+    uint32_t e[4];
+    exc_pairs(ent, e);
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
-        const int tok = 16 * x + (lane & 15);
+    for (int q = 0; q < 8; q++) {
+        const bool mine = (own >> q) & 1u;
+        if (!__any(mine)) continue;
+        uint32_t p[4];
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const int vec = 4 * c + (lane >> 4);
-            uint4 w = make_uint4(0u, 0u, 0u, 0u);
-            if ((word >> tok) & 1u) w = load_row8<BF16>(p + (t + tok) * R.st + 8 * vec);
-            put_k(lds, tok, vec, w);
+        for (int i = 0; i < 4; i++)     // the token's own pairs of dimensions
+            p[i] = __builtin_amdgcn_perm(vp[q >> 1][2 * i + 1], vp[q >> 1][2 * i], q & 1 ? 0x07060302u : 0x05040100u);
+        pull_entry(r, m, e, mine, y.hi[0], rank + __builtin_popcount(own & ((1u << q) - 1u)), p);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t &w0 = vp[q >> 1][2 * i], &w1 = vp[q >> 1][2 * i + 1];
+            w0 = __builtin_amdgcn_perm(p[i], w0, q & 1 ? 0x05040100u : 0x03020504u);
+            w1 = __builtin_amdgcn_perm(p[i], w1, q & 1 ? 0x07060100u : 0x03020706u);
         }
     }
 }
 
-// V of the lane's eight tokens as decode_v gives it; returns whether one of the wave's
-// values is an infinity or a NaN
+// fp16 / bf16 rows: 32 tokens from t on, of which the first `have` exist (one at least);
+// the others read the last that does.
 template <bool BF16>
-__device__ __forceinline__ bool rows_v(const Rows& R, int64_t b, int64_t h, int64_t t, uint32_t word, int lane,
+__device__ __forceinline__ void rows_k(const uint16_t* p, int64_t st, int64_t t, int have, int lane, char* lds) {
+    uint4 w[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const int tok = 16 * (j >> 2) + (lane & 15);
+        w[j] = *reinterpret_cast<const uint4*>(p + (t + min(tok, have - 1)) * st + 8 * (4 * (j & 3) + (lane >> 4)));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        put_k(lds, 16 * (j >> 2) + (lane & 15), 4 * (j & 3) + (lane >> 4), BF16 ? bf_to_h(w[j]) : w[j]);
+}
+
+// V of the lane's eight tokens as decode_v gives it, tokens outside the word cleared
+template <bool BF16>
+__device__ __forceinline__ void rows_v(const uint16_t* p, int64_t st, int64_t t, int have, uint32_t word, int lane,
                                        uint32_t vp[4][8]) {
-    const uint16_t* p = R.p + b * R.sb + h * R.sh;
     const int n = lane & 15, k8 = lane >> 4;
-    uint32_t bad = 0u;
+    uint4 w[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) w[j] = *reinterpret_cast<const uint4*>(p + (t + min(8 * k8 + j, have - 1)) * st + 8 * n);
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (BF16) w[j] = bf_to_h(w[j]);
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        const int tok = 8 * k8 + 2 * k;
-        uint4 w0 = make_uint4(0u, 0u, 0u, 0u), w1 = w0;
-        if ((word >> tok) & 1u) w0 = load_row8<BF16>(p + (t + tok) * R.st + 8 * n);
-        if ((word >> (tok + 1)) & 1u) w1 = load_row8<BF16>(p + (t + tok + 1) * R.st + 8 * n);
+        const uint4 w0 = w[2 * k], w1 = w[2 * k + 1];
         const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             vp[k][2 * i] = __builtin_amdgcn_perm(x1[i], x0[i], 0x05040100u);
             vp[k][2 * i + 1] = __builtin_amdgcn_perm(x1[i], x0[i], 0x07060302u);
         }
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            bad |= (uint32_t)((vp[k][i] & 0x7c00u) == 0x7c00u) | (uint32_t)((vp[k][i] & 0x7c000000u) == 0x7c000000u);
     }
-    return __any(bad != 0u);
+    if (word != ~0u) clear_v(word, k8, vp);
+}
+
+// A draft's infinities and NaN must reach the rows that see it and no others, but 0 times
+// one of them is a NaN: they are cleared here, and join_teams adds them to the rows that
+// see them.  Returns whether the wave has any.
+__device__ __forceinline__ bool clear_odd(uint32_t vp[4][8]) {
+    bool bad = false;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const bool lo = (vp[k][i] & 0x7c00u) == 0x7c00u, hi = (vp[k][i] & 0x7c000000u) == 0x7c000000u;
+            bad = bad || lo || hi;
+            vp[k][i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+        }
+    return __any(bad);
 }
 
 // ---------------------------------------------------------- 32 x 32 of it --
 
 struct RowState {
-    float m, l;      // running maximum (base 2), the lane's part of the sum
+    float m, l;      // reference (base 2), the lane's part of the sum
     f16_t o[4];      // O^T: column lane % 32, row of MFMA dt: V row 32 dt + 8 (i / 4) + 4 (lane / 32) + i % 4
 };
 
@@ -429,80 +494,71 @@ __device__ __forceinline__ float quarters_max(float v) {
     return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
 
-// One subtile for the wave's 32 rows: word has the visible tokens of the lane's
-// row; every: all of them, for every lane; odd (with DRAFT): V is not finite.
-template <bool DRAFT>
-__device__ __forceinline__ void sub_attend(const char* lds, const h8_t q[8], uint32_t word, bool every, bool odd,
-                                           int lane, RowState& st) {
+// A row's reference m need not be its maximum: it is raised (and l and o rescaled) once
+// a score passes it by more than kLazy, so that P stays below 2^(kPShift + kLazy), in
+// fp16's range.  With 32 rows a wave some row finds a new maximum in nearly every tile;
+// passing the old one by 2^5 is rare after the first.
+constexpr float kLazy = 5.0f;
+
+// U subtiles for the wave's 32 rows, of which the lane's row sees the tokens of word (with
+// MASK, one subtile) or all.  The subtiles' products are independent, so one's softmax
+// runs beside the other's MFMA.
+template <int U, bool MASK>
+__device__ __forceinline__ void sub_attend(const char* lds, const h8_t q[8], uint32_t word, int lane, RowState& st) {
     const float c0 = 1.4426950408889634f / 11.313708498984761f;   // log2(e) / sqrt(128)
     const int n = lane & 31, g = lane >> 5;
     const int tok = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
-    f16_t s = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    f16_t s[U];
 #pragma unroll
-    for (int c = 0; c < 8; c++) {
-        const h8_t ka = *reinterpret_cast<const h8_t*>(lds + tok * kKRow + 32 * c + 16 * g);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, q[c], s, 0, 0, 0);
+    for (int u = 0; u < U; u++) {
+        s[u] = f16_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            const h8_t ka = *reinterpret_cast<const h8_t*>(lds + u * kSub + tok * kKRow + 32 * c + 16 * g);
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, q[c], s[u], 0, 0, 0);
+        }
     }
-    const uint32_t own = word >> (8 * g);
-    if (!every) {
+    float mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = (own >> tok_of(i)) & 1u ? s[i] : -INFINITY;
+    for (int u = 0; u < U; u++) {
+        if (MASK) {
+            const uint32_t own = word >> (8 * g);
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[u][i] = (own >> tok_of(i)) & 1u ? s[u][i] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
     }
-    float mx = s[0];
-#pragma unroll
-    for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
-    const float mn = fmaxf(st.m, halves_max(mx) * c0);
-    if (__any(mn > st.m)) {
+    const float mn = halves_max(mx) * c0;
+    if (__any(mn > st.m + kLazy)) {
         // a row that has seen nothing has m = -inf, l = 0 and o = 0
-        const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - mn);
+        const float up = fmaxf(st.m, mn);
+        const float al = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - up);
         st.l *= al;
 #pragma unroll
         for (int d = 0; d < 4; d++)
 #pragma unroll
             for (int i = 0; i < 16; i++) st.o[d][i] *= al;
-        st.m = mn;
+        st.m = up;
     }
-    const float off = (mn == -INFINITY ? 0.f : -mn) + kPShift;
-    float p[16];
-    float l = 0.f;
+    const float off = (st.m == -INFINITY ? 0.f : -st.m) + kPShift;
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c0, off));
-        l += p[i];
-    }
-    st.l += l;
-    const char* vl = lds + 32 * kKRow;
-    if (!DRAFT || !odd) {
+    for (int u = 0; u < U; u++) {
+        const char* vl = lds + u * kSub + 32 * kKRow;
 #pragma unroll
         for (int sx = 0; sx < 2; sx++) {
-            const h8_t pb = as_h8(pair_h(p[8 * sx + 0], p[8 * sx + 1]), pair_h(p[8 * sx + 2], p[8 * sx + 3]),
-                                  pair_h(p[8 * sx + 4], p[8 * sx + 5]), pair_h(p[8 * sx + 6], p[8 * sx + 7]));
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * sx + i], c0, off));
+                st.l += p[i];
+            }
+            const h8_t pb = as_h8(pair_h(p[0], p[1]), pair_h(p[2], p[3]), pair_h(p[4], p[5]), pair_h(p[6], p[7]));
 #pragma unroll
             for (int d = 0; d < 4; d++) {
                 const h8_t va = *reinterpret_cast<const h8_t*>(vl + (32 * d + n) * kVRow + 16 * (2 * sx + g));
                 st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb, st.o[d], 0, 0, 0);
             }
-        }
-        return;
-    }
-    // A draft's V with infinities or NaN: they reach the rows that see it and no others,
-    // so the products are taken token by token.
-#pragma unroll 1
-    for (int t = 0; t < 32; t++) {
-        float pv = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; i++) pv = 8 * g + tok_of(i) == t ? p[i] : pv;
-        const float other = __shfl_xor(pv, 32, 64);
-        pv = ((t >> 3) & 1) == g ? pv : other;
-        if ((word >> t) & 1u) {
-#pragma unroll
-            for (int d = 0; d < 4; d++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int row = 32 * d + 8 * (i >> 2) + 4 * g + (i & 3);
-                    const _Float16 v = *reinterpret_cast<const _Float16*>(vl + row * kVRow + 2 * t);
-                    st.o[d][i] = __builtin_fmaf(pv, (float)v, st.o[d][i]);
-                }
         }
     }
 }
@@ -554,26 +610,45 @@ __device__ __forceinline__ void out_pair(const TreeArgs& A, bool bf16, int64_t b
                                            : (uint32_t)f2h(x) | ((uint32_t)f2h(y) << 16);
 }
 
-// Split sp's share of the tiles: `per` of the cache's, the draft's all to the last.
+// Split sp's share of the tiles: `per` of the cache's, the draft's besides to the last.
 struct Share {
     int first, end;
 };
 __device__ __forceinline__ Share share_of(const TreeArgs& A, int sp) {
-    const int per = (A.tiles + A.nsp - 1) / A.nsp, cache = A.np + A.nt;
-    return {min(sp * per, cache), sp == A.nsp - 1 ? A.tiles : min((sp + 1) * per, cache)};
+    const int cache = A.np + A.nt;
+    return {min(sp * A.per, cache), sp == A.nsp - 1 ? A.tiles : min((sp + 1) * A.per, cache)};
+}
+
+struct Place {       // what a workgroup works on
+    int64_t hd, b, kvh, len, start;
+    int sp, row0;
+    int first;       // prefix tile (of 32 tokens) that holds the first visible token
+};
+__device__ __forceinline__ Place place_of(const TreeArgs& A, int rows_wg) {
+    Place p;
+    const uint32_t rest = blockIdx.x / (uint32_t)A.rb, hd = rest / (uint32_t)A.nsp;
+    p.row0 = (int)(blockIdx.x % (uint32_t)A.rb) * rows_wg;
+    p.sp = (int)(rest % (uint32_t)A.nsp);
+    p.hd = hd;
+    p.b = hd / (uint32_t)A.heads;
+    p.kvh = hd % (uint32_t)A.heads;
+    p.len = A.tail_cap ? (A.tail_len ? min((int64_t)max(A.tail_len[p.b], 0), A.tail_cap) : A.tail_cap) : 0;
+    p.start = A.start ? A.start[p.b] : 0;
+    p.first = (int)(min(max(p.start, (int64_t)0), A.t_prefix) / 32);
+    return p;
 }
 
 // The teams' (m, l, O) of a workgroup's rows (in s_m, s_l and buf by wave and column,
 // COLS columns a wave, C waves a team) joined, to the record of the split or to out.
 template <int C, int COLS, bool BF16>
-__device__ __forceinline__ void join_teams(const TreeArgs& A, int64_t hd, int sp, int row0, const float* buf,
-                                           const float (*s_m)[32], const float (*s_l)[32],
-                                           const uint32_t (*vis)[kVisWords], int tid) {
+__device__ __forceinline__ void join_teams(const TreeArgs& A, const Place& P, const float* buf, const float (*s_m)[32],
+                                           const float (*s_l)[32],
+                                           const uint32_t (*vis)[kVisWords], const int* odd, int tid) {
     constexpr int T = kWaves / C;
-    const bool last = sp == A.nsp - 1;
+    const bool last = P.sp == A.nsp - 1;
     for (int idx = tid; idx < COLS * C * (kHd / 2); idx += kWaves * 64) {
         const int lr = idx / (kHd / 2), d = 2 * (idx % (kHd / 2));
-        const int rr = row0 + lr;
+        const int rr = P.row0 + lr;
         if (rr >= A.rows) break;               // idx grows with the row
         const int w0 = lr / COLS, c = lr % COLS;
         float M = -INFINITY;
@@ -591,35 +666,25 @@ __device__ __forceinline__ void join_teams(const TreeArgs& A, int64_t hd, int sp
         }
         const int nd = rr / A.group;
         const bool empty = last && !((vis[nd][nd >> 5] >> (nd & 31)) & 1u);
+        if (last && *odd) {
+            const uint16_t* p = A.dv.p + P.b * A.dv.sb + P.kvh * A.dv.sh + d;
+            for (int t = 0; t <= nd; t++) {
+                if (!((vis[nd][t >> 5] >> (t & 31)) & 1u)) continue;
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(p + t * A.dv.st);
+                const float u = BF16 ? bf2h2f((uint16_t)w) : h2f((uint16_t)w), v = BF16 ? bf2h2f((uint16_t)(w >> 16)) : h2f((uint16_t)(w >> 16));
+                if (!(fabsf(u) < INFINITY)) x += u;
+                if (!(fabsf(v) < INFINITY)) y += v;
+            }
+        }
         if (A.nsp == 1) {
             const float inv = 1.f / L;
-            out_pair(A, BF16, hd / A.heads, hd % A.heads, rr, d, empty ? 0.f : x * inv, empty ? 0.f : y * inv);
+            out_pair(A, BF16, P.b, P.kvh, rr, d, empty ? 0.f : x * inv, empty ? 0.f : y * inv);
         } else {
-            float* rec = A.rec + ((hd * A.nsp + sp) * A.rows + rr) * kRecF;
+            float* rec = A.rec + ((P.hd * A.nsp + P.sp) * A.rows + rr) * kRecF;
             *reinterpret_cast<float2*>(rec + 4 + d) = make_float2(x, y);
             if (d == 0) *reinterpret_cast<float2*>(rec) = make_float2(M, empty ? kEmpty : L);
         }
     }
-}
-
-struct Place {       // what a workgroup works on
-    int64_t hd, b, kvh, len, start;
-    int sp, row0;
-    int first;       // prefix tile (of 32 tokens) that holds the first visible token
-};
-__device__ __forceinline__ Place place_of(const TreeArgs& A, int rows_wg) {
-    Place p;
-    int64_t bid = blockIdx.x;
-    p.row0 = (int)(bid % A.rb) * rows_wg;
-    bid /= A.rb;
-    p.sp = (int)(bid % A.nsp);
-    p.hd = bid / A.nsp;
-    p.b = p.hd / A.heads;
-    p.kvh = p.hd % A.heads;
-    p.len = A.tail_cap ? (A.tail_len ? min((int64_t)max(A.tail_len[p.b], 0), A.tail_cap) : A.tail_cap) : 0;
-    p.start = A.start ? A.start[p.b] : 0;
-    p.first = (int)(min(max(p.start, (int64_t)0), A.t_prefix) / 32);
-    return p;
 }
 
 // 8 values of query row r from dimension d on
@@ -635,23 +700,56 @@ template <int C, bool BF16>
 __global__ __launch_bounds__(kWaves * 64) void k_tree_many(TreeArgs A) {
     constexpr int S = C / 2;                   // subtiles of a tile: waves 0 .. S - 1 of a team decode their K, the others V
     constexpr int T = kWaves / C;              // teams
-    constexpr int kStage = T * S * kSub, kMerge = kWaves * 32 * kMRow * 4;
-    __shared__ __align__(16) char s_buf[kStage > kMerge ? kStage : kMerge];
+    constexpr int kStage = 2 * T * S * kSub;   // two tiles a team: one is read while the next is decoded
+    static_assert(kStage >= kWaves * 32 * (kMRow + 2) * 4 && kStage >= kMaxNodes * 4, "the join and the tree fit the stage");
+    __shared__ __align__(16) char s_buf[kStage];
     __shared__ uint32_t s_vis[kMaxNodes][kVisWords];
-    __shared__ int s_up[kMaxNodes];
-    __shared__ int s_bad[T][S];
-    __shared__ float s_m[kWaves][32], s_l[kWaves][32];
+    __shared__ uint32_t s_place[kWaves][64];
+    __shared__ int s_odd;                      // a draft's V has infinities or NaN
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int team = wave / C, ct = wave % C;
     const Place P = place_of(A, 32 * C);
-    if (P.sp == A.nsp - 1) tree_words(A.parents + P.b * A.nodes, A.nodes, s_vis, s_up, tid);
+    const Share sh = share_of(A, P.sp);
+    char* buf = s_buf + team * 2 * S * kSub;
+    const bool isk = ct < S;                   // wave-uniform
+    const int mine = ct % S;                   // the subtile whose K or V the wave decodes
+    const bool rows_here = P.row0 + 32 * ct < A.rows;
+    // the share's tiles of the prefix that the sequence sees whole; the others (cut by its
+    // start or by the prefix's end, the tail's, the draft's) follow in a loop of their own
+    const int seen = max(sh.first, P.first / S);
+    const int h1 = min(sh.end, (int)(A.t_prefix / (32 * S)));
+    const int h0 = min(max(sh.first, (int)((max(P.start, (int64_t)0) + 32 * S - 1) / (32 * S))), max(h1, seen));
+    const bool prefix = h0 < h1;
 
+    // The wave's records of its next tile are in flight while it works on this one, and the
+    // bases of the tile after.  Reloads are unconditional (past the share they read the
+    // last tile again), so that they land in place and nothing waits on them before their use.
+    const lq_resident& res = isk ? A.k : A.v;
+    const Lay lay = lay_of(isk, lane);
+    Raw raw;
+    Meta meta, ahead;
+    uint4 ent;
+    auto at = [&](int tile) { return ((int64_t)min(tile, h1 - 1) * S + mine) * 32; };
+    auto fetch = [&](int tile) {               // `ahead` has the tile's bases
+        ent = load_entry(res, ahead, lane);
+        meta = ahead;
+        load_raw(res, P.hd, at(tile), A.t_prefix, lay, raw);
+        ahead = load_meta(res, P.hd, at(tile + T), A.t_prefix, lane);
+    };
+    if (prefix) {
+        ahead = load_meta(res, P.hd, at(h0 + team), A.t_prefix, lane);
+        fetch(h0 + team);
+    }
     // the wave's rows: column lane % 32
     const int r = P.row0 + 32 * ct + (lane & 31);
     const int node = r < A.rows ? r / A.group : 0;
     h8_t q[8];
 #pragma unroll
     for (int c = 0; c < 8; c++) q[c] = load_q<BF16>(A, P, r, node, 16 * c + 8 * (lane >> 5));
+    if (P.sp == A.nsp - 1) {
+        if (tid == 0) s_odd = 0;
+        tree_words(A.parents + P.b * A.nodes, A.nodes, s_vis, reinterpret_cast<int*>(s_buf), tid);
+    }
     RowState st;
     st.m = -INFINITY;
     st.l = 0.f;
@@ -660,86 +758,77 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_many(TreeArgs A) {
 #pragma unroll
         for (int i = 0; i < 16; i++) st.o[d][i] = 0.f;
 
-    const Share sh = share_of(A, P.sp);
-    char* buf = s_buf + team * S * kSub;
-    const bool isk = ct < S;                   // wave-uniform
-    const int mine = ct % S;                   // the subtile whose K or V the wave decodes
-    const bool rows_here = P.row0 + 32 * ct < A.rows;
-    const int split = min(sh.end, A.np);       // prefix tiles, then rows: two loops, each with the registers it needs
-    int t0 = max(sh.first, P.first / S);
-    if (t0 < split) {
-        // The wave's records of its next tile are in flight while it works on this one.  The
-        // reload is unconditional (past the share it reads the team's last tile again), so
-        // that it lands in place; nothing waits on it before the next decode.
-        const lq_resident& res = isk ? A.k : A.v;
-        const Lay lay = lay_of(isk, lane);
-        Raw raw;
-        auto fetch = [&](int tile) {
-            const int64_t t = min(((int64_t)min(tile, split - 1) * S + mine) * 32, A.t_prefix - kRB);
-            load_raw(res, P.hd, t, A.t_prefix, lay, isk ? lane & 1 : lane >> 5, raw);
-        };
-        fetch(t0 + team);
-        for (; t0 < split; t0 += T) {
-            const int tile = t0 + team;
-            const Sub sb = sub_of<S>(A, tile, mine, P.len, P.start);
-            char* lds = buf + mine * kSub;
-            if (isk) {
-                stage_k(A.k, raw, lane, lds);
-            } else {
-                uint32_t vp[4][8];
-                decode_v(A.v, raw, sb.word, lane, vp);
-                put_v(lds, lane & 15, lane >> 4, vp);
-            }
-            __builtin_amdgcn_sched_barrier(0);   // every use of the records before their reload
-            fetch(tile + T);
-            __syncthreads();
-            if (tile < split && rows_here) {
-#pragma unroll 1
-                for (int u = 0; u < S; u++) {
-                    const Sub su = sub_of<S>(A, tile, u, P.len, P.start);
-                    if (su.word) sub_attend<false>(buf + u * kSub, q, su.word, su.word == ~0u, false, lane, st);
-                }
-            }
+    // K or V of a tile's records into LDS, by the wave that decodes it
+    auto put = [&](const Raw& d, const Meta& m, const uint4& e, uint32_t word, char* lds) {
+        if (isk) {
+            stage_k(d, lane, lds);
+        } else {
+            uint32_t vp[4][8];
+            decode_v(d, vp);
+            scale_v(d, word, lane, vp);
+            put_v(lds, lane & 15, lane >> 4, vp);
+        }
+        patch_lds(isk, res, d, lay, m, e, word, lane, s_place[wave], lds);
+    };
+    if (prefix) {
+        put(raw, meta, ent, ~0u, buf + mine * kSub);
+        __builtin_amdgcn_sched_barrier(0);     // every use of the records before their reload
+        fetch(h0 + team + T);
+        __syncthreads();
+        for (int t = h0, half = 0; t < h1; t += T, half ^= 1) {
+            put(raw, meta, ent, ~0u, buf + ((half ^ 1) * S + mine) * kSub);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch(t + team + 2 * T);
+            if (t + team < h1 && rows_here) sub_attend<S, false>(buf + half * S * kSub, q, 0u, lane, st);
             __syncthreads();
         }
     }
-    for (t0 = max(sh.first, A.np); t0 < sh.end; t0 += T) {
-        const int tile = t0 + team;
-        if (tile < sh.end) {
+    const int before = prefix ? h0 - seen : 0, after = prefix ? h1 : seen, edge = before + max(0, sh.end - after);
+#pragma unroll 1
+    for (int j = 0; j < edge; j += T) {
+        const int tile = j + team < before ? seen + j + team : after + j + team - before;
+        if (j + team < edge) {
             const Sub sb = sub_of<S>(A, tile, mine, P.len, P.start);
             char* lds = buf + mine * kSub;
-            if (sb.word) {
+            if (sb.word && sb.kind == 0) {
+                Raw d;
+                const Meta m = load_meta(res, P.hd, sb.t, A.t_prefix, lane);
+                load_raw(res, P.hd, sb.t, A.t_prefix, lay, d);
+                put(d, m, load_entry(res, m, lane), sb.word, lds);
+            } else if (sb.word) {
+                const bool draft = sb.kind == 2;
+                const Rows& R = isk ? (draft ? A.dk : A.tk) : (draft ? A.dv : A.tv);
+                const uint16_t* p = R.p + P.b * R.sb + P.kvh * R.sh;
                 if (isk) {
-                    rows_k<BF16>(sb.kind == 1 ? A.tk : A.dk, P.b, P.kvh, sb.t, sb.word, lane, lds);
+                    rows_k<BF16>(p, R.st, sb.t, sb.have, lane, lds);
                 } else {
                     uint32_t vp[4][8];
-                    const bool bad = rows_v<BF16>(sb.kind == 1 ? A.tv : A.dv, P.b, P.kvh, sb.t, sb.word, lane, vp);
+                    rows_v<BF16>(p, R.st, sb.t, sb.have, sb.word, lane, vp);
+                    if (draft && clear_odd(vp) && lane == 0) s_odd = 1;
                     put_v(lds, lane & 15, lane >> 4, vp);
-                    if (lane == 0) s_bad[team][mine] = bad;
                 }
             }
         }
         __syncthreads();
-        if (tile < sh.end && rows_here) {
+        if (j + team < edge && rows_here) {
 #pragma unroll 1
             for (int u = 0; u < S; u++) {
                 const Sub sb = sub_of<S>(A, tile, u, P.len, P.start);
                 if (!sb.word) continue;
-                const bool draft = sb.kind == 2;
-                const uint32_t w = draft ? sb.word & s_vis[node][sb.t >> 5] : sb.word;
-                sub_attend<true>(buf + u * kSub, q, w, !draft && w == ~0u,
-                                 draft && __builtin_amdgcn_readfirstlane(s_bad[team][u]), lane, st);
+                sub_attend<1, true>(buf + u * kSub, q, sb.kind == 2 ? sb.word & s_vis[node][sb.t >> 5] : sb.word, lane, st);
             }
         }
         __syncthreads();
     }
 
+    float* dst = reinterpret_cast<float*>(s_buf) + (wave * 32 + (lane & 31)) * kMRow;
+    float(*s_m)[32] = reinterpret_cast<float(*)[32]>(reinterpret_cast<float*>(s_buf) + kWaves * 32 * kMRow);
+    float(*s_l)[32] = s_m + kWaves;
     const float l = st.l + __shfl_xor(st.l, 32, 64);
     if (lane < 32) {
         s_m[wave][lane] = st.m;
         s_l[wave][lane] = l;
     }
-    float* dst = reinterpret_cast<float*>(s_buf) + (wave * 32 + (lane & 31)) * kMRow;
 #pragma unroll
     for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -751,78 +840,52 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_many(TreeArgs A) {
                                                    st.o[3][8 + 4 * j + i]};
         }
     __syncthreads();
-    join_teams<C, 32, BF16>(A, P.hd, P.sp, P.row0, reinterpret_cast<const float*>(s_buf), s_m, s_l, s_vis, tid);
+    join_teams<C, 32, BF16>(A, P, reinterpret_cast<const float*>(s_buf), s_m, s_l, s_vis, &s_odd, tid);
 }
 
 // The softmax and P V of one column of 16 rows and 32 tokens: s[y][i] is the score of
 // token 8 (lane / 16) + 2 i + y, word the tokens that the lane's row sees (every: all of
-// them, for every lane), odd (with DRAFT) that V is not finite.
+// them, for every lane).
 struct FewState {
-    float m, l;      // running maximum (base 2), the lane's part of the sum
+    float m, l;      // reference (base 2), the lane's part of the sum
     f4_t o[8];       // O^T: column lane % 16; o[mm][i]: dimension 8 (4 (lane / 16) + i) + mm
 };
-template <bool DRAFT>
-__device__ __forceinline__ void few_attend(f4_t s[2], uint32_t word, bool every, bool odd, const uint32_t vp[4][8],
-                                           int lane, FewState& st) {
+__device__ __forceinline__ void few_attend(f4_t s[2], uint32_t word, bool every, const uint32_t vp[4][8], int lane,
+                                           FewState& st) {
     const float c0 = 1.4426950408889634f / 11.313708498984761f;   // log2(e) / sqrt(128)
-    const int col = lane & 15, g = lane >> 4;
     if (!every) {
+        const uint32_t own = word >> (8 * (lane >> 4));
 #pragma unroll
         for (int y = 0; y < 2; y++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[y][i] = (word >> (8 * g + 2 * i + y)) & 1u ? s[y][i] : -INFINITY;
+            for (int i = 0; i < 4; i++) s[y][i] = (own >> (2 * i + y)) & 1u ? s[y][i] : -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
     for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[i >> 2][i & 3]);
-    const float mn = fmaxf(st.m, quarters_max(mx) * c0);
-    if (__any(mn > st.m)) {
-        // a row that has seen nothing has m = -inf, l = 0 and o = 0
-        const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - mn);
+    const float mn = quarters_max(mx) * c0;
+    if (__any(mn > st.m + kLazy)) {
+        const float up = fmaxf(st.m, mn);
+        const float al = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - up);
         st.l *= al;
 #pragma unroll
         for (int mm = 0; mm < 8; mm++)
 #pragma unroll
             for (int i = 0; i < 4; i++) st.o[mm][i] *= al;
-        st.m = mn;
+        st.m = up;
     }
-    const float off = (mn == -INFINITY ? 0.f : -mn) + kPShift;
+    const float off = (st.m == -INFINITY ? 0.f : -st.m) + kPShift;
     float p[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {              // in the order of the tokens
         p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i & 1][i >> 1], c0, off));
         st.l += p[i];
     }
-    if (!DRAFT || !odd) {
-        const h8_t pb = as_h8(pair_h(p[0], p[1]), pair_h(p[2], p[3]), pair_h(p[4], p[5]), pair_h(p[6], p[7]));
+    const h8_t pb = as_h8(pair_h(p[0], p[1]), pair_h(p[2], p[3]), pair_h(p[4], p[5]), pair_h(p[6], p[7]));
 #pragma unroll
-        for (int mm = 0; mm < 8; mm++)
-            st.o[mm] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(vp[0][mm], vp[1][mm], vp[2][mm], vp[3][mm]), pb,
-                                                              st.o[mm], 0, 0, 0);
-        return;
-    }
-    // A draft's V with infinities or NaN: they reach the rows that see it and no others, so
-    // the products are taken token by token.
-#pragma unroll 1
-    for (int t = 0; t < 32; t++) {
-        float pv = p[0];
-#pragma unroll
-        for (int i = 1; i < 8; i++) pv = (t & 7) == i ? p[i] : pv;
-        pv = __shfl(pv, col + 16 * (t >> 3), 64);
-        const bool see = (word >> t) & 1u;
-#pragma unroll
-        for (int mm = 0; mm < 8; mm++) {
-            uint32_t w = vp[0][mm];
-#pragma unroll
-            for (int k = 1; k < 4; k++) w = ((t >> 1) & 3) == k ? vp[k][mm] : w;
-            w = t & 1 ? w >> 16 : w & 0xffffu;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float v = h2f((uint16_t)__shfl((int)w, 4 * g + i + 16 * (t >> 3), 64));
-                if (see) st.o[mm][i] = __builtin_fmaf(pv, v, st.o[mm][i]);
-            }
-        }
-    }
+    for (int mm = 0; mm < 8; mm++)
+        st.o[mm] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(vp[0][mm], vp[1][mm], vp[2][mm], vp[3][mm]), pb, st.o[mm],
+                                                          0, 0, 0);
 }
 
 // Up to 16 Q rows of a kv head, Q columns of 16 a wave, tokens dealt to the waves.
@@ -832,28 +895,40 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_few(TreeArgs A) {
     __shared__ __align__(16) float s_buf[kWaves * 16 * Q * kMRow];
     __shared__ uint32_t s_vis[N][kVisWords];
     __shared__ int s_up[N];
+    __shared__ int s_odd;                      // a draft's V has infinities or NaN
     __shared__ float s_m[kWaves][32], s_l[kWaves][32];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     const Place P = place_of(A, 16 * Q);
-    if (P.sp == A.nsp - 1) tree_words(A.parents + P.b * A.nodes, A.nodes, s_vis, s_up, tid);
 
     const Share sh = share_of(A, P.sp);
     const int split = min(sh.end, A.np);       // prefix tiles, then rows: two loops, each with the registers it needs
-    // The records of the wave's next tile are in flight during the products of this one.  The
-    // reload is unconditional (past the share it reads the last tile again), so that it
-    // lands in place; nothing waits on it before the next decode.
+    // The records of the wave's next tile are in flight during the products of this one, and
+    // the bases of the tile after.  Reloads are unconditional (past the share they read the
+    // last tile again), so that they land in place and nothing waits on them before their use.
     const Lay lay = lay_of(false, lane);
     KFew kr;
     Raw vr;
-    auto fetch = [&](int tile) {
-        const int64_t t = (int64_t)min(tile, split - 1) * 32;
-        load_few(A.k, P.hd, t, A.t_prefix, lane, kr);
-        load_raw(A.v, P.hd, t, A.t_prefix, lay, lane >> 5, vr);
+    Meta mk, mv, nk, nv;
+    uint4 ek, ev;
+    auto at = [&](int tile) { return (int64_t)min(tile, split - 1) * 32; };
+    auto fetch = [&](int tile) {               // nk, nv have the tile's bases
+        ek = load_entry(A.k, nk, lane);
+        ev = load_entry(A.v, nv, lane);
+        mk = nk;
+        mv = nv;
+        load_few(A.k, P.hd, at(tile), A.t_prefix, lane, kr);
+        load_raw(A.v, P.hd, at(tile), A.t_prefix, lay, vr);
+        nk = load_meta(A.k, P.hd, at(tile + kWaves), A.t_prefix, lane);
+        nv = load_meta(A.v, P.hd, at(tile + kWaves), A.t_prefix, lane);
     };
     int tile = max(sh.first, P.first) + wave;
     const bool prefix = max(sh.first, P.first) < split;
-    if (prefix) fetch(tile);
+    if (prefix) {
+        nk = load_meta(A.k, P.hd, at(tile), A.t_prefix, lane);
+        nv = load_meta(A.v, P.hd, at(tile), A.t_prefix, lane);
+        fetch(tile);
+    }
     h8_t q[Q][4];
     int node[Q];
     FewState st[Q];
@@ -868,23 +943,35 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_few(TreeArgs A) {
 #pragma unroll
         for (int mm = 0; mm < 8; mm++) st[x].o[mm] = f4_t{0.f, 0.f, 0.f, 0.f};
     }
+    if (P.sp == A.nsp - 1) {
+        if (tid == 0) s_odd = 0;
+        tree_words(A.parents + P.b * A.nodes, A.nodes, s_vis, s_up, tid);
+    }
     for (; tile < split; tile += kWaves) {
         const Sub sb = sub_of<1>(A, tile, 0, P.len, P.start);
         f4_t s[Q][2];
         uint32_t vp[4][8];
 #pragma unroll
         for (int x = 0; x < Q; x++) s[x][0] = s[x][1] = f4_t{0.f, 0.f, 0.f, 0.f};
-        ExcFew ex;
-        exc_few(A.k, kr, lane, ex);
+        uint32_t e[4], before = 0u;
+        exc_pairs(ek, e);
 #pragma unroll
         for (int c = 0; c < 4; c++) {
+            const FewMask fm = few_mask(kr, c, lane);
+            const int bit = 16 * g + 8 * ((col >> 2) & 1) + 2 * (col & 3);
+            const uint32_t two = (uint32_t)(fm.m >> bit) & 3u;
+            uint32_t rank = 0u;
+            if (fm.any) {                      // wave-uniform
+                rank = before + __builtin_popcountll(fm.m & ((1ull << bit) - 1ull));
+                before += __builtin_popcountll(fm.m);
+            }
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 uint32_t p[4];
                 rec_pairs(y ? kr.a[c].y : kr.a[c].x, (kr.b[c] >> (8 * y)) & 0xffu, p);
 #pragma unroll
                 for (int i = 0; i < 4; i++) p[i] = unbias(p[i]);
-                exc_select((ex.any >> (2 * c + y)) & 1u, (ex.own >> (2 * c + y)) & 1u, ex.e[c][y], p);
+                if (fm.any) pull_entry(A.k, mk, e, (two >> y) & 1u, col >> 3, rank + (y ? two & 1u : 0u), p);
                 mul_pairs<4>(p, __builtin_amdgcn_perm(0u, kr.s, y ? 0x03020302u : 0x01000100u));
 #pragma unroll
                 for (int x = 0; x < Q; x++)
@@ -892,11 +979,13 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_few(TreeArgs A) {
             }
             __builtin_amdgcn_sched_barrier(0);   // one record group's operands live at a time
         }
-        decode_v(A.v, vr, sb.word, lane, vp);
-        __builtin_amdgcn_sched_barrier(0);       // every use of the records before their reload: it lands in place
+        decode_v(vr, vp);
+        pull_v(A.v, vr, lay, mv, ev, lane, vp);
+        scale_v(vr, sb.word, lane, vp);
+        __builtin_amdgcn_sched_barrier(0);       // every use of the records before their reload
         fetch(tile + kWaves);
 #pragma unroll
-        for (int x = 0; x < Q; x++) few_attend<false>(s[x], sb.word, sb.word == ~0u, false, vp, lane, st[x]);
+        for (int x = 0; x < Q; x++) few_attend(s[x], sb.word, sb.word == ~0u, vp, lane, st[x]);
     }
     if (!prefix) tile = max(sh.first, split) + wave;
     for (; tile < sh.end; tile += kWaves) {
@@ -904,28 +993,30 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_few(TreeArgs A) {
         if (!sb.word) continue;
         f4_t s[Q][2];
         uint32_t vp[4][8];
-        const Rows& R = sb.kind == 1 ? A.tk : A.dk;
-        const uint16_t* p = R.p + P.b * R.sb + P.kvh * R.sh;
+        const bool draft = sb.kind == 2;
+        const Rows &rk = draft ? A.dk : A.tk, &rv = draft ? A.dv : A.tv;
+        const uint16_t* p = rk.p + P.b * rk.sb + P.kvh * rk.sh;
+        uint4 w[2][4];
 #pragma unroll
-        for (int x = 0; x < Q; x++) s[x][0] = s[x][1] = f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int y = 0; y < 2; y++) {
-            const int tok = 8 * (col >> 2) + 2 * (col & 3) + y;
+        for (int y = 0; y < 2; y++)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if ((sb.word >> tok) & 1u) w = load_row8<BF16>(p + (sb.t + tok) * R.st + 32 * c + 8 * g);
-#pragma unroll
-                for (int x = 0; x < Q; x++)
-                    s[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, w), q[x][c], s[x][y], 0, 0, 0);
+                const int tok = min(8 * (col >> 2) + 2 * (col & 3) + y, sb.have - 1);
+                w[y][c] = *reinterpret_cast<const uint4*>(p + (sb.t + tok) * rk.st + 32 * c + 8 * g);
             }
-        }
-        const bool bad = rows_v<BF16>(sb.kind == 1 ? A.tv : A.dv, P.b, P.kvh, sb.t, sb.word, lane, vp);
-        const bool draft = sb.kind == 2;
+        rows_v<BF16>(rv.p + P.b * rv.sb + P.kvh * rv.sh, rv.st, sb.t, sb.have, sb.word, lane, vp);
+        if (draft && clear_odd(vp) && lane == 0) s_odd = 1;
 #pragma unroll
         for (int x = 0; x < Q; x++) {
-            const uint32_t w = draft ? sb.word & s_vis[node[x]][sb.t >> 5] : sb.word;
-            few_attend<true>(s[x], w, !draft && w == ~0u, draft && bad, vp, lane, st[x]);
+            s[x][0] = s[x][1] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int y = 0; y < 2; y++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    s[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        __builtin_bit_cast(h8_t, BF16 ? bf_to_h(w[y][c]) : w[y][c]), q[x][c], s[x][y], 0, 0, 0);
+            const uint32_t word = draft ? sb.word & s_vis[node[x]][sb.t >> 5] : sb.word;
+            few_attend(s[x], word, !draft && word == ~0u, vp, lane, st[x]);
         }
     }
 #pragma unroll
@@ -945,33 +1036,69 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_few(TreeArgs A) {
         }
     }
     __syncthreads();
-    join_teams<1, 16 * Q, BF16>(A, P.hd, P.sp, 0, s_buf, s_m, s_l, s_vis, tid);
+    join_teams<1, 16 * Q, BF16>(A, P, s_buf, s_m, s_l, s_vis, &s_odd, tid);
 }
 
-// one wave per row: the splits' records of it, in order
-__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs A, int64_t n, int bf16) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= n) return;
-    const int64_t hd = row / A.rows;
-    const int r = (int)(row % A.rows);
+// One workgroup per row: thread (sub, dq) sums dimensions 4 dq .. + 3 of the records sub,
+// sub + 8, .. (their loads go out together), then the eight sums are joined in order.
+__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs A, int bf16) {
+    constexpr int kUp = 8;                     // records in flight per thread
+    __shared__ __align__(16) f4_t s_o[8][32];
+    __shared__ float s_m[8], s_l[8];
+    const int dq = threadIdx.x & 31, sub = threadIdx.x >> 5;
+    const int64_t hd = blockIdx.x / (uint32_t)A.rows;
+    const int r = (int)(blockIdx.x % (uint32_t)A.rows);
     const float* rec = A.rec + (hd * A.nsp * A.rows + r) * kRecF;
     const int64_t step = (int64_t)A.rows * kRecF;
-    float M = -INFINITY;
-    for (int p = lane; p < A.nsp; p += 64) M = fmaxf(M, rec[p * step]);
+    const float tail_l = rec[(A.nsp - 1) * step + 1];
+    float m = -INFINITY, l = 0.f;
+    f4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (int p0 = sub; p0 < A.nsp; p0 += 8 * kUp) {
+        float2 ml[kUp];
+        f4_t v[kUp];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+        for (int k = 0; k < kUp; k++) {
+            const float* x = rec + min(p0 + 8 * k, A.nsp - 1) * step;
+            ml[k] = *reinterpret_cast<const float2*>(x);
+            v[k] = *reinterpret_cast<const f4_t*>(x + 4 + 4 * dq);
+        }
+        float M = m;
+#pragma unroll
+        for (int k = 0; k < kUp; k++) M = p0 + 8 * k < A.nsp ? fmaxf(M, ml[k].x) : M;
+        const float f0 = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - M);
+        o *= f0;
+        l *= f0;
+#pragma unroll
+        for (int k = 0; k < kUp; k++) {
+            if (p0 + 8 * k >= A.nsp) continue;
+            const float f = ml[k].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[k].x - M);
+            l = __builtin_fmaf(ml[k].y, f, l);
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(v[k][c], f, o[c]);
+        }
+        m = M;
+    }
+    s_o[sub][dq] = o;
+    if (dq == 0) {
+        s_m[sub] = m;
+        s_l[sub] = l;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    const int lane = threadIdx.x;
+    float M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 8; k++) M = fmaxf(M, s_m[k]);
     float L = 0.f, x = 0.f, y = 0.f;
-#pragma unroll 8
-    for (int p = 0; p < A.nsp; p++) {
-        const float2 ml = *reinterpret_cast<const float2*>(rec + p * step);
-        const float2 v = *reinterpret_cast<const float2*>(rec + p * step + 4 + 2 * lane);
-        const float f = ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
-        L = __builtin_fmaf(ml.y, f, L);
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const float f = s_m[k] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[k] - M);
+        const float2 v = reinterpret_cast<const float2*>(s_o[k])[lane];
+        L = __builtin_fmaf(s_l[k], f, L);
         x = __builtin_fmaf(v.x, f, x);
         y = __builtin_fmaf(v.y, f, y);
     }
-    const bool empty = rec[(A.nsp - 1) * step + 1] == kEmpty;
+    const bool empty = tail_l == kEmpty;
     const float inv = 1.f / L;
     out_pair(A, bf16 != 0, hd / A.heads, hd % A.heads, r, 2 * lane, empty ? 0.f : x * inv, empty ? 0.f : y * inv);
 }
@@ -979,13 +1106,13 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs A, int64_t n, int b
 // ------------------------------------------------------------------- plan --
 
 struct Plan {
-    int c, rb, np, nt, nd, nsp;
+    int c, rb, np, nt, nd, nsp, per;
 };
 
 // Waves of a team: as many 32-row columns as there are rows, four at most (their
-// O is 64 registers each).  Splits: of the counts that leave one, the one whose
-// longest CU has the fewest tiles; among those the fewest splits (records are
-// written and read once more).
+// O is 64 registers each).  A split's share is whole rounds of its teams' tiles; of the
+// shares, the one whose longest CU has the fewest rounds (a workgroup's prologue and
+// join count as two), among those the fewest splits (records are written and read again).
 bool plan(int64_t n_seq, int64_t heads, int64_t nodes, int64_t group, int64_t t_prefix, int64_t tail_cap, Plan* p) {
     if (n_seq < 1 || heads < 1 || nodes < 1 || nodes > kMaxNodes || group < 1 || group > 16 || t_prefix < 0 ||
         t_prefix % kRB || tail_cap < 0 || t_prefix > INT_MAX / 2 || tail_cap > INT_MAX / 4)
@@ -999,17 +1126,25 @@ bool plan(int64_t n_seq, int64_t heads, int64_t nodes, int64_t group, int64_t t_
     p->nd = (int)((nodes + tt - 1) / tt);
     const int64_t base = n_seq * heads * p->rb;
     if (base > INT_MAX / 256) return false;
-    const int64_t tiles = p->np + p->nt + p->nd;
+    const int64_t cache = p->np + p->nt;
     int64_t best = -1;
-    for (int64_t n = 1; n <= 256 && (n - 1) * teams < tiles; n++) {
-        const int64_t per = (tiles + n - 1) / n;
-        const int64_t cost = ((base * n + 255) / 256) * ((per + teams - 1) / teams + 2);
+    for (int64_t rounds = (cache + teams - 1) / teams; ; ) {
+        const int64_t per = (rounds > 0 ? rounds : 1) * teams, n = cache > 0 ? (cache + per - 1) / per : 1;
+        if (n > 256) break;
+        // the last split has the draft's tiles beside its share
+        const int64_t last = (cache - (n - 1) * per + p->nd + teams - 1) / teams;
+        const int64_t cost = ((base * n + 255) / 256) * (rounds + 2) + (last > rounds ? last - rounds : 0);
         if (best < 0 || cost < best) {
             best = cost;
             p->nsp = (int)n;
+            p->per = (int)per;
         }
+        if (rounds <= 1) break;
+        // the next smaller share that changes the number of splits
+        const int64_t next = (cache + (n + 1) * teams - 1) / ((n + 1) * teams);
+        rounds = next < rounds ? next : rounds - 1;
     }
-    return true;
+    return best >= 0;
 }
 
 bool tree_res_ok(const lq_resident* r) {
@@ -1059,7 +1194,13 @@ int lq_resident_tree_attention(const lq_resident *k, const lq_resident *v, int64
     Plan p;
     if (!plan(n_seq, heads, n_nodes, group, t_prefix, tail_cap, &p) || heads > INT_MAX) return LQ_ERR_ARG;
     TreeArgs A{};
-    if (t_prefix > 0) { A.k = *k; A.v = *v; }
+    if (t_prefix > 0) {
+        A.k = *k;
+        A.v = *v;
+        // an empty exception list is read at its first entry and the value not used
+        if (!A.k.exc || A.k.exc_cap == 0) A.k.exc = reinterpret_cast<int16_t*>(A.k.a);
+        if (!A.v.exc || A.v.exc_cap == 0) A.v.exc = reinterpret_cast<int16_t*>(A.v.a);
+    }
     A.t_prefix = t_prefix;
     A.q = rows_of(q);
     A.dk = rows_of(draft_k);
@@ -1081,14 +1222,14 @@ int lq_resident_tree_attention(const lq_resident *k, const lq_resident *v, int64
     A.nsp = p.nsp;
     A.np = p.np;
     A.nt = p.nt;
+    A.per = p.per;
     A.tiles = p.np + p.nt + p.nd;
     A.rec = static_cast<float*>(d_work);
     const int64_t grid = k->n_heads * p.nsp * p.rb;
     if (dtype == LQ_BF16) tree_launch<true>(A, p.c, grid, s);
     else tree_launch<false>(A, p.c, grid, s);
     if (p.nsp > 1) {
-        const int64_t n = k->n_heads * A.rows;
-        hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, s, A, n, dtype == LQ_BF16);
+        hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)(k->n_heads * A.rows)), dim3(256), 0, s, A, dtype == LQ_BF16);
     }
     return launch_status();
 }
