@@ -125,8 +125,6 @@ __device__ __forceinline__ uint4 bf_to_h(const uint4& w) {
     return make_uint4(y[0], y[1], y[2], y[3]);
 }
 
-__device__ __forceinline__ float bf2h2f(uint16_t u) { return h2f(f2h(bf2f(u))); }   // a bf16 value as the products take it
-
 template <bool BF16>
 __device__ __forceinline__ uint4 load_row8(const uint16_t* p) {
     const uint4 w = *reinterpret_cast<const uint4*>(p);
@@ -566,11 +564,11 @@ __device__ __forceinline__ void sub_attend(const char* lds, const h8_t q[8], uin
 // ------------------------------------------------------------------ kernel --
 
 // vis[i]: node i and its ancestors, or nothing where its chain of parents does not end
-// in a root (-1).  Pointer doubling: after round k the words hold 2^k generations.
-__device__ void tree_words(const int32_t* __restrict__ parents, int n, uint32_t (*vis)[kVisWords], int* up, int tid) {
+// in a root (-1).  p: node tid's parent.  Pointer doubling: after round k the words hold
+// 2^k generations.
+__device__ void tree_words(int p, int n, uint32_t (*vis)[kVisWords], int* up, int tid) {
     const bool mine = tid < n;
     if (mine) {
-        const int p = parents[tid];
         up[tid] = p == -1 ? -1 : p >= 0 && p < tid ? p : -2;
 #pragma unroll
         for (int w = 0; w < kVisWords; w++) vis[tid][w] = w == tid >> 5 ? 1u << (tid & 31) : 0u;
@@ -610,6 +608,22 @@ __device__ __forceinline__ void out_pair(const TreeArgs& A, bool bf16, int64_t b
                                            : (uint32_t)f2h(x) | ((uint32_t)f2h(y) << 16);
 }
 
+// eight values of a row from dimension d on; none of a row that sees nothing
+__device__ __forceinline__ void out8(const TreeArgs& A, bool bf16, int64_t b, int64_t kvh, int r, int d, const f4_t& x,
+                                     const f4_t& y, bool empty) {
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    if (!empty) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float u = i < 2 ? x[2 * i] : y[2 * i - 4], v = i < 2 ? x[2 * i + 1] : y[2 * i - 3];
+            w[i] = bf16 ? (uint32_t)f2bf(u) | ((uint32_t)f2bf(v) << 16) : pair_h(u, v);
+        }
+    }
+    const int node = r / A.group, g = r % A.group;
+    *reinterpret_cast<uint4*>(A.out + b * A.ob + (kvh * A.group + g) * A.oh + (int64_t)node * A.ot + d) =
+        make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Split sp's share of the tiles: `per` of the cache's, the draft's besides to the last.
 struct Share {
     int first, end;
@@ -646,42 +660,51 @@ __device__ __forceinline__ void join_teams(const TreeArgs& A, const Place& P, co
                                            const uint32_t (*vis)[kVisWords], const int* odd, int tid) {
     constexpr int T = kWaves / C;
     const bool last = P.sp == A.nsp - 1;
-    for (int idx = tid; idx < COLS * C * (kHd / 2); idx += kWaves * 64) {
-        const int lr = idx / (kHd / 2), d = 2 * (idx % (kHd / 2));
+    const int d = 8 * (tid & 15);              // 16 lanes a row, eight dimensions a lane
+    for (int lr = tid >> 4; lr < COLS * C; lr += kWaves * 4) {
         const int rr = P.row0 + lr;
-        if (rr >= A.rows) break;               // idx grows with the row
+        if (rr >= A.rows) break;
         const int w0 = lr / COLS, c = lr % COLS;
-        float M = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < T; t++) M = fmaxf(M, s_m[t * C + w0][c]);
-        float L = 0.f, x = 0.f, y = 0.f;
+        float m[T], M = -INFINITY, L = 0.f;
 #pragma unroll
         for (int t = 0; t < T; t++) {
-            const int w = t * C + w0;
-            const float f = s_m[w][c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[w][c] - M);
-            const float2 o = *reinterpret_cast<const float2*>(buf + (w * COLS + c) * kMRow + d);
-            L += s_l[w][c] * f;
-            x += o.x * f;
-            y += o.y * f;
+            m[t] = s_m[t * C + w0][c];
+            M = fmaxf(M, m[t]);
         }
-        const int nd = rr / A.group;
-        const bool empty = last && !((vis[nd][nd >> 5] >> (nd & 31)) & 1u);
-        if (last && *odd) {
-            const uint16_t* p = A.dv.p + P.b * A.dv.sb + P.kvh * A.dv.sh + d;
-            for (int t = 0; t <= nd; t++) {
-                if (!((vis[nd][t >> 5] >> (t & 31)) & 1u)) continue;
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(p + t * A.dv.st);
-                const float u = BF16 ? bf2h2f((uint16_t)w) : h2f((uint16_t)w), v = BF16 ? bf2h2f((uint16_t)(w >> 16)) : h2f((uint16_t)(w >> 16));
-                if (!(fabsf(u) < INFINITY)) x += u;
-                if (!(fabsf(v) < INFINITY)) y += v;
+        f4_t x = {0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            const float f = m[t] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] - M);
+            const float* o = buf + ((t * C + w0) * COLS + c) * kMRow + d;
+            L += s_l[t * C + w0][c] * f;
+            x += *reinterpret_cast<const f4_t*>(o) * f;
+            y += *reinterpret_cast<const f4_t*>(o + 4) * f;
+        }
+        bool empty = false;
+        if (last) {
+            const int nd = rr / A.group;
+            empty = !((vis[nd][nd >> 5] >> (nd & 31)) & 1u);
+            if (*odd) {
+                const uint16_t* p = A.dv.p + P.b * A.dv.sb + P.kvh * A.dv.sh + d;
+                for (int t = 0; t <= nd; t++) {
+                    if (!((vis[nd][t >> 5] >> (t & 31)) & 1u)) continue;
+                    const uint4 w = load_row8<BF16>(p + t * A.dv.st);
+                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float v = h2f((uint16_t)(u[i >> 1] >> (16 * (i & 1))));
+                        if (!(fabsf(v) < INFINITY)) (i < 4 ? x : y)[i & 3] += v;
+                    }
+                }
             }
         }
         if (A.nsp == 1) {
             const float inv = 1.f / L;
-            out_pair(A, BF16, P.b, P.kvh, rr, d, empty ? 0.f : x * inv, empty ? 0.f : y * inv);
+            out8(A, BF16, P.b, P.kvh, rr, d, x * inv, y * inv, empty);
         } else {
             float* rec = A.rec + ((P.hd * A.nsp + P.sp) * A.rows + rr) * kRecF;
-            *reinterpret_cast<float2*>(rec + 4 + d) = make_float2(x, y);
+            *reinterpret_cast<f4_t*>(rec + 4 + d) = x;
+            *reinterpret_cast<f4_t*>(rec + 8 + d) = y;
             if (d == 0) *reinterpret_cast<float2*>(rec) = make_float2(M, empty ? kEmpty : L);
         }
     }
@@ -738,18 +761,15 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_many(TreeArgs A) {
     };
     if (prefix) {
         ahead = load_meta(res, P.hd, at(h0 + team), A.t_prefix, lane);
-        fetch(h0 + team);
+        load_raw(res, P.hd, at(h0 + team), A.t_prefix, lay, raw);
     }
+    const int parent = P.sp == A.nsp - 1 && tid < A.nodes ? A.parents[P.b * A.nodes + tid] : -2;
     // the wave's rows: column lane % 32
     const int r = P.row0 + 32 * ct + (lane & 31);
     const int node = r < A.rows ? r / A.group : 0;
     h8_t q[8];
 #pragma unroll
     for (int c = 0; c < 8; c++) q[c] = load_q<BF16>(A, P, r, node, 16 * c + 8 * (lane >> 5));
-    if (P.sp == A.nsp - 1) {
-        if (tid == 0) s_odd = 0;
-        tree_words(A.parents + P.b * A.nodes, A.nodes, s_vis, reinterpret_cast<int*>(s_buf), tid);
-    }
     RowState st;
     st.m = -INFINITY;
     st.l = 0.f;
@@ -771,17 +791,27 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_many(TreeArgs A) {
         patch_lds(isk, res, d, lay, m, e, word, lane, s_place[wave], lds);
     };
     if (prefix) {
+        ent = load_entry(res, ahead, lane);
+        meta = ahead;
+        ahead = load_meta(res, P.hd, at(h0 + team + T), A.t_prefix, lane);
         put(raw, meta, ent, ~0u, buf + mine * kSub);
         __builtin_amdgcn_sched_barrier(0);     // every use of the records before their reload
         fetch(h0 + team + T);
         __syncthreads();
-        for (int t = h0, half = 0; t < h1; t += T, half ^= 1) {
+        int t = h0, half = 0;
+        for (; t + T < h1; t += T, half ^= 1) {
             put(raw, meta, ent, ~0u, buf + ((half ^ 1) * S + mine) * kSub);
             __builtin_amdgcn_sched_barrier(0);
             fetch(t + team + 2 * T);
-            if (t + team < h1 && rows_here) sub_attend<S, false>(buf + half * S * kSub, q, 0u, lane, st);
+            if (rows_here) sub_attend<S, false>(buf + half * S * kSub, q, 0u, lane, st);
             __syncthreads();
         }
+        if (t + team < h1 && rows_here) sub_attend<S, false>(buf + half * S * kSub, q, 0u, lane, st);
+        __syncthreads();
+    }
+    if (P.sp == A.nsp - 1) {
+        if (tid == 0) s_odd = 0;
+        tree_words(parent, A.nodes, s_vis, reinterpret_cast<int*>(s_buf), tid);
     }
     const int before = prefix ? h0 - seen : 0, after = prefix ? h1 : seen, edge = before + max(0, sh.end - after);
 #pragma unroll 1
@@ -925,10 +955,14 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_few(TreeArgs A) {
     int tile = max(sh.first, P.first) + wave;
     const bool prefix = max(sh.first, P.first) < split;
     if (prefix) {
-        nk = load_meta(A.k, P.hd, at(tile), A.t_prefix, lane);
-        nv = load_meta(A.v, P.hd, at(tile), A.t_prefix, lane);
-        fetch(tile);
+        mk = load_meta(A.k, P.hd, at(tile), A.t_prefix, lane);
+        mv = load_meta(A.v, P.hd, at(tile), A.t_prefix, lane);
+        load_few(A.k, P.hd, at(tile), A.t_prefix, lane, kr);
+        load_raw(A.v, P.hd, at(tile), A.t_prefix, lay, vr);
+        nk = load_meta(A.k, P.hd, at(tile + kWaves), A.t_prefix, lane);
+        nv = load_meta(A.v, P.hd, at(tile + kWaves), A.t_prefix, lane);
     }
+    const int parent = P.sp == A.nsp - 1 && tid < A.nodes ? A.parents[P.b * A.nodes + tid] : -2;
     h8_t q[Q][4];
     int node[Q];
     FewState st[Q];
@@ -943,9 +977,13 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_few(TreeArgs A) {
 #pragma unroll
         for (int mm = 0; mm < 8; mm++) st[x].o[mm] = f4_t{0.f, 0.f, 0.f, 0.f};
     }
+    if (prefix) {
+        ek = load_entry(A.k, mk, lane);
+        ev = load_entry(A.v, mv, lane);
+    }
     if (P.sp == A.nsp - 1) {
         if (tid == 0) s_odd = 0;
-        tree_words(A.parents + P.b * A.nodes, A.nodes, s_vis, s_up, tid);
+        tree_words(parent, A.nodes, s_vis, s_up, tid);
     }
     for (; tile < split; tile += kWaves) {
         const Sub sb = sub_of<1>(A, tile, 0, P.len, P.start);
@@ -1111,8 +1149,9 @@ struct Plan {
 
 // Waves of a team: as many 32-row columns as there are rows, four at most (their
 // O is 64 registers each).  A split's share is whole rounds of its teams' tiles; of the
-// shares, the one whose longest CU has the fewest rounds (a workgroup's prologue and
-// join count as two), among those the fewest splits (records are written and read again).
+// shares, the one whose longest CU takes the least: a round counts 2, a workgroup's
+// prologue and join 3, a further round of the draft's tiles 1; of equals the fewest splits
+// (records are written and read again).
 bool plan(int64_t n_seq, int64_t heads, int64_t nodes, int64_t group, int64_t t_prefix, int64_t tail_cap, Plan* p) {
     if (n_seq < 1 || heads < 1 || nodes < 1 || nodes > kMaxNodes || group < 1 || group > 16 || t_prefix < 0 ||
         t_prefix % kRB || tail_cap < 0 || t_prefix > INT_MAX / 2 || tail_cap > INT_MAX / 4)
@@ -1133,7 +1172,7 @@ bool plan(int64_t n_seq, int64_t heads, int64_t nodes, int64_t group, int64_t t_
         if (n > 256) break;
         // the last split has the draft's tiles beside its share
         const int64_t last = (cache - (n - 1) * per + p->nd + teams - 1) / teams;
-        const int64_t cost = ((base * n + 255) / 256) * (rounds + 2) + (last > rounds ? last - rounds : 0);
+        const int64_t cost = ((base * n + 255) / 256) * (2 * rounds + 3) + (last > rounds ? last - rounds : 0);
         if (best < 0 || cost < best) {
             best = cost;
             p->nsp = (int)n;
