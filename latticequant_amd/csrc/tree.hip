@@ -498,6 +498,13 @@ __device__ __forceinline__ float quarters_max(float v) {
 // passing the old one by 2^5 is rare after the first.
 constexpr float kLazy = 5.0f;
 
+// The weights of two scores as fp16, added to the sum as they are rounded (fp32).
+__device__ __forceinline__ uint32_t weights(float s0, float s1, float c0, float off, float& l) {
+    const uint32_t p = pair_h(__builtin_amdgcn_exp2f(__builtin_fmaf(s0, c0, off)), __builtin_amdgcn_exp2f(__builtin_fmaf(s1, c0, off)));
+    l = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, p), h2_t{(_Float16)1.f, (_Float16)1.f}, l, false);
+    return p;
+}
+
 // U subtiles for the wave's 32 rows, of which the lane's row sees the tokens of word (with
 // MASK, one subtile) or all.  The subtiles' products are independent, so one's softmax
 // runs beside the other's MFMA.
@@ -516,6 +523,7 @@ __device__ __forceinline__ void sub_attend(const char* lds, const h8_t q[8], uin
             s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, q[c], s[u], 0, 0, 0);
         }
     }
+    __builtin_amdgcn_sched_barrier(0);   // V is read once the scores stand: both at a time take more registers than there are
     float mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -545,13 +553,12 @@ __device__ __forceinline__ void sub_attend(const char* lds, const h8_t q[8], uin
         const char* vl = lds + u * kSub + 32 * kKRow;
 #pragma unroll
         for (int sx = 0; sx < 2; sx++) {
-            float p[8];
+            uint32_t p[4];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * sx + i], c0, off));
-                st.l += p[i];
+            for (int i = 0; i < 4; i++) {
+                p[i] = weights(s[u][8 * sx + 2 * i], s[u][8 * sx + 2 * i + 1], c0, off, st.l);
             }
-            const h8_t pb = as_h8(pair_h(p[0], p[1]), pair_h(p[2], p[3]), pair_h(p[4], p[5]), pair_h(p[6], p[7]));
+            const h8_t pb = as_h8(p[0], p[1], p[2], p[3]);
 #pragma unroll
             for (int d = 0; d < 4; d++) {
                 const h8_t va = *reinterpret_cast<const h8_t*>(vl + (32 * d + n) * kVRow + 16 * (2 * sx + g));
@@ -722,6 +729,7 @@ __device__ __forceinline__ h8_t load_q(const TreeArgs& A, const Place& P, int r,
 template <int C, bool BF16>
 __global__ __launch_bounds__(kWaves * 64) void k_tree_many(TreeArgs A) {
     constexpr int S = C / 2;                   // subtiles of a tile: waves 0 .. S - 1 of a team decode their K, the others V
+    constexpr int U = S < 2 ? S : 2;           // subtiles taken together
     constexpr int T = kWaves / C;              // teams
     constexpr int kStage = 2 * T * S * kSub;   // two tiles a team: one is read while the next is decoded
     static_assert(kStage >= kWaves * 32 * (kMRow + 2) * 4 && kStage >= kMaxNodes * 4, "the join and the tree fit the stage");
@@ -803,10 +811,16 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_many(TreeArgs A) {
             put(raw, meta, ent, ~0u, buf + ((half ^ 1) * S + mine) * kSub);
             __builtin_amdgcn_sched_barrier(0);
             fetch(t + team + 2 * T);
-            if (rows_here) sub_attend<S, false>(buf + half * S * kSub, q, 0u, lane, st);
+            if (rows_here) {
+#pragma unroll 1
+                for (int u = 0; u < S; u += U) sub_attend<U, false>(buf + (half * S + u) * kSub, q, 0u, lane, st);
+            }
             __syncthreads();
         }
-        if (t + team < h1 && rows_here) sub_attend<S, false>(buf + half * S * kSub, q, 0u, lane, st);
+        if (t + team < h1 && rows_here) {
+#pragma unroll 1
+            for (int u = 0; u < S; u += U) sub_attend<U, false>(buf + (half * S + u) * kSub, q, 0u, lane, st);
+        }
         __syncthreads();
     }
     if (P.sp == A.nsp - 1) {
@@ -905,13 +919,10 @@ __device__ __forceinline__ void few_attend(f4_t s[2], uint32_t word, bool every,
         st.m = up;
     }
     const float off = (st.m == -INFINITY ? 0.f : -st.m) + kPShift;
-    float p[8];
+    uint32_t p[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {              // in the order of the tokens
-        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i & 1][i >> 1], c0, off));
-        st.l += p[i];
-    }
-    const h8_t pb = as_h8(pair_h(p[0], p[1]), pair_h(p[2], p[3]), pair_h(p[4], p[5]), pair_h(p[6], p[7]));
+    for (int i = 0; i < 4; i++) p[i] = weights(s[0][i], s[1][i], c0, off, st.l);   // in the order of the tokens
+    const h8_t pb = as_h8(p[0], p[1], p[2], p[3]);
 #pragma unroll
     for (int mm = 0; mm < 8; mm++)
         st.o[mm] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(vp[0][mm], vp[1][mm], vp[2][mm], vp[3][mm]), pb, st.o[mm],
@@ -1157,7 +1168,7 @@ bool plan(int64_t n_seq, int64_t heads, int64_t nodes, int64_t group, int64_t t_
         t_prefix % kRB || tail_cap < 0 || t_prefix > INT_MAX / 2 || tail_cap > INT_MAX / 4)
         return false;
     const int64_t rows = nodes * group;
-    p->c = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;   // 1: k_tree_few
+    p->c = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;   // 1: k_tree_few
     const int64_t s = p->c > 1 ? p->c / 2 : 1, teams = kWaves / p->c, tt = 32 * s;
     p->rb = (int)((rows + 32 * p->c - 1) / (32 * p->c));
     p->np = (int)((t_prefix + tt - 1) / tt);
@@ -1199,7 +1210,8 @@ Rows rows_of(const lq_rows* r) { return {static_cast<const uint16_t*>(r->p), r->
 template <bool BF16>
 void tree_launch(const TreeArgs& A, int c, int64_t grid, hipStream_t s) {
     const dim3 g((unsigned)grid), wg(kWaves * 64);
-    if (c == 4) hipLaunchKernelGGL((k_tree_many<4, BF16>), g, wg, 0, s, A);
+    if (c == 8) hipLaunchKernelGGL((k_tree_many<8, BF16>), g, wg, 0, s, A);
+    else if (c == 4) hipLaunchKernelGGL((k_tree_many<4, BF16>), g, wg, 0, s, A);
     else if (c == 2) hipLaunchKernelGGL((k_tree_many<2, BF16>), g, wg, 0, s, A);
     else if (A.rows > 16) hipLaunchKernelGGL((k_tree_few<2, BF16>), g, wg, 0, s, A);
     else hipLaunchKernelGGL((k_tree_few<1, BF16>), g, wg, 0, s, A);
