@@ -606,8 +606,9 @@ typedef struct {
 
 #define LQ_TREE_MAX_NODES 256   /* drafted nodes per sequence */
 
-/* Workspace (bytes) of lq_resident_tree_attention.  Needs no initialisation; the
- * bytes are in use until the call's work on the stream is done. */
+/* Workspace (bytes) of lq_resident_tree_attention, 16-byte aligned.  Needs no
+ * initialisation; the bytes are in use until the call's work on the stream is done.  The
+ * call refuses a workspace of fewer bytes (work_bytes); likewise those below. */
 int64_t lq_tree_attn_workspace(int64_t n_seq, int64_t heads, int64_t n_nodes, int group, int64_t t_prefix,
                                int64_t tail_cap);
 
@@ -629,7 +630,7 @@ int lq_resident_tree_attention(const lq_resident *k, const lq_resident *v, int64
                                const lq_rows *draft_k, const lq_rows *draft_v, const int32_t *d_parents,
                                int64_t n_seq, int64_t n_nodes, int group, const lq_rows *tail_k, const lq_rows *tail_v,
                                int64_t tail_cap, const int32_t *d_tail_len, const int32_t *d_start, int dtype,
-                               void *d_work, const lq_rows *out, hipStream_t s);
+                               void *d_work, int64_t work_bytes, const lq_rows *out, hipStream_t s);
 
 /* Workspace (bytes) of lq_accept_drafts with logits; uninitialised. */
 int64_t lq_accept_workspace(int64_t n_seq, int64_t n_nodes, int64_t vocab);
@@ -645,7 +646,7 @@ int64_t lq_accept_workspace(int64_t n_seq, int64_t n_nodes, int64_t vocab);
  * alignment of the rows); vocab < 2^31, n_seq * n_nodes <= 65535 with logits. */
 int lq_accept_drafts(const void *d_logits, int dtype, int64_t stride_b, int64_t stride_n, int64_t vocab,
                      const int64_t *d_choice, const int64_t *d_tokens, const int32_t *d_parents, int64_t n_seq,
-                     int64_t n_nodes, void *d_work, int32_t *d_path, int32_t *d_count, int64_t *d_next, hipStream_t s);
+                     int64_t n_nodes, void *d_work, int64_t work_bytes, int32_t *d_path, int32_t *d_count, int64_t *d_next, hipStream_t s);
 
 /* Accepted rows behind the tails, n (tail, draft) pairs in one launch per 128:
  * dst[b, h, d_len[b] + j] = src[b, h, d_path[b][j]] for j < d_count[b];
@@ -679,11 +680,13 @@ int64_t lq_select_workspace(int64_t heads_out, int64_t n_blocks);
  * d_blocks[r][j] (null: j) of sequence d_index[r] of src, which has src_blocks blocks in
  * use per head; dst holds n_out * (src heads per sequence) heads.  Writes dst's
  * planes with the exception offsets of a list that has the chosen blocks' entries
- * in block order, and their number to *dst->n_exc; dst->exc is then sized by the
- * caller and filled by lq_resident_select_exceptions (same arguments).  Indices are
- * clamped to their ranges. */
+ * in block order, and their number to *dst->n_exc, clears *dst->status; dst->exc is then
+ * sized by the caller and filled by lq_resident_select_exceptions (same arguments).
+ * With h_total (host, nullable) the call waits for that number, not for the planes, and
+ * is not for a stream that is being captured.  Indices are clamped to their ranges. */
 int lq_resident_select(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index, int64_t n_out,
-                       const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst, void *d_work, hipStream_t s);
+                       const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst, void *d_work,
+                       int64_t work_bytes, int64_t *h_total, hipStream_t s);
 int lq_resident_select_exceptions(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index,
                                   int64_t n_out, const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst,
                                   hipStream_t s);

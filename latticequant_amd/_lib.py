@@ -7,6 +7,7 @@ pointers).  The library is required: there is no CPU fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -22,6 +23,7 @@ LQ_SYM_STRIDE = 4352
 LQ_MAXSYM = 1028
 LQ_STREAMS = 16
 LQ_F16, LQ_BF16, LQ_F32 = 0, 1, 2
+LQ_ERR_ARG = -1
 LQ_ST_SYM_OVERFLOW, LQ_ST_ALPHABET, LQ_ST_TIE_UNPINNED = 1, 2, 4
 LQ_V_VALID, LQ_V_HALF, LQ_V_INRANGE = 1, 2, 4
 TABLE_BYTES = 16 + 4 * LQ_MAXSYM   # sizeof(lq_table)
@@ -95,16 +97,16 @@ _SIGS = {
     "lq_resident_attention": ([_P, _P, _I64, _P, _INT, _P, _P, _I64, _P, _P, _P], _INT),
     "lq_resident_attention_noalloc": ([_P, _P, _I64, _P, _INT, _P, _P, _I64, _P, _P], _INT),
     "lq_accept_workspace": ([_I64, _I64, _I64], _I64),
-    "lq_accept_drafts": ([_P, _INT, _I64, _I64, _I64, _P, _P, _P, _I64, _I64] + [_P] * 5, _INT),
+    "lq_accept_drafts": ([_P, _INT, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I64] + [_P] * 4, _INT),
     "lq_append_rows": ([_P, _P, _I64, _P, _P] + [_I64] * 5 + [_P] * 5, _INT),
     "lq_gather_rows": ([_P, _P, _I64, _P, _P] + [_I64] * 5 + [_P] * 2, _INT),
     "lq_resident_reorder": ([_P, _I64, _I64, _P, _I64, _I64, _P], _INT),
     "lq_select_workspace": ([_I64, _I64], _I64),
-    "lq_resident_select": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P], _INT),
+    "lq_resident_select": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _P, _P], _INT),
     "lq_resident_select_exceptions": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P], _INT),
     "lq_tree_attn_workspace": ([_I64, _I64, _I64, _INT, _I64, _I64], _I64),
-    "lq_resident_tree_attention": ([_P, _P, _I64] + [_P] * 4 + [_I64, _I64, _INT, _P, _P, _I64, _P, _P, _INT] + [_P] * 3,
-                                   _INT),
+    "lq_resident_tree_attention": ([_P, _P, _I64] + [_P] * 4 + [_I64, _I64, _INT, _P, _P, _I64, _P, _P, _INT, _P, _I64] +
+                                   [_P] * 2, _INT),
 }
 
 
@@ -188,6 +190,19 @@ def lib():
 
 def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def raw_stream(device) -> int:
+    """stream_ptr of a device with an index, without a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def on_device(device):
+    """Context in which `device` (with an index) is current."""
+    return _HERE_ALREADY if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
 
 
 def ptr(t) -> int | None:

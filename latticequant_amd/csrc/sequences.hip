@@ -4,6 +4,7 @@
 #include <climits>
 
 #include "lq_device.h"
+#include "lq_readpool.h"
 
 using namespace lq;
 
@@ -246,11 +247,10 @@ __device__ __forceinline__ Unit unit_of(const Planes& p, int64_t w, int64_t nb) 
 template <int R>
 __global__ __launch_bounds__(256) void k_reorder(PlaneTable P, int64_t heads, int n_seq,
                                                  const int32_t* __restrict__ index, int64_t blk0, int64_t nb) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t h = i / (nb * kUnits);
-    if (h >= heads) return;
-    const Planes& p = P.r[blockIdx.y];
-    const Unit u = unit_of(p, i % (nb * kUnits), nb);
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+    if (i >= nb * kUnits) return;
+    const Planes& p = P.r[blockIdx.z];
+    const Unit u = unit_of(p, i, nb);
     const int64_t row = heads * p.cap * u.per * 16;
     char* at = u.plane + ((h * p.cap + blk0) * u.per + u.at) * 16;
     uint4 v[R];
@@ -271,11 +271,10 @@ constexpr int kMaxReorder = 128;
 __global__ __launch_bounds__(64) void k_reorder_lds(PlaneTable P, int64_t heads, int n_seq,
                                                     const int32_t* __restrict__ index, int64_t blk0, int64_t nb) {
     __shared__ uint4 s_v[kMaxReorder][64];
-    const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    const int64_t h = i / (nb * kUnits);
-    if (h >= heads) return;
-    const Planes& p = P.r[blockIdx.y];
-    const Unit u = unit_of(p, i % (nb * kUnits), nb);
+    const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x, h = blockIdx.y;
+    if (i >= nb * kUnits) return;
+    const Planes& p = P.r[blockIdx.z];
+    const Unit u = unit_of(p, i, nb);
     const int64_t row = heads * p.cap * u.per * 16;
     char* at = u.plane + ((h * p.cap + blk0) * u.per + u.at) * 16;
     for (int s = 0; s < n_seq; s++) {
@@ -293,29 +292,31 @@ struct Choice {
     const int32_t* blocks;   // [n_out][nb] blocks, or null: the first nb
     int64_t n_seq, heads, n_out, nb, src_blocks;
 };
-// source block (resident head, block) of output block k = (r * heads + h) * nb + j
-__device__ __forceinline__ int64_t source_of(const Choice& C, int64_t k, int64_t cap) {
-    const int64_t j = k % C.nb, rh = k / C.nb, r = rh / C.heads, h = rh % C.heads;
+// source block (resident head, block) of block j of output head rh = r * heads + h
+__device__ __forceinline__ int64_t source_of(const Choice& C, uint32_t rh, uint32_t j, int64_t cap) {
+    const uint32_t r = rh / (uint32_t)C.heads, h = rh % (uint32_t)C.heads;
     const int64_t s = min((int64_t)max(C.index[r], 0), C.n_seq - 1);
-    const int64_t blk = C.blocks ? min((int64_t)max(C.blocks[r * C.nb + j], 0), C.src_blocks - 1) : j;
+    const int64_t blk = C.blocks ? min((int64_t)max(C.blocks[r * C.nb + j], 0), C.src_blocks - 1) : (int64_t)j;
     return (s * C.heads + h) * cap + blk;
 }
 
-constexpr int kScan = 2048;   // blocks of a scan tile
+constexpr int kScan = 1024;   // blocks of a scan tile
 
 // exception counts of kScan output blocks: each one's sum of those before it in the
 // tile (off), and the tile's sum
-__global__ __launch_bounds__(256) void k_select_count(const uint32_t* __restrict__ meta, int64_t cap, Choice C,
+__global__ __launch_bounds__(256) void k_select_count(const uint32_t* __restrict__ meta, int64_t cap, Choice C, uint32_t n,
                                                       uint32_t* __restrict__ off, uint32_t* __restrict__ sums) {
-    __shared__ uint32_t s_w[4];
+    __shared__ uint32_t s_c[kScan], s_w[4];
     const int tid = threadIdx.x, lane = tid & 63;
-    const int64_t n = C.n_out * C.heads * C.nb, k0 = (int64_t)blockIdx.x * kScan + tid * 8;
-    uint32_t c[8], mine = 0;
+    const uint32_t k0 = blockIdx.x * kScan;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        c[i] = k0 + i < n ? meta[source_of(C, k0 + i, cap) * 4 + 3] : 0u;
-        mine += c[i];
+    for (int i = 0; i < kScan / 256; i++) {
+        const uint32_t k = k0 + i * 256 + tid;
+        s_c[i * 256 + tid] = k < n ? meta[source_of(C, k / (uint32_t)C.nb, k % (uint32_t)C.nb, cap) * 4 + 3] : 0u;
     }
+    __syncthreads();
+    const uint4 c = reinterpret_cast<const uint4*>(s_c)[tid];
+    const uint32_t mine = c.x + c.y + c.z + c.w;
     uint32_t run = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -330,16 +331,17 @@ __global__ __launch_bounds__(256) void k_select_count(const uint32_t* __restrict
         if (w < (tid >> 6)) before += s_w[w];
         total += s_w[w];
     }
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        if (k0 + i < n) off[k0 + i] = before;
-        before += c[i];
-    }
+    const uint32_t k = k0 + 4 * tid;
+    if (k < n) off[k] = before;
+    if (k + 1 < n) off[k + 1] = before + c.x;
+    if (k + 2 < n) off[k + 2] = before + c.x + c.y;
+    if (k + 3 < n) off[k + 3] = before + c.x + c.y + c.z;
     if (tid == 0) sums[blockIdx.x] = total;
 }
 
-// sums[i]: the sum of those before it; the total to n_exc.  One wave.
-__global__ __launch_bounds__(64) void k_select_bases(uint32_t* sums, int64_t tiles, int32_t* n_exc) {
+// sums[i]: the sum of those before it; the total to n_exc (and to the host).  One wave.
+__global__ __launch_bounds__(64) void k_select_bases(uint32_t* sums, int64_t tiles, int32_t* n_exc, int32_t* status,
+                                                     int64_t* h_total) {
     const int lane = threadIdx.x;
     uint32_t carry = 0;
     for (int64_t t0 = 0; t0 < tiles; t0 += 64) {
@@ -353,17 +355,21 @@ __global__ __launch_bounds__(64) void k_select_bases(uint32_t* sums, int64_t til
         if (t0 + lane < tiles) sums[t0 + lane] = carry + run - v;
         carry += (uint32_t)__shfl((int)run, 63, 64);
     }
-    if (lane == 0) *n_exc = (int32_t)carry;
+    if (lane == 0) {
+        *n_exc = (int32_t)carry;
+        *status = 0;
+        if (h_total) *h_total = carry;
+    }
 }
 
+// grid (units of a head, output heads)
 __global__ __launch_bounds__(256) void k_select_planes(Planes S, Planes D, Choice C, const uint32_t* __restrict__ off,
                                                        const uint32_t* __restrict__ sums) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t rh = i / (C.nb * kUnits);
-    if (rh >= C.n_out * C.heads) return;
-    const Unit u = unit_of(D, i % (C.nb * kUnits), C.nb);
-    const int64_t j = u.at / u.per, e = u.at % u.per, k = rh * C.nb + j;
-    const int64_t from = source_of(C, k, S.cap);
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x, rh = blockIdx.y;
+    if (i >= (uint32_t)C.nb * kUnits) return;
+    const Unit u = unit_of(D, i, C.nb);
+    const uint32_t j = (uint32_t)u.at / (uint32_t)u.per, e = (uint32_t)u.at % (uint32_t)u.per, k = rh * (uint32_t)C.nb + j;
+    const int64_t from = source_of(C, rh, j, S.cap);
     const char* src = u.plane == D.a ? S.a : u.plane == D.b ? S.b : u.plane == D.mask ? S.mask
                       : u.plane == D.scale ? S.scale : S.meta;
     uint4 w = *reinterpret_cast<const uint4*>(src + (from * u.per + e) * 16);
@@ -376,11 +382,11 @@ __global__ __launch_bounds__(256) void k_select_exc(const uint4* __restrict__ sr
                                                     int64_t src_cap, int64_t src_exc, const uint4* __restrict__ dst_meta,
                                                     int16_t* __restrict__ dst, int64_t dst_cap, int64_t dst_exc,
                                                     Choice C, int32_t* status) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, k = i >> 3;
-    if (k >= C.n_out * C.heads * C.nb) return;
-    const uint4 d = dst_meta[(k / C.nb) * dst_cap + k % C.nb];
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x, k = i >> 3, rh = k / (uint32_t)C.nb, j = k % (uint32_t)C.nb;
+    if (rh >= C.n_out * C.heads) return;
+    const uint4 d = dst_meta[rh * dst_cap + j];
     if (!d.w) return;
-    const int64_t from = src_meta[source_of(C, k, src_cap)].z;
+    const int64_t from = src_meta[source_of(C, rh, j, src_cap)].z;
     for (uint32_t e = i & 7; e < d.w; e += 8) {
         if ((int64_t)d.z + e >= dst_exc) {
             atomicOr(status, LQ_RES_ST_EXC_OVERFLOW);
@@ -403,7 +409,12 @@ bool choice_of(const lq_resident* src, const lq_resident* dst, int64_t n_seq, in
         dst->n_heads != src->n_heads / n_seq * n_out || dst->a == src->a)
         return false;
     *c = {index, blocks, n_seq, src->n_heads / n_seq, n_out, nb, src_blocks};
-    return n_out * c->heads * nb <= (int64_t)INT_MAX / 4;
+    return n_out * c->heads <= 65535 && n_out * c->heads * nb <= (int64_t)INT_MAX / 128;
+}
+
+ReadPool& read_pool() {
+    static ReadPool p;   // trivially destroyed: the HIP runtime may be gone by then
+    return p;
 }
 
 }  // namespace
@@ -419,13 +430,14 @@ int64_t lq_accept_workspace(int64_t n_seq, int64_t n_nodes, int64_t vocab) {
 
 int lq_accept_drafts(const void *d_logits, int dtype, int64_t stride_b, int64_t stride_n, int64_t vocab,
                      const int64_t *d_choice, const int64_t *d_tokens, const int32_t *d_parents, int64_t n_seq,
-                     int64_t n_nodes, void *d_work, int32_t *d_path, int32_t *d_count, int64_t *d_next, hipStream_t s) {
+                     int64_t n_nodes, void *d_work, int64_t work_bytes, int32_t *d_path, int32_t *d_count, int64_t *d_next, hipStream_t s) {
     if ((!d_logits == !d_choice) || !d_tokens || !d_parents || !d_path || !d_count || !d_next || n_seq < 1 ||
         n_seq > INT_MAX || n_nodes < 1 || n_nodes > LQ_TREE_MAX_NODES)
         return LQ_ERR_ARG;
     int64_t parts = 0;
     if (d_logits) {
         if (!d_work || dtype < 0 || dtype > 2 || lq_accept_workspace(n_seq, n_nodes, vocab) < 0 ||
+            work_bytes < lq_accept_workspace(n_seq, n_nodes, vocab) || ((uintptr_t)d_work & 7) ||
             ((uintptr_t)d_logits & (dtype == LQ_F32 ? 3 : 1)))
             return LQ_ERR_ARG;
         parts = argmax_parts(n_seq * n_nodes, vocab);
@@ -499,14 +511,14 @@ int lq_resident_reorder(const lq_resident *h_res, int64_t n, int64_t n_seq, cons
         if (!res_planes_ok(h_res + i) || h_res[i].n_heads != n_heads || n_heads % n_seq ||
             blk0 + n_blocks > h_res[i].cap_blocks)
             return LQ_ERR_ARG;
-    const int64_t heads = n_heads / n_seq, units = heads * n_blocks * kUnits, wg = n_seq <= 16 ? 256 : 64;
+    const int64_t heads = n_heads / n_seq, units = n_blocks * kUnits, wg = n_seq <= 16 ? 256 : 64;
     const int64_t grid = (units + wg - 1) / wg;
-    if (grid > INT_MAX) return LQ_ERR_ARG;
+    if (grid > INT_MAX || heads > 65535) return LQ_ERR_ARG;
     for (int64_t i = 0; i < n; i += kMaxRes) {
         const int64_t k = n - i < kMaxRes ? n - i : kMaxRes;
         PlaneTable P{};
         for (int64_t j = 0; j < k; j++) P.r[j] = planes_of(h_res + i + j);
-        const dim3 g((unsigned)grid, (unsigned)k);
+        const dim3 g((unsigned)grid, (unsigned)heads, (unsigned)k);
         if (n_seq <= 4) hipLaunchKernelGGL(k_reorder<4>, g, dim3(256), 0, s, P, heads, (int)n_seq, d_index, blk0, n_blocks);
         else if (n_seq <= 8) hipLaunchKernelGGL(k_reorder<8>, g, dim3(256), 0, s, P, heads, (int)n_seq, d_index, blk0, n_blocks);
         else if (n_seq <= 16) hipLaunchKernelGGL(k_reorder<16>, g, dim3(256), 0, s, P, heads, (int)n_seq, d_index, blk0, n_blocks);
@@ -516,24 +528,39 @@ int lq_resident_reorder(const lq_resident *h_res, int64_t n, int64_t n_seq, cons
 }
 
 int64_t lq_select_workspace(int64_t heads_out, int64_t n_blocks) {
-    if (heads_out < 1 || n_blocks < 1 || heads_out * n_blocks > (int64_t)INT_MAX / 4) return -1;
+    if (heads_out < 1 || n_blocks < 1 || heads_out > 65535 || heads_out * n_blocks > (int64_t)INT_MAX / 128) return -1;
     const int64_t n = heads_out * n_blocks;
     return (n + (n + kScan - 1) / kScan) * (int64_t)sizeof(uint32_t);
 }
 
 int lq_resident_select(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index, int64_t n_out,
-                       const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst, void *d_work, hipStream_t s) {
+                       const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst, void *d_work,
+                       int64_t work_bytes, int64_t *h_total, hipStream_t s) {
     Choice C;
-    if (!choice_of(src, dst, n_seq, src_blocks, d_index, n_out, d_blocks, n_blocks, &C) || !d_work || !dst->n_exc)
+    if (!choice_of(src, dst, n_seq, src_blocks, d_index, n_out, d_blocks, n_blocks, &C) || !d_work || !dst->n_exc ||
+        !dst->status || work_bytes < lq_select_workspace(dst->n_heads, n_blocks) || ((uintptr_t)d_work & 3))
         return LQ_ERR_ARG;
     const int64_t n = C.n_out * C.heads * C.nb, tiles = (n + kScan - 1) / kScan;
     uint32_t* off = static_cast<uint32_t*>(d_work);
     uint32_t* sums = off + n;
-    hipLaunchKernelGGL(k_select_count, dim3((unsigned)tiles), dim3(256), 0, s, src->meta, src->cap_blocks, C, off, sums);
-    hipLaunchKernelGGL(k_select_bases, dim3(1), dim3(64), 0, s, sums, tiles, dst->n_exc);
-    const int64_t grid = (n * kUnits + 255) / 256;
-    hipLaunchKernelGGL(k_select_planes, dim3((unsigned)grid), dim3(256), 0, s, planes_of(src), planes_of(dst), C, off, sums);
-    return launch_status();
+    ReadSlot slot;
+    if (h_total && !read_pool().take(s, &slot)) return LQ_ERR_LAUNCH;
+    hipLaunchKernelGGL(k_select_count, dim3((unsigned)tiles), dim3(256), 0, s, src->meta, src->cap_blocks, C, (uint32_t)n,
+                       off, sums);
+    hipLaunchKernelGGL(k_select_bases, dim3(1), dim3(64), 0, s, sums, tiles, dst->n_exc, dst->status,
+                       h_total ? slot.host : nullptr);
+    bool ok = !h_total || hipEventRecord(slot.event, s) == hipSuccess;
+    hipLaunchKernelGGL(k_select_planes, dim3((unsigned)((C.nb * kUnits + 255) / 256), (unsigned)(C.n_out * C.heads)),
+                       dim3(256), 0, s, planes_of(src), planes_of(dst), C, off, sums);
+    ok = hipGetLastError() == hipSuccess && ok;
+    if (h_total) {
+        // the planes are copied while the caller reads on
+        ok = ok && hipEventSynchronize(slot.event) == hipSuccess;
+        if (ok) *h_total = slot.host[0];
+        else (void)hipStreamSynchronize(s);   // no launch may still write the slot
+        read_pool().give(slot);
+    }
+    return ok ? LQ_OK : LQ_ERR_LAUNCH;
 }
 
 int lq_resident_select_exceptions(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index,

@@ -1232,7 +1232,7 @@ int lq_resident_tree_attention(const lq_resident *k, const lq_resident *v, int64
                                const lq_rows *draft_k, const lq_rows *draft_v, const int32_t *d_parents,
                                int64_t n_seq, int64_t n_nodes, int group, const lq_rows *tail_k, const lq_rows *tail_v,
                                int64_t tail_cap, const int32_t *d_tail_len, const int32_t *d_start, int dtype,
-                               void *d_work, const lq_rows *out, hipStream_t s) {
+                               void *d_work, int64_t work_bytes, const lq_rows *out, hipStream_t s) {
     if (!k || !v || k->n_heads < 1 || n_seq < 1 || k->n_heads != v->n_heads || k->n_heads % n_seq || !d_parents ||
         !d_work || !rows_ok(q) || !rows_ok(draft_k) || !rows_ok(draft_v) || !rows_ok(out) ||
         (dtype != LQ_F16 && dtype != LQ_BF16))
@@ -1244,6 +1244,8 @@ int lq_resident_tree_attention(const lq_resident *k, const lq_resident *v, int64
     const int64_t heads = k->n_heads / n_seq;
     Plan p;
     if (!plan(n_seq, heads, n_nodes, group, t_prefix, tail_cap, &p) || heads > INT_MAX) return LQ_ERR_ARG;
+    if (work_bytes < lq_tree_attn_workspace(n_seq, heads, n_nodes, group, t_prefix, tail_cap) || ((uintptr_t)d_work & 15))
+        return LQ_ERR_ARG;
     TreeArgs A{};
     if (t_prefix > 0) {
         A.k = *k;

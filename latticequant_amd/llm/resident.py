@@ -179,8 +179,11 @@ class ResidentKV:
         self._st = None
 
     def exceptions(self) -> torch.Tensor:
-        """(n, 8) int16: the exception entries in use (one host read of their number)."""
-        return self.exc[:min(int(self.n_exc.item()), self.exc_cap) * 8].view(-1, 8)
+        """(n, 8) int16: the exception entries in use (a host read of their number unless
+        the host knows it)."""
+        known = self._exc_since == 0 and self._exc_read is None
+        n = self._exc_known if known else int(self.n_exc.item())
+        return self.exc[:min(n, self.exc_cap) * 8].view(-1, 8)
 
     def reorder(self, index: torch.Tensor, t_from: int = 0) -> None:
         """reorder_sequences of this prefix alone."""
@@ -216,39 +219,40 @@ class ResidentKV:
         new = ResidentKV._bare(R * (self.n_heads // n_seq), cap, dev)
         if nb == 0:
             new.n_exc.zero_()
+            new.status.zero_()
             return new
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a selection reads its exception count back: not while a graph is captured")
         lib = L.lib()
         need = lib.lq_select_workspace(new.n_heads, nb)
         if need < 0:
-            raise ValueError("too many blocks for one selection")
-        with torch.cuda.device(dev):
+            raise ValueError("too many heads or blocks for one selection")
+        total = ctypes.c_int64()
+        with L.on_device(dev):
             idx = index.to(device=dev, dtype=torch.int32).contiguous()
             blk = None if blocks is None else blocks.to(device=dev, dtype=torch.int32).contiguous()
-            work = torch.empty(int(need), dtype=torch.uint8, device=dev)
-            src, dst = self.struct(), new.struct()
-            args = (ctypes.addressof(src), n_seq, used, idx.data_ptr(), R, L.ptr(blk), nb)
-            L.check(lib.lq_resident_select(*args, ctypes.addressof(dst), work.data_ptr(), L.stream_ptr(dev)),
-                    "lq_resident_select")
-            n = int(new.n_exc.item())
+            work = torch.empty(need, dtype=torch.uint8, device=dev)
+            args = (ctypes.addressof(self.struct()), n_seq, used, idx.data_ptr(), R, L.ptr(blk), nb)
+            L.check(lib.lq_resident_select(*args, ctypes.addressof(new.struct()), work.data_ptr(), need,
+                                           ctypes.addressof(total), L.raw_stream(dev)), "lq_resident_select")
+            n = total.value
             if n:
                 new.exc = torch.empty(n * 8, dtype=torch.int16, device=dev)
                 new._st = None
-                dst = new.struct()
-                L.check(lib.lq_resident_select_exceptions(*args, ctypes.addressof(dst), L.stream_ptr(dev)),
+                L.check(lib.lq_resident_select_exceptions(*args, ctypes.addressof(new.struct()), L.raw_stream(dev)),
                         "lq_resident_select_exceptions")
         new._exc_known, new.n_tokens = n, nb * RB
         return new
 
     @classmethod
     def _bare(cls, n_heads: int, nb: int, dev) -> "ResidentKV":
-        """nb blocks of room per head, uninitialised, an empty exception list."""
+        """nb blocks of room per head, everything uninitialised (counters too)."""
         r = cls.__new__(cls)
         r.device, r.n_heads, r.cap_blocks = dev, n_heads, nb
         for name, per, dt in (("a", 256, torch.int32), ("b", 256, torch.uint8), ("mask", 4, torch.int64),
                               ("meta", 4, torch.int32), ("scale", RB, torch.float16)):
             setattr(r, name, torch.empty(n_heads * nb * per, dtype=dt, device=dev))
-        r.n_exc = torch.empty(1, dtype=torch.int32, device=dev)
-        r.status = torch.zeros(1, dtype=torch.int32, device=dev)
+        r.n_exc, r.status = torch.empty((2, 1), dtype=torch.int32, device=dev).unbind(0)
         r.exc = torch.empty(8, dtype=torch.int16, device=dev)
         r.n_tokens = r._exc_known = r._exc_since = 0
         r._exc_read = r._st = None
@@ -298,9 +302,11 @@ def reorder_sequences(residents: Sequence[ResidentKV], index: torch.Tensor, t_fr
     if B < 1 or B > MAX_REORDER or r0.n_heads % B:
         raise ValueError(f"index must name 1..{MAX_REORDER} sequences that the heads divide into evenly "
                          "(more: ResidentKV.select makes a reordered copy)")
-    if any(r.n_heads != r0.n_heads or r.n_tokens != r0.n_tokens or r.a.device != dev for r in residents):
-        raise ValueError("the prefixes must have the same heads, tokens and device")
-    if len({r.a.data_ptr() for r in residents}) != len(residents):
+    H, T = r0.n_heads, r0.n_tokens
+    for r in residents:
+        if r.n_heads != H or r.n_tokens != T or r.a.device != dev:
+            raise ValueError("the prefixes must have the same heads, tokens and device")
+    if len(set(map(id, residents))) != len(residents):
         raise ValueError("a prefix stands twice in the list")
     if t_from < 0 or t_from % RB or t_from > r0.n_tokens or r0.n_tokens % RB:
         raise ValueError("t_from must be a multiple of 16 within the prefix")
@@ -308,13 +314,13 @@ def reorder_sequences(residents: Sequence[ResidentKV], index: torch.Tensor, t_fr
     if nb == 0 or B == 1:
         return
     lib = L.lib()
-    with torch.cuda.device(dev):
+    with L.on_device(dev):
         idx = index.to(device=dev, dtype=torch.int32).contiguous()
         if L.debug_checks() and (bool((idx < 0).any()) or bool((idx >= B).any())):
             raise ValueError("sequence out of range")
-        table = (L.Resident * len(residents))(*(r.struct() for r in residents))
-        L.check(lib.lq_resident_reorder(ctypes.addressof(table), len(residents), B, idx.data_ptr(), t_from // RB, nb,
-                                        L.stream_ptr(dev)), "lq_resident_reorder")
+        table = b"".join([r.struct() for r in residents])   # lq_resident[]
+        L.check(lib.lq_resident_reorder(table, len(residents), B, idx.data_ptr(), t_from // RB, nb, L.raw_stream(dev)),
+                "lq_resident_reorder")
 
 
 def attn_workspace(n_heads: int, group: int, t_prefix: int, t_tail: int, device=None) -> torch.Tensor:

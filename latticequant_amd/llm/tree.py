@@ -16,6 +16,8 @@ None of it waits for the device; lengths, trees and counts stay there.
 from __future__ import annotations
 
 import ctypes
+from array import array
+from operator import attrgetter
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -28,19 +30,25 @@ _DTYPES = (torch.float16, torch.bfloat16)
 
 
 def _rows(t: torch.Tensor):
-    """(tensor, its lq_rows): t (B, H, T, 128) as it lies where the kernels can read
-    16 bytes at a time, else a contiguous copy."""
-    if t.stride(3) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
+    """(t, pointer and strides of (B, H, T, 128) rows): as it lies where the kernels can
+    read 16 bytes at a time, else a contiguous copy."""
+    sb, sh, st, se = t.stride()
+    p = t.data_ptr()
+    if se != 1 or (sb | sh | st) & 7 or p & 15:
         t = t.contiguous()
-    return t, L.Rows(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+        sb, sh, st, _ = t.stride()
+        p = t.data_ptr()
+    return t, (p, sb, sh, st)
 
 
 def _ints(t, shape, name: str, dev) -> torch.Tensor:
     """Whole numbers of the given shape as a contiguous int32 tensor on dev."""
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be an int32 or int64 tensor")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    if t.dtype is torch.int32 and t.device == dev and t.is_contiguous():
+        return t
     return t.to(device=dev, dtype=torch.int32).contiguous()
 
 
@@ -88,10 +96,11 @@ def resident_tree_attention(k: ResidentKV, v: ResidentKV, q: torch.Tensor, draft
     same bits."""
     lib = L.lib()
     dev = k.a.device
-    if q.dim() != 4 or q.shape[3] != HD or q.dtype not in _DTYPES:
+    if q.dim() != 4 or q.dtype not in _DTYPES or q.shape[3] != HD:
         raise ValueError("q must be (B, Hq, N, 128) fp16 or bf16")
+    dt = q.dtype
     B, Hq, N, _ = q.shape
-    if k.n_heads != v.n_heads or k.n_tokens != v.n_tokens or k.a.device != v.a.device:
+    if k.n_heads != v.n_heads or k.n_tokens != v.n_tokens or dev != v.a.device:
         raise ValueError("K and V resident prefixes must have the same geometry and device")
     if B < 1 or k.n_heads % B:
         raise ValueError("the resident prefix must hold B * H_kv heads")
@@ -103,45 +112,53 @@ def resident_tree_attention(k: ResidentKV, v: ResidentKV, q: torch.Tensor, draft
     tp = k.n_tokens if t_prefix is None else int(t_prefix)
     if tp < 0 or tp > k.n_tokens or tp % RB:
         raise ValueError("t_prefix must be a multiple of 16 within the resident prefix")
-    if (tail_k is None) != (tail_v is None):
-        raise ValueError("tail K and V go together")
-    given = [q, draft_k, draft_v] + ([tail_k, tail_v] if tail_k is not None else [])
-    if any(t.dtype != q.dtype or t.device != dev for t in given):
-        raise ValueError("q, the drafts and the tail must be of one type, on the resident prefix's device")
     if draft_k.shape != (B, Hkv, N, HD) or draft_v.shape != draft_k.shape:
         raise ValueError("draft K / V must be (B, H_kv, N, 128)")
+    given = [q, draft_k, draft_v]
     cap = 0
-    if tail_k is not None:
+    if tail_k is not None and tail_v is not None:
         if tail_k.dim() != 4 or tail_k.shape != tail_v.shape or tail_k.shape[:2] != (B, Hkv) or tail_k.shape[3] != HD:
             raise ValueError("tail K / V must be (B, H_kv, cap, 128)")
-        cap = int(tail_k.shape[2])
+        cap = tail_k.shape[2]
+        given += [tail_k, tail_v]
+    elif tail_k is not None or tail_v is not None:
+        raise ValueError("tail K and V go together")
     elif tail_len is not None:
         raise ValueError("tail_len without a tail")
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif (out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(3) != 1 or
-          any(s % 8 or (s == 0 and n > 1) for s, n in zip(out.stride()[:3], out.shape)) or out.data_ptr() % 16):
+    for t in given:
+        if t.dtype is not dt or t.device != dev:
+            raise ValueError("q, the drafts and the tail must be of one type, on the resident prefix's device")
+    if out is not None and (out.shape != q.shape or out.dtype is not dt or out.device != dev or out.stride(3) != 1 or
+                            any(s % 8 or (s == 0 and n > 1) for s, n in zip(out.stride()[:3], out.shape)) or
+                            out.data_ptr() % 16):
         raise ValueError("out must be like q, its rows 16-byte aligned and apart")
-    need = lib.lq_tree_attn_workspace(B, Hkv, N, Hq // Hkv, tp, cap)
-    if need < 0:
-        raise ValueError("bad tree attention geometry")
-    with torch.cuda.device(dev):
-        if work is None:
-            work = torch.empty(int(need), dtype=torch.uint8, device=dev)
-        elif work.device != dev or not work.is_contiguous() or work.numel() * work.element_size() < need:
-            raise ValueError("attention workspace too small, or on another device")
+    with L.on_device(dev):
         par = _parents(parents, B, N, dev)
         tl = None if tail_len is None else _ints(tail_len, (B,), "tail_len", dev)
         st = None if start is None else _ints(start, (B,), "start", dev)
-        keep, rows = zip(*(_rows(t) for t in given))
-        refs = [ctypes.addressof(r) for r in rows] + [None, None]
-        ks, vs = k.struct(), v.struct()
-        ro = L.Rows(out.data_ptr(), out.stride(0), out.stride(1), out.stride(2))
-        L.check(lib.lq_resident_tree_attention(ctypes.addressof(ks), ctypes.addressof(vs), tp, refs[0], refs[1],
-                                               refs[2], par.data_ptr(), B, N, Hq // Hkv, refs[3] if cap else None,
-                                               refs[4] if cap else None, cap, L.ptr(tl), L.ptr(st),
-                                               L.dtype_code(q.dtype), work.data_ptr(), ctypes.addressof(ro),
-                                               L.stream_ptr(dev)), "lq_resident_tree_attention")
+        if work is None:
+            work = tree_attn_workspace(k.n_heads, Hq // Hkv, N, tp, cap, device=dev)
+        elif work.device != dev or not work.is_contiguous():
+            raise ValueError("the attention workspace must be contiguous, on the resident prefix's device")
+        if out is None:
+            out = torch.empty(q.shape, dtype=dt, device=dev)
+        keep, flat = [], array("q")            # the copies stay until the launch; six lq_rows
+        for t in given:
+            t, r = _rows(t)
+            keep.append(t)
+            flat.extend(r)
+        flat.extend((out.data_ptr(),) + out.stride()[:3])
+        at = flat.buffer_info()[0]
+        rc = lib.lq_resident_tree_attention(
+            ctypes.addressof(k.struct()), ctypes.addressof(v.struct()), tp, at, at + 32, at + 64, par.data_ptr(), B, N,
+            Hq // Hkv, at + 96 if cap else None, at + 128 if cap else None, cap, None if tl is None else tl.data_ptr(),
+            None if st is None else st.data_ptr(), 0 if dt is torch.float16 else 1, work.data_ptr(),
+            work.numel() * work.element_size(), at + 32 * len(given), L.raw_stream(dev))
+        if rc:
+            if rc == L.LQ_ERR_ARG and work.numel() * work.element_size() < lib.lq_tree_attn_workspace(
+                    B, Hkv, N, Hq // Hkv, tp, cap):
+                raise ValueError("attention workspace too small")
+            L.check(rc, "lq_resident_tree_attention")
     return out
 
 
@@ -167,69 +184,101 @@ def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, logits: Optional[
     dev = tokens.device
     if B < 1 or not 1 <= N <= MAX_NODES:
         raise ValueError(f"at least one sequence of 1..{MAX_NODES} nodes")
-    vocab = dt = need = 0
+    vocab = dt = sb = sn = 0
     if logits is not None:
         if logits.dim() != 3 or logits.shape[:2] != (B, N) or logits.device != dev or logits.shape[2] < 1:
             raise ValueError("logits must be (B, N, V) on the tokens' device")
-        if logits.dtype not in _DTYPES + (torch.float32,):
+        if logits.dtype not in _DTYPES and logits.dtype is not torch.float32:
             raise ValueError("logits must be fp16, bf16 or fp32")
         vocab, dt = logits.shape[2], L.dtype_code(logits.dtype)
-        need = lib.lq_accept_workspace(B, N, vocab)
-        if need < 0:
-            raise ValueError("too many nodes (65535 in all) or too large a vocabulary")
-    elif tuple(choice.shape) != (B, N) or choice.dtype != torch.int64 or choice.device != dev:
+    elif choice.shape != (B, N) or choice.dtype is not torch.int64 or choice.device != dev:
         raise ValueError("choice must be (B, N) int64 on the tokens' device")
-    with torch.cuda.device(dev):
+    with L.on_device(dev):
+        nbytes = 0
         if logits is not None:
             if logits.stride(2) != 1:
                 logits = logits.contiguous()
+            sb, sn, _ = logits.stride()
             if work is None:
-                work = torch.empty(need, dtype=torch.uint8, device=dev)
-            elif work.device != dev or not work.is_contiguous() or work.numel() * work.element_size() < need:
-                raise ValueError("acceptance workspace too small, or on another device")
+                nbytes = lib.lq_accept_workspace(B, N, vocab)
+                if nbytes < 0:
+                    raise ValueError("too many nodes (65535 in all) or too large a vocabulary")
+                work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            elif work.device != dev or not work.is_contiguous():
+                raise ValueError("the acceptance workspace must be contiguous, on the tokens' device")
+            else:
+                nbytes = work.numel() * work.element_size()
         else:
             choice = choice.contiguous()
         par, tok = _parents(parents, B, N, dev), tokens.contiguous()
-        path = torch.empty(B, N, dtype=torch.int32, device=dev)
+        path = torch.empty((B, N), dtype=torch.int32, device=dev)
         count = torch.empty(B, dtype=torch.int32, device=dev)
         nxt = torch.empty(B, dtype=torch.int64, device=dev)
-        sb, sn = (0, 0) if logits is None else logits.stride()[:2]
-        L.check(lib.lq_accept_drafts(L.ptr(logits), dt, sb, sn, vocab, L.ptr(choice), tok.data_ptr(), par.data_ptr(),
-                                     B, N, L.ptr(work), path.data_ptr(), count.data_ptr(), nxt.data_ptr(),
-                                     L.stream_ptr(dev)), "lq_accept_drafts")
+        rc = lib.lq_accept_drafts(None if logits is None else logits.data_ptr(), dt, sb, sn, vocab, L.ptr(choice),
+                                  tok.data_ptr(), par.data_ptr(), B, N, None if logits is None else work.data_ptr(),
+                                  nbytes, path.data_ptr(), count.data_ptr(), nxt.data_ptr(), L.raw_stream(dev))
+        if rc:
+            if logits is not None and not 0 <= lib.lq_accept_workspace(B, N, vocab) <= nbytes:
+                raise ValueError("acceptance workspace too small, or too many nodes")
+            L.check(rc, "lq_accept_drafts")
     return path, count, nxt
+
+
+def accept_workspace(n_seq: int, n_nodes: int, vocab: int, device=None) -> torch.Tensor:
+    """Workspace of accept_drafts with logits; uninitialised."""
+    n = L.load().lq_accept_workspace(n_seq, n_nodes, vocab)
+    if n < 0:
+        raise ValueError("bad acceptance geometry")
+    return torch.empty(int(n), dtype=torch.uint8, device=device)
+
+
+_stride, _data_ptr, _get_device = torch.Tensor.stride, torch.Tensor.data_ptr, torch.Tensor.get_device
+_shape, _dtype = attrgetter("shape"), attrgetter("dtype")
 
 
 def _pairs(dst: Sequence[torch.Tensor], src: Sequence[torch.Tensor], what: str):
     """Checked (destination, source) lists of row tensors (B, H, rows, width), grouped by
-    layout: [(pointers, pointers, strides, strides, sources kept alive)]."""
+    layout: [(how many, pointers, pointers, strides, strides in bytes, sources kept)].
+    A model's lists are long (K and V of every layer): their properties are taken by
+    maps over the list, a tenth of a microsecond each, and compared as sets."""
     if not len(dst) or len(dst) != len(src):
         raise ValueError(f"{what}: as many destinations as sources, one at least")
-    d0, s0 = dst[0], src[0]
-    if d0.dim() != 4 or s0.dim() != 4:
+    ds, ss = set(map(_shape, dst)), set(map(_shape, src))
+    if len(ds) != 1 or len(ss) != 1 or len(set(map(_dtype, dst)) | set(map(_dtype, src))) != 1:
+        raise ValueError(f"{what}: destinations of one shape, sources of one shape, all of one type")
+    ds, ss, el = ds.pop(), ss.pop(), dst[0].element_size()
+    if len(ds) != 4 or len(ss) != 4:
         raise ValueError(f"{what}: tensors of (B, H, rows, width)")
-    if any(t.shape != d0.shape or t.dtype != d0.dtype or t.device != d0.device for t in dst):
-        raise ValueError(f"{what}: destinations of one shape, type and device")
-    if any(t.shape != s0.shape or t.dtype != d0.dtype or t.device != d0.device for t in src):
-        raise ValueError(f"{what}: sources of one shape, and of the destinations' type and device")
-    el = d0.element_size()
-    if not d0.is_cuda or d0.shape[3] != s0.shape[3] or d0.shape[3] * el % 16 or not 16 <= d0.shape[3] * el <= 4096:
-        raise ValueError(f"{what}: rows on the GPU, of one width, a multiple of 16 bytes")
+    on = set(map(_get_device, dst)) | set(map(_get_device, src))
+    if len(on) != 1 or on.pop() < 0 or ds[3] != ss[3] or ds[3] * el % 16 or not 16 <= ds[3] * el <= 4096:
+        raise ValueError(f"{what}: rows on one GPU, of one width, a multiple of 16 bytes")
 
-    def fits(t):
-        return t.stride(3) == 1 and not any(x * el % 16 for x in t.stride()[:3]) and t.data_ptr() % 16 == 0
-    if any(not fits(t) or any(x == 0 and n > 1 for x, n in zip(t.stride(), t.shape)) for t in dst):
+    def fits(strides):
+        return strides[3] == 1 and not any(x * el % 16 for x in strides[:3])
+    dt, st = list(map(_stride, dst)), list(map(_stride, src))
+    dp, sp = list(map(_data_ptr, dst)), list(map(_data_ptr, src))
+    if (not all(fits(t) and not any(x == 0 and n > 1 for x, n in zip(t, ds)) for t in set(dt)) or
+            any(p & 15 for p in dp)):
         raise ValueError(f"{what}: destination rows must be contiguous, apart and 16-byte aligned")
-    groups = {}
-    for d, s in zip(dst, src):
-        s = s if fits(s) else s.contiguous()
-        groups.setdefault((d.stride(), s.stride()), []).append((d.data_ptr(), s.data_ptr(), s))
+    src = list(src)
+    if not all(map(fits, set(st))) or any(p & 15 for p in sp):
+        for i, t in enumerate(src):
+            if not fits(st[i]) or sp[i] & 15:
+                src[i] = t.contiguous()
+                st[i], sp[i] = src[i].stride(), src[i].data_ptr()
+    kinds = set(zip(dt, st))
     out = []
-    for (sd, ss), g in groups.items():
-        n = len(g)
-        out.append((n, (ctypes.c_void_p * n)(*(x[0] for x in g)), (ctypes.c_void_p * n)(*(x[1] for x in g)),
-                    (ctypes.c_int64 * 3)(*(x * el for x in sd[:3])), (ctypes.c_int64 * 3)(*(x * el for x in ss[:3])), g))
+    for kind in kinds:
+        at = range(len(dst)) if len(kinds) == 1 else [i for i in range(len(dst)) if (dt[i], st[i]) == kind]
+        out.append((len(at), array("Q", (dp[i] for i in at)), array("Q", (sp[i] for i in at)),
+                    array("q", (x * el for x in kind[0][:3])), array("q", (x * el for x in kind[1][:3])), src))
     return out
+
+
+def _addresses(group):
+    """A group of _pairs as the C ABI takes it."""
+    n, d, s, sd, ss, _ = group
+    return d.buffer_info()[0], s.buffer_info()[0], n, sd.buffer_info()[0], ss.buffer_info()[0]
 
 
 def append_accepted(tails: Sequence[torch.Tensor], drafts: Sequence[torch.Tensor], path: torch.Tensor,
@@ -246,15 +295,15 @@ def append_accepted(tails: Sequence[torch.Tensor], drafts: Sequence[torch.Tensor
     N, dev = drafts[0].shape[2], tails[0].device
     if drafts[0].shape[:2] != (B, H) or B < 1 or H < 1 or cap < 1 or not 1 <= N <= MAX_NODES:
         raise ValueError(f"drafts must be (B, H, N, width) of the tails' B and H, N 1..{MAX_NODES}")
-    with torch.cuda.device(dev):
+    with L.on_device(dev):
         pt, ct = _ints(path, (B, N), "path", dev), _ints(count, (B,), "count", dev)
         ln = _ints(tail_len, (B,), "tail_len", dev)
         if L.debug_checks() and (bool((ln + ct > cap).any()) or bool((ct > N).any())):
             raise ValueError("accepted rows do not fit the tails")
         new = torch.empty(B, dtype=torch.int32, device=dev)
-        for n, d, s, sd, ss, _ in groups:
-            L.check(lib.lq_append_rows(d, s, n, sd, ss, B, H, cap, N, width * tails[0].element_size(), pt.data_ptr(),
-                                       ct.data_ptr(), ln.data_ptr(), new.data_ptr(), L.stream_ptr(dev)),
+        for g in groups:
+            L.check(lib.lq_append_rows(*_addresses(g), B, H, cap, N, width * tails[0].element_size(), pt.data_ptr(),
+                                       ct.data_ptr(), ln.data_ptr(), new.data_ptr(), L.raw_stream(dev)),
                     "lq_append_rows")
     return new
 
@@ -274,11 +323,11 @@ def gather_tails(tails: Sequence[torch.Tensor], index: torch.Tensor) -> list:
         return out
     groups = _pairs(out, tails, "gather_tails")
     B, H, T, width = t0.shape
-    with torch.cuda.device(t0.device):
+    with L.on_device(t0.device):
         idx = _ints(index, (index.numel(),), "index", t0.device)
         if B < 1:
             raise ValueError("no sequences to choose from")
-        for n, d, s, sd, ss, _ in groups:
-            L.check(lib.lq_gather_rows(d, s, n, sd, ss, B, index.numel(), H, T, width * t0.element_size(),
-                                       idx.data_ptr(), L.stream_ptr(t0.device)), "lq_gather_rows")
+        for g in groups:
+            L.check(lib.lq_gather_rows(*_addresses(g), B, index.numel(), H, T, width * t0.element_size(),
+                                       idx.data_ptr(), L.raw_stream(t0.device)), "lq_gather_rows")
     return out
