@@ -242,48 +242,77 @@ __device__ __forceinline__ Unit unit_of(const Planes& p, int64_t w, int64_t nb) 
     return {p.meta, kUT, w - nb * kUS};
 }
 
-// In place: a thread has one unit of all sequences, reads the ones that move before it
-// writes any.  R: the sequences, at most (their units in registers).
+// Workgroups of a head by plane, so that a workgroup's plane is uniform: those of plane p
+// end before end[p].
+struct Cuts {
+    uint32_t end[5];
+};
+// Where a workgroup works: its plane's unit 0 of head h and block blk0 in sequence 0, the
+// bytes from a sequence to the next, its first unit and the plane's units of the head.
+struct Part {
+    char* at;
+    int64_t row;
+    uint32_t first, units;
+};
+__device__ __forceinline__ Part part_of(const Planes& p, const Cuts& c, uint32_t wg, int64_t heads, int64_t h, int64_t blk0,
+                                        uint32_t nb, uint32_t threads) {
+    const int k = wg < c.end[0] ? 0 : wg < c.end[1] ? 1 : wg < c.end[2] ? 2 : wg < c.end[3] ? 3 : 4;
+    const uint32_t per = k == 0 ? kUA : k == 1 ? kUB : k == 2 ? kUM : k == 3 ? kUS : kUT;
+    char* base = k == 0 ? p.a : k == 1 ? p.b : k == 2 ? p.mask : k == 3 ? p.scale : p.meta;
+    return {base + (h * p.cap + blk0) * per * 16, heads * p.cap * per * 16, (wg - (k ? c.end[k - 1] : 0u)) * threads, nb * per};
+}
+
+// In place: a thread has one unit of all sequences and reads the ones that move before it
+// writes any.  R: the sequences, at most (their units in registers).  Every load is issued
+// before the first wait; where a sequence stays (or its index names none) the load is
+// that of one that moves, from cache.  Bound by memory: 8 sequences of 2048 tokens of 64
+// prefixes, 1.25 GB read and written, take 255 us (4.9 TB/s); loads that each waited
+// for their own took 407.
 template <int R>
-__global__ __launch_bounds__(256) void k_reorder(PlaneTable P, int64_t heads, int n_seq,
-                                                 const int32_t* __restrict__ index, int64_t blk0, int64_t nb) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
-    if (i >= nb * kUnits) return;
-    const Planes& p = P.r[blockIdx.z];
-    const Unit u = unit_of(p, i, nb);
-    const int64_t row = heads * p.cap * u.per * 16;
-    char* at = u.plane + ((h * p.cap + blk0) * u.per + u.at) * 16;
-    uint4 v[R];
+__global__ __launch_bounds__(256) void k_reorder(PlaneTable P, Cuts cuts, int64_t heads, int n_seq,
+                                                 const int32_t* __restrict__ index, int64_t blk0, uint32_t nb) {
+    int f[R], any = -1;
+#pragma unroll
+    for (int s = 0; s < R; s++) f[s] = index[s < n_seq ? s : 0];
 #pragma unroll
     for (int s = 0; s < R; s++) {
-        const int f = s < n_seq ? index[s] : s;   // uniform; an index out of range moves nothing
-        if (f != s && f >= 0 && f < n_seq) v[s] = *reinterpret_cast<const uint4*>(at + f * row);
+        if (s >= n_seq || f[s] == s || f[s] < 0 || f[s] >= n_seq) f[s] = -1;
+        else any = f[s];
     }
+    if (any < 0) return;
+    const Part w = part_of(P.r[blockIdx.z], cuts, blockIdx.x, heads, blockIdx.y, blk0, nb, 256);
+    const uint32_t u = w.first + threadIdx.x;
+    if (u >= w.units) return;
+    u32x4_t v[R];   // (a native vector: arrays of the HIP type go through scratch here)
 #pragma unroll
-    for (int s = 0; s < R; s++) {
-        const int f = s < n_seq ? index[s] : s;
-        if (f != s && f >= 0 && f < n_seq) *reinterpret_cast<uint4*>(at + s * row) = v[s];
-    }
+    for (int s = 0; s < R; s++) v[s] = reinterpret_cast<const u32x4_t*>(w.at + (f[s] < 0 ? any : f[s]) * w.row)[u];
+#pragma unroll
+    for (int s = 0; s < R; s++)
+        if (f[s] >= 0) reinterpret_cast<u32x4_t*>(w.at + s * w.row)[u] = v[s];
 }
 
 // The same for more sequences, their units in LDS (1 KB a sequence and wave).
 constexpr int kMaxReorder = 128;
-__global__ __launch_bounds__(64) void k_reorder_lds(PlaneTable P, int64_t heads, int n_seq,
-                                                    const int32_t* __restrict__ index, int64_t blk0, int64_t nb) {
-    __shared__ uint4 s_v[kMaxReorder][64];
-    const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x, h = blockIdx.y;
-    if (i >= nb * kUnits) return;
-    const Planes& p = P.r[blockIdx.z];
-    const Unit u = unit_of(p, i, nb);
-    const int64_t row = heads * p.cap * u.per * 16;
-    char* at = u.plane + ((h * p.cap + blk0) * u.per + u.at) * 16;
-    for (int s = 0; s < n_seq; s++) {
-        const int f = index[s];
-        if (f != s && f >= 0 && f < n_seq) s_v[s][threadIdx.x] = *reinterpret_cast<const uint4*>(at + f * row);
+__global__ __launch_bounds__(64) void k_reorder_lds(PlaneTable P, Cuts cuts, int64_t heads, int n_seq,
+                                                    const int32_t* __restrict__ index, int64_t blk0, uint32_t nb) {
+    __shared__ u32x4_t s_v[kMaxReorder][64];
+    const Part w = part_of(P.r[blockIdx.z], cuts, blockIdx.x, heads, blockIdx.y, blk0, nb, 64);
+    const uint32_t u = w.first + threadIdx.x;
+    if (u >= w.units) return;
+    for (int s0 = 0; s0 < n_seq; s0 += 8) {
+        u32x4_t v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int s = min(s0 + k, n_seq - 1), f = index[s];
+            v[k] = reinterpret_cast<const u32x4_t*>(w.at + (f >= 0 && f < n_seq ? f : s) * w.row)[u];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (s0 + k < n_seq) s_v[s0 + k][threadIdx.x] = v[k];
     }
     for (int s = 0; s < n_seq; s++) {
         const int f = index[s];
-        if (f != s && f >= 0 && f < n_seq) *reinterpret_cast<uint4*>(at + s * row) = s_v[s][threadIdx.x];
+        if (f != s && f >= 0 && f < n_seq) reinterpret_cast<u32x4_t*>(w.at + s * w.row)[u] = s_v[s][threadIdx.x];
     }
 }
 
@@ -511,18 +540,22 @@ int lq_resident_reorder(const lq_resident *h_res, int64_t n, int64_t n_seq, cons
         if (!res_planes_ok(h_res + i) || h_res[i].n_heads != n_heads || n_heads % n_seq ||
             blk0 + n_blocks > h_res[i].cap_blocks)
             return LQ_ERR_ARG;
-    const int64_t heads = n_heads / n_seq, units = n_blocks * kUnits, wg = n_seq <= 16 ? 256 : 64;
-    const int64_t grid = (units + wg - 1) / wg;
-    if (grid > INT_MAX || heads > 65535) return LQ_ERR_ARG;
+    const int64_t heads = n_heads / n_seq, wg = n_seq <= 16 ? 256 : 64;
+    if (n_blocks > INT_MAX / kUnits || heads > 65535) return LQ_ERR_ARG;
+    Cuts cuts;
+    const int per[5] = {kUA, kUB, kUM, kUS, kUT};
+    uint32_t grid = 0;
+    for (int p = 0; p < 5; p++) cuts.end[p] = grid += (uint32_t)((n_blocks * per[p] + wg - 1) / wg);
     for (int64_t i = 0; i < n; i += kMaxRes) {
         const int64_t k = n - i < kMaxRes ? n - i : kMaxRes;
         PlaneTable P{};
         for (int64_t j = 0; j < k; j++) P.r[j] = planes_of(h_res + i + j);
-        const dim3 g((unsigned)grid, (unsigned)heads, (unsigned)k);
-        if (n_seq <= 4) hipLaunchKernelGGL(k_reorder<4>, g, dim3(256), 0, s, P, heads, (int)n_seq, d_index, blk0, n_blocks);
-        else if (n_seq <= 8) hipLaunchKernelGGL(k_reorder<8>, g, dim3(256), 0, s, P, heads, (int)n_seq, d_index, blk0, n_blocks);
-        else if (n_seq <= 16) hipLaunchKernelGGL(k_reorder<16>, g, dim3(256), 0, s, P, heads, (int)n_seq, d_index, blk0, n_blocks);
-        else hipLaunchKernelGGL(k_reorder_lds, g, dim3(64), 0, s, P, heads, (int)n_seq, d_index, blk0, n_blocks);
+        const dim3 g(grid, (unsigned)heads, (unsigned)k), t((unsigned)wg);
+        const uint32_t nb = (uint32_t)n_blocks;
+        if (n_seq <= 4) hipLaunchKernelGGL(k_reorder<4>, g, t, 0, s, P, cuts, heads, (int)n_seq, d_index, blk0, nb);
+        else if (n_seq <= 8) hipLaunchKernelGGL(k_reorder<8>, g, t, 0, s, P, cuts, heads, (int)n_seq, d_index, blk0, nb);
+        else if (n_seq <= 16) hipLaunchKernelGGL(k_reorder<16>, g, t, 0, s, P, cuts, heads, (int)n_seq, d_index, blk0, nb);
+        else hipLaunchKernelGGL(k_reorder_lds, g, t, 0, s, P, cuts, heads, (int)n_seq, d_index, blk0, nb);
     }
     return launch_status();
 }

@@ -220,6 +220,7 @@ class ResidentKV:
         if nb == 0:
             new.n_exc.zero_()
             new.status.zero_()
+            new.exc = torch.empty(8, dtype=torch.int16, device=dev)
             return new
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a selection reads its exception count back: not while a graph is captured")
@@ -232,15 +233,15 @@ class ResidentKV:
             idx = index.to(device=dev, dtype=torch.int32).contiguous()
             blk = None if blocks is None else blocks.to(device=dev, dtype=torch.int32).contiguous()
             work = torch.empty(need, dtype=torch.uint8, device=dev)
-            args = (ctypes.addressof(self.struct()), n_seq, used, idx.data_ptr(), R, L.ptr(blk), nb)
-            L.check(lib.lq_resident_select(*args, ctypes.addressof(new.struct()), work.data_ptr(), need,
-                                           ctypes.addressof(total), L.raw_stream(dev)), "lq_resident_select")
+            dst, stream = new.struct(), L.raw_stream(dev)
+            args = (ctypes.addressof(self.struct()), n_seq, used, idx.data_ptr(), R, L.ptr(blk), nb, ctypes.addressof(dst))
+            L.check(lib.lq_resident_select(*args, work.data_ptr(), need, ctypes.addressof(total), stream),
+                    "lq_resident_select")
             n = total.value
+            new.exc = torch.empty(max(1, n) * 8, dtype=torch.int16, device=dev)
+            dst.exc, dst.exc_cap = new.exc.data_ptr(), max(1, n)
             if n:
-                new.exc = torch.empty(n * 8, dtype=torch.int16, device=dev)
-                new._st = None
-                L.check(lib.lq_resident_select_exceptions(*args, ctypes.addressof(new.struct()), L.raw_stream(dev)),
-                        "lq_resident_select_exceptions")
+                L.check(lib.lq_resident_select_exceptions(*args, stream), "lq_resident_select_exceptions")
         new._exc_known, new.n_tokens = n, nb * RB
         return new
 
@@ -253,7 +254,7 @@ class ResidentKV:
                               ("meta", 4, torch.int32), ("scale", RB, torch.float16)):
             setattr(r, name, torch.empty(n_heads * nb * per, dtype=dt, device=dev))
         r.n_exc, r.status = torch.empty((2, 1), dtype=torch.int32, device=dev).unbind(0)
-        r.exc = torch.empty(8, dtype=torch.int16, device=dev)
+        r.exc = r.scale.view(torch.int16)[:8]   # no entry yet
         r.n_tokens = r._exc_known = r._exc_since = 0
         r._exc_read = r._st = None
         return r
