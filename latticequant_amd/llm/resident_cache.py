@@ -18,7 +18,14 @@ compresses every update and hands HF attention fully decompressed fp16 K / V
   ``lq_resident_attention`` over resident prefix + tail (no fp16 prefix is
   ever materialised); for a prompt (several query tokens) it returns the
   materialised K / V (resident prefix dequantised as ``_decompress_chunk``
-  writes it, then the tail) for HF's causal SDPA.
+  writes it, then the tail) for HF's causal SDPA;
+* drafted tokens (``draft`` / ``verify``): the next forward's tokens are the nodes of
+  a tree that attend to the cache and their own ancestors
+  (:func:`resident_tree_attention`); the path that the model confirms goes into the
+  cache, the rest is dropped;
+* beams: ``reorder_cache`` permutes the sequences in place
+  (:func:`reorder_sequences`), ``batch_repeat_interleave`` and
+  ``batch_select_indices`` make the cache of chosen ones.
 
 Use::
 
@@ -26,6 +33,10 @@ Use::
     register()                                   # adds attn_implementation "lq_resident"
     model = AutoModelForCausalLM.from_config(cfg, attn_implementation="lq_resident")
     out = model.generate(ids, past_key_values=ResidentKVCache(bits_per_dim=4), ...)
+
+    cache.draft(parents)                         # the tree: parents[i] < i, -1 for node 0
+    logits = model(tokens, position_ids=cache.draft_positions(), past_key_values=cache).logits
+    accepted, nxt = cache.verify(tokens, logits=logits)
 """
 from __future__ import annotations
 
@@ -35,7 +46,9 @@ import torch
 from transformers.cache_utils import DynamicCache
 
 from .. import codec
-from .resident import RB, ResidentKV, attn_workspace, resident_decode_attention
+from .resident import MAX_REORDER, RB, ResidentKV, attn_workspace, reorder_sequences, resident_decode_attention
+from .tree import (MAX_NODES, accept_drafts, append_accepted, gather_tails, node_depths, resident_tree_attention,
+                   tree_workspace_size)
 
 ATTN_NAME = "lq_resident"
 
@@ -58,6 +71,10 @@ class ResidentKVCache(DynamicCache):
         self.chunks: List[list] = []          # per layer: [(_AtRest K, _AtRest V)] rANS chunks at rest
         self._work = None
         self._work_heads = 0
+        self._parents = self._start = None    # drafted tree of the next forward
+        self._drafts = {}                     # layer -> the drafts' (K, V)
+        self._room = {}                       # layer -> (K, V) buffers that the tails are the first tokens of
+        self._tree_work = None
 
     # -- storage ----------------------------------------------------------
     def _ensure(self, layer_idx: int):
@@ -93,6 +110,11 @@ class ResidentKVCache(DynamicCache):
         if key_states.shape[-1] != 128:
             raise ValueError("ResidentKVCache needs head_dim 128")
         self._ensure(layer_idx)
+        if self._parents is not None:
+            if (key_states.shape[0], key_states.shape[2]) != tuple(self._parents.shape):
+                raise ValueError("the forward's tokens are not the drafted nodes: verify() or discard() the draft first")
+            self._drafts[layer_idx] = (key_states, value_states)
+            return self._marked(key_states, value_states, layer_idx)
         if self.tail_k[layer_idx] is None:
             self.tail_k[layer_idx] = key_states.contiguous()
             self.tail_v[layer_idx] = value_states.contiguous()
@@ -105,11 +127,14 @@ class ResidentKVCache(DynamicCache):
         if key_states.shape[2] == 1:
             # decode step: marker views carrying the cache; the attention reads
             # the resident prefix and the tail itself
-            mk, mv = key_states.view_as(key_states), value_states.view_as(value_states)
-            mk._lq_cache = mv._lq_cache = self
-            mk._lq_layer = mv._lq_layer = layer_idx
-            return mk, mv
+            return self._marked(key_states, value_states, layer_idx)
         return self.materialise(layer_idx)
+
+    def _marked(self, k, v, layer_idx: int):
+        mk, mv = k.view_as(k), v.view_as(v)
+        mk._lq_cache = mv._lq_cache = self
+        mk._lq_layer = mv._lq_layer = layer_idx
+        return mk, mv
 
     def materialise(self, layer_idx: int):
         """Full (B, H, T, hd) K / V of the layer: the resident prefix dequantised
@@ -127,10 +152,7 @@ class ResidentKVCache(DynamicCache):
         """One decode step of the layer: query (B, Hq, 1, 128) -> (B, Hq, 1, 128)."""
         tk, tv = self.tail_k[layer_idx], self.tail_v[layer_idx]
         B, H = tk.shape[:2]
-        rk, rv = self.res_k[layer_idx], self.res_v[layer_idx]
-        if rk is None:   # nothing flushed yet: an empty prefix
-            rk = self.res_k[layer_idx] = ResidentKV(B * H, 1024, device=tk.device)
-            rv = self.res_v[layer_idx] = ResidentKV(B * H, 1024, device=tk.device)
+        rk, rv = self._prefix(layer_idx, B * H, tk.device)
         group = query.shape[1] // H
         n = attn_workspace_size(B * H, group, rk.n_tokens, tk.shape[2])
         # the workspace's completion counters sit at [0, 256 * kv heads): a new
@@ -142,6 +164,187 @@ class ResidentKVCache(DynamicCache):
         out = resident_decode_attention(rk, rv, query.to(torch.float16), tk.to(torch.float16),
                                         tv.to(torch.float16), work=self._work)
         return out.to(query.dtype)
+
+    def _prefix(self, layer_idx: int, heads: int, device):
+        if self.res_k[layer_idx] is None:   # nothing flushed yet: an empty prefix
+            self.res_k[layer_idx] = ResidentKV(heads, 1024, device=device)
+            self.res_v[layer_idx] = ResidentKV(heads, 1024, device=device)
+        return self.res_k[layer_idx], self.res_v[layer_idx]
+
+    # -- drafted trees ------------------------------------------------------
+    def draft(self, parents, start=None) -> None:
+        """The next forward's tokens are drafted nodes: parents (B, N) or (N,) whole
+        numbers (tensor or nested lists), an earlier node, -1 for the root, node 0 (the
+        newest token, not in the cache yet); -2 for padding.  start (B,): the first cached
+        token each sequence sees (left padding).  The forward leaves the cache as it is;
+        its attention is the tree's (the model's mask is not read), so its positions are
+        draft_positions().  verify() or discard() ends the draft."""
+        if self._parents is not None:
+            raise ValueError("a draft is pending: verify() or discard() it first")
+        if not self.tail_k:
+            raise ValueError("nothing is cached yet: the prompt comes first")
+        B, dev = self.tail_k[0].shape[0], self.tail_k[0].device
+        par = torch.as_tensor(parents)
+        if par.is_floating_point() or par.dtype == torch.bool or par.dim() not in (1, 2):
+            raise ValueError("parents must be (B, N) or (N,) whole numbers")
+        if par.dim() == 1:
+            par = par[None].expand(B, -1)
+        if par.shape[0] != B or not 1 <= par.shape[1] <= MAX_NODES:
+            raise ValueError(f"one tree of 1..{MAX_NODES} nodes per sequence")
+        st = None if start is None else torch.as_tensor(start)
+        if st is not None and (st.shape != (B,) or st.dtype not in (torch.int32, torch.int64)):
+            raise ValueError("start must be (B,) whole numbers")
+        self._parents = par.to(device=dev, dtype=torch.int32).contiguous()
+        self._start = None if st is None else st.to(device=dev, dtype=torch.int32)
+        self._drafts = {}
+
+    def draft_positions(self) -> torch.Tensor:
+        """(B, N) int64: the nodes' positions, cached tokens + depth in the tree."""
+        if self._parents is None:
+            raise ValueError("no draft is pending")
+        pos = self.get_seq_length() + node_depths(self._parents)
+        return pos if self._start is None else pos - self._start[:, None].long()
+
+    def attend_drafts(self, layer_idx: int, query: torch.Tensor) -> torch.Tensor:
+        """The drafted nodes' attention: query (B, Hq, N, 128) -> (B, N, Hq, 128)."""
+        dk, dv = self._drafts[layer_idx]
+        tk, tv = self.tail_k[layer_idx], self.tail_v[layer_idx]
+        dt = query.dtype if query.dtype in (torch.float16, torch.bfloat16) else torch.float16
+        rk, rv = self._prefix(layer_idx, tk.shape[0] * tk.shape[1], tk.device)
+        B, Hq, N, hd = query.shape
+        n = tree_workspace_size(rk.n_heads, Hq // tk.shape[1], N, rk.n_tokens, tk.shape[2])
+        if self._tree_work is None or self._tree_work.numel() < n or self._tree_work.device != tk.device:
+            self._tree_work = torch.empty(n, dtype=torch.uint8, device=tk.device)
+        out = torch.empty((B, N, Hq, hd), dtype=dt, device=tk.device)
+        resident_tree_attention(rk, rv, query.to(dt), dk.to(dt), dv.to(dt), self._parents, tk.to(dt), tv.to(dt),
+                                start=self._start, work=self._tree_work, out=out.transpose(1, 2))
+        return out.to(query.dtype)
+
+    def verify(self, tokens: torch.Tensor, logits: Optional[torch.Tensor] = None,
+               choice: Optional[torch.Tensor] = None):
+        """End the draft: the path of nodes that the model's choices confirm
+        (accept_drafts: the argmax of logits (B, N, V), or choice (B, N)) goes into the
+        cache, the other nodes are dropped.  tokens: (B, N), the forward's.  Sequences of a
+        batch advance together, by the shortest accepted path.  Returns (accepted (B, A):
+        the tokens now cached, node 0's first; next (B, 1): the token after them)."""
+        if self._parents is None or len(self._drafts) != len(self.tail_k):
+            raise ValueError("no drafted forward to verify")
+        path, count, nxt = accept_drafts(tokens, self._parents, logits=logits, choice=choice)
+        n = int(count.min())                       # the tails' length: the host has to know it
+        if n == 0:
+            raise ValueError("a sequence's node 0 is padding")
+        taken = path[:, :n].long()
+        accepted = tokens.gather(1, taken)
+        if path.shape[1] > n:                      # a sequence cut short goes on with its next accepted node
+            more = path[:, n].long()
+            nxt = torch.where(more >= 0, tokens.gather(1, more.clamp_min(0)[:, None])[:, 0], nxt)
+        self.accept(path[:, :n])
+        return accepted, nxt[:, None]
+
+    def accept(self, path: torch.Tensor) -> None:
+        """End the draft with the nodes path (B, A), whole numbers, in the cache."""
+        if self._parents is None or len(self._drafts) != len(self.tail_k):
+            raise ValueError("no drafted forward to accept")
+        B, N = self._parents.shape
+        if path.dim() != 2 or path.shape[0] != B or not 1 <= path.shape[1] <= N:
+            raise ValueError("path must be (B, A), 1 <= A <= nodes")
+        A, dev = path.shape[1], self._parents.device
+        full = torch.full((B, N), -1, dtype=torch.int32, device=dev)
+        full[:, :A] = path
+        groups = {}                                # layers of one shape, type and tail length: all of them, as a rule
+        for i in range(len(self.tail_k)):
+            t = self.tail_k[i].shape[2]
+            key = (t, self._buffers(i, t + A)[0].shape, self.tail_k[i].dtype, self._drafts[i][0].dtype)
+            groups.setdefault(key, []).append(i)
+        for (t, _, dt, _), layers in groups.items():
+            count, at = (torch.full((B,), n, dtype=torch.int32, device=dev) for n in (A, t))
+            append_accepted([b for i in layers for b in self._room[i]],
+                            [d.to(dt) for i in layers for d in self._drafts[i]], full, count, at)
+            for i in layers:
+                self.tail_k[i], self.tail_v[i] = (b[:, :, :t + A] for b in self._room[i])
+        self.discard()
+        for i in range(len(self.tail_k)):
+            over = self.tail_k[i].shape[2] - self.tail_tokens
+            if over >= RB:
+                self._flush(i, over // RB * RB)
+
+    def discard(self) -> None:
+        """End the draft, the cache as it was."""
+        self._parents = self._start = None
+        self._drafts = {}
+
+    def _buffers(self, layer_idx: int, need: int):
+        """The layer's tails as the first tokens of buffers with room for `need`."""
+        tk, tv = self.tail_k[layer_idx], self.tail_v[layer_idx]
+        buf = self._room.get(layer_idx)
+        if buf is None or buf[0].data_ptr() != tk.data_ptr() or buf[0].shape[2] < need:
+            B, H, t, hd = tk.shape
+            buf = tuple(torch.empty((B, H, need + 64, hd), dtype=x.dtype, device=x.device) for x in (tk, tv))
+            for b, x in zip(buf, (tk, tv)):
+                b[:, :, :t] = x
+            self._room[layer_idx] = buf
+        return buf
+
+    # -- beams --------------------------------------------------------------
+    def reorder_cache(self, beam_idx: torch.Tensor) -> None:
+        """Sequence i becomes sequence beam_idx[i] as it was, in place."""
+        if not self.tail_k:
+            return
+        if beam_idx.dim() != 1 or beam_idx.numel() != self.tail_k[0].shape[0] or beam_idx.numel() > MAX_REORDER:
+            return self.batch_select_indices(beam_idx)
+        self._no_draft()
+        idx = beam_idx.to(self.tail_k[0].device)
+        by_length = {}
+        for r in self.res_k + self.res_v:
+            if r is not None:
+                by_length.setdefault(r.n_tokens, []).append(r)
+        for group in by_length.values():
+            reorder_sequences(group, idx)
+        self._select_rest(idx)
+
+    def batch_select_indices(self, indices: torch.Tensor) -> None:
+        """Keep the sequences indices[r], in that order (a sequence may stand several
+        times); the others' resident blocks and exceptions are freed."""
+        if not self.tail_k:
+            return
+        self._no_draft()
+        B = self.tail_k[0].shape[0]
+        idx = torch.arange(B)[indices.cpu()] if indices.dtype == torch.bool else indices
+        if idx.dim() != 1 or idx.numel() < 1:
+            raise ValueError("indices must be a list of sequences")
+        idx = idx.to(self.tail_k[0].device)
+        for res in (self.res_k, self.res_v):
+            for i, r in enumerate(res):
+                if r is not None:
+                    res[i] = r.select(idx, B, cap_tokens=r.cap_blocks * RB)
+        self._select_rest(idx)
+
+    def batch_repeat_interleave(self, repeats: int) -> None:
+        """Every sequence `repeats` times in a row (a prompt's beams)."""
+        if self.tail_k:
+            self.batch_select_indices(torch.arange(self.tail_k[0].shape[0]).repeat_interleave(repeats))
+
+    def _no_draft(self):
+        if self._parents is not None:
+            raise ValueError("a draft is pending: verify() or discard() it first")
+
+    def _select_rest(self, idx):
+        """Tails and at-rest chunks of the sequences idx."""
+        shapes = {}
+        for i, (tk, tv) in enumerate(zip(self.tail_k, self.tail_v)):
+            shapes.setdefault((tk.shape, tk.dtype, tv.dtype), []).append(i)
+        for layers in shapes.values():
+            if self.tail_k[layers[0]].dtype == self.tail_v[layers[0]].dtype:
+                new = gather_tails([t for i in layers for t in (self.tail_k[i], self.tail_v[i])], idx)
+            else:
+                new = [t.index_select(0, idx) for i in layers for t in (self.tail_k[i], self.tail_v[i])]
+            for j, i in enumerate(layers):
+                self.tail_k[i], self.tail_v[i] = new[2 * j], new[2 * j + 1]
+        self._room = {}
+        for ch in self.chunks:
+            for pair in ch:
+                for e in pair:
+                    e.rows = idx.long() if e.rows is None else e.rows[idx.long()]
 
     def get_seq_length(self, layer_idx=0):
         if layer_idx >= len(self.tail_k) or self.tail_k[layer_idx] is None:
@@ -173,14 +376,14 @@ class ResidentKVCache(DynamicCache):
         pending encodes (one host sync).  Returns the host bytes held."""
         for ch in self.chunks:
             for i, pair in enumerate(ch):
-                ch[i] = tuple(e if isinstance(e, _HostAtRest) else _HostAtRest(e.batch) for e in pair)
+                ch[i] = tuple(e if isinstance(e, _HostAtRest) else _HostAtRest(e.batch, e.rows) for e in pair)
         return self.at_rest_host_bytes()
 
     def restore_at_rest(self):
         """Bring offloaded chunk pairs back to the device (codec.from_bytes)."""
         for ch in self.chunks:
             for i, pair in enumerate(ch):
-                ch[i] = tuple(_DeviceAtRest(e.batch) if isinstance(e, _HostAtRest) else e for e in pair)
+                ch[i] = tuple(_DeviceAtRest(e.batch, e.rows) if isinstance(e, _HostAtRest) else e for e in pair)
 
     def at_rest_host_bytes(self) -> int:
         return sum(e.nbytes for ch in self.chunks for pair in ch for e in pair if isinstance(e, _HostAtRest))
@@ -201,7 +404,11 @@ class ResidentKVCache(DynamicCache):
 
 
 class _AtRest:
-    """One K or V half of a flushed chunk pair, settled on first access."""
+    """One K or V half of a flushed chunk pair, settled on first access.  rows: the
+    chunk's sequence that each sequence of the cache is (None: the same one); a chunk's
+    bitstreams are its own whole, so reordering and selecting move only this."""
+
+    rows = None
 
     def __init__(self, pend, index: int):
         self._pend, self._index = pend, index
@@ -217,8 +424,8 @@ class _AtRest:
 class _DeviceAtRest:
     """An at-rest half held on the device as a settled batch."""
 
-    def __init__(self, batch):
-        self.batch = batch
+    def __init__(self, batch, rows=None):
+        self.batch, self.rows = batch, rows
 
     def reference_bytes(self) -> int:
         return int(self.batch.reference_bytes().sum())
@@ -228,7 +435,8 @@ class _HostAtRest:
     """An at-rest half held in host memory in the wire form; .batch restores
     it to the current device (a new device copy per access)."""
 
-    def __init__(self, batch):
+    def __init__(self, batch, rows=None):
+        self.rows = rows
         self.blob = codec.to_bytes(batch)
         self.nbytes = len(self.blob)
         self._ref = int(batch.reference_bytes().sum())
@@ -251,10 +459,17 @@ def attn_workspace_size(n_heads: int, group: int, t_prefix: int, t_tail: int) ->
 
 def resident_attention(module, query, key, value, attention_mask, dropout: float = 0.0, scaling=None, **kwargs):
     """HF attention function "lq_resident": one-token decode steps over a
-    ResidentKVCache run lq_resident_attention; everything else (prompts,
+    ResidentKVCache run lq_resident_attention, drafted tokens
+    lq_resident_tree_attention; everything else (prompts,
     plain tensors) goes to HF's SDPA over the materialised K / V."""
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
     cache = getattr(key, "_lq_cache", None)
+    if cache is not None and cache._parents is not None:
+        # drafted nodes: the tree is the mask, whatever mask the model built for a chain
+        if (kwargs.get("sliding_window") is not None or kwargs.get("softcap") is not None or
+                (scaling is not None and abs(scaling - 128 ** -0.5) > 1e-12)):
+            raise ValueError("drafted trees need plain attention: no sliding window or soft-capping, scale 1/sqrt(128)")
+        return cache.attend_drafts(key._lq_layer, query), None
     if cache is None or query.shape[2] != 1:
         return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout, scaling=scaling,
                                       **kwargs)

@@ -63,14 +63,34 @@ def _parents(parents, B: int, N: int, dev) -> torch.Tensor:
     return p
 
 
-def tree_attn_workspace(n_heads: int, group: int, n_nodes: int, t_prefix: int, tail_cap: int,
-                        device=None) -> torch.Tensor:
-    """Workspace of resident_tree_attention over n_heads resident heads (all
-    sequences' kv heads), n_nodes nodes per sequence; uninitialised."""
+def node_depths(parents: torch.Tensor) -> torch.Tensor:
+    """(B, N) int64: how many ancestors each node has (0 for roots and padding), by
+    doubling: after k rounds up[i] is the node 2^k generations above i."""
+    B, N = parents.shape
+    idx = torch.arange(N, device=parents.device)
+    up = torch.where((parents >= 0) & (parents < idx), parents.long(), idx)
+    depth = (up != idx).long()
+    k = 1
+    while k < N:
+        depth = depth + depth.gather(1, up)
+        up = up.gather(1, up)
+        k *= 2
+    return depth
+
+
+def tree_workspace_size(n_heads: int, group: int, n_nodes: int, t_prefix: int, tail_cap: int) -> int:
+    """Bytes of workspace of resident_tree_attention over n_heads resident heads (all
+    sequences' kv heads), n_nodes nodes per sequence."""
     n = L.load().lq_tree_attn_workspace(1, n_heads, n_nodes, group, t_prefix, tail_cap)
     if n < 0:
         raise ValueError("bad tree attention geometry")
-    return torch.empty(int(n), dtype=torch.uint8, device=device)
+    return n
+
+
+def tree_attn_workspace(n_heads: int, group: int, n_nodes: int, t_prefix: int, tail_cap: int,
+                        device=None) -> torch.Tensor:
+    """tree_workspace_size bytes on the device, uninitialised."""
+    return torch.empty(tree_workspace_size(n_heads, group, n_nodes, t_prefix, tail_cap), dtype=torch.uint8, device=device)
 
 
 def resident_tree_attention(k: ResidentKV, v: ResidentKV, q: torch.Tensor, draft_k: torch.Tensor,

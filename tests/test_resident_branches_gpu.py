@@ -1,0 +1,270 @@
+"""ResidentKVCache along several continuations: drafted trees verified by a model, and
+beams (sequences reordered, selected and repeated)."""
+import pytest
+import torch
+
+from tests.test_hf_resident_gpu import _model
+
+gpu = pytest.mark.gpu
+
+
+def _cache(model, ids, tail=32, **kw):
+    from latticequant_amd.llm.resident_cache import ResidentKVCache
+    c = ResidentKVCache(bits_per_dim=4, tail_tokens=tail)
+    with torch.no_grad():
+        lo = model(ids, past_key_values=c, use_cache=True, **kw).logits[:, -1]
+    return c, lo
+
+
+def _step(model, c, tokens):
+    with torch.no_grad():
+        return model(tokens, past_key_values=c, use_cache=True).logits
+
+
+def _tree_around(path, vocab, g):
+    """A tree that holds the path's tokens among others: (tokens, parents, path nodes)."""
+    tokens, parents, nodes = [int(path[0])], [-1], [0]
+    for t in path[1:]:
+        for _ in range(2):                                   # siblings that are wrong
+            w = int(torch.randint(0, vocab, (1,), generator=g))
+            if w != int(t):
+                tokens.append(w)
+                parents.append(nodes[-1])
+        tokens.append(int(t))
+        parents.append(nodes[-1])
+        nodes.append(len(tokens) - 1)
+        tokens.append(int(torch.randint(0, vocab, (1,), generator=g)))
+        parents.append(len(tokens) - 2)
+    return tokens, parents, nodes
+
+
+@gpu
+@pytest.mark.parametrize("prompt,tail,heads,kv", [(100, 32, 4, 2), (41, 0, 8, 2), (70, 128, 4, 4)])
+def test_drafted_tree_matches_single_steps_gpu(prompt, tail, heads, kv):
+    """A tree that holds the greedy continuation: its nodes' logits on that path are those
+    of one-token steps (the attention's tolerance carried into the logits, as in
+    test_hf_resident_gpu), verify() accepts the path, and the cache goes on as the
+    stepped one does, drafts again (into the same buffers) and one-token steps.  Both
+    caches keep what comes after the prompt in their tails until the end: a step that
+    flushed 16 of them in between would leave the stepped one with other, quantised K / V
+    than the drafts saw.  A last draft then flushes."""
+    model, cfg = _model(heads=heads, kv_heads=kv)
+    g = torch.Generator().manual_seed(3)
+    ids = torch.randint(0, cfg.vocab_size, (1, prompt), generator=g).cuda()
+    a, lo = _cache(model, ids, tail)
+    b, _ = _cache(model, ids, tail)
+    first = lo.argmax(-1)
+    a.tail_tokens = b.tail_tokens = 1 << 20
+    for _ in range(3):
+        path, want = [int(first)], []
+        for _ in range(5):
+            lb = _step(model, b, torch.tensor([[path[-1]]], device="cuda"))[:, -1].float()
+            want.append(lb)
+            path.append(int(lb.argmax()))
+        path = path[:5]                                      # b has cached exactly these
+        tokens, parents, nodes = _tree_around(path, cfg.vocab_size, g)
+        t = torch.tensor([tokens], device="cuda")
+        before = a.get_seq_length()
+        a.draft(parents)
+        assert a.draft_positions().tolist() == [[before + d for d in _depths(parents)]]
+        with torch.no_grad():
+            logits = model(t, position_ids=a.draft_positions(), past_key_values=a, use_cache=True).logits
+        assert a.get_seq_length() == before
+        for i, w in zip(nodes, want):
+            err = ((logits[:, i].float() - w).abs().max() / w.abs().max()).item()
+            assert err < 5e-3, err
+        choice = torch.zeros(1, len(tokens), dtype=torch.int64, device="cuda")   # b's choices: a near tie cannot decide
+        choice[0, nodes] = torch.tensor([int(w.argmax()) for w in want], device="cuda")
+        accepted, nxt = a.verify(t, choice=choice)
+        assert accepted.tolist() == [path] and int(nxt) == int(want[-1].argmax())
+        assert a.get_seq_length() == before + 5 == b.get_seq_length()
+        la = _step(model, a, nxt)[:, -1].float()
+        lb = _step(model, b, nxt)[:, -1].float()
+        assert ((la - lb).abs().max() / lb.abs().max()).item() < 5e-3
+        first = lb.argmax(-1)
+    a.tail_tokens = tail
+    before, flushed = a.get_seq_length(), a.res_k[0].n_tokens if a.res_k[0] is not None else 0
+    last = [x.clone() for x in a.materialise(1)]
+    t = torch.tensor([[int(first), 1, 2]], device="cuda")
+    a.draft([-1, 0, 0])
+    with torch.no_grad():
+        model(t, position_ids=a.draft_positions(), past_key_values=a, use_cache=True)
+    drafts = [x.clone() for x in a._drafts[1]]
+    a.accept(torch.tensor([[0, 2]], device="cuda"))
+    assert a.get_seq_length() == before + 2
+    n = a.res_k[1].n_tokens
+    assert n % 16 == 0 and before + 2 - n == a.tail_k[1].shape[2] and a.tail_k[1].shape[2] < tail + 16
+    for now, old, d in zip(a.materialise(1), last, drafts):
+        kept = max(n - flushed, 0) + flushed                  # the first n tokens are compressed by now, the rest as they were
+        if kept < before:
+            assert torch.equal(now[:, :, kept:before], old[:, :, kept:])
+        if kept <= before:
+            assert torch.equal(now[:, :, before:], d[:, :, [0, 2]])
+
+
+def _depths(parents):
+    d = []
+    for p in parents:
+        d.append(0 if p < 0 else d[p] + 1)
+    return d
+
+
+@gpu
+def test_verify_logits_batch_and_bookkeeping_gpu():
+    """Two sequences whose accepted paths differ in length advance by the shorter; the
+    longer one's next token is its next accepted draft.  discard() leaves the cache."""
+    model, cfg = _model()
+    g = torch.Generator().manual_seed(5)
+    ids = torch.randint(0, cfg.vocab_size, (2, 50), generator=g).cuda()
+    c, lo = _cache(model, ids, 32)
+    t = torch.tensor([[int(lo[0].argmax()), 7, 8, 9], [int(lo[1].argmax()), 3, 4, 5]], device="cuda")
+    c.draft([-1, 0, 1, 0])
+    kv = [x.clone() for x in c.materialise(1)]
+    with torch.no_grad():
+        model(t, position_ids=c.draft_positions(), past_key_values=c, use_cache=True)
+    c.discard()
+    assert c.get_seq_length() == 50 and all(torch.equal(x, y) for x, y in zip(c.materialise(1), kv))
+    c.draft([-1, 0, 1, 0])
+    with torch.no_grad():
+        logits = model(t, position_ids=c.draft_positions(), past_key_values=c, use_cache=True).logits
+    drafts = [(k.clone(), v.clone()) for k, v in (c._drafts[i] for i in range(2))]
+    fake = torch.zeros_like(logits)
+    fake[0, 0, 7] = fake[0, 1, 8] = fake[0, 2, 100] = 5.0    # accepts nodes 0, 1, 2
+    fake[1, 0, 5] = fake[1, 3, 200] = 5.0                    # accepts nodes 0, 3
+    accepted, nxt = c.verify(t, logits=fake)
+    assert accepted.tolist() == [[int(t[0, 0]), 7], [int(t[1, 0]), 5]] and nxt.tolist() == [[8], [200]]
+    assert c.get_seq_length() == 52
+    for i in range(2):
+        for half in range(2):
+            full = c.materialise(i)[half]
+            for b, nodes in enumerate(([0, 1], [0, 3])):
+                assert torch.equal(full[b, :, 50:52], drafts[i][half][b][:, nodes])
+
+
+@gpu
+def test_left_padded_drafts_gpu():
+    """Sequences of different lengths, left-padded: drafts with start= see no padding and
+    agree with the same sequence drafted alone."""
+    model, cfg = _model()
+    g = torch.Generator().manual_seed(8)
+    ids = torch.randint(0, cfg.vocab_size, (2, 60), generator=g).cuda()
+    mask = torch.ones(2, 60, dtype=torch.long, device="cuda")
+    mask[0, :13] = 0
+    pos = (mask.cumsum(-1) - 1).clamp_min(0)
+    c, _ = _cache(model, ids, 128, attention_mask=mask, position_ids=pos)
+    alone, _ = _cache(model, ids[:1, 13:], 128)
+    t = torch.randint(0, cfg.vocab_size, (2, 6), generator=g).cuda()
+    par = [-1, 0, 0, 1, 3, 2]
+    c.draft(par, start=[13, 0])
+    alone.draft(par)
+    assert torch.equal(c.draft_positions()[:1], alone.draft_positions())
+    with torch.no_grad():
+        both = model(t, position_ids=c.draft_positions(), past_key_values=c, use_cache=True).logits[0].float()
+        one = model(t[:1], position_ids=alone.draft_positions(), past_key_values=alone, use_cache=True).logits[0].float()
+    assert ((both - one).abs().max() / one.abs().max()).item() < 5e-3
+
+
+def _filled(B, layers=3, tail=32, tokens=90, seed=1, dtype=torch.float16):
+    from latticequant_amd.llm.resident_cache import ResidentKVCache
+    g = torch.Generator().manual_seed(seed)
+    c = ResidentKVCache(bits_per_dim=4, tail_tokens=tail)
+    for i in range(layers):
+        k, v = (torch.randn(B, 2, tokens, 128, generator=g).to(dtype).cuda() for _ in range(2))
+        k[..., 5] *= 12
+        c.update(k, v, i)
+    return c
+
+
+@gpu
+@pytest.mark.parametrize("tail", [0, 32, 128])
+def test_reorder_select_and_repeat_gpu(tail):
+    from latticequant_amd import codec
+    c = _filled(4, tail=tail)
+    q = torch.randn(4, 8, 1, 128, device="cuda").half()
+    ref = [[x.clone() for x in c.materialise(i)] for i in range(3)]
+    at = torch.arange(4)
+    for how, idx in (("reorder", [2, 0, 2, 1]), ("reorder", [0, 1, 2, 3]), ("select", [3, 1, 0]), ("repeat", 2),
+                     ("reorder", [5, 0, 1, 1, 4, 2])):
+        if how == "reorder":
+            c.reorder_cache(torch.tensor(idx, device="cuda"))
+        elif how == "select":
+            c.batch_select_indices(torch.tensor(idx))
+        else:
+            c.batch_repeat_interleave(idx)
+            idx = torch.arange(at.numel()).repeat_interleave(idx).tolist()
+        at = at[idx]
+        for i in range(3):
+            for x, y in zip(c.materialise(i), ref[i]):
+                assert torch.equal(x, y[at.cuda()]), (how, i)
+        assert c.get_seq_length() == 90
+        if c.chunks[0]:
+            half = c.chunks[1][0][0]
+            rows = codec.decode_batch(half.batch).reshape(4, 2, -1, 128)
+            now = torch.arange(4) if half.rows is None else half.rows.cpu()
+            assert torch.equal(now, at) or how == "reorder" and idx == [0, 1, 2, 3]
+            assert torch.equal(rows[now.cuda()], c.materialise(1)[0][:, :, :rows.shape[2]])
+    held = c.compressed_bytes()
+    c.offload_at_rest()
+    c.restore_at_rest()
+    assert c.compressed_bytes() == held and (not c.chunks[0] or torch.equal(c.chunks[0][0][0].rows.cpu(), at))
+    # the cache is used on: a step whose tail flushes, attention over it
+    new = torch.randn(6, 2, 16, 128, device="cuda").half()
+    c.update(new, new, 0)
+    out = c.attend(0, torch.randn(6, 8, 1, 128, device="cuda").half())
+    assert torch.isfinite(out).all() and q is not None
+
+
+@gpu
+def test_reorder_leaves_callers_tensors_gpu():
+    """The prompt's own K / V may be the tail (nothing flushed): reordering must not write them."""
+    from latticequant_amd.llm.resident_cache import ResidentKVCache
+    c = ResidentKVCache(bits_per_dim=4, tail_tokens=128)
+    k = torch.randn(3, 2, 20, 128, device="cuda").half()
+    keep = k.clone()
+    c.update(k, k, 0)
+    c.reorder_cache(torch.tensor([1, 2, 0], device="cuda"))
+    assert torch.equal(k, keep) and torch.equal(c.materialise(0)[0], keep[[1, 2, 0]])
+
+
+@gpu
+def test_generate_with_beams_gpu():
+    """HF's beam search over the cache: with nothing flushed the cache holds the model's own
+    fp16 K / V, and the beams found are as likely as DynamicCache's (the same up to a near
+    tie); over a compressed prefix it runs."""
+    from transformers.cache_utils import DynamicCache
+    from latticequant_amd.llm.resident_cache import ResidentKVCache
+    model, cfg = _model()
+    ids = torch.randint(0, cfg.vocab_size, (2, 40), generator=torch.Generator().manual_seed(2)).cuda()
+    kw = dict(num_beams=3, max_new_tokens=12, do_sample=False, return_dict_in_generate=True, output_scores=True,
+              pad_token_id=0, eos_token_id=None)
+    a = model.generate(ids, past_key_values=ResidentKVCache(bits_per_dim=4, tail_tokens=256), **kw)
+    b = model.generate(ids, past_key_values=DynamicCache(), **kw)
+    assert (a.sequences_scores - b.sequences_scores).abs().max() < 2e-2
+    c = model.generate(ids, past_key_values=ResidentKVCache(bits_per_dim=5, tail_tokens=16), **kw)
+    assert c.sequences.shape == b.sequences.shape
+
+
+def test_draft_refusals():
+    from latticequant_amd.llm.resident_cache import ResidentKVCache
+    c = ResidentKVCache(bits_per_dim=4, tail_tokens=128)
+    with pytest.raises(ValueError):
+        c.draft([-1, 0])                                     # nothing cached
+    k = torch.randn(2, 1, 4, 128).half()
+    c.update(k, k, 0)
+    for bad in ([[-1, 0]], [[-1.0], [-1.0]], [], [[[-1]], [[-1]]], [-1] * 257):
+        with pytest.raises((ValueError, TypeError)):
+            c.draft(bad)
+    with pytest.raises(ValueError):
+        c.draft([-1, 0], start=[1])
+    with pytest.raises(ValueError):
+        c.draft_positions()
+    c.draft([-1, 0, 0])
+    assert c.draft_positions().tolist() == [[4, 5, 5]] * 2
+    for f in (lambda: c.draft([-1]), lambda: c.update(k, k, 0), lambda: c.reorder_cache(torch.tensor([0, 1])),
+              lambda: c.batch_select_indices(torch.tensor([0])), lambda: c.verify(torch.zeros(2, 3, dtype=torch.int64)),
+              lambda: c.accept(torch.zeros(2, 1, dtype=torch.int64))):
+        with pytest.raises(ValueError):
+            f()
+    c.discard()
+    c.update(k, k, 0)
+    assert c.get_seq_length() == 8
