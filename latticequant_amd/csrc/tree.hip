@@ -219,6 +219,39 @@ struct Raw {
     uint2 s[2];
     uint2 mask[2];   // exceptions of the records' group
 };
+// The records and metas of a wave's tiles in a loop over whole ones: bases that advance by
+// a round at a time and offsets that stay, so a reload is its loads and little else.
+struct Walk {
+    const char *a, *b, *s, *m, *t;
+    uint32_t left;   // rounds that are still to come
+};
+__device__ __forceinline__ Walk walk_of(const lq_resident& r, int64_t block, uint32_t rounds) {
+    return {reinterpret_cast<const char*>(r.a + block * 256), reinterpret_cast<const char*>(r.b + block * 256),
+            reinterpret_cast<const char*>(r.scale + block * kRB), reinterpret_cast<const char*>(r.mask + block * 4),
+            reinterpret_cast<const char*>(r.meta + block * 4 + 2), rounds};
+}
+__device__ __forceinline__ void step(Walk& w, uint32_t blocks) {   // stays at the last round
+    const uint32_t n = w.left ? blocks : 0u;
+    w.left -= w.left ? 1u : 0u;
+    w.a += n * 1024;
+    w.b += n * 256;
+    w.s += n * 32;
+    w.m += n * 32;
+    w.t += n * 16;
+}
+__device__ __forceinline__ void load_walk(const Walk& w, const Lay& y, Raw& d) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        d.a[j] = at32<uint4>(w.a, (y.hi[j] * 256 + y.rec[j]) * 4);
+        d.b[j] = at32<uint32_t>(w.b, y.hi[j] * 256 + y.rec[j]);
+        d.s[j] = at32<uint2>(w.s, (y.hi[j] * kRB + (y.rec[j] & 15)) * 2);
+        d.mask[j] = at32<uint2>(w.m, (y.hi[j] * 4 + (y.rec[j] >> 6)) * 8);
+    }
+}
+__device__ __forceinline__ Meta load_meta(const Walk& w, uint32_t lane) {
+    const uint2 x = at32<uint2>(w.t, (lane >> 5) * 16);
+    return {x.x, x.y};
+}
 __device__ __forceinline__ void load_raw(const lq_resident& r, int64_t hd, int64_t t, int64_t T, const Lay& y, Raw& d) {
     const Blocks B = blocks_of(r, hd, t, T);
 #pragma unroll
@@ -505,36 +538,50 @@ __device__ __forceinline__ uint32_t weights(float s0, float s1, float c0, float 
     return p;
 }
 
-// U subtiles for the wave's 32 rows, of which the lane's row sees the tokens of word (with
-// MASK, one subtile) or all.  The subtiles' products are independent, so one's softmax
-// runs beside the other's MFMA.
-template <int U, bool MASK>
-__device__ __forceinline__ void sub_attend(const char* lds, const h8_t q[8], uint32_t word, int lane, RowState& st) {
-    const float c0 = 1.4426950408889634f / 11.313708498984761f;   // log2(e) / sqrt(128)
+// Scores of U subtiles for the wave's 32 rows: eight steps of U MFMA each, K read two
+// steps ahead (left to itself the compiler reads each step's K just before it).
+template <int U>
+__device__ __forceinline__ void scores(const char* lds, const h8_t q[8], int lane, f16_t s[U]) {
     const int n = lane & 31, g = lane >> 5;
     const int tok = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
-    f16_t s[U];
+    const char* kl = lds + tok * kKRow + 16 * g;
+    h8_t ka[3][U];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        s[u] = f16_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < 2; c++)
 #pragma unroll
-        for (int c = 0; c < 8; c++) {
-            const h8_t ka = *reinterpret_cast<const h8_t*>(lds + u * kSub + tok * kKRow + 32 * c + 16 * g);
-            s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, q[c], s[u], 0, 0, 0);
+        for (int u = 0; u < U; u++) ka[c][u] = *reinterpret_cast<const h8_t*>(kl + u * kSub + 32 * c);
+#pragma unroll
+    for (int u = 0; u < U; u++) s[u] = f16_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 8; c++) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (c < 6) ka[(c + 2) % 3][u] = *reinterpret_cast<const h8_t*>(kl + u * kSub + 32 * (c + 2));
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[c % 3][u], q[c], s[u], 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_barrier(0);   // V is read once the scores stand: both at a time take more registers than there are
-    float mx = -INFINITY;
+}
+
+// Softmax and P V of U subtiles' scores.  The weights of a half subtile (16 tokens) are
+// taken beside the products of the half before, V is read three products ahead.
+template <int U>
+__device__ __forceinline__ void products(const char* lds, const f16_t s[U], int lane, RowState& st) {
+    const float c0 = 1.4426950408889634f / 11.313708498984761f;   // log2(e) / sqrt(128)
+    const int n = lane & 31, g = lane >> 5;
+    constexpr int N = 8 * U;                   // products: half h, 32 dimensions d: number 4 h + d
+    const char* vl = lds + 32 * kKRow + n * kVRow + 16 * g;
+    auto read = [&](int f) __attribute__((always_inline)) {
+        return *reinterpret_cast<const h8_t*>(vl + (f >> 3) * kSub + 32 * (f & 3) * kVRow + 32 * ((f >> 2) & 1));
+    };
+    h8_t va[4];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        if (MASK) {
-            const uint32_t own = word >> (8 * g);
+    for (int f = 0; f < 3; f++) va[f] = read(f);
+    float mx = s[0][0];
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[u][i] = (own >> tok_of(i)) & 1u ? s[u][i] : -INFINITY;
-        }
+    for (int u = 0; u < U; u++)
 #pragma unroll
         for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
-    }
     const float mn = halves_max(mx) * c0;
     if (__any(mn > st.m + kLazy)) {
         // a row that has seen nothing has m = -inf, l = 0 and o = 0
@@ -548,24 +595,39 @@ __device__ __forceinline__ void sub_attend(const char* lds, const h8_t q[8], uin
         st.m = up;
     }
     const float off = (st.m == -INFINITY ? 0.f : -st.m) + kPShift;
+    uint32_t p[2][4];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const char* vl = lds + u * kSub + 32 * kKRow;
+    for (int i = 0; i < 4; i++) p[0][i] = weights(s[0][2 * i], s[0][2 * i + 1], c0, off, st.l);
 #pragma unroll
-        for (int sx = 0; sx < 2; sx++) {
-            uint32_t p[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                p[i] = weights(s[u][8 * sx + 2 * i], s[u][8 * sx + 2 * i + 1], c0, off, st.l);
-            }
-            const h8_t pb = as_h8(p[0], p[1], p[2], p[3]);
-#pragma unroll
-            for (int d = 0; d < 4; d++) {
-                const h8_t va = *reinterpret_cast<const h8_t*>(vl + (32 * d + n) * kVRow + 16 * (2 * sx + g));
-                st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb, st.o[d], 0, 0, 0);
-            }
+    for (int f = 0; f < N; f++) {
+        const int h = f >> 2, d = f & 3;
+        if (f + 3 < N) va[(f + 3) & 3] = read(f + 3);
+        st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[f & 3], as_h8(p[h & 1][0], p[h & 1][1], p[h & 1][2], p[h & 1][3]),
+                                                         st.o[d], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (h + 1 < 2 * U) {
+            const int u = (h + 1) >> 1, i = 8 * ((h + 1) & 1) + 2 * d;
+            p[(h + 1) & 1][d] = weights(s[u][i], s[u][i + 1], c0, off, st.l);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
+}
+
+template <int U>
+__device__ __forceinline__ void sub_attend(const char* lds, const h8_t q[8], int lane, RowState& st) {
+    f16_t s[U];
+    scores<U>(lds, q, lane, s);
+    products<U>(lds, s, lane, st);
+}
+
+// one subtile of which the lane's row sees the tokens of word
+__device__ __forceinline__ void sub_masked(const char* lds, const h8_t q[8], uint32_t word, int lane, RowState& st) {
+    f16_t s[1];
+    scores<1>(lds, q, lane, s);
+    const uint32_t own = word >> (8 * (lane >> 5));
+#pragma unroll
+    for (int i = 0; i < 16; i++) s[0][i] = (own >> tok_of(i)) & 1u ? s[0][i] : -INFINITY;
+    products<1>(lds, s, lane, st);
 }
 
 // ------------------------------------------------------------------ kernel --
@@ -760,16 +822,23 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_many(TreeArgs A) {
     Raw raw;
     Meta meta, ahead;
     uint4 ent;
-    auto at = [&](int tile) { return ((int64_t)min(tile, h1 - 1) * S + mine) * 32; };
-    auto fetch = [&](int tile) {               // `ahead` has the tile's bases
+    // the team's rounds; a team without a tile in the last one reads that of the one before
+    const uint32_t tiles = h1 - h0 > team ? (uint32_t)(h1 - h0 - team + T - 1) / T : 0u;
+    Walk wr = walk_of(res, P.hd * res.cap_blocks + ((int64_t)(tiles ? h0 + team : h0) * S + mine) * 2, tiles ? tiles - 1 : 0u);
+    Walk wm = wr;
+    auto fetch = [&]() __attribute__((always_inline)) {   // `ahead` has the tile's bases
         ent = load_entry(res, ahead, lane);
         meta = ahead;
-        load_raw(res, P.hd, at(tile), A.t_prefix, lay, raw);
-        ahead = load_meta(res, P.hd, at(tile + T), A.t_prefix, lane);
+        step(wr, 2 * T * S);
+        load_walk(wr, lay, raw);
+        step(wm, 2 * T * S);
+        ahead = load_meta(wm, lane);
     };
     if (prefix) {
-        ahead = load_meta(res, P.hd, at(h0 + team), A.t_prefix, lane);
-        load_raw(res, P.hd, at(h0 + team), A.t_prefix, lay, raw);
+        meta = load_meta(wm, lane);
+        load_walk(wr, lay, raw);
+        step(wm, 2 * T * S);
+        ahead = load_meta(wm, lane);
     }
     const int parent = P.sp == A.nsp - 1 && tid < A.nodes ? A.parents[P.b * A.nodes + tid] : -2;
     // the wave's rows: column lane % 32
@@ -799,27 +868,25 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_many(TreeArgs A) {
         patch_lds(isk, res, d, lay, m, e, word, lane, s_place[wave], lds);
     };
     if (prefix) {
-        ent = load_entry(res, ahead, lane);
-        meta = ahead;
-        ahead = load_meta(res, P.hd, at(h0 + team + T), A.t_prefix, lane);
+        ent = load_entry(res, meta, lane);
         put(raw, meta, ent, ~0u, buf + mine * kSub);
         __builtin_amdgcn_sched_barrier(0);     // every use of the records before their reload
-        fetch(h0 + team + T);
+        fetch();
         __syncthreads();
         int t = h0, half = 0;
         for (; t + T < h1; t += T, half ^= 1) {
             put(raw, meta, ent, ~0u, buf + ((half ^ 1) * S + mine) * kSub);
             __builtin_amdgcn_sched_barrier(0);
-            fetch(t + team + 2 * T);
+            fetch();
             if (rows_here) {
 #pragma unroll 1
-                for (int u = 0; u < S; u += U) sub_attend<U, false>(buf + (half * S + u) * kSub, q, 0u, lane, st);
+                for (int u = 0; u < S; u += U) sub_attend<U>(buf + (half * S + u) * kSub, q, lane, st);
             }
             __syncthreads();
         }
         if (t + team < h1 && rows_here) {
 #pragma unroll 1
-            for (int u = 0; u < S; u += U) sub_attend<U, false>(buf + (half * S + u) * kSub, q, 0u, lane, st);
+            for (int u = 0; u < S; u += U) sub_attend<U>(buf + (half * S + u) * kSub, q, lane, st);
         }
         __syncthreads();
     }
@@ -859,7 +926,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_many(TreeArgs A) {
             for (int u = 0; u < S; u++) {
                 const Sub sb = sub_of<S>(A, tile, u, P.len, P.start);
                 if (!sb.word) continue;
-                sub_attend<1, true>(buf + u * kSub, q, sb.kind == 2 ? sb.word & s_vis[node][sb.t >> 5] : sb.word, lane, st);
+                sub_masked(buf + u * kSub, q, sb.kind == 2 ? sb.word & s_vis[node][sb.t >> 5] : sb.word, lane, st);
             }
         }
         __syncthreads();
