@@ -242,10 +242,11 @@ __device__ __forceinline__ void step(Walk& w, uint32_t blocks) {   // stays at t
 __device__ __forceinline__ void load_walk(const Walk& w, const Lay& y, Raw& d) {
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-        d.a[j] = at32<uint4>(w.a, (y.hi[j] * 256 + y.rec[j]) * 4);
-        d.b[j] = at32<uint32_t>(w.b, y.hi[j] * 256 + y.rec[j]);
-        d.s[j] = at32<uint2>(w.s, (y.hi[j] * kRB + (y.rec[j] & 15)) * 2);
-        d.mask[j] = at32<uint2>(w.m, (y.hi[j] * 4 + (y.rec[j] >> 6)) * 8);
+        const uint32_t blk = y.hi[j];
+        d.a[j] = at32<uint4>(w.a, (blk * 256 + y.rec[j]) * 4);
+        d.b[j] = at32<uint32_t>(w.b, blk * 256 + y.rec[j]);
+        d.s[j] = at32<uint2>(w.s, (blk * kRB + (y.rec[j] & 15)) * 2);
+        d.mask[j] = at32<uint2>(w.m, (blk * 4 + (y.rec[j] >> 6)) * 8);
     }
 }
 __device__ __forceinline__ Meta load_meta(const Walk& w, uint32_t lane) {
@@ -339,16 +340,18 @@ __device__ __forceinline__ void patch_lds(bool isk, const lq_resident& r, const 
     for (uint32_t r0 = 0; r0 < most; r0 += 32) {
         if (r0) ent = load_entry(r, {m.base + r0, m.count > r0 ? m.count - r0 : 0u}, lane);
         wave_lds_sync();
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t e = rank[j] + __builtin_popcount(own[j] & ((1u << i) - 1u)) - r0;
-                const uint32_t sw = i < 2 ? d.s[j].x : d.s[j].y;
-                if (((own[j] >> i) & 1u) && e < 32u)   // scale, token of the 32, vector
-                    place[32 * y.hi[j] + e] = (i & 1 ? sw & 0xffff0000u : sw << 16) |
-                                              ((16 * y.hi[j] + (y.rec[j] & 15) + i) << 4) | (y.rec[j] >> 4);
-            }
+#pragma unroll 1
+        for (uint32_t left = own[0] | (own[1] << 4); __any(left != 0u);) {   // a lane rarely has more than one
+            const uint32_t b = (uint32_t)__ffs((int)left) - 1u, j = b >> 2, i = b & 3u;   // (none: b is 2^32 - 1, nothing is written)
+            const uint32_t o = j ? own[1] : own[0], e = (j ? rank[1] : rank[0]) + __builtin_popcount(o & ((1u << i) - 1u)) - r0;
+            const uint2 s2 = j ? d.s[1] : d.s[0];
+            const uint32_t sw = i < 2 ? s2.x : s2.y;
+            if (left && e < 32u)   // scale, token of the 32, vector
+                place[32 * (j ? y.hi[1] : y.hi[0]) + e] =
+                    (i & 1 ? sw & 0xffff0000u : sw << 16) |
+                    ((16 * (j ? y.hi[1] : y.hi[0]) + ((j ? y.rec[1] : y.rec[0]) & 15) + i) << 4) | ((j ? y.rec[1] : y.rec[0]) >> 4);
+            left &= left - 1u;
+        }
         wave_lds_sync();
         const uint32_t e = r0 + (lane & 31);
         if (e < m.count && (int64_t)m.base + e < r.exc_cap) {
