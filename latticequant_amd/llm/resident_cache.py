@@ -102,6 +102,7 @@ class ResidentKVCache(DynamicCache):
                 r.reserve(max(2 * r.cap_blocks * RB, r.n_tokens + n))
             r.append(x, s32[i], s16[i])
         self.chunks[layer_idx].append((_AtRest(pend, 0), _AtRest(pend, 1)))
+        self._room.pop(layer_idx, None)
         self.tail_k[layer_idx] = tk[:, :, n:].contiguous()
         self.tail_v[layer_idx] = tv[:, :, n:].contiguous()
 
@@ -115,6 +116,7 @@ class ResidentKVCache(DynamicCache):
                 raise ValueError("the forward's tokens are not the drafted nodes: verify() or discard() the draft first")
             self._drafts[layer_idx] = (key_states, value_states)
             return self._marked(key_states, value_states, layer_idx)
+        self._room.pop(layer_idx, None)
         if self.tail_k[layer_idx] is None:
             self.tail_k[layer_idx] = key_states.contiguous()
             self.tail_v[layer_idx] = value_states.contiguous()
@@ -242,7 +244,8 @@ class ResidentKVCache(DynamicCache):
         return accepted, nxt[:, None]
 
     def accept(self, path: torch.Tensor) -> None:
-        """End the draft with the nodes path (B, A), whole numbers, in the cache."""
+        """End the draft with the nodes path (B, A), whole numbers (clamped to the nodes), in
+        the cache."""
         if self._parents is None or len(self._drafts) != len(self.tail_k):
             raise ValueError("no drafted forward to accept")
         B, N = self._parents.shape
@@ -250,7 +253,7 @@ class ResidentKVCache(DynamicCache):
             raise ValueError("path must be (B, A), 1 <= A <= nodes")
         A, dev = path.shape[1], self._parents.device
         full = torch.full((B, N), -1, dtype=torch.int32, device=dev)
-        full[:, :A] = path
+        full[:, :A] = path.clamp(0, N - 1)
         groups = {}                                # layers of one shape, type and tail length: all of them, as a rule
         for i in range(len(self.tail_k)):
             t = self.tail_k[i].shape[2]
@@ -277,7 +280,7 @@ class ResidentKVCache(DynamicCache):
         """The layer's tails as the first tokens of buffers with room for `need`."""
         tk, tv = self.tail_k[layer_idx], self.tail_v[layer_idx]
         buf = self._room.get(layer_idx)
-        if buf is None or buf[0].data_ptr() != tk.data_ptr() or buf[0].shape[2] < need:
+        if buf is None or buf[0].shape[2] < need:
             B, H, t, hd = tk.shape
             buf = tuple(torch.empty((B, H, need + 64, hd), dtype=x.dtype, device=x.device) for x in (tk, tv))
             for b, x in zip(buf, (tk, tv)):
@@ -287,13 +290,14 @@ class ResidentKVCache(DynamicCache):
 
     # -- beams --------------------------------------------------------------
     def reorder_cache(self, beam_idx: torch.Tensor) -> None:
-        """Sequence i becomes sequence beam_idx[i] as it was, in place."""
+        """Sequence i becomes sequence beam_idx[i] as it was, in place (-1: the last one;
+        what is out of range is clamped)."""
         if not self.tail_k:
             return
         if beam_idx.dim() != 1 or beam_idx.numel() != self.tail_k[0].shape[0] or beam_idx.numel() > MAX_REORDER:
             return self.batch_select_indices(beam_idx)
         self._no_draft()
-        idx = beam_idx.to(self.tail_k[0].device)
+        idx = self._numbers(beam_idx)
         by_length = {}
         for r in self.res_k + self.res_v:
             if r is not None:
@@ -304,7 +308,8 @@ class ResidentKVCache(DynamicCache):
 
     def batch_select_indices(self, indices: torch.Tensor) -> None:
         """Keep the sequences indices[r], in that order (a sequence may stand several
-        times); the others' resident blocks and exceptions are freed."""
+        times; -1 is the last one, what is out of range is clamped); the others' resident
+        blocks and exceptions are freed."""
         if not self.tail_k:
             return
         self._no_draft()
@@ -312,7 +317,7 @@ class ResidentKVCache(DynamicCache):
         idx = torch.arange(B)[indices.cpu()] if indices.dtype == torch.bool else indices
         if idx.dim() != 1 or idx.numel() < 1:
             raise ValueError("indices must be a list of sequences")
-        idx = idx.to(self.tail_k[0].device)
+        idx = self._numbers(idx)
         for res in (self.res_k, self.res_v):
             for i, r in enumerate(res):
                 if r is not None:
@@ -327,6 +332,14 @@ class ResidentKVCache(DynamicCache):
     def _no_draft(self):
         if self._parents is not None:
             raise ValueError("a draft is pending: verify() or discard() it first")
+
+    def _numbers(self, idx: torch.Tensor) -> torch.Tensor:
+        """Sequence numbers as the prefixes, the tails and the chunks all read them."""
+        if idx.dtype not in (torch.int32, torch.int64):
+            raise ValueError("sequence numbers must be int32 or int64")
+        B = self.tail_k[0].shape[0]
+        idx = idx.to(self.tail_k[0].device)
+        return torch.where(idx < 0, idx + B, idx).clamp(0, B - 1)
 
     def _select_rest(self, idx):
         """Tails and at-rest chunks of the sequences idx."""

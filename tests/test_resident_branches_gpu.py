@@ -227,6 +227,47 @@ def test_reorder_leaves_callers_tensors_gpu():
 
 
 @gpu
+@pytest.mark.parametrize("tail", [0, 128])
+def test_sequence_numbers_beyond_the_batch_gpu(tail):
+    """Negative numbers count from the end and others are clamped, in the prefix, the tail
+    and the chunks alike."""
+    for how in ("reorder_cache", "batch_select_indices"):
+        c = _filled(3, layers=1, tail=tail)
+        ref = [x.clone() for x in c.materialise(0)]
+        getattr(c, how)(torch.tensor([-1, 7, 0]))
+        for x, y in zip(c.materialise(0), ref):
+            assert torch.equal(x, y[[2, 2, 0]]), how
+        assert all(e.rows.tolist() == [2, 2, 0] for pair in c.chunks[0] for e in pair)
+        with pytest.raises(ValueError):
+            getattr(c, how)(torch.tensor([0.0, 1.0, 2.0]))
+
+
+@gpu
+def test_accept_keeps_within_the_nodes_and_the_buffers_gpu():
+    """A path's numbers are clamped to the nodes; the tails' buffers are the tails' own
+    after a step or a flush in between."""
+    c = _filled(2, layers=2, tail=64, tokens=20)
+    want = [[x.clone() for x in c.materialise(i)] for i in range(2)]
+    g = torch.Generator().manual_seed(5)
+    for path, between in (([[0, 9], [-3, 1]], True), ([[0, 2], [0, 1]], True), ([[0, 1, 2], [0, 1, 2]], False)):
+        c.draft([-1, 0, 1])
+        d = [[torch.randn(2, 2, 3, 128, generator=g).half().cuda() for _ in range(2)] for _ in range(2)]
+        for i in range(2):
+            c.update(*d[i], i)
+        c.accept(torch.tensor(path, device="cuda"))
+        at = torch.tensor(path).clamp(0, 2).cuda()[:, None, :, None].expand(-1, 2, -1, 128)
+        for i in range(2):
+            want[i] = [torch.cat([w, x.gather(2, at)], 2) for w, x in zip(want[i], d[i])]
+        if between:
+            one = torch.randn(2, 2, 1, 128, generator=g).half().cuda()
+            for i in range(2):
+                c.update(one, one, i)
+                want[i] = [torch.cat([w, one], 2) for w in want[i]]
+        for i in range(2):
+            assert all(torch.equal(x, w) for x, w in zip(c.materialise(i), want[i]))
+
+
+@gpu
 def test_generate_with_beams_gpu():
     """HF's beam search over the cache: with nothing flushed the cache holds the model's own
     fp16 K / V, and the beams found are as likely as DynamicCache's (the same up to a near
