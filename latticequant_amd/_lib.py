@@ -199,7 +199,7 @@ def raw_stream(device) -> int:
 
 def on_device(device):
     """Context in which `device` (with an index) is current."""
-    return _HERE_ALREADY if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE_ALREADY if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 _HERE_ALREADY = contextlib.nullcontext()

@@ -195,13 +195,19 @@ __global__ __launch_bounds__(256) void k_gather(RowMoves M, RowShape S, int64_t 
         *reinterpret_cast<const uint4*>(M.src[blockIdx.y] + b * S.sb + h * S.sh + t * S.st + 16 * u);
 }
 
-bool moves_ok(void* const* dst, const void* const* src, int64_t n, RowMoves* m) {
-    for (int64_t i = 0; i < n; i++) {
+bool pointers_ok(void* const* dst, const void* const* src, int64_t n) {
+    for (int64_t i = 0; i < n; i++)
         if (!dst[i] || !src[i] || ((uintptr_t)dst[i] | (uintptr_t)src[i]) & 15) return false;
-        m->dst[i] = static_cast<char*>(dst[i]);
-        m->src[i] = static_cast<const char*>(src[i]);
-    }
     return true;
+}
+
+RowMoves moves_of(void* const* dst, const void* const* src, int64_t n) {
+    RowMoves m{};
+    for (int64_t i = 0; i < n; i++) {
+        m.dst[i] = static_cast<char*>(dst[i]);
+        m.src[i] = static_cast<const char*>(src[i]);
+    }
+    return m;
 }
 
 // -------------------------------------------------------- resident blocks --
@@ -428,7 +434,8 @@ __global__ __launch_bounds__(256) void k_select_exc(const uint4* __restrict__ sr
 }
 
 bool res_planes_ok(const lq_resident* r) {
-    return r && r->a && r->b && r->mask && r->meta && r->scale && r->n_heads > 0 && r->cap_blocks > 0;
+    return r && r->a && r->b && r->mask && r->meta && r->scale && r->n_heads > 0 && r->cap_blocks > 0 &&
+           (((uintptr_t)r->a | (uintptr_t)r->b | (uintptr_t)r->mask | (uintptr_t)r->meta | (uintptr_t)r->scale) & 15) == 0;
 }
 
 bool choice_of(const lq_resident* src, const lq_resident* dst, int64_t n_seq, int64_t src_blocks, const int32_t* index,
@@ -500,11 +507,10 @@ int lq_append_rows(void *const *h_dst, const void *const *h_src, int64_t n, cons
     for (int i = 0; i < 3; i++)
         if (h_dst_stride[i] % 16 || h_src_stride[i] % 16) return LQ_ERR_ARG;
     const int64_t grid = (n_seq * heads * slots * S.units + 255) / 256;
-    if (grid > INT_MAX) return LQ_ERR_ARG;
+    if (grid > INT_MAX || !pointers_ok(h_dst, h_src, n)) return LQ_ERR_ARG;
     for (int64_t i = 0; i < n; i += kPairs) {
-        RowMoves m;
         const int64_t k = n - i < kPairs ? n - i : kPairs;
-        if (!moves_ok(h_dst + i, h_src + i, k, &m)) return LQ_ERR_ARG;
+        const RowMoves m = moves_of(h_dst + i, h_src + i, k);
         hipLaunchKernelGGL(k_append, dim3((unsigned)grid, (unsigned)k), dim3(256), 0, s, m, S, slots, d_path, d_count,
                            d_len, d_new_len);
     }
@@ -522,11 +528,10 @@ int lq_gather_rows(void *const *h_dst, const void *const *h_src, int64_t n, cons
     for (int i = 0; i < 3; i++)
         if (h_dst_stride[i] % 16 || h_src_stride[i] % 16) return LQ_ERR_ARG;
     const int64_t grid = (n_out * heads * rows * S.units + 255) / 256;
-    if (grid > INT_MAX) return LQ_ERR_ARG;
+    if (grid > INT_MAX || !pointers_ok(h_dst, h_src, n)) return LQ_ERR_ARG;
     for (int64_t i = 0; i < n; i += kPairs) {
-        RowMoves m;
         const int64_t k = n - i < kPairs ? n - i : kPairs;
-        if (!moves_ok(h_dst + i, h_src + i, k, &m)) return LQ_ERR_ARG;
+        const RowMoves m = moves_of(h_dst + i, h_src + i, k);
         hipLaunchKernelGGL(k_gather, dim3((unsigned)grid, (unsigned)k), dim3(256), 0, s, m, S, n_src, d_index);
     }
     return launch_status();

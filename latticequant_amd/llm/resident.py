@@ -216,11 +216,11 @@ class ResidentKV:
         if L.debug_checks() and (bool((index < 0).any()) or bool((index >= n_seq).any()) or
                                  (blocks is not None and nb and (bool((blocks < 0).any()) or bool((blocks >= used).any())))):
             raise ValueError("sequence or block out of range")
-        new = ResidentKV._bare(R * (self.n_heads // n_seq), cap, dev)
+        new = self._bare(R * (self.n_heads // n_seq), cap)
         if nb == 0:
             new.n_exc.zero_()
             new.status.zero_()
-            new.exc = torch.empty(8, dtype=torch.int16, device=dev)
+            new.exc = self.exc.new_empty(8)
             return new
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a selection reads its exception count back: not while a graph is captured")
@@ -232,28 +232,28 @@ class ResidentKV:
         with L.on_device(dev):
             idx = index.to(device=dev, dtype=torch.int32).contiguous()
             blk = None if blocks is None else blocks.to(device=dev, dtype=torch.int32).contiguous()
-            work = torch.empty(need, dtype=torch.uint8, device=dev)
+            work = idx.new_empty(need + 3 >> 2)
             dst, stream = new.struct(), L.raw_stream(dev)
             args = (ctypes.addressof(self.struct()), n_seq, used, idx.data_ptr(), R, L.ptr(blk), nb, ctypes.addressof(dst))
             L.check(lib.lq_resident_select(*args, work.data_ptr(), need, ctypes.addressof(total), stream),
                     "lq_resident_select")
             n = total.value
-            new.exc = torch.empty(max(1, n) * 8, dtype=torch.int16, device=dev)
+            new.exc = self.exc.new_empty(max(1, n) * 8)
             dst.exc, dst.exc_cap = new.exc.data_ptr(), max(1, n)
             if n:
                 L.check(lib.lq_resident_select_exceptions(*args, stream), "lq_resident_select_exceptions")
         new._exc_known, new.n_tokens = n, nb * RB
         return new
 
-    @classmethod
-    def _bare(cls, n_heads: int, nb: int, dev) -> "ResidentKV":
-        """nb blocks of room per head, everything uninitialised (counters too)."""
-        r = cls.__new__(cls)
-        r.device, r.n_heads, r.cap_blocks = dev, n_heads, nb
-        for name, per, dt in (("a", 256, torch.int32), ("b", 256, torch.uint8), ("mask", 4, torch.int64),
-                              ("meta", 4, torch.int32), ("scale", RB, torch.float16)):
-            setattr(r, name, torch.empty(n_heads * nb * per, dtype=dt, device=dev))
-        r.n_exc, r.status = torch.empty((2, 1), dtype=torch.int32, device=dev).unbind(0)
+    def _bare(self, n_heads: int, nb: int) -> "ResidentKV":
+        """nb blocks of room per head where this prefix lies, everything uninitialised
+        (counters too)."""
+        r = ResidentKV.__new__(ResidentKV)
+        r.device, r.n_heads, r.cap_blocks = self.a.device, n_heads, nb
+        n = n_heads * nb
+        r.a, r.b, r.mask = self.a.new_empty(n * 256), self.b.new_empty(n * 256), self.mask.new_empty(n * 4)
+        r.meta, r.scale = self.meta.new_empty(n * 4), self.scale.new_empty(n * RB)
+        r.n_exc, r.status = self.n_exc.new_empty(1), self.status.new_empty(1)
         r.exc = r.scale.view(torch.int16)[:8]   # no entry yet
         r.n_tokens = r._exc_known = r._exc_since = 0
         r._exc_read = r._st = None

@@ -17,7 +17,8 @@ from __future__ import annotations
 
 import ctypes
 from array import array
-from operator import attrgetter
+from functools import reduce
+from operator import attrgetter, or_
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -161,14 +162,15 @@ def resident_tree_attention(k: ResidentKV, v: ResidentKV, q: torch.Tensor, draft
         elif work.device != dev or not work.is_contiguous():
             raise ValueError("the attention workspace must be contiguous, on the resident prefix's device")
         if out is None:
-            out = torch.empty(q.shape, dtype=dt, device=dev)
-        keep, flat = [], array("q")            # the copies stay until the launch; six lq_rows
+            out = q.new_empty(q.shape)
+        keep, flat = [], []                    # the copies stay until the launch; six lq_rows
         for t in given:
             t, r = _rows(t)
             keep.append(t)
-            flat.extend(r)
-        flat.extend((out.data_ptr(),) + out.stride()[:3])
-        at = flat.buffer_info()[0]
+            flat += r
+        flat += (out.data_ptr(),) + out.stride()[:3]
+        rows = array("q", flat)
+        at = rows.buffer_info()[0]
         rc = lib.lq_resident_tree_attention(
             ctypes.addressof(k.struct()), ctypes.addressof(v.struct()), tp, at, at + 32, at + 64, par.data_ptr(), B, N,
             Hq // Hkv, at + 96 if cap else None, at + 128 if cap else None, cap, None if tl is None else tl.data_ptr(),
@@ -223,7 +225,7 @@ def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, logits: Optional[
                 nbytes = lib.lq_accept_workspace(B, N, vocab)
                 if nbytes < 0:
                     raise ValueError("too many nodes (65535 in all) or too large a vocabulary")
-                work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+                work = tokens.new_empty(nbytes + 7 >> 3)
             elif work.device != dev or not work.is_contiguous():
                 raise ValueError("the acceptance workspace must be contiguous, on the tokens' device")
             else:
@@ -231,9 +233,7 @@ def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, logits: Optional[
         else:
             choice = choice.contiguous()
         par, tok = _parents(parents, B, N, dev), tokens.contiguous()
-        path = torch.empty((B, N), dtype=torch.int32, device=dev)
-        count = torch.empty(B, dtype=torch.int32, device=dev)
-        nxt = torch.empty(B, dtype=torch.int64, device=dev)
+        path, count, nxt = par.new_empty((B, N)), par.new_empty(B), tokens.new_empty(B)
         rc = lib.lq_accept_drafts(None if logits is None else logits.data_ptr(), dt, sb, sn, vocab, L.ptr(choice),
                                   tok.data_ptr(), par.data_ptr(), B, N, None if logits is None else work.data_ptr(),
                                   nbytes, path.data_ptr(), count.data_ptr(), nxt.data_ptr(), L.raw_stream(dev))
@@ -278,21 +278,24 @@ def _pairs(dst: Sequence[torch.Tensor], src: Sequence[torch.Tensor], what: str):
     dt, st = list(map(_stride, dst)), list(map(_stride, src))
     dp, sp = list(map(_data_ptr, dst)), list(map(_data_ptr, src))
     if (not all(fits(t) and not any(x == 0 and n > 1 for x, n in zip(t, ds)) for t in set(dt)) or
-            any(p & 15 for p in dp)):
+            reduce(or_, dp) & 15 or len(set(dp)) < len(dp)):
         raise ValueError(f"{what}: destination rows must be contiguous, apart and 16-byte aligned")
     src = list(src)
-    if not all(map(fits, set(st))) or any(p & 15 for p in sp):
+    if not all(map(fits, set(st))) or reduce(or_, sp) & 15:
         for i, t in enumerate(src):
             if not fits(st[i]) or sp[i] & 15:
                 src[i] = t.contiguous()
                 st[i], sp[i] = src[i].stride(), src[i].data_ptr()
-    kinds = set(zip(dt, st))
-    out = []
-    for kind in kinds:
-        at = range(len(dst)) if len(kinds) == 1 else [i for i in range(len(dst)) if (dt[i], st[i]) == kind]
-        out.append((len(at), array("Q", (dp[i] for i in at)), array("Q", (sp[i] for i in at)),
-                    array("q", (x * el for x in kind[0][:3])), array("q", (x * el for x in kind[1][:3])), src))
-    return out
+
+    def group(td, ts, d, s):
+        return (len(d), array("Q", d), array("Q", s), array("q", [x * el for x in td[:3]]),
+                array("q", [x * el for x in ts[:3]]), src)
+    n = len(dst)
+    if dt.count(dt[0]) == n and st.count(st[0]) == n:
+        return [group(dt[0], st[0], dp, sp)]
+    kinds = list(zip(dt, st))
+    return [group(*kind, [p for p, x in zip(dp, kinds) if x == kind], [p for p, x in zip(sp, kinds) if x == kind])
+            for kind in dict.fromkeys(kinds)]
 
 
 def _addresses(group):
@@ -307,7 +310,7 @@ def append_accepted(tails: Sequence[torch.Tensor], drafts: Sequence[torch.Tensor
     (B, H, cap, width) becomes row path[b][j] of its draft (B, H, N, width), j < count[b];
     the other rows stay.  tails / drafts: lists (K and V of all layers: one launch per
     128 of one layout); path (B, N), count and tail_len (B,) as accept_drafts and the
-    tails have them.  Returns the new lengths (B,) int32, tail_len + count.  The caller
+    tails have them.  No draft may lie in a tail.  Returns the new lengths (B,) int32, tail_len + count.  The caller
     keeps cap >= tail_len + count: rows past cap are left out (the length stops there)."""
     lib = L.lib()
     groups = _pairs(tails, drafts, "append_accepted")
@@ -320,7 +323,7 @@ def append_accepted(tails: Sequence[torch.Tensor], drafts: Sequence[torch.Tensor
         ln = _ints(tail_len, (B,), "tail_len", dev)
         if L.debug_checks() and (bool((ln + ct > cap).any()) or bool((ct > N).any())):
             raise ValueError("accepted rows do not fit the tails")
-        new = torch.empty(B, dtype=torch.int32, device=dev)
+        new = ln.new_empty(B)
         for g in groups:
             L.check(lib.lq_append_rows(*_addresses(g), B, H, cap, N, width * tails[0].element_size(), pt.data_ptr(),
                                        ct.data_ptr(), ln.data_ptr(), new.data_ptr(), L.raw_stream(dev)),

@@ -203,6 +203,17 @@ def test_row_moves_refusals_gpu():
             gather_tails(*a)
 
 
+@gpu
+def test_a_tail_twice_is_refused_gpu():
+    """Two drafts of one tail would be written in no order."""
+    from latticequant_amd.llm.tree import append_accepted
+    t = torch.zeros(1, 1, 8, 128, dtype=torch.float16, device="cuda")
+    d, n = t[:, :, :2].contiguous(), torch.ones(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        append_accepted([t, t], [d, d + 1], torch.zeros(1, 2, dtype=torch.int32, device="cuda"), n, n)
+    assert not t.any()
+
+
 def _prefix(B, H, T, seed):
     from latticequant_amd import codec
     from latticequant_amd.llm.resident import ResidentKV
