@@ -27,6 +27,7 @@
 // Decoding 32 tokens of K and V is about 430 VALU instructions, a column's softmax 60
 // (16 rows) or 110 (32 rows) and its 16 MFMA 256 or 512 cycles: with few rows the
 // decode bounds the loop and sharing it through LDS costs more than it saves.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -1228,43 +1229,66 @@ struct Plan {
     int c, rb, np, nt, nd, nsp, per;
 };
 
-// Waves of a team: as many 32-row columns as there are rows, four at most (their
-// O is 64 registers each).  A split's share is whole rounds of its teams' tiles; of the
-// shares, the one whose longest CU takes the least: a round counts 2, a workgroup's
-// prologue and join 3, a further round of the draft's tiles 1; of equals the fewest splits
-// (records are written and read again).
+// Waves of a team (c): as many 32-row columns as there are rows, eight at most (their O is
+// 64 registers each), so that a tile is decoded once for all of them.  Where little is to
+// be read, decoding it for two halves of the rows on twice the CUs is faster: a round is
+// 128 tokens in all three forms, and takes 5 us (c = 8, beside 16 us before and after the
+// rounds), 3.7 us (4, beside 11 us).  Measured, one sequence of 8 heads with a tail of
+// 100, 256 rows a head: 8192 tokens (2 rounds a CU with c = 8) 38.0 us with c = 8, 35.8
+// with 4; 16384 tokens 47.7 / 47.3; 32768 tokens (8 rounds) 67 / 75.  128 rows: 4096
+// tokens (1 round with c = 4) 25.6 us with c = 4, 23.7 with 2; 16384 (4 rounds) 34.8 / 38.6.
+constexpr int64_t kRounds8 = 3, kRounds4 = 2;
+// Costs of the choice of splits, in units of half a round: a round over whole prefix
+// tiles, one over the others (the tail's, the draft's, the prefix's last), and a
+// workgroup's prologue and join.  A split's share is whole rounds of its teams' tiles; of
+// the splits whose longest CU takes the least the fewest (records are written and read
+// again).  The last one has the draft and whatever the equal shares leave: a share more
+// for the draft alone is often the best (one head of 16384 tokens, 64 rows: 17.6 us;
+// 20.1 with the draft beside a full share).
+constexpr uint32_t kHotCost = 2, kEdgeCost = 2, kFixedCost = 3;
 bool plan(int64_t n_seq, int64_t heads, int64_t nodes, int64_t group, int64_t t_prefix, int64_t tail_cap, Plan* p) {
     if (n_seq < 1 || heads < 1 || nodes < 1 || nodes > kMaxNodes || group < 1 || group > 16 || t_prefix < 0 ||
         t_prefix % kRB || tail_cap < 0 || t_prefix > INT_MAX / 2 || tail_cap > INT_MAX / 4)
         return false;
     const int64_t rows = nodes * group;
     p->c = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;   // 1: k_tree_few
-    const int64_t s = p->c > 1 ? p->c / 2 : 1, teams = kWaves / p->c, tt = 32 * s;
-    p->rb = (int)((rows + 32 * p->c - 1) / (32 * p->c));
+    const auto blocks = [=](int c) { return (rows + 32 * c - 1) / (32 * c); };
+    const auto rounds_a_cu = [=](int c) { return n_seq * heads * blocks(c) * ((t_prefix + tail_cap + 127) / 128) / 256; };
+    if (n_seq > INT_MAX / heads) return false;
+    if (p->c == 8 && rounds_a_cu(8) <= kRounds8) p->c = 4;
+    if (p->c == 4 && rounds_a_cu(4) <= kRounds4) p->c = 2;
+    const int64_t s = p->c > 1 ? p->c / 2 : 1, tt = 32 * s;
+    p->rb = (int)blocks(p->c);
     p->np = (int)((t_prefix + tt - 1) / tt);
     p->nt = (int)((tail_cap + tt - 1) / tt);
     p->nd = (int)((nodes + tt - 1) / tt);
     const int64_t base = n_seq * heads * p->rb;
     if (base > INT_MAX / 256) return false;
-    const int64_t cache = p->np + p->nt;
+    const int lg = p->c > 1 ? (p->c == 8 ? 0 : p->c == 4 ? 1 : 2) : 3;   // teams = 1 << lg
+    const auto rounds_of = [lg](uint32_t n) { return (n + (1u << lg) - 1) >> lg; };
+    const uint32_t np = (uint32_t)p->np, cache = np + (uint32_t)p->nt, tiles = cache + (uint32_t)p->nd, whole = (uint32_t)(t_prefix / tt);
     int64_t best = -1;
-    for (int64_t rounds = (cache + teams - 1) / teams; ; ) {
-        const int64_t per = (rounds > 0 ? rounds : 1) * teams, n = cache > 0 ? (cache + per - 1) / per : 1;
-        if (n > 256) break;
-        // the last split has the draft's tiles beside its share
-        const int64_t last = (cache - (n - 1) * per + p->nd + teams - 1) / teams;
-        const int64_t cost = ((base * n + 255) / 256) * (2 * rounds + 3) + (last > rounds ? last - rounds : 0);
-        if (best < 0 || cost < best) {
-            best = cost;
-            p->nsp = (int)n;
-            p->per = (int)per;
+    const uint32_t most = (uint32_t)std::min<int64_t>(256, std::max<int64_t>(4, 512 / base));
+    for (uint32_t n = 1; n <= most && (n == 1 || n <= tiles); n++) {
+        // n splits share the prefix, the cache or all tiles in equal parts; the last takes what is left
+        const uint32_t of[3] = {np, cache, tiles};
+        uint32_t was = 0;
+        for (uint32_t x : of) {
+            const uint32_t rounds = std::max(rounds_of((x + n - 1) / n), 1u);
+            if (rounds == was) continue;
+            was = rounds;
+            const uint32_t first = std::min<uint64_t>((uint64_t)(n - 1) * rounds << lg, cache), hot = whole > first ? whole - first : 0u;
+            const uint32_t last = kHotCost * rounds_of(hot) + kEdgeCost * rounds_of(tiles - first - hot);
+            const int64_t cost = (base * n + 255) / 256 * (int64_t)(kHotCost * rounds + kFixedCost) +
+                                 (last > kHotCost * rounds ? last - kHotCost * rounds : 0u);
+            if (best < 0 || cost < best) {
+                best = cost;
+                p->nsp = (int)n;
+                p->per = (int)(rounds << lg);
+            }
         }
-        if (rounds <= 1) break;
-        // the next smaller share that changes the number of splits
-        const int64_t next = (cache + (n + 1) * teams - 1) / ((n + 1) * teams);
-        rounds = next < rounds ? next : rounds - 1;
     }
-    return best >= 0;
+    return true;
 }
 
 bool tree_res_ok(const lq_resident* r) {
