@@ -18,7 +18,7 @@
 //                   8 (lane / 16) .. + 7 of the B operand: P never leaves its lane.
 //                   MFMA mm's row n is dimension 8 n + mm, the order in which a lane has
 //                   the eight dimensions of a decoded vector
-// k_tree_many, more rows: two or four waves (a team) hold 32 rows each and share their
+// k_tree_many, more rows: two, four or eight waves (a team) hold 32 rows each and share their
 // tokens: a tile is decoded once into LDS, K as rows, V with its dimensions as rows.
 //   S^T = K Q^T     8 MFMA 32x32x16 per 32 tokens, K's row m is token
 //                   16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4: a lane's scores are
@@ -172,19 +172,27 @@ __device__ __forceinline__ T at32(const void* base, uint32_t bytes) {
 }
 
 // Exceptions (vectors outside the 5-bit range): a block's entries lie in record order
-// from its base, so an entry's number is the base plus the set bits of the block's
-// masks before it.  The first 32 of both blocks are loaded with the tile, one a lane
-// (lanes 0..31 of the first block's, 32..63 of the second's), from the bases and counts
-// of a tile further on: taken when the masks are known, their latency would stand in
-// every tile that has one (with outlier channels all of them: 32768 tokens, 16 rows a
-// head, 5.6 % of K's vectors: 41 us against 32 without any, at first).
+// from its base.  The first 32 of both blocks are loaded with the tile, one a lane (lanes
+// 0..31 of the first block's, 32..63 of the second's), from the bases and counts of a tile
+// further on: taken when the masks are known, their latency would stand in every tile that
+// has one (with outlier channels all of them: 32768 tokens, 16 rows a head, 5.6 % of K's
+// vectors, 9 us more).  A tile's cost is that of writing them over the decoded values
+// (25.3 us without any, 27.3 with one vector in 1200, 30.9 with outlier channels).
 struct Meta {
-    uint32_t base, count;   // of the lane's half
+    uint32_t h0, h1, base, count;   // of the lane's half
 };
 __device__ __forceinline__ Meta load_meta(const lq_resident& r, int64_t hd, int64_t t, int64_t T, uint32_t lane) {
     const Blocks B = blocks_of(r, hd, t, T);
-    const uint2 w = at32<uint2>(r.meta + B.rb0 * 4 + 2, ((lane >> 5) & B.d) * 16);
-    return {w.x, w.y};
+    const uint4 w = at32<uint4>(r.meta + B.rb0 * 4, ((lane >> 5) & B.d) * 16);
+    return {w.x, w.y, w.z, w.w};
+}
+// the record of the lane's entry as the block's header has it: of the first seven
+__device__ __forceinline__ uint32_t head_rec(const Meta& m, uint32_t lane) {
+    return (uint32_t)(((((uint64_t)m.h1 << 32) | m.h0) >> 8) >> (8 * (lane & 7))) & 255u;
+}
+// exceptions of the block that has more; wave-uniform
+__device__ __forceinline__ uint32_t most_of(const Meta& m) {
+    return max((uint32_t)__builtin_amdgcn_readlane((int)m.count, 0), (uint32_t)__builtin_amdgcn_readlane((int)m.count, 32));
 }
 __device__ __forceinline__ uint4 load_entry(const lq_resident& r, const Meta& m, uint32_t lane) {
     const uint32_t e = lane & 31;
@@ -229,7 +237,7 @@ struct Walk {
 __device__ __forceinline__ Walk walk_of(const lq_resident& r, int64_t block, uint32_t rounds) {
     return {reinterpret_cast<const char*>(r.a + block * 256), reinterpret_cast<const char*>(r.b + block * 256),
             reinterpret_cast<const char*>(r.scale + block * kRB), reinterpret_cast<const char*>(r.mask + block * 4),
-            reinterpret_cast<const char*>(r.meta + block * 4 + 2), rounds};
+            reinterpret_cast<const char*>(r.meta + block * 4), rounds};
 }
 __device__ __forceinline__ void step(Walk& w, uint32_t blocks) {   // stays at the last round
     const uint32_t n = w.left ? blocks : 0u;
@@ -251,8 +259,8 @@ __device__ __forceinline__ void load_walk(const Walk& w, const Lay& y, Raw& d) {
     }
 }
 __device__ __forceinline__ Meta load_meta(const Walk& w, uint32_t lane) {
-    const uint2 x = at32<uint2>(w.t, (lane >> 5) * 16);
-    return {x.x, x.y};
+    const uint4 x = at32<uint4>(w.t, (lane >> 5) * 16);
+    return {x.x, x.y, x.z, x.w};
 }
 __device__ __forceinline__ void load_raw(const lq_resident& r, int64_t hd, int64_t t, int64_t T, const Lay& y, Raw& d) {
     const Blocks B = blocks_of(r, hd, t, T);
@@ -302,18 +310,44 @@ __device__ __forceinline__ void scale_v(const Raw& d, uint32_t word, int lane, u
     if (word != ~0u) clear_v(word, lane >> 4, vp);
 }
 
-// How many exceptions stand before the lane's four records from rec[j] on in their block:
-// those of the record groups before (popcounts of the other lanes' masks) and in the group.
-__device__ __forceinline__ uint32_t rank_of(bool isk, const Raw& d, const Lay& y, int j, int lane) {
-    const uint64_t m = ((uint64_t)d.mask[j].y << 32) | d.mask[j].x;
-    const int pc = __builtin_popcountll(m), g = (int)(y.rec[j] >> 6);
-    uint32_t n = __builtin_popcountll(m & ((1ull << (y.rec[j] & 63)) - 1ull));
+// The record of number k among a block's exceptions (there are as many): the k-th set bit
+// of its masks m, found by halving.
+__device__ __forceinline__ uint32_t nth_record(const uint2 m[4], uint32_t k) {
+    uint2 w = m[0];
+    uint32_t at = 0u;
 #pragma unroll
-    for (int c = 0; c < 3; c++) {   // group c: K lane 16 c; V lane 4 c of the first block, 32 + 4 c of the second
-        const int lo = __builtin_amdgcn_readlane(pc, isk ? 16 * c : 4 * c), hi = __builtin_amdgcn_readlane(pc, isk ? 16 * c : 32 + 4 * c);
-        n += g > c ? (lane >> 5 ? hi : lo) : 0;
+    for (uint32_t c = 0; c < 3; c++) {
+        const uint32_t n = __builtin_popcount(w.x) + __builtin_popcount(w.y);
+        if (at == 64 * c && k >= n) {
+            k -= n;
+            w = m[c + 1];
+            at += 64u;
+        }
     }
-    return n;
+    const uint32_t n = __builtin_popcount(w.x);
+    const bool up = k >= n;
+    uint32_t x = up ? w.y : w.x;
+    k -= up ? n : 0u;
+    at += up ? 32u : 0u;
+#pragma unroll
+    for (uint32_t s = 16; s; s >>= 1) {
+        const uint32_t b = __builtin_popcount(x & ((1u << s) - 1u));
+        const bool over = k >= b;
+        x = over ? x >> s : x;
+        k -= over ? b : 0u;
+        at += over ? s : 0u;
+    }
+    return at;
+}
+// Masks of block lane / 32 of a tile: group c's in lane l0 + step c of the first register
+// for its first block, in lane l1 + step c of the second for its second
+__device__ __forceinline__ void half_masks(const uint2& a, int l0, const uint2& b, int l1, int step, int lane, uint2 m[4]) {
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const uint32_t x0 = (uint32_t)__builtin_amdgcn_readlane((int)a.x, l0 + step * c), y0 = (uint32_t)__builtin_amdgcn_readlane((int)a.y, l0 + step * c);
+        const uint32_t x1 = (uint32_t)__builtin_amdgcn_readlane((int)b.x, l1 + step * c), y1 = (uint32_t)__builtin_amdgcn_readlane((int)b.y, l1 + step * c);
+        m[c] = lane >> 5 ? make_uint2(x1, y1) : make_uint2(x0, y0);
+    }
 }
 
 __device__ __forceinline__ void wave_lds_sync() {
@@ -322,44 +356,45 @@ __device__ __forceinline__ void wave_lds_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// The exceptions of 32 tokens whose records are staged in LDS: a record's lane leaves its
-// place and scale for the lane that holds its entry (place: 64 words of the wave's own),
-// which writes the eight values over the staged ones.  Rounds of 32 entries a block;
-// `ent` has the first.
-__device__ __forceinline__ void patch_lds(bool isk, const lq_resident& r, const Raw& d, const Lay& y, const Meta& m, uint4 ent,
-                                          uint32_t word, int lane, uint32_t* place, char* lds) {
-    if (!__any(((d.mask[0].x | d.mask[0].y) | (d.mask[1].x | d.mask[1].y)) != 0u)) return;
-    uint32_t rank[2], own[2];
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-        const uint64_t mk = ((uint64_t)d.mask[j].y << 32) | d.mask[j].x;
-        rank[j] = rank_of(isk, d, y, j, lane);
-        own[j] = (uint32_t)(mk >> (y.rec[j] & 63)) & 15u;
-    }
-    const uint32_t most = max(__builtin_amdgcn_readlane((int)m.count, 0), __builtin_amdgcn_readlane((int)m.count, 32));
+// put(rec, e): the lane's entry (pairs e) over record rec of block lane / 32, for all
+// entries of a tile, a block's by rounds of 32; `ent` has the first.  Which record an entry
+// is stands in the block's header where neither block has more than seven, as most tiles.
+template <typename M, typename P>
+__device__ __forceinline__ void each_entry(const lq_resident& r, const Meta& m, uint4 ent, uint32_t most, int lane, M masks, P put) {
+    uint2 mk[4];
+    if (most > 7) masks(mk);
 #pragma unroll 1
     for (uint32_t r0 = 0; r0 < most; r0 += 32) {
-        if (r0) ent = load_entry(r, {m.base + r0, m.count > r0 ? m.count - r0 : 0u}, lane);
-        wave_lds_sync();
-#pragma unroll 1
-        for (uint32_t left = own[0] | (own[1] << 4); __any(left != 0u);) {   // a lane rarely has more than one
-            const uint32_t b = (uint32_t)__ffs((int)left) - 1u, j = b >> 2, i = b & 3u;   // (none: b is 2^32 - 1, nothing is written)
-            const uint32_t o = j ? own[1] : own[0], e = (j ? rank[1] : rank[0]) + __builtin_popcount(o & ((1u << i) - 1u)) - r0;
-            const uint2 s2 = j ? d.s[1] : d.s[0];
-            const uint32_t sw = i < 2 ? s2.x : s2.y;
-            if (left && e < 32u)   // scale, token of the 32, vector
-                place[32 * (j ? y.hi[1] : y.hi[0]) + e] =
-                    (i & 1 ? sw & 0xffff0000u : sw << 16) |
-                    ((16 * (j ? y.hi[1] : y.hi[0]) + ((j ? y.rec[1] : y.rec[0]) & 15) + i) << 4) | ((j ? y.rec[1] : y.rec[0]) >> 4);
-            left &= left - 1u;
+        const uint32_t k = r0 + (lane & 31);
+        if (r0) ent = load_entry(r, {0u, 0u, m.base + r0, m.count > r0 ? m.count - r0 : 0u}, lane);
+        const uint32_t rec = most > 7 ? nth_record(mk, k) & 255u : head_rec(m, lane);
+        if (k < m.count && (int64_t)m.base + k < r.exc_cap) {
+            uint32_t e[4];
+            exc_pairs(ent, e);
+            put(rec, e);
         }
-        wave_lds_sync();
-        const uint32_t e = r0 + (lane & 31);
-        if (e < m.count && (int64_t)m.base + e < r.exc_cap) {
-            const uint32_t got = place[lane], v = got & 15u, tok = (got >> 4) & 31u;
-            uint32_t p[4];
-            exc_pairs(ent, p);
-            mul_pairs<4>(p, __builtin_amdgcn_perm(0u, got, 0x03020302u));
+    }
+}
+
+// The exceptions of 32 tokens whose records are staged in LDS, over the staged ones; the
+// tokens' scales go through `scales`, 32 of the wave's own.
+__device__ __forceinline__ void patch_lds(bool isk, const lq_resident& r, const Raw& d, const Meta& m, const uint4& ent,
+                                          uint32_t word, int lane, uint2* scales, char* lds) {
+    const uint32_t most = most_of(m);
+    if (!most) return;
+    wave_lds_sync();
+    if (isk ? lane < 4 : (lane & 15) == 0) {   // four tokens each
+#pragma unroll
+        for (int j = 0; j < 2; j++) scales[isk ? lane + 4 * j : 2 * (lane >> 4) + j] = d.s[j];
+    }
+    wave_lds_sync();
+    each_entry(r, m, ent, most, lane,
+        [&](uint2 mk[4]) __attribute__((always_inline)) {
+            half_masks(d.mask[0], 0, isk ? d.mask[1] : d.mask[0], isk ? 0 : 32, isk ? 16 : 4, lane, mk);
+        },
+        [&](uint32_t rec, uint32_t p[4]) __attribute__((always_inline)) {
+            const uint32_t tok = 16 * (lane >> 5) + (rec & 15), v = rec >> 4;
+            mul_pairs<4>(p, __builtin_amdgcn_perm(0u, reinterpret_cast<const uint16_t*>(scales)[tok], 0x01000100u));
             if (isk) {
                 put_k(lds, tok, v, make_uint4(p[0], p[1], p[2], p[3]));
             } else if ((word >> tok) & 1u) {
@@ -368,8 +403,7 @@ __device__ __forceinline__ void patch_lds(bool isk, const lq_resident& r, const 
                     *reinterpret_cast<uint16_t*>(lds + 32 * kKRow + (16 * i + v) * kVRow + 2 * tok) =
                         (uint16_t)(i & 1 ? p[i >> 1] >> 16 : p[i >> 1]);
             }
-        }
-    }
+        });
 }
 
 // K for the operands of k_tree_few: a lane has tokens 8 g + 2 i, + 1 (lane % 16 = 4 g + i)
@@ -394,63 +428,56 @@ __device__ __forceinline__ void load_few(const lq_resident& r, int64_t hd, int64
     d.mask = at32<uint2>(r.mask + B.rb0 * 4, ((lane >> 2) & B.d) * 32 + (lane & 3) * 8);
 }
 
-// The converted entry (pairs e of the lane that holds it) of the record of rank `rank` in
-// block `blk`, over p, for the lanes that own one.  Entries past the first 32 of a block
-// are loaded here.
-__device__ __forceinline__ void pull_entry(const lq_resident& r, const Meta& m, const uint32_t e[4], bool own, uint32_t blk,
-                                           uint32_t rank, uint32_t p[4]) {
-    if (!__any(own)) return;
-    uint32_t x[4];
+// Exceptions of a wave's decoded pairs: these go through 8 KB of LDS of the wave's own,
+// where the lanes that hold the entries write over them, all at once.  (Pulled into the
+// registers of the records' lanes, one record group after the other, they cost as much as
+// decoding the tile: 32768 tokens, 16 rows a head, 30.4 us a call against 27.1; 25.3
+// without any exception.)
+// Over the pairs of K's records 2 c + y:
+__device__ __forceinline__ void patch_k(const lq_resident& r, const KFew& d, const Meta& m, const uint4& ent, uint32_t most,
+                                        int lane, u32x4_t* area, uint32_t p[8][4]) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(4 * (32 * blk + (rank & 31))), (int)e[i]);
-    const uint32_t b0 = (uint32_t)__builtin_amdgcn_readlane((int)m.base, 0), b1 = (uint32_t)__builtin_amdgcn_readlane((int)m.base, 32);
-    const int64_t at = (int64_t)(blk ? b1 : b0) + rank;
-    own = own && at < r.exc_cap;
-    if (__any(own && rank >= 32u)) {
-        uint32_t f[4];
-        exc_pairs(reinterpret_cast<const uint4*>(r.exc)[own ? at : 0], f);
+    for (int j = 0; j < 8; j++) area[64 * j + lane] = u32x4_t{p[j][0], p[j][1], p[j][2], p[j][3]};
+    wave_lds_sync();
+    each_entry(r, m, ent, most, lane,
+        [&](uint2 mk[4]) __attribute__((always_inline)) { half_masks(d.mask, 0, d.mask, 4, 1, lane, mk); },
+        [&](uint32_t rec, const uint32_t e[4]) __attribute__((always_inline)) {
+            area[64 * (2 * (rec >> 6) + (rec & 1)) + 16 * ((rec >> 4) & 3) + 8 * (lane >> 5) + ((rec & 15) >> 1)] =
+                u32x4_t{e[0], e[1], e[2], e[3]};
+        });
+    wave_lds_sync();
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = rank >= 32u ? f[i] : x[i];
+    for (int j = 0; j < 8; j++) {
+        const u32x4_t w = area[64 * j + lane];
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[j][i] = w[i];
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++) p[i] = own ? x[i] : p[i];
+    wave_lds_sync();
 }
-
-// K's masks of record group c in the lane's block, and how many stand before group c
-struct FewMask {
-    uint64_t m;
-    uint32_t any;   // wave-uniform
-};
-__device__ __forceinline__ FewMask few_mask(const KFew& d, int c, int lane) {
-    const uint32_t l0 = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.x, c), h0 = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.y, c);
-    const uint32_t l1 = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.x, 4 + c), h1 = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.y, 4 + c);
-    return {(lane & 8) ? ((uint64_t)h1 << 32) | l1 : ((uint64_t)h0 << 32) | l0, l0 | h0 | l1 | h1};
-}
-
-// V's exceptions over the pairs of decode_v
-__device__ __forceinline__ void pull_v(const lq_resident& r, const Raw& d, const Lay& y, const Meta& m, uint4 ent, int lane,
-                                       uint32_t vp[4][8]) {
-    if (!__any((d.mask[0].x | d.mask[0].y) != 0u)) return;
-    const uint64_t mk = ((uint64_t)d.mask[0].y << 32) | d.mask[0].x;
-    const uint32_t rank = rank_of(false, d, y, 0, lane), own = (uint32_t)(mk >> (y.rec[0] & 63)) & 0xffu;
-    uint32_t e[4];
-    exc_pairs(ent, e);
+// over the pairs of decode_v:
+__device__ __forceinline__ void patch_v(const lq_resident& r, const Raw& d, const Meta& m, const uint4& ent, uint32_t most,
+                                        int lane, u32x4_t* area, uint32_t vp[4][8]) {
 #pragma unroll
-    for (int q = 0; q < 8; q++) {
-        const bool mine = (own >> q) & 1u;
-        if (!__any(mine)) continue;
-        uint32_t p[4];
+    for (int j = 0; j < 8; j++)
+        area[64 * j + lane] = u32x4_t{vp[j >> 1][4 * (j & 1)], vp[j >> 1][4 * (j & 1) + 1], vp[j >> 1][4 * (j & 1) + 2],
+                                      vp[j >> 1][4 * (j & 1) + 3]};
+    wave_lds_sync();
+    each_entry(r, m, ent, most, lane,
+        [&](uint2 mk[4]) __attribute__((always_inline)) { half_masks(d.mask[0], 0, d.mask[0], 32, 4, lane, mk); },
+        [&](uint32_t rec, const uint32_t e[4]) __attribute__((always_inline)) {
+            const uint32_t tok = 16 * (lane >> 5) + (rec & 15);   // of the tile's 32: pair (tok / 2) % 4 of lane vector + 16 (tok / 8)
+            uint16_t* w = reinterpret_cast<uint16_t*>(area + 64 * (tok & 6) + 16 * (tok >> 3) + (rec >> 4)) + (tok & 1);
 #pragma unroll
-        for (int i = 0; i < 4; i++)     // the token's own pairs of dimensions
-            p[i] = __builtin_amdgcn_perm(vp[q >> 1][2 * i + 1], vp[q >> 1][2 * i], q & 1 ? 0x07060302u : 0x05040100u);
-        pull_entry(r, m, e, mine, y.hi[0], rank + __builtin_popcount(own & ((1u << q) - 1u)), p);
+            for (int i = 0; i < 8; i++) w[(i & 4) * 128 + (i & 3) * 2] = (uint16_t)(i & 1 ? e[i >> 1] >> 16 : e[i >> 1]);
+        });
+    wave_lds_sync();
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            uint32_t &w0 = vp[q >> 1][2 * i], &w1 = vp[q >> 1][2 * i + 1];
-            w0 = __builtin_amdgcn_perm(p[i], w0, q & 1 ? 0x05040100u : 0x03020504u);
-            w1 = __builtin_amdgcn_perm(p[i], w1, q & 1 ? 0x07060100u : 0x03020706u);
-        }
+    for (int j = 0; j < 8; j++) {
+        const u32x4_t w = area[64 * j + lane];
+#pragma unroll
+        for (int i = 0; i < 4; i++) vp[j >> 1][4 * (j & 1) + i] = w[i];
     }
+    wave_lds_sync();
 }
 
 // fp16 / bf16 rows: 32 tokens from t on, of which the first `have` exist (one at least);
@@ -801,7 +828,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_many(TreeArgs A) {
     static_assert(kStage >= kWaves * 32 * (kMRow + 2) * 4 && kStage >= kMaxNodes * 4, "the join and the tree fit the stage");
     __shared__ __align__(16) char s_buf[kStage];
     __shared__ uint32_t s_vis[kMaxNodes][kVisWords];
-    __shared__ uint32_t s_place[kWaves][64];
+    __shared__ uint2 s_scale[kWaves][8];
     __shared__ int s_odd;                      // a draft's V has infinities or NaN
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int team = wave / C, ct = wave % C;
@@ -869,7 +896,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_many(TreeArgs A) {
             scale_v(d, word, lane, vp);
             put_v(lds, lane & 15, lane >> 4, vp);
         }
-        patch_lds(isk, res, d, lay, m, e, word, lane, s_place[wave], lds);
+        patch_lds(isk, res, d, m, e, word, lane, s_scale[wave], lds);
     };
     if (prefix) {
         ent = load_entry(res, meta, lane);
@@ -1012,6 +1039,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_few(TreeArgs A) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     const Place P = place_of(A, 16 * Q);
+    u32x4_t* area = reinterpret_cast<u32x4_t*>(s_buf + wave * 16 * Q * kMRow);   // the wave's own until the join
+    static_assert(16 * kMRow * 4 >= 8 * 64 * 16, "a tile's pairs fit it");
 
     const Share sh = share_of(A, P.sp);
     const int split = min(sh.end, A.np);       // prefix tiles, then rows: two loops, each with the registers it needs
@@ -1073,34 +1102,24 @@ __global__ __launch_bounds__(kWaves * 64) void k_tree_few(TreeArgs A) {
         uint32_t vp[4][8];
 #pragma unroll
         for (int x = 0; x < Q; x++) s[x][0] = s[x][1] = f4_t{0.f, 0.f, 0.f, 0.f};
-        uint32_t e[4], before = 0u;
-        exc_pairs(ek, e);
+        uint32_t p[8][4];                        // records 2 c + y
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const FewMask fm = few_mask(kr, c, lane);
-            const int bit = 16 * g + 8 * ((col >> 2) & 1) + 2 * (col & 3);
-            const uint32_t two = (uint32_t)(fm.m >> bit) & 3u;
-            uint32_t rank = 0u;
-            if (fm.any) {                      // wave-uniform
-                rank = before + __builtin_popcountll(fm.m & ((1ull << bit) - 1ull));
-                before += __builtin_popcountll(fm.m);
-            }
+        for (int j = 0; j < 8; j++) {
+            rec_pairs(j & 1 ? kr.a[j >> 1].y : kr.a[j >> 1].x, (kr.b[j >> 1] >> (8 * (j & 1))) & 0xffu, p[j]);
 #pragma unroll
-            for (int y = 0; y < 2; y++) {
-                uint32_t p[4];
-                rec_pairs(y ? kr.a[c].y : kr.a[c].x, (kr.b[c] >> (8 * y)) & 0xffu, p);
+            for (int i = 0; i < 4; i++) p[j][i] = unbias(p[j][i]);
+        }
+        if (const uint32_t most = most_of(mk)) patch_k(A.k, kr, mk, ek, most, lane, area, p);
 #pragma unroll
-                for (int i = 0; i < 4; i++) p[i] = unbias(p[i]);
-                if (fm.any) pull_entry(A.k, mk, e, (two >> y) & 1u, col >> 3, rank + (y ? two & 1u : 0u), p);
-                mul_pairs<4>(p, __builtin_amdgcn_perm(0u, kr.s, y ? 0x03020302u : 0x01000100u));
+        for (int j = 0; j < 8; j++) {
+            mul_pairs<4>(p[j], __builtin_amdgcn_perm(0u, kr.s, j & 1 ? 0x03020302u : 0x01000100u));
 #pragma unroll
-                for (int x = 0; x < Q; x++)
-                    s[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(p[0], p[1], p[2], p[3]), q[x][c], s[x][y], 0, 0, 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);   // one record group's operands live at a time
+            for (int x = 0; x < Q; x++)
+                s[x][j & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(p[j][0], p[j][1], p[j][2], p[j][3]), q[x][j >> 1],
+                                                                     s[x][j & 1], 0, 0, 0);
         }
         decode_v(vr, vp);
-        pull_v(A.v, vr, lay, mv, ev, lane, vp);
+        if (const uint32_t most = most_of(mv)) patch_v(A.v, vr, mv, ev, most, lane, area, vp);
         scale_v(vr, sb.word, lane, vp);
         __builtin_amdgcn_sched_barrier(0);       // every use of the records before their reload
         fetch(tile + kWaves);

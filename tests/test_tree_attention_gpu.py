@@ -225,6 +225,66 @@ def test_tree_attention_infinite_draft_seen_gpu():
 
 
 @gpu
+@pytest.mark.parametrize("B,H,G,N,T,cap,dtype", [
+    (4, 8, 16, 5, 4096, 70, torch.float16),      # 80 rows, much to read: teams of four
+    (4, 8, 13, 11, 4112, 40, torch.bfloat16),    # 143 rows: teams of eight, half a tile at the end
+    (3, 6, 16, 14, 8192, 0, torch.float16),      # 224 rows, no tail
+])
+def test_tree_attention_wide_teams_gpu(B, H, G, N, T, cap, dtype):
+    c = _case(B, H, G, N, T, cap, seed=21, dtype=dtype, ragged=cap > 0, start=True)
+    _check(_run(c), c)
+
+
+@gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_tree_attention_wide_teams_masked_values_gpu(bad):
+    """As test_tree_attention_masked_values_gpu, in the kernel's widest form; rows that see
+    nothing that is not finite keep their bits."""
+    c = _case(4, 8, 16, 10, 4096, 48, seed=23, kind="roots", ragged=True, start=True)
+    c["len"][:] = torch.tensor([20, 33, 0, 48])
+    c["start"][:] = torch.tensor([0, 4100, 17, 4096])
+    clean = _run(c)
+    for n in ("tk", "tv"):
+        c[n][0, :, 20:] = bad
+        c[n][1, :, 33:] = bad
+        c[n][2] = bad
+        c[n][1, :, :4] = bad
+    out = _run(c)
+    assert torch.equal(out, clean)
+    for n in ("dk", "dv"):
+        c[n][1, :, 3, 7] = bad                           # its own row alone sees it
+    out = _run(c)
+    others = torch.arange(10, device="cuda") != 3
+    assert torch.isfinite(out[:, :, others]).all() and torch.equal(out[[0, 2, 3]], clean[[0, 2, 3]])
+    assert torch.equal(out[1][:, others], clean[1][:, others])
+
+
+@gpu
+@pytest.mark.parametrize("rows", [16, 32, 64])
+def test_tree_attention_exception_counts_gpu(rows):
+    """0 to 64 exceptions a block of 16 tokens, spread at random (the header names seven, a
+    round takes 32): vectors with a coordinate outside the 5-bit range."""
+    from latticequant_amd.llm.resident import ResidentKV
+    B, H, T = 1, 2, 16 * 66
+    c = _case(B, H, 4, rows // 4, 0, 20, seed=27, dtype=torch.float16)
+    g = torch.Generator().manual_seed(28)
+    for n in "kv":
+        x = torch.randn(B * H, T // 16, 256, 8, generator=g).clamp(-3, 3)   # vectors of blocks
+        for h in range(B * H):
+            for i in range(T // 16):
+                at = torch.randperm(256, generator=g)[:(i if h == 0 else [0, 1, 7, 8, 9, 31, 32, 33, 64, 2][i % 10])]
+                x[h, i, at, i % 8] = 9.0                 # 36 steps of 0.25
+        x = x.reshape(B, H, T, 128).half().cuda()
+        s = torch.full((B * H,), 0.25, device="cuda")
+        r = ResidentKV(B * H, T, device="cuda")
+        r.append(x, s, s.half())
+        counts = r.meta.view(B * H, -1, 4)[0, :T // 16, 3].cpu()
+        assert counts.min() == 0 and (counts == 7).any() and (counts == 8).any() and counts.max() > 60
+        c[n] = r
+    _check(_run(c), c)
+
+
+@gpu
 def test_tree_attention_large_scores_gpu():
     """A far maximum, found late, and weights that underflow: the running maximum's rescaling."""
     c = _case(1, 2, 4, 4, 512, 40, seed=9)
