@@ -344,6 +344,35 @@ def test_tree_attention_prefix_part_stream_and_graph_gpu():
 
 
 @gpu
+def test_tree_workspace_shared_by_geometries_gpu():
+    """One workspace for calls of other rows, heads and lengths, eager and replayed in turn:
+    the results are those of a workspace of each call's own, whatever it held before."""
+    from latticequant_amd.llm.tree import tree_workspace_size
+    cases = [_case(*a, seed=31) for a in ((1, 2, 4, 1, 1024, 30), (2, 8, 4, 8, 2048, 0), (1, 1, 3, 1, 4096, 5),
+                                          (1, 2, 8, 20, 512, 40), (3, 4, 1, 7, 1040, 9), (1, 1, 1, 1, 8192, 0))]
+    size = [tree_workspace_size(c["k"].n_heads, c["q"].shape[1] * c["q"].shape[0] // c["k"].n_heads, c["q"].shape[2],
+                                c["k"].n_tokens, 0 if c["tk"] is None else c["tk"].shape[2]) for c in cases]
+    work = torch.empty(max(size), dtype=torch.uint8, device="cuda").fill_(0x7f)
+    for c in cases:
+        c["par"] = c["par"].cuda()
+    want = [_run(c) for c in cases]
+    for c, w in zip(cases, want):
+        _check(w, c)
+    graph, held = torch.cuda.CUDAGraph(), []
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        held = [_run(c, work=work) for c in cases]
+    for turn in range(4):
+        for h in held:
+            h.fill_(float("nan"))
+        graph.replay()
+        eager = [_run(c, work=work) for c in cases[::-1]][::-1]
+        torch.cuda.synchronize()
+        for h, e, w in zip(held, eager, want):
+            assert torch.equal(h, w) and torch.equal(e, w), turn
+
+
+@gpu
 def test_tree_attention_refusals_gpu():
     from latticequant_amd.llm.tree import resident_tree_attention, tree_attn_workspace
     c = _case(1, 2, 4, 5, 32, 10, seed=1)
