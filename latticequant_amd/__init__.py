@@ -14,5 +14,9 @@ merge / decode-attention step, as hand-written HIP kernels behind a C ABI
   latticequant_amd.llm.fused_triton_merge  (llm/fused_triton_merge.py)
   latticequant_amd.llm.triton_kv_integration (llm/triton_kv_integration.py)
   latticequant_amd.llm.decode_attention     (decode step over the compressed prefix)
+  latticequant_amd.llm.resident             (decode step over its resident fixed-width form;
+                                             sequences reordered, selected, forked)
+  latticequant_amd.llm.tree                 (drafted trees over it: attention, acceptance)
+  latticequant_amd.llm.resident_cache       (HF cache and attention of the resident form)
 """
 __version__ = "0.1.0"
