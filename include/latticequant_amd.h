@@ -681,7 +681,8 @@ int64_t lq_select_workspace(int64_t heads_out, int64_t n_blocks);
  * use per head; dst holds n_out * (src heads per sequence) heads.  Writes dst's
  * planes with the exception offsets of a list that has the chosen blocks' entries
  * in block order, and their number to *dst->n_exc, clears *dst->status; dst->exc is then
- * sized by the caller and filled by lq_resident_select_exceptions (same arguments).
+ * sized by the caller and filled by lq_resident_select_exceptions (same arguments;
+ * entries that src's list has dropped set LQ_RES_ST_EXC_OVERFLOW in *dst->status).
  * With h_total (host, nullable) the call waits for that number, not for the planes, and
  * is not for a stream that is being captured.  Indices are clamped to their ranges. */
 int lq_resident_select(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index, int64_t n_out,

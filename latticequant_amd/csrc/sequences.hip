@@ -439,6 +439,7 @@ __global__ __launch_bounds__(256) void k_select_exc(const uint4* __restrict__ sr
         }
         uint4 w = make_uint4(0u, 0u, 0u, 0u);
         if (from + e < src_exc) w = reinterpret_cast<const uint4*>(src)[from + e];
+        else atomicOr(status, LQ_RES_ST_EXC_OVERFLOW);   // dropped before already
         reinterpret_cast<uint4*>(dst)[(int64_t)d.z + e] = w;
     }
 }

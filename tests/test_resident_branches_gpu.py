@@ -268,6 +268,28 @@ def test_accept_keeps_within_the_nodes_and_the_buffers_gpu():
 
 
 @gpu
+def test_drafts_behind_an_empty_tail_gpu():
+    """Everything cached is compressed: the drafts follow the prefix at once."""
+    from latticequant_amd.llm.tree import resident_tree_attention
+    c = _filled(2, layers=2, tail=0, tokens=48)
+    assert c.tail_k[0].shape[2] == 0
+    g = torch.Generator().manual_seed(6)
+    c.draft([-1, 0, 0])
+    d = [[torch.randn(2, 2, 3, 128, generator=g).half().cuda() for _ in range(2)] for _ in range(2)]
+    q = torch.randn(2, 8, 3, 128, generator=g).half().cuda()
+    for i in range(2):
+        c.update(*d[i], i)
+        out = c.attend_drafts(i, q)
+        want = resident_tree_attention(c.res_k[i], c.res_v[i], q, *d[i], torch.tensor([-1, 0, 0]))
+        assert torch.equal(out.transpose(1, 2), want)
+    before = [c.materialise(i)[0].clone() for i in range(2)]
+    c.accept(torch.tensor([[0, 2], [0, 1]], device="cuda"))
+    for i in range(2):
+        new = torch.stack([d[i][0][0][:, [0, 2]], d[i][0][1][:, [0, 1]]])
+        assert torch.equal(c.materialise(i)[0], torch.cat([before[i], new], 2))
+
+
+@gpu
 def test_generate_with_beams_gpu():
     """HF's beam search over the cache: with nothing flushed the cache holds the model's own
     fp16 K / V, and the beams found are as likely as DynamicCache's (the same up to a near

@@ -305,6 +305,20 @@ def test_select_gpu(B, H, T, R, keep):
 
 
 @gpu
+def test_select_reports_dropped_exceptions_gpu():
+    """A prefix whose exception list was too short stays marked when it is selected from."""
+    r = _prefix(2, 1, 64, 3)
+    n = r.exceptions().shape[0]
+    assert n > 8
+    s = r.select(torch.tensor([1, 0]), 2)
+    assert int(s.status.item()) == 0 and s.exceptions().shape[0] == n
+    r.exc, r._st = r.exc[:8 * 8].clone(), None           # the first eight alone are left
+    s = r.select(torch.tensor([1, 0]), 2)
+    assert int(s.status.item()) == 1                     # LQ_RES_ST_EXC_OVERFLOW
+    assert s.exceptions().shape[0] == n and int((s.exceptions() != 0).any(1).sum()) <= 8
+
+
+@gpu
 def test_reorder_and_select_refusals_gpu():
     from latticequant_amd.llm.resident import ResidentKV, reorder_sequences
     r, s = _prefix(4, 1, 32, 1), _prefix(4, 1, 48, 2)
