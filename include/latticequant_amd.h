@@ -673,21 +673,28 @@ int lq_gather_rows(void *const *h_dst, const void *const *h_src, int64_t n, cons
 int lq_resident_reorder(const lq_resident *h_res, int64_t n, int64_t n_seq, const int32_t *d_index, int64_t blk0,
                         int64_t n_blocks, hipStream_t s);
 
-/* Workspace (bytes) of lq_resident_select for heads_out heads of n_blocks blocks. */
+/* Workspace (bytes) of a selection of heads_out heads of n_blocks blocks. */
 int64_t lq_select_workspace(int64_t heads_out, int64_t n_blocks);
 
 /* A new prefix of chosen sequences and blocks: block j of output sequence r is block
  * d_blocks[r][j] (null: j) of sequence d_index[r] of src, which has src_blocks blocks in
- * use per head; dst holds n_out * (src heads per sequence) heads.  Writes dst's
- * planes with the exception offsets of a list that has the chosen blocks' entries
- * in block order, and their number to *dst->n_exc, clears *dst->status; dst->exc is then
- * sized by the caller and filled by lq_resident_select_exceptions (same arguments;
- * entries that src's list has dropped set LQ_RES_ST_EXC_OVERFLOW in *dst->status).
- * With h_total (host, nullable) the call waits for that number, not for the planes, and
- * is not for a stream that is being captured.  Indices are clamped to their ranges. */
+ * use per head; dst holds n_out * (src heads per sequence) heads.  Indices are clamped to
+ * their ranges.  In three calls with the same arguments on one stream:
+ * lq_select_count numbers the chosen blocks' exceptions (in d_work), writes their number
+ * to *d_n_exc (dst's n_exc) and clears *d_status; with h_read (nullable; not for a stream
+ * that is being captured) it leaves there a read of that number for lq_select_total, which
+ * waits for it, not for what is queued behind, and is to be called once for each.
+ * lq_resident_select writes dst's planes, with the offsets of an exception list that has
+ * the chosen blocks' entries in block order.
+ * lq_resident_select_exceptions fills that list, dst->exc, sized by the caller; entries that
+ * src's list has dropped set LQ_RES_ST_EXC_OVERFLOW in *dst->status. */
+int lq_select_count(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index, int64_t n_out,
+                    const int32_t *d_blocks, int64_t n_blocks, void *d_work, int64_t work_bytes, int32_t *d_n_exc,
+                    int32_t *d_status, void **h_read, hipStream_t s);
+int lq_select_total(void *h_read, int64_t *h_total);
 int lq_resident_select(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index, int64_t n_out,
-                       const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst, void *d_work,
-                       int64_t work_bytes, int64_t *h_total, hipStream_t s);
+                       const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst, const void *d_work,
+                       int64_t work_bytes, hipStream_t s);
 int lq_resident_select_exceptions(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index,
                                   int64_t n_out, const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst,
                                   hipStream_t s);

@@ -102,7 +102,9 @@ _SIGS = {
     "lq_gather_rows": ([_P, _P, _I64, _P, _P] + [_I64] * 5 + [_P] * 2, _INT),
     "lq_resident_reorder": ([_P, _I64, _I64, _P, _I64, _I64, _P], _INT),
     "lq_select_workspace": ([_I64, _I64], _I64),
-    "lq_resident_select": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _P, _P], _INT),
+    "lq_select_count": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P], _INT),
+    "lq_select_total": ([_P, _P], _INT),
+    "lq_resident_select": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _P], _INT),
     "lq_resident_select_exceptions": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P], _INT),
     "lq_tree_attn_workspace": ([_I64, _I64, _I64, _INT, _I64, _I64], _I64),
     "lq_resident_tree_attention": ([_P, _P, _I64] + [_P] * 4 + [_I64, _I64, _INT, _P, _P, _I64, _P, _P, _INT, _P, _I64] +

@@ -2,6 +2,7 @@
 // into the tails, sequences of resident prefixes reordered in place, and new
 // prefixes made of chosen sequences and blocks.
 #include <climits>
+#include <new>
 
 #include "lq_device.h"
 #include "lq_readpool.h"
@@ -449,14 +450,16 @@ bool res_planes_ok(const lq_resident* r) {
            (((uintptr_t)r->a | (uintptr_t)r->b | (uintptr_t)r->mask | (uintptr_t)r->meta | (uintptr_t)r->scale) & 15) == 0;
 }
 
-bool choice_of(const lq_resident* src, const lq_resident* dst, int64_t n_seq, int64_t src_blocks, const int32_t* index,
-               int64_t n_out, const int32_t* blocks, int64_t nb, Choice* c) {
-    if (!res_planes_ok(src) || !res_planes_ok(dst) || !index || n_seq < 1 || n_out < 1 || nb < 1 || src_blocks < 1 ||
-        src->n_heads % n_seq || src_blocks > src->cap_blocks || nb > dst->cap_blocks || (!blocks && nb > src_blocks) ||
-        dst->n_heads != src->n_heads / n_seq * n_out || dst->a == src->a)
+bool choice_of(const lq_resident* src, int64_t n_seq, int64_t src_blocks, const int32_t* index, int64_t n_out,
+               const int32_t* blocks, int64_t nb, Choice* c) {
+    if (!res_planes_ok(src) || !index || n_seq < 1 || n_out < 1 || n_out > 65535 || nb < 1 || src_blocks < 1 ||
+        src->n_heads % n_seq || src_blocks > src->cap_blocks || (!blocks && nb > src_blocks))
         return false;
     *c = {index, blocks, n_seq, src->n_heads / n_seq, n_out, nb, src_blocks};
-    return n_out * c->heads <= 65535 && n_out * c->heads * nb <= (int64_t)INT_MAX / 128;
+    return c->heads <= 65535 && n_out * c->heads <= 65535 && nb <= INT_MAX && n_out * c->heads * nb <= (int64_t)INT_MAX / 128;
+}
+bool takes(const lq_resident* dst, const lq_resident* src, const Choice& c) {
+    return res_planes_ok(dst) && dst->a != src->a && dst->n_heads == c.n_out * c.heads && c.nb <= dst->cap_blocks;
 }
 
 ReadPool& read_pool() {
@@ -582,42 +585,71 @@ int64_t lq_select_workspace(int64_t heads_out, int64_t n_blocks) {
     return (n + (n + kScan - 1) / kScan) * (int64_t)sizeof(uint32_t);
 }
 
-int lq_resident_select(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index, int64_t n_out,
-                       const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst, void *d_work,
-                       int64_t work_bytes, int64_t *h_total, hipStream_t s) {
+int lq_select_count(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index, int64_t n_out,
+                    const int32_t *d_blocks, int64_t n_blocks, void *d_work, int64_t work_bytes, int32_t *d_n_exc,
+                    int32_t *d_status, void **h_read, hipStream_t s) {
     Choice C;
-    if (!choice_of(src, dst, n_seq, src_blocks, d_index, n_out, d_blocks, n_blocks, &C) || !d_work || !dst->n_exc ||
-        !dst->status || work_bytes < lq_select_workspace(dst->n_heads, n_blocks) || ((uintptr_t)d_work & 3))
+    if (h_read) *h_read = nullptr;
+    if (!choice_of(src, n_seq, src_blocks, d_index, n_out, d_blocks, n_blocks, &C) || !d_work || !d_n_exc || !d_status ||
+        work_bytes < lq_select_workspace(C.n_out * C.heads, n_blocks) || ((uintptr_t)d_work & 3))
         return LQ_ERR_ARG;
     const int64_t n = C.n_out * C.heads * C.nb, tiles = (n + kScan - 1) / kScan;
     uint32_t* off = static_cast<uint32_t*>(d_work);
     uint32_t* sums = off + n;
-    ReadSlot slot;
-    if (h_total && !read_pool().take(s, &slot)) return LQ_ERR_LAUNCH;
+    ReadSlot* slot = nullptr;
+    if (h_read) {
+        slot = new (std::nothrow) ReadSlot;
+        if (!slot || !read_pool().take(s, slot)) {
+            delete slot;
+            return LQ_ERR_LAUNCH;
+        }
+    }
     hipLaunchKernelGGL(k_select_count, dim3((unsigned)tiles), dim3(256), 0, s, src->meta, src->cap_blocks, C, (uint32_t)n,
                        off, sums);
-    hipLaunchKernelGGL(k_select_bases, dim3(1), dim3(64), 0, s, sums, tiles, dst->n_exc, dst->status,
-                       h_total ? slot.host : nullptr);
-    bool ok = !h_total || hipEventRecord(slot.event, s) == hipSuccess;
-    hipLaunchKernelGGL(k_select_planes, dim3((unsigned)((C.nb * kUnits + 255) / 256), (unsigned)(C.n_out * C.heads)),
-                       dim3(256), 0, s, planes_of(src), planes_of(dst), C, off, sums);
-    ok = hipGetLastError() == hipSuccess && ok;
-    if (h_total) {
-        // the planes are copied while the caller reads on
-        ok = ok && hipEventSynchronize(slot.event) == hipSuccess;
-        if (ok) *h_total = slot.host[0];
-        else (void)hipStreamSynchronize(s);   // no launch may still write the slot
-        read_pool().give(slot);
+    hipLaunchKernelGGL(k_select_bases, dim3(1), dim3(64), 0, s, sums, tiles, d_n_exc, d_status, slot ? slot->host : nullptr);
+    bool ok = hipGetLastError() == hipSuccess;
+    if (slot) {
+        ok = hipEventRecord(slot->event, s) == hipSuccess && ok;
+        if (ok) {
+            *h_read = slot;
+        } else {
+            (void)hipStreamSynchronize(s);   // no launch may still write the slot
+            read_pool().give(*slot);
+            delete slot;
+        }
     }
     return ok ? LQ_OK : LQ_ERR_LAUNCH;
+}
+
+int lq_select_total(void *h_read, int64_t *h_total) {
+    if (!h_read) return LQ_ERR_ARG;
+    ReadSlot* slot = static_cast<ReadSlot*>(h_read);
+    const bool ok = hipEventSynchronize(slot->event) == hipSuccess;
+    if (ok && h_total) *h_total = slot->host[0];
+    if (ok) read_pool().give(*slot);         // (else a launch may still write it: it is left)
+    delete slot;
+    return ok ? LQ_OK : LQ_ERR_LAUNCH;
+}
+
+int lq_resident_select(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index, int64_t n_out,
+                       const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst, const void *d_work,
+                       int64_t work_bytes, hipStream_t s) {
+    Choice C;
+    if (!choice_of(src, n_seq, src_blocks, d_index, n_out, d_blocks, n_blocks, &C) || !takes(dst, src, C) || !d_work ||
+        work_bytes < lq_select_workspace(dst->n_heads, n_blocks) || ((uintptr_t)d_work & 3))
+        return LQ_ERR_ARG;
+    const uint32_t* off = static_cast<const uint32_t*>(d_work);
+    hipLaunchKernelGGL(k_select_planes, dim3((unsigned)((C.nb * kUnits + 255) / 256), (unsigned)(C.n_out * C.heads)),
+                       dim3(256), 0, s, planes_of(src), planes_of(dst), C, off, off + C.n_out * C.heads * C.nb);
+    return launch_status();
 }
 
 int lq_resident_select_exceptions(const lq_resident *src, int64_t n_seq, int64_t src_blocks, const int32_t *d_index,
                                   int64_t n_out, const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst,
                                   hipStream_t s) {
     Choice C;
-    if (!choice_of(src, dst, n_seq, src_blocks, d_index, n_out, d_blocks, n_blocks, &C) || !src->exc || !dst->exc ||
-        !dst->status || src->exc_cap < 0 || dst->exc_cap < 0)
+    if (!choice_of(src, n_seq, src_blocks, d_index, n_out, d_blocks, n_blocks, &C) || !takes(dst, src, C) || !src->exc ||
+        !dst->exc || !dst->status || src->exc_cap < 0 || dst->exc_cap < 0)
         return LQ_ERR_ARG;
     const int64_t n = C.n_out * C.heads * C.nb;
     hipLaunchKernelGGL(k_select_exc, dim3((unsigned)((n * 8 + 255) / 256)), dim3(256), 0, s,

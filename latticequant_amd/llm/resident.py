@@ -216,44 +216,52 @@ class ResidentKV:
         if L.debug_checks() and (bool((index < 0).any()) or bool((index >= n_seq).any()) or
                                  (blocks is not None and nb and (bool((blocks < 0).any()) or bool((blocks >= used).any())))):
             raise ValueError("sequence or block out of range")
-        new = self._bare(R * (self.n_heads // n_seq), cap)
+        heads = R * (self.n_heads // n_seq)
         if nb == 0:
-            new.n_exc.zero_()
-            new.status.zero_()
+            new = self._bare(heads, cap, self.n_exc.new_zeros(1), self.status.new_zeros(1))
             new.exc = self.exc.new_empty(8)
             return new
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a selection reads its exception count back: not while a graph is captured")
         lib = L.lib()
-        need = lib.lq_select_workspace(new.n_heads, nb)
+        need = lib.lq_select_workspace(heads, nb)
         if need < 0:
             raise ValueError("too many heads or blocks for one selection")
-        total = ctypes.c_int64()
+        read, total = ctypes.c_void_p(), ctypes.c_int64()
         with L.on_device(dev):
             idx = index.to(device=dev, dtype=torch.int32).contiguous()
             blk = None if blocks is None else blocks.to(device=dev, dtype=torch.int32).contiguous()
-            work = idx.new_empty(need + 3 >> 2)
-            dst, stream = new.struct(), L.raw_stream(dev)
-            args = (ctypes.addressof(self.struct()), n_seq, used, idx.data_ptr(), R, L.ptr(blk), nb, ctypes.addressof(dst))
-            L.check(lib.lq_resident_select(*args, work.data_ptr(), need, ctypes.addressof(total), stream),
-                    "lq_resident_select")
+            work, n_exc, status = idx.new_empty(need + 3 >> 2), self.n_exc.new_empty(1), self.status.new_empty(1)
+            stream = L.raw_stream(dev)
+            args = (ctypes.addressof(self.struct()), n_seq, used, idx.data_ptr(), R, L.ptr(blk), nb)
+            L.check(lib.lq_select_count(*args, work.data_ptr(), need, n_exc.data_ptr(), status.data_ptr(),
+                                        ctypes.addressof(read), stream), "lq_select_count")
+            try:                               # the planes are allocated while the device counts
+                new = self._bare(heads, cap, n_exc, status)
+                dst = new.struct()
+                L.check(lib.lq_resident_select(*args, ctypes.addressof(dst), work.data_ptr(), need, stream),
+                        "lq_resident_select")
+            finally:
+                rc = lib.lq_select_total(read, ctypes.addressof(total))
+            L.check(rc, "lq_select_total")
             n = total.value
             new.exc = self.exc.new_empty(max(1, n) * 8)
             dst.exc, dst.exc_cap = new.exc.data_ptr(), max(1, n)
             if n:
-                L.check(lib.lq_resident_select_exceptions(*args, stream), "lq_resident_select_exceptions")
+                L.check(lib.lq_resident_select_exceptions(*args, ctypes.addressof(dst), stream),
+                        "lq_resident_select_exceptions")
         new._exc_known, new.n_tokens = n, nb * RB
         return new
 
-    def _bare(self, n_heads: int, nb: int) -> "ResidentKV":
-        """nb blocks of room per head where this prefix lies, everything uninitialised
-        (counters too)."""
+    def _bare(self, n_heads: int, nb: int, n_exc: torch.Tensor, status: torch.Tensor) -> "ResidentKV":
+        """nb blocks of room per head where this prefix lies, uninitialised, with the given
+        counters."""
         r = ResidentKV.__new__(ResidentKV)
         r.device, r.n_heads, r.cap_blocks = self.a.device, n_heads, nb
         n = n_heads * nb
         r.a, r.b, r.mask = self.a.new_empty(n * 256), self.b.new_empty(n * 256), self.mask.new_empty(n * 4)
         r.meta, r.scale = self.meta.new_empty(n * 4), self.scale.new_empty(n * RB)
-        r.n_exc, r.status = self.n_exc.new_empty(1), self.status.new_empty(1)
+        r.n_exc, r.status = n_exc, status
         r.exc = r.scale.view(torch.int16)[:8]   # no entry yet
         r.n_tokens = r._exc_known = r._exc_since = 0
         r._exc_read = r._st = None

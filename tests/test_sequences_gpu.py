@@ -305,6 +305,26 @@ def test_select_gpu(B, H, T, R, keep):
 
 
 @gpu
+def test_select_after_a_failed_allocation_gpu(monkeypatch):
+    """A selection whose planes cannot be allocated gives its read back; the next one works."""
+    from latticequant_amd.llm.resident import ResidentKV
+    r = _prefix(2, 1, 64, 4)
+    want = r.select(torch.tensor([1, 1, 0]), 2)
+    bare = ResidentKV._bare
+
+    def fails(*a):
+        raise torch.OutOfMemoryError("no room")
+    for _ in range(40):                                  # more than the reads that are kept
+        monkeypatch.setattr(ResidentKV, "_bare", fails)
+        with pytest.raises(torch.OutOfMemoryError):
+            r.select(torch.tensor([1, 1, 0]), 2)
+        monkeypatch.setattr(ResidentKV, "_bare", bare)
+    s = r.select(torch.tensor([1, 1, 0]), 2)
+    assert all(torch.equal(getattr(s, p), getattr(want, p)) for p in PLANES)
+    assert torch.equal(s.exceptions(), want.exceptions())
+
+
+@gpu
 def test_select_reports_dropped_exceptions_gpu():
     """A prefix whose exception list was too short stays marked when it is selected from."""
     r = _prefix(2, 1, 64, 3)
@@ -390,6 +410,11 @@ def test_moves_streams_and_graph_gpu():
             assert not tail[b, :, i + n:].any()
         after = res.dequant().reshape(3, 2, 64, 128)
         assert torch.equal(after[:, :, 16:], before[[1, 2, 0]][:, :, 16:]) and torch.equal(after[:, :, :16], before[:, :, :16])
+
+
+def test_select_total_of_no_read():
+    from latticequant_amd import _lib as L
+    assert L.load().lq_select_total(None, None) == L.LQ_ERR_ARG
 
 
 def test_workspaces_geometry():
