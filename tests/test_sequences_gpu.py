@@ -48,7 +48,8 @@ def _drafts(B, N, V, seed, agree=0.7):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("B,N,V", [(1, 1, 1), (2, 5, 7), (3, 9, 1001), (1, 64, 32003), (2, 256, 130), (5, 3, 128256)])
+@pytest.mark.parametrize("B,N,V", [(1, 1, 1), (2, 5, 7), (3, 9, 1001), (1, 64, 32003), (2, 256, 130), (5, 3, 128256),
+                                   (3, 17, 15420), (2, 256, 1024), (1, 1, 262144), (2, 6, 43690), (1, 15, 4001)])
 def test_accept_logits_gpu(B, N, V, dtype):
     from latticequant_amd.llm.tree import accept_drafts
     tokens, parents, g = _drafts(B, N, V, B * 100 + N)
