@@ -221,14 +221,14 @@ class ResidentKV:
             new = self._bare(heads, cap, self.n_exc.new_zeros(1), self.status.new_zeros(1))
             new.exc = self.exc.new_empty(8)
             return new
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a selection reads its exception count back: not while a graph is captured")
         lib = L.lib()
         need = lib.lq_select_workspace(heads, nb)
         if need < 0:
             raise ValueError("too many heads or blocks for one selection")
         read, total = ctypes.c_void_p(), ctypes.c_int64()
         with L.on_device(dev):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a selection reads its exception count back: not while a graph is captured")
             idx = index.to(device=dev, dtype=torch.int32).contiguous()
             blk = None if blocks is None else blocks.to(device=dev, dtype=torch.int32).contiguous()
             work, n_exc, status = idx.new_empty(need + 3 >> 2), self.n_exc.new_empty(1), self.status.new_empty(1)

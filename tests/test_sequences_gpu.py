@@ -306,6 +306,22 @@ def test_select_gpu(B, H, T, R, keep):
 
 
 @gpu
+def test_select_not_while_captured_gpu():
+    r, x = _prefix(2, 1, 64, 5), torch.zeros(4, device="cuda")
+    want = r.select(torch.tensor([1, 0]), 2)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        with pytest.raises(RuntimeError):
+            r.select(torch.tensor([1, 0]), 2)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert (x == 3).all() and torch.equal(r.select(torch.tensor([1, 0]), 2).a, want.a)
+
+
+@gpu
 def test_select_after_a_failed_allocation_gpu(monkeypatch):
     """A selection whose planes cannot be allocated gives its read back; the next one works."""
     from latticequant_amd.llm.resident import ResidentKV
