@@ -31,15 +31,24 @@ HD = 128
 
 
 class ResidentKV:
-    """Resident prefix of n_heads kv heads (B * H_kv), capacity cap_tokens tokens each."""
+    """Resident prefix of n_heads kv heads (B * H_kv), capacity cap_tokens tokens each.
 
-    def __init__(self, n_heads: int, cap_tokens: int, device=None, exc_cap: Optional[int] = None):
+    n_seq: of how many sequences the heads are (B), where a selection is to know without
+    being told: given here, or that of the rows appended; None where rows of different
+    groupings were."""
+
+    def __init__(self, n_heads: int, cap_tokens: int, device=None, exc_cap: Optional[int] = None,
+                 n_seq: Optional[int] = None):
         if n_heads <= 0 or cap_tokens <= 0:
             raise ValueError("n_heads and cap_tokens must be positive")
+        if n_seq is not None and (n_seq < 1 or n_heads % n_seq):
+            raise ValueError("n_heads must be a multiple of n_seq")
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         nb = (cap_tokens + RB - 1) // RB
         self.device = dev
         self.n_heads = int(n_heads)
+        self.n_seq = n_seq
+        self._n_seq_given = n_seq is not None
         self.cap_blocks = nb
         self.a = torch.zeros(n_heads * nb * 64 * 4, dtype=torch.int32, device=dev)
         self.b = torch.zeros(n_heads * nb * 64 * 4, dtype=torch.uint8, device=dev)
@@ -116,6 +125,8 @@ class ResidentKV:
         B, H, T, _ = x.shape
         if B * H != self.n_heads:
             raise ValueError(f"x has {B * H} heads, the resident prefix {self.n_heads}")
+        if self._n_seq_given and B != self.n_seq:
+            raise ValueError(f"x has {B} sequences, the resident prefix {self.n_seq}")
         if T % RB:
             raise ValueError(f"resident blocks hold {RB} tokens: append a multiple of {RB} (keep the rest in the tail)")
         if self.n_tokens % RB:
@@ -169,6 +180,8 @@ class ResidentKV:
                     self.n_exc.fill_(n0)
                     self.status.zero_()
                 self._exc_known, self._exc_since, self._exc_read = n1, 0, None
+        if B != self.n_seq:
+            self.n_seq = None if self.n_tokens else B
         self.n_tokens += T
 
     def _grow_exc(self, cap: int, keep: int) -> None:
@@ -189,16 +202,21 @@ class ResidentKV:
         """reorder_sequences of this prefix alone."""
         reorder_sequences([self], index, t_from)
 
-    def select(self, index: torch.Tensor, n_seq: int, blocks: Optional[torch.Tensor] = None,
+    def select(self, index: torch.Tensor, n_seq: Optional[int] = None, blocks: Optional[torch.Tensor] = None,
                cap_tokens: Optional[int] = None) -> "ResidentKV":
         """A new prefix of chosen sequences, and of chosen blocks of each: fork, drop,
-        evict and compact.  This prefix is n_seq sequences of n_heads / n_seq heads;
-        sequence r of the new one is sequence index[r] (index: (R,) whole numbers) and,
-        with blocks (R, n), holds that sequence's 16-token blocks blocks[r] in the order
-        given, else all of them.  The new prefix has its own exception list, with the
-        entries of the chosen blocks only (their number is read back: one host wait), and
-        room for cap_tokens tokens (those it holds by default).  Indices are clamped to
-        their ranges."""
+        evict and compact.  This prefix is n_seq sequences of n_heads / n_seq heads (by
+        default its own n_seq: that of the rows appended, of its construction or of the
+        selection that made it); sequence r of the new one is sequence index[r] (index: (R,)
+        whole numbers) and, with blocks (R, n), holds that sequence's 16-token blocks blocks[r]
+        in the order given, else all of them.  The new prefix has its own exception list,
+        with the entries of the chosen blocks only (their number is read back: one host
+        wait), and room for cap_tokens tokens (those it holds by default).  Indices are
+        clamped to their ranges."""
+        if n_seq is None:
+            n_seq = self.n_seq
+            if n_seq is None:
+                raise ValueError("how many sequences the prefix holds is not known: give n_seq")
         if n_seq < 1 or self.n_heads % n_seq:
             raise ValueError("n_heads must be a multiple of n_seq")
         if index.dim() != 1 or index.numel() < 1 or index.dtype not in (torch.int32, torch.int64):
@@ -219,7 +237,7 @@ class ResidentKV:
         heads = R * (self.n_heads // n_seq)
         if nb == 0:
             new = self._bare(heads, cap, self.n_exc.new_zeros(1), self.status.new_zeros(1))
-            new.exc = self.exc.new_empty(8)
+            new.exc, new.n_seq = self.exc.new_empty(8), R
             return new
         lib = L.lib()
         need = lib.lq_select_workspace(heads, nb)
@@ -250,14 +268,14 @@ class ResidentKV:
             if n:
                 L.check(lib.lq_resident_select_exceptions(*args, ctypes.addressof(dst), stream),
                         "lq_resident_select_exceptions")
-        new._exc_known, new.n_tokens = n, nb * RB
+        new._exc_known, new.n_tokens, new.n_seq = n, nb * RB, R
         return new
 
     def _bare(self, n_heads: int, nb: int, n_exc: torch.Tensor, status: torch.Tensor) -> "ResidentKV":
         """nb blocks of room per head where this prefix lies, uninitialised, with the given
         counters."""
         r = ResidentKV.__new__(ResidentKV)
-        r.device, r.n_heads, r.cap_blocks = self.a.device, n_heads, nb
+        r.device, r.n_heads, r.cap_blocks, r.n_seq, r._n_seq_given = self.a.device, n_heads, nb, None, False
         n = n_heads * nb
         r.a, r.b, r.mask = self.a.new_empty(n * 256), self.b.new_empty(n * 256), self.mask.new_empty(n * 4)
         r.meta, r.scale = self.meta.new_empty(n * 4), self.scale.new_empty(n * RB)

@@ -442,3 +442,46 @@ def test_workspaces_geometry():
         assert lib.lq_accept_workspace(*bad) == -1
     for bad in ((0, 5), (5, 0), (1 << 20, 1 << 20)):
         assert lib.lq_select_workspace(*bad) == -1
+
+
+def test_select_needs_to_know_the_sequences():
+    """Without n_seq, and none known of the prefix (or rows appended in two groupings),
+    there is nothing to select from."""
+    from latticequant_amd.llm.resident import ResidentKV
+    i = torch.arange(2)
+    r = ResidentKV(4, 16, device="cpu")
+    with pytest.raises(ValueError):
+        r.select(i)
+    for n in (0, -1, 3):
+        with pytest.raises(ValueError):
+            ResidentKV(4, 16, device="cpu", n_seq=n)
+    r = ResidentKV(4, 16, device="cpu", n_seq=2)
+    with pytest.raises(ValueError):                      # rows of four sequences, by a prefix of two
+        r.append(torch.zeros(4, 1, 16, 128), torch.ones(4), torch.ones(4).half())
+
+
+@gpu
+def test_select_of_known_sequences_gpu():
+    """n_seq is the prefix's own by default: that of the rows appended, of its construction,
+    or of the selection that made it."""
+    from latticequant_amd.llm.resident import ResidentKV
+    r = _prefix(3, 2, 64, 9)
+    index, blocks = torch.tensor([2, 0, 2, 1], device="cuda"), torch.randint(0, 4, (4, 3), device="cuda")
+    planes = ResidentKV(6, 112, device="cuda", n_seq=3)   # planes made elsewhere
+    for p in PLANES + ("exc", "n_exc"):
+        setattr(planes, p, getattr(r, p))
+    planes.n_tokens = 64
+    for b in (None, blocks):
+        want = r.select(index, 3, blocks=b)
+        for src in (r, planes):
+            got = src.select(index, blocks=b)
+            assert got.n_seq == 4 and torch.equal(got.dequant(), want.dequant())
+            assert torch.equal(got.select(index[:2]).dequant(), want.select(index[:2], 4).dequant())
+    assert ResidentKV(6, 16, device="cuda", n_seq=3).select(index).n_seq == 4
+    flat = ResidentKV(6, 64, device="cuda")
+    x, s = torch.randn(3, 2, 16, 128, device="cuda").half(), torch.full((6,), 0.25, device="cuda")
+    flat.append(x, s, s.half())
+    flat.append(x.reshape(1, 6, 16, 128), s, s.half())    # two groupings: which one is meant?
+    with pytest.raises(ValueError):
+        flat.select(index)
+    assert torch.equal(flat.select(torch.tensor([1]), 3).dequant(), flat.dequant()[2:4])
