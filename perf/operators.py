@@ -241,7 +241,7 @@ def _blocks(lead, case, seed):
 def _resident(case, planes, exc=None):
     """A ResidentKV whose planes are these tensors (layers allocated together)."""
     from latticequant_amd.llm.resident import ResidentKV
-    r = ResidentKV(case["batch"] * case["heads"], case["tokens"], device="cuda")
+    r = ResidentKV(case["batch"] * case["heads"], case["tokens"], device="cuda", n_seq=case["batch"])
     for p, t in planes.items():
         setattr(r, p, t.reshape(-1))
     if exc is not None:
@@ -416,7 +416,7 @@ def run(state):
         return st["planes"]
     out = []
     for r in st["res"]:
-        n = r.select(st["index"], st["case"]["batch"], blocks=st["blocks"])
+        n = r.select(st["index"], blocks=st["blocks"])
         out.append({**{p: getattr(n, p) for p in PLANES}, "exc": n.exceptions().reshape(-1)})
     return out
 
