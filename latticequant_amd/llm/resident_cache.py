@@ -254,17 +254,17 @@ class ResidentKVCache(DynamicCache):
         A, dev = path.shape[1], self._parents.device
         full = torch.full((B, N), -1, dtype=torch.int32, device=dev)
         full[:, :A] = path.clamp(0, N - 1)
-        groups = {}                                # layers of one shape, type and tail length: all of them, as a rule
+        groups = {}                                # rows of one shape, type and tail length: K and V of all layers, as a rule
         for i in range(len(self.tail_k)):
             t = self.tail_k[i].shape[2]
-            key = (t, self._buffers(i, t + A)[0].shape, self.tail_k[i].dtype, self._drafts[i][0].dtype)
-            groups.setdefault(key, []).append(i)
-        for (t, _, dt, _), layers in groups.items():
+            for buf, d in zip(self._buffers(i, t + A), self._drafts[i]):
+                groups.setdefault((t, buf.shape, buf.dtype), []).append((buf, d.to(buf.dtype)))
+        for (t, _, _), pairs in groups.items():
             count, at = (torch.full((B,), n, dtype=torch.int32, device=dev) for n in (A, t))
-            append_accepted([b for i in layers for b in self._room[i]],
-                            [d.to(dt) for i in layers for d in self._drafts[i]], full, count, at)
-            for i in layers:
-                self.tail_k[i], self.tail_v[i] = (b[:, :, :t + A] for b in self._room[i])
+            append_accepted(*zip(*pairs), full, count, at)
+        for i in range(len(self.tail_k)):          # (the tails end before the new rows until here)
+            t = self.tail_k[i].shape[2]
+            self.tail_k[i], self.tail_v[i] = (b[:, :, :t + A] for b in self._room[i])
         self.discard()
         for i in range(len(self.tail_k)):
             over = self.tail_k[i].shape[2] - self.tail_tokens

@@ -331,3 +331,24 @@ def test_draft_refusals():
     c.discard()
     c.update(k, k, 0)
     assert c.get_seq_length() == 8
+
+
+@gpu
+def test_accept_of_keys_and_values_of_two_types_gpu():
+    """K and V of different types (a model under autocast rotates K in float32)."""
+    from latticequant_amd.llm.resident_cache import ResidentKVCache
+    c, g = ResidentKVCache(bits_per_dim=4, tail_tokens=64), torch.Generator().manual_seed(3)
+    new = lambda n: (torch.randn(2, 2, n, 128, generator=g).cuda(),   # noqa: E731
+                     torch.randn(2, 2, n, 128, generator=g).bfloat16().cuda())
+    for i in range(2):
+        c.update(*new(20), i)
+    want = [[x.clone() for x in c.materialise(i)] for i in range(2)]
+    c.draft([-1, 0, 0])
+    d = [new(3) for _ in range(2)]
+    for i in range(2):
+        c.update(*d[i], i)
+    c.accept(torch.tensor([[0, 2], [0, 1]], device="cuda"))
+    for i in range(2):
+        for x, w, y in zip(c.materialise(i), want[i], d[i]):
+            assert x.dtype == y.dtype
+            assert torch.equal(x, torch.cat([w, torch.stack([y[0][:, [0, 2]], y[1][:, [0, 1]]])], 2))
