@@ -254,12 +254,12 @@ class ResidentKVCache(DynamicCache):
         A, dev = path.shape[1], self._parents.device
         full = torch.full((B, N), -1, dtype=torch.int32, device=dev)
         full[:, :A] = path.clamp(0, N - 1)
-        groups = {}                                # rows of one shape, type and tail length: K and V of all layers, as a rule
+        groups = {}                                # rows of one shape, type, device and tail length: K and V of all layers, as a rule
         for i in range(len(self.tail_k)):
             t = self.tail_k[i].shape[2]
             for buf, d in zip(self._buffers(i, t + A), self._drafts[i]):
-                groups.setdefault((t, buf.shape, buf.dtype), []).append((buf, d.to(buf.dtype)))
-        for (t, _, _), pairs in groups.items():
+                groups.setdefault((t, buf.shape, buf.dtype, buf.device), []).append((buf, d.to(buf.dtype)))
+        for (t, *_), pairs in groups.items():
             count, at = (torch.full((B,), n, dtype=torch.int32, device=dev) for n in (A, t))
             append_accepted(*zip(*pairs), full, count, at)
         for i in range(len(self.tail_k)):          # (the tails end before the new rows until here)

@@ -352,3 +352,55 @@ def test_accept_of_keys_and_values_of_two_types_gpu():
         for x, w, y in zip(c.materialise(i), want[i], d[i]):
             assert x.dtype == y.dtype
             assert torch.equal(x, torch.cat([w, torch.stack([y[0][:, [0, 2]], y[1][:, [0, 1]]])], 2))
+
+
+class _Stand:
+    """What the cache asks of a prefix, without a GPU."""
+
+    def __init__(self, n_heads, n_tokens, device, log):
+        self.n_heads, self.n_tokens, self.cap_blocks, self.log = n_heads, n_tokens, n_tokens // 16, log
+        self.a = torch.empty(0, device=device)
+
+    def select(self, index, n_seq=None, blocks=None, cap_tokens=None):
+        self.log.append(self.n_heads)
+        return _Stand(index.numel() * self.n_heads // n_seq, self.n_tokens, self.a.device, self.log)
+
+
+def _two_devices(monkeypatch, heads=(2, 2)):
+    """A cache of two layers on two devices, the moves replaced by their checks (rows and
+    prefixes of one device and shape) and a record."""
+    from latticequant_amd.llm import resident_cache as rc
+    c, log = rc.ResidentKVCache(bits_per_dim=4, tail_tokens=64), []
+    for i, dev in enumerate(("cpu", "meta")):
+        c.update(*(torch.zeros(2, heads[i], 20, 128, device=dev) for _ in range(2)), i)
+        c.res_k[i], c.res_v[i] = (_Stand(2 * heads[i], 32, dev, log) for _ in range(2))
+
+    def one(ts):
+        if len({(t.device, t.shape, t.dtype) for t in ts}) != 1:
+            raise ValueError("rows on one GPU, of one shape and type")
+
+    def gather(tails, index):
+        one(tails)
+        return [t.new_empty((index.numel(),) + t.shape[1:]) for t in tails]
+
+    def append(tails, drafts, path, count, tail_len):
+        one(tails)
+        one(drafts)
+        log.append(len(tails))
+
+    def reorder(res, index, t_from=0):
+        if len({(r.a.device, r.n_heads, r.n_tokens) for r in res}) != 1:
+            raise ValueError("the prefixes must have the same heads, tokens and device")
+        log.append(len(res))
+    for name, f in (("gather_tails", gather), ("append_accepted", append), ("reorder_sequences", reorder)):
+        monkeypatch.setattr(rc, name, f)
+    return c, log
+
+
+def test_accept_of_layers_on_two_devices(monkeypatch):
+    c, log = _two_devices(monkeypatch)
+    c.draft([-1, 0, 0])
+    for i, dev in enumerate(("cpu", "meta")):
+        c.update(*(torch.zeros(2, 2, 3, 128, device=dev) for _ in range(2)), i)
+    c.accept(torch.tensor([[0, 2], [0, 1]]))
+    assert log == [2, 2] and [t.shape[2] for t in c.tail_k + c.tail_v] == [22] * 4
