@@ -298,11 +298,11 @@ class ResidentKVCache(DynamicCache):
             return self.batch_select_indices(beam_idx)
         self._no_draft()
         idx = self._numbers(beam_idx)
-        by_length = {}
+        groups = {}                                # prefixes of one length, head count and device: all of them, as a rule
         for r in self.res_k + self.res_v:
             if r is not None:
-                by_length.setdefault(r.n_tokens, []).append(r)
-        for group in by_length.values():
+                groups.setdefault((r.n_tokens, r.n_heads, r.a.device), []).append(r)
+        for group in groups.values():
             reorder_sequences(group, idx)
         self._select_rest(idx)
 
@@ -343,16 +343,14 @@ class ResidentKVCache(DynamicCache):
 
     def _select_rest(self, idx):
         """Tails and at-rest chunks of the sequences idx."""
-        shapes = {}
-        for i, (tk, tv) in enumerate(zip(self.tail_k, self.tail_v)):
-            shapes.setdefault((tk.shape, tk.dtype, tv.dtype), []).append(i)
-        for layers in shapes.values():
-            if self.tail_k[layers[0]].dtype == self.tail_v[layers[0]].dtype:
-                new = gather_tails([t for i in layers for t in (self.tail_k[i], self.tail_v[i])], idx)
-            else:
-                new = [t.index_select(0, idx) for i in layers for t in (self.tail_k[i], self.tail_v[i])]
-            for j, i in enumerate(layers):
-                self.tail_k[i], self.tail_v[i] = new[2 * j], new[2 * j + 1]
+        layers, tails = len(self.tail_k), self.tail_k + self.tail_v
+        groups = {}                                # tails of one shape, type and device
+        for j, t in enumerate(tails):
+            groups.setdefault((t.shape, t.dtype, t.device), []).append(j)
+        for group in groups.values():
+            for j, t in zip(group, gather_tails([tails[j] for j in group], idx)):
+                tails[j] = t
+        self.tail_k, self.tail_v = tails[:layers], tails[layers:]
         self._room = {}
         for ch in self.chunks:
             for pair in ch:

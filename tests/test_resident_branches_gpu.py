@@ -404,3 +404,14 @@ def test_accept_of_layers_on_two_devices(monkeypatch):
         c.update(*(torch.zeros(2, 2, 3, 128, device=dev) for _ in range(2)), i)
     c.accept(torch.tensor([[0, 2], [0, 1]]))
     assert log == [2, 2] and [t.shape[2] for t in c.tail_k + c.tail_v] == [22] * 4
+
+
+@pytest.mark.parametrize("heads", [(2, 2), (2, 1)])
+def test_sequences_of_layers_on_two_devices(monkeypatch, heads):
+    """Also where the layers have different numbers of heads."""
+    c, log = _two_devices(monkeypatch, heads)
+    c.reorder_cache(torch.tensor([1, 0]))
+    assert log == [2, 2]
+    c.batch_select_indices(torch.tensor([1, 0, 1]))
+    assert [r.n_heads for r in c.res_k + c.res_v] == [3 * h for h in heads] * 2
+    assert [tuple(t.shape[:3]) for t in c.tail_k + c.tail_v] == [(3, h, 20) for h in heads] * 2
