@@ -302,14 +302,16 @@ class ResidentKVCache(DynamicCache):
         for r in self.res_k + self.res_v:
             if r is not None:
                 groups.setdefault((r.n_tokens, r.n_heads, r.a.device), []).append(r)
+        tails = self._tails_of(idx)                # before anything moves: it may find no room
         for group in groups.values():
             reorder_sequences(group, idx)
-        self._select_rest(idx)
+        self._continue_as(idx, tails)
 
     def batch_select_indices(self, indices: torch.Tensor) -> None:
         """Keep the sequences indices[r], in that order (a sequence may stand several
         times; -1 is the last one, what is out of range is clamped); the others' resident
-        blocks and exceptions are freed."""
+        blocks and exceptions are freed, once all layers' new ones are there: a selection
+        that finds no room leaves the cache as it was."""
         if not self.tail_k:
             return
         self._no_draft()
@@ -318,11 +320,10 @@ class ResidentKVCache(DynamicCache):
         if idx.dim() != 1 or idx.numel() < 1:
             raise ValueError("indices must be a list of sequences")
         idx = self._numbers(idx)
-        for res in (self.res_k, self.res_v):
-            for i, r in enumerate(res):
-                if r is not None:
-                    res[i] = r.select(idx, B, cap_tokens=r.cap_blocks * RB)
-        self._select_rest(idx)
+        new = [None if r is None else r.select(idx, B, cap_tokens=r.cap_blocks * RB) for r in self.res_k + self.res_v]
+        tails = self._tails_of(idx)
+        self.res_k, self.res_v = new[:len(self.res_k)], new[len(self.res_k):]
+        self._continue_as(idx, tails)
 
     def batch_repeat_interleave(self, repeats: int) -> None:
         """Every sequence `repeats` times in a row (a prompt's beams)."""
@@ -341,15 +342,20 @@ class ResidentKVCache(DynamicCache):
         idx = idx.to(self.tail_k[0].device)
         return torch.where(idx < 0, idx + B, idx).clamp(0, B - 1)
 
-    def _select_rest(self, idx):
-        """Tails and at-rest chunks of the sequences idx."""
-        layers, tails = len(self.tail_k), self.tail_k + self.tail_v
+    def _tails_of(self, idx) -> list:
+        """New tails of the sequences idx: K of all layers, then V."""
+        tails = self.tail_k + self.tail_v
         groups = {}                                # tails of one shape, type and device
         for j, t in enumerate(tails):
             groups.setdefault((t.shape, t.dtype, t.device), []).append(j)
         for group in groups.values():
             for j, t in zip(group, gather_tails([tails[j] for j in group], idx)):
                 tails[j] = t
+        return tails
+
+    def _continue_as(self, idx, tails) -> None:
+        """The tails of the sequences idx, and their at-rest chunks."""
+        layers = len(self.tail_k)
         self.tail_k, self.tail_v = tails[:layers], tails[layers:]
         self._room = {}
         for ch in self.chunks:

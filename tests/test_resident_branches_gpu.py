@@ -415,3 +415,29 @@ def test_sequences_of_layers_on_two_devices(monkeypatch, heads):
     c.batch_select_indices(torch.tensor([1, 0, 1]))
     assert [r.n_heads for r in c.res_k + c.res_v] == [3 * h for h in heads] * 2
     assert [tuple(t.shape[:3]) for t in c.tail_k + c.tail_v] == [(3, h, 20) for h in heads] * 2
+
+
+@pytest.mark.parametrize("fails", ["gather_tails", "select"])
+def test_a_selection_that_fails_changes_nothing(monkeypatch, fails):
+    from latticequant_amd.llm import resident_cache as rc
+    c, _ = _two_devices(monkeypatch)
+    n = 0
+
+    def no_room(*a, **kw):
+        nonlocal n
+        n += 1
+        if n > 1:                                        # the second call: the first one's result is there already
+            raise torch.OutOfMemoryError("no room")
+        return done(*a, **kw)
+    done = getattr(rc, fails) if fails == "gather_tails" else _Stand.select
+    monkeypatch.setattr(*((rc, fails) if fails == "gather_tails" else (_Stand, fails)), no_room)
+    before = list(map(id, c.res_k + c.res_v + c.tail_k + c.tail_v))
+    with pytest.raises(torch.OutOfMemoryError):
+        c.batch_select_indices(torch.tensor([1, 1, 0]))
+    assert list(map(id, c.res_k + c.res_v + c.tail_k + c.tail_v)) == before
+    if fails == "gather_tails":
+        n, moved = 0, []
+        monkeypatch.setattr(rc, "reorder_sequences", lambda *a, **kw: moved.append(a))
+        with pytest.raises(torch.OutOfMemoryError):
+            c.reorder_cache(torch.tensor([1, 0]))
+        assert not moved and list(map(id, c.tail_k + c.tail_v)) == before[4:]
