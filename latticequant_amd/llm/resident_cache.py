@@ -69,6 +69,7 @@ class ResidentKVCache(DynamicCache):
         self.tail_k: List[Optional[torch.Tensor]] = []
         self.tail_v: List[Optional[torch.Tensor]] = []
         self.chunks: List[list] = []          # per layer: [(_AtRest K, _AtRest V)] rANS chunks at rest
+        self._epochs = _Epochs()
         self._work = None
         self._work_heads = 0
         self._parents = self._start = None    # drafted tree of the next forward
@@ -101,7 +102,8 @@ class ResidentKVCache(DynamicCache):
             elif r.n_tokens + n > r.cap_blocks * RB:
                 r.reserve(max(2 * r.cap_blocks * RB, r.n_tokens + n))
             r.append(x, s32[i], s16[i])
-        self.chunks[layer_idx].append((_AtRest(pend, 0), _AtRest(pend, 1)))
+        since = self._epochs.now()
+        self.chunks[layer_idx].append((_AtRest(pend, 0, since), _AtRest(pend, 1, since)))
         self._room.pop(layer_idx, None)
         self.tail_k[layer_idx] = tk[:, :, n:].contiguous()
         self.tail_v[layer_idx] = tv[:, :, n:].contiguous()
@@ -358,10 +360,7 @@ class ResidentKVCache(DynamicCache):
         layers = len(self.tail_k)
         self.tail_k, self.tail_v = tails[:layers], tails[layers:]
         self._room = {}
-        for ch in self.chunks:
-            for pair in ch:
-                for e in pair:
-                    e.rows = idx.long() if e.rows is None else e.rows[idx.long()]
+        self._epochs.select(idx)
 
     def get_seq_length(self, layer_idx=0):
         if layer_idx >= len(self.tail_k) or self.tail_k[layer_idx] is None:
@@ -393,14 +392,14 @@ class ResidentKVCache(DynamicCache):
         pending encodes (one host sync).  Returns the host bytes held."""
         for ch in self.chunks:
             for i, pair in enumerate(ch):
-                ch[i] = tuple(e if isinstance(e, _HostAtRest) else _HostAtRest(e.batch, e.rows) for e in pair)
+                ch[i] = tuple(e if isinstance(e, _HostAtRest) else _HostAtRest(e.batch, e.since) for e in pair)
         return self.at_rest_host_bytes()
 
     def restore_at_rest(self):
         """Bring offloaded chunk pairs back to the device (codec.from_bytes)."""
         for ch in self.chunks:
             for i, pair in enumerate(ch):
-                ch[i] = tuple(_DeviceAtRest(e.batch, e.rows) if isinstance(e, _HostAtRest) else e for e in pair)
+                ch[i] = tuple(_DeviceAtRest(e.batch, e.since) if isinstance(e, _HostAtRest) else e for e in pair)
 
     def at_rest_host_bytes(self) -> int:
         return sum(e.nbytes for ch in self.chunks for pair in ch for e in pair if isinstance(e, _HostAtRest))
@@ -420,14 +419,52 @@ class ResidentKVCache(DynamicCache):
         return sum(t.numel() * t.element_size() for t in self.tail_k + self.tail_v if t is not None)
 
 
-class _AtRest:
-    """One K or V half of a flushed chunk pair, settled on first access.  rows: the
-    chunk's sequence that each sequence of the cache is (None: the same one); a chunk's
-    bitstreams are its own whole, so reordering and selecting move only this."""
+class _Epochs:
+    """Which of its sequences a chunk has for each sequence of the cache.  A chunk's
+    bitstreams are its own whole, so reordering and selecting move only these numbers: one
+    row of a table for all chunks flushed between two selections, (epochs, sequences) int64
+    on the device, so that a selection is the same few launches however many chunks there
+    are."""
 
-    rows = None
+    def __init__(self):
+        self.table, self._open = None, False   # _open: chunks since the last selection, which have no row yet
 
-    def __init__(self, pend, index: int):
+    def now(self) -> tuple:
+        """The epoch of a chunk that is flushed now."""
+        self._open = True
+        return self, 0 if self.table is None else self.table.shape[0]
+
+    def rows(self, epoch: int) -> Optional[torch.Tensor]:
+        """The chunk's sequence that each of the cache's is; None: the same one."""
+        return None if self.table is None or epoch == self.table.shape[0] else self.table[epoch]
+
+    def select(self, idx: torch.Tensor) -> None:
+        idx = idx.long()
+        held = [] if self.table is None else [self.table.index_select(1, idx)]
+        if self._open:
+            held.append(idx[None])
+        if held:
+            self.table, self._open = torch.cat(held), False
+
+
+class _Half:
+    """One K or V half of a flushed chunk pair; since: _Epochs.now() when it was flushed."""
+
+    def __init__(self, since):
+        self.since = since
+
+    @property
+    def rows(self) -> Optional[torch.Tensor]:
+        """The chunk's sequence that each sequence of the cache is (None: the same one)."""
+        epochs, at = self.since
+        return epochs.rows(at)
+
+
+class _AtRest(_Half):
+    """A half as it was flushed, settled on first access."""
+
+    def __init__(self, pend, index: int, since):
+        super().__init__(since)
         self._pend, self._index = pend, index
 
     @property
@@ -438,22 +475,23 @@ class _AtRest:
         return int(self.batch.reference_bytes().sum())
 
 
-class _DeviceAtRest:
-    """An at-rest half held on the device as a settled batch."""
+class _DeviceAtRest(_Half):
+    """A half held on the device as a settled batch."""
 
-    def __init__(self, batch, rows=None):
-        self.batch, self.rows = batch, rows
+    def __init__(self, batch, since):
+        super().__init__(since)
+        self.batch = batch
 
     def reference_bytes(self) -> int:
         return int(self.batch.reference_bytes().sum())
 
 
-class _HostAtRest:
-    """An at-rest half held in host memory in the wire form; .batch restores
-    it to the current device (a new device copy per access)."""
+class _HostAtRest(_Half):
+    """A half held in host memory in the wire form; .batch restores it to the current
+    device (a new device copy per access)."""
 
-    def __init__(self, batch, rows=None):
-        self.rows = rows
+    def __init__(self, batch, since):
+        super().__init__(since)
         self.blob = codec.to_bytes(batch)
         self.nbytes = len(self.blob)
         self._ref = int(batch.reference_bytes().sum())

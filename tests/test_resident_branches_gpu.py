@@ -441,3 +441,47 @@ def test_a_selection_that_fails_changes_nothing(monkeypatch, fails):
         with pytest.raises(torch.OutOfMemoryError):
             c.reorder_cache(torch.tensor([1, 0]))
         assert not moved and list(map(id, c.tail_k + c.tail_v)) == before[4:]
+
+
+@gpu
+@pytest.mark.parametrize("how", ["reorder_cache", "batch_select_indices"])
+def test_launches_of_a_reorder_do_not_grow_with_the_chunks_gpu(how):
+    """As many operations after 3 as after 24 flushes, chunks of many epochs, some of them
+    held by the host; the maps are those of chunk by chunk."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from latticequant_amd import codec
+
+    class Count(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.n = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.n += 1
+            return func(*args, **(kwargs or {}))
+    g = torch.Generator().manual_seed(7)
+    c, ops, maps = _filled(3, layers=2, tail=16, tokens=40), [], [[], []]
+    for turn in range(24):
+        for i in range(2):
+            k, v = (torch.randn(3, 2, 16, 128, generator=g).half().cuda() for _ in range(2))
+            c.update(k, v, i)
+            maps[i] += [list(range(3))] * (len(c.chunks[i]) - len(maps[i]))
+        idx = torch.randint(0, 3, (3,), generator=g)
+        with Count() as n:
+            getattr(c, how)(idx.cuda())
+        ops.append(n.n)
+        maps = [[[m[j] for j in idx.tolist()] for m in x] for x in maps]
+        if turn % 2 == 0:
+            getattr(c, how)(torch.tensor([1, 1, 2]).cuda())   # no flush since the last one
+            maps = [[[m[j] for j in (1, 1, 2)] for m in x] for x in maps]
+        if turn == 9:
+            c.offload_at_rest()
+        elif turn == 14:
+            c.restore_at_rest()
+    for i in range(2):
+        assert [[e.rows.tolist() for e in pair] for pair in c.chunks[i]] == [[m, m] for m in maps[i]]
+    half = c.chunks[1][3][0]
+    rows = codec.decode_batch(half.batch).reshape(3, 2, -1, 128)[half.rows]
+    at = sum(pair[0].batch.shape[2] for pair in c.chunks[1][:3])
+    assert torch.equal(rows, c.materialise(1)[0][:, :, at:at + rows.shape[2]])
+    assert len(set(ops[2:])) == 1, ops
