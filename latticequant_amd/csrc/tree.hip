@@ -615,9 +615,10 @@ __device__ __forceinline__ void products(const char* lds, const f16_t s[U], int 
         for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
     const float mn = halves_max(mx) * c0;
     if (__any(mn > st.m + kLazy)) {
-        // a row that has seen nothing has m = -inf, l = 0 and o = 0
-        const float up = fmaxf(st.m, mn);
-        const float al = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - up);
+        // only the rows that passed it: a row's roundings do not depend on the others of its
+        // wave.  (One that has seen nothing has m = -inf, l = 0 and o = 0.)
+        const float up = mn > st.m + kLazy ? mn : st.m;
+        const float al = up == st.m ? 1.f : __builtin_amdgcn_exp2f(st.m - up);
         st.l *= al;
 #pragma unroll
         for (int d = 0; d < 4; d++)
@@ -1007,8 +1008,8 @@ __device__ __forceinline__ void few_attend(f4_t s[2], uint32_t word, bool every,
     for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[i >> 2][i & 3]);
     const float mn = quarters_max(mx) * c0;
     if (__any(mn > st.m + kLazy)) {
-        const float up = fmaxf(st.m, mn);
-        const float al = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - up);
+        const float up = mn > st.m + kLazy ? mn : st.m;   // as in products
+        const float al = up == st.m ? 1.f : __builtin_amdgcn_exp2f(st.m - up);
         st.l *= al;
 #pragma unroll
         for (int mm = 0; mm < 8; mm++)

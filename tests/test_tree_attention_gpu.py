@@ -407,3 +407,25 @@ def test_tree_workspace_geometry():
                 (1, 8, 5, 0, 32, 0), (1, 8, 5, 17, 32, 0), (1, 8, 5, 4, 33, 0), (1, 8, 5, 4, -16, 0),
                 (1, 8, 5, 4, 32, -1)):
         assert f(*bad) == -1, bad
+
+
+FORMS = [(1, 2, 4, 4, 512, 20),                          # k_tree_few: 16 rows,
+         (1, 2, 4, 8, 512, 20),                          # 32 rows
+         (1, 2, 4, 16, 512, 20),                         # k_tree_many: two waves,
+         (4, 8, 10, 10, 4096, 20),                       # four,
+         (4, 8, 16, 10, 4096, 20)]                       # eight
+
+
+@gpu
+@pytest.mark.parametrize("B,H,G,N,T,cap", FORMS)
+def test_tree_attention_rows_apart_gpu(B, H, G, N, T, cap):
+    """A node that no other sees changes nobody's bits, however large its finite q, K and V."""
+    c = _case(B, H, G, N, T, cap, seed=41, kind="roots")
+    c["par"][:] = -1
+    clean = _run(c)
+    others = torch.arange(N, device="cuda") != 2
+    for n, f in (("q", 30.0), ("dk", 50.0), ("dv", 1000.0)):
+        c[n][:, :, 2] *= f
+        out = _run(c)
+        assert torch.equal(out[:, :, others], clean[:, :, others]), n
+    assert torch.isfinite(out).all() and not torch.equal(out, clean)
