@@ -532,7 +532,7 @@ typedef struct {
     int64_t exc_cap;
 } lq_resident;
 
-#define LQ_RES_ST_EXC_OVERFLOW 1  /* more exceptions than exc_cap: entries beyond it were dropped */
+#define LQ_RES_ST_EXC_OVERFLOW 1  /* more exceptions than exc_cap: entries beyond it were dropped (zero vectors) */
 
 /* Workspace (bytes) of lq_resident_quantize for n_heads x t_tokens. */
 int64_t lq_resident_workspace(int64_t n_heads, int64_t t_tokens);

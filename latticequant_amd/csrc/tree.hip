@@ -368,9 +368,11 @@ __device__ __forceinline__ void each_entry(const lq_resident& r, const Meta& m, 
         const uint32_t k = r0 + (lane & 31);
         if (r0) ent = load_entry(r, {0u, 0u, m.base + r0, m.count > r0 ? m.count - r0 : 0u}, lane);
         const uint32_t rec = most > 7 ? nth_record(mk, k) & 255u : head_rec(m, lane);
-        if (k < m.count && (int64_t)m.base + k < r.exc_cap) {
+        if (k < m.count) {
+            // an entry that the list had no room for is zero (numbers of entries are below 2^31)
+            const uint32_t keep = m.base + k < (uint32_t)min(r.exc_cap, (int64_t)INT_MAX) ? ~0u : 0u;
             uint32_t e[4];
-            exc_pairs(ent, e);
+            exc_pairs(make_uint4(ent.x & keep, ent.y & keep, ent.z & keep, ent.w & keep), e);
             put(rec, e);
         }
     }

@@ -429,3 +429,17 @@ def test_tree_attention_rows_apart_gpu(B, H, G, N, T, cap):
         out = _run(c)
         assert torch.equal(out[:, :, others], clean[:, :, others]), n
     assert torch.isfinite(out).all() and not torch.equal(out, clean)
+
+
+@gpu
+@pytest.mark.parametrize("B,H,G,N,T,cap", FORMS)
+def test_tree_attention_dropped_exceptions_gpu(B, H, G, N, T, cap):
+    """Vectors that a too short exception list dropped are zero, as dequant() has them."""
+    c = _case(B, H, G, N, T, cap, seed=43)
+    for n in "kv":
+        r = c[n]
+        counts = r.meta.view(B * H, -1, 4)[:, :T // 16, 3]
+        total = int(counts.sum())
+        assert total > 200
+        r.exc, r._st = r.exc[:(total // 2 + 3) * 8].clone(), None
+    _check(_run(c), c)
