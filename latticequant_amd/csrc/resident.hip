@@ -375,8 +375,9 @@ __device__ __forceinline__ void tile_k(const AttnArgs& A, const TileRaw& d, int 
             const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.x, 4 * x + c);
             const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)d.mask.y, 4 * x + c);
             const int64_t idx = base + __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0u));
-            mine[c] = (((lane & 32) ? hi : lo) >> (lane & 31)) & 1u && idx < A.k.exc_cap;
-            if (mine[c]) ex[c] = reinterpret_cast<const uint4*>(A.k.exc)[idx];
+            mine[c] = (((lane & 32) ? hi : lo) >> (lane & 31)) & 1u;
+            ex[c] = make_uint4(0u, 0u, 0u, 0u);   // an entry that the list had no room for is zero
+            if (mine[c] && idx < A.k.exc_cap) ex[c] = reinterpret_cast<const uint4*>(A.k.exc)[idx];
             base += __builtin_popcount(lo) + __builtin_popcount(hi);
         }
     }
@@ -436,8 +437,9 @@ __device__ __forceinline__ void tile_v(const AttnArgs& A, const TileRaw& d, int 
             for (int j = 0; j < 4; j++) {
                 const int q = q0 + j;
                 const int64_t idx = base + __builtin_popcount(own & ((1u << q) - 1u));
-                mine[j] = ((own >> q) & 1u) && idx < A.v.exc_cap;
-                if (mine[j]) ex[j] = reinterpret_cast<const uint4*>(A.v.exc)[idx];
+                mine[j] = (own >> q) & 1u;
+                ex[j] = make_uint4(0u, 0u, 0u, 0u);
+                if (mine[j] && idx < A.v.exc_cap) ex[j] = reinterpret_cast<const uint4*>(A.v.exc)[idx];
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) {

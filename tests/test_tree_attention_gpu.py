@@ -443,3 +443,15 @@ def test_tree_attention_dropped_exceptions_gpu(B, H, G, N, T, cap):
         assert total > 200
         r.exc, r._st = r.exc[:(total // 2 + 3) * 8].clone(), None
     _check(_run(c), c)
+
+
+@gpu
+def test_decode_attention_dropped_exceptions_gpu():
+    """The one-token step has them as zero too."""
+    from latticequant_amd.llm.resident import resident_decode_attention
+    c = _case(2, 4, 4, 1, 1040, 30, seed=45)
+    for n in "kv":
+        r = c[n]
+        r.exc, r._st = r.exc[:(int(r.n_exc.item()) // 2 + 3) * 8].clone(), None
+    _check(resident_decode_attention(c["k"], c["v"], c["q"], torch.cat([c["tk"], c["dk"]], 2),
+                                     torch.cat([c["tv"], c["dv"]], 2)), c)
