@@ -32,11 +32,12 @@ _DTYPES = (torch.float16, torch.bfloat16)
 
 def _rows(t: torch.Tensor):
     """(t, pointer and strides of (B, H, T, 128) rows): as it lies where the kernels can
-    read 16 bytes at a time, else a contiguous copy."""
+    read 16 bytes at a time, else a copy.  (contiguous() makes none of a tensor that is
+    contiguous and unaligned, or whose odd stride is that of a length of one.)"""
     sb, sh, st, se = t.stride()
     p = t.data_ptr()
     if se != 1 or (sb | sh | st) & 7 or p & 15:
-        t = t.contiguous()
+        t = t.clone(memory_format=torch.contiguous_format)
         sb, sh, st, _ = t.stride()
         p = t.data_ptr()
     return t, (p, sb, sh, st)
@@ -284,7 +285,7 @@ def _pairs(dst: Sequence[torch.Tensor], src: Sequence[torch.Tensor], what: str):
     if not all(map(fits, set(st))) or reduce(or_, sp) & 15:
         for i, t in enumerate(src):
             if not fits(st[i]) or sp[i] & 15:
-                src[i] = t.contiguous()
+                src[i] = t.clone(memory_format=torch.contiguous_format)
                 st[i], sp[i] = src[i].stride(), src[i].data_ptr()
 
     def group(td, ts, d, s):

@@ -485,3 +485,22 @@ def test_select_of_known_sequences_gpu():
     with pytest.raises(ValueError):
         flat.select(index)
     assert torch.equal(flat.select(torch.tensor([1]), 3).dequant(), flat.dequant()[2:4])
+
+
+@gpu
+def test_row_moves_of_unaligned_sources_gpu():
+    """Sources that are contiguous but start between 16-byte boundaries are copied, as those of
+    odd strides are."""
+    from latticequant_amd.llm.tree import append_accepted, gather_tails
+    flat = torch.randn(2 * 3 * 5 * 128 + 8, device="cuda").half()
+    tail = torch.zeros(2, 3, 8, 128, dtype=torch.float16, device="cuda")
+    path = torch.arange(5, dtype=torch.int32, device="cuda").expand(2, 5).contiguous()
+    for off in (1, 3, 4):
+        d = flat[off:off + 2 * 3 * 5 * 128].view(2, 3, 5, 128)
+        assert d.data_ptr() % 16
+        new = append_accepted([tail], [d], path, torch.tensor([5, 2], device="cuda"), torch.tensor([0, 1], device="cuda"))
+        assert new.tolist() == [5, 3] and torch.equal(tail[0, :, :5], d[0]) and torch.equal(tail[1, :, 1:3], d[1, :, :2])
+        assert torch.equal(gather_tails([d], torch.tensor([1, 1, 0]))[0], d[[1, 1, 0]])
+    d = torch.randn(3, 5, 128, 1, device="cuda").half().movedim(3, 0)   # a length of one whose stride is 1
+    assert d.stride(0) == 1
+    assert torch.equal(gather_tails([d], torch.tensor([0, 0]))[0], d[[0, 0]])

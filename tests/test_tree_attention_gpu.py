@@ -455,3 +455,21 @@ def test_decode_attention_dropped_exceptions_gpu():
         r.exc, r._st = r.exc[:(int(r.n_exc.item()) // 2 + 3) * 8].clone(), None
     _check(resident_decode_attention(c["k"], c["v"], c["q"], torch.cat([c["tk"], c["dk"]], 2),
                                      torch.cat([c["tv"], c["dv"]], 2)), c)
+
+
+@gpu
+def test_tree_attention_unaligned_rows_gpu():
+    """Rows that are contiguous but start between 16-byte boundaries, or have an odd stride
+    over a length of one, are copied like those of other odd strides."""
+    c = _case(1, 2, 4, 9, 160, 40, seed=3)
+    want = _run(c)
+    for off in (1, 4):
+        d = dict(c)
+        for n in ("q", "dk", "dv", "tk", "tv"):
+            flat = torch.empty(c[n].numel() + 8, dtype=torch.float16, device="cuda")
+            d[n] = flat[off:off + c[n].numel()].view(c[n].shape)
+            d[n].copy_(c[n])
+            assert d[n].data_ptr() % 16
+        assert torch.equal(_run(d), want)
+    d = dict(c, q=c["q"][0].unsqueeze(-1).movedim(3, 0))
+    assert d["q"].stride(0) == 1 and torch.equal(_run(d), want)
