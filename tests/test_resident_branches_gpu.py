@@ -485,3 +485,33 @@ def test_launches_of_a_reorder_do_not_grow_with_the_chunks_gpu(how):
     at = sum(pair[0].batch.shape[2] for pair in c.chunks[1][:3])
     assert torch.equal(rows, c.materialise(1)[0][:, :, at:at + rows.shape[2]])
     assert len(set(ops[2:])) == 1, ops
+
+
+@gpu
+def test_generate_with_beams_over_a_compressed_prefix_gpu():
+    """Every reorder of a beam search over flushed tokens gives each layer the rows that plain
+    indexing of the materialised cache gives, and the search goes as it does with selections
+    that copy the sequences."""
+    from latticequant_amd.llm.resident_cache import ResidentKVCache
+    seen = []
+
+    class Checked(ResidentKVCache):
+        def reorder_cache(self, beam_idx):
+            before = [[x.clone() for x in self.materialise(i)] for i in range(len(self))]
+            super().reorder_cache(beam_idx)
+            for i, old in enumerate(before):
+                for x, y in zip(self.materialise(i), old):
+                    assert torch.equal(x, y[beam_idx])
+            seen.append((self.res_k[0].n_tokens, beam_idx.tolist() != list(range(beam_idx.numel()))))
+
+    class Copied(ResidentKVCache):
+        def reorder_cache(self, beam_idx):
+            self.batch_select_indices(beam_idx)
+    model, cfg = _model()
+    ids = torch.randint(0, cfg.vocab_size, (2, 40), generator=torch.Generator().manual_seed(2)).cuda()
+    kw = dict(num_beams=3, max_new_tokens=40, do_sample=False, return_dict_in_generate=True, output_scores=True,
+              pad_token_id=0, eos_token_id=None)
+    a = model.generate(ids, past_key_values=Checked(bits_per_dim=5, tail_tokens=16), **kw)
+    b = model.generate(ids, past_key_values=Copied(bits_per_dim=5, tail_tokens=16), **kw)
+    assert max(n for n, _ in seen) >= 48 and any(moved for _, moved in seen)
+    assert torch.equal(a.sequences, b.sequences) and torch.equal(a.sequences_scores, b.sequences_scores)

@@ -473,3 +473,36 @@ def test_tree_attention_unaligned_rows_gpu():
         assert torch.equal(_run(d), want)
     d = dict(c, q=c["q"][0].unsqueeze(-1).movedim(3, 0))
     assert d["q"].stride(0) == 1 and torch.equal(_run(d), want)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["chain", "tree"])
+@pytest.mark.parametrize("G,N,cap,dtype", [
+    (2, 50, 40, torch.float16),          # 100 rows: teams of four, drafts over two subtiles
+    (4, 40, 0, torch.bfloat16),          # 160 rows: teams of eight, a draft tile with empty subtiles
+    (4, 100, 70, torch.float16),         # 400 rows: two row blocks, drafts cut within the tile
+])
+def test_tree_attention_wide_teams_deep_trees_gpu(G, N, cap, dtype, kind):
+    """Drafts of several words of nodes where a tile holds two or four subtiles."""
+    c = _case(4, 8, G, N, 4096, cap, seed=47, kind=kind, dtype=dtype, ragged=cap > 0)
+    _check(_run(c), c)
+
+
+@gpu
+@pytest.mark.parametrize("G,N", [(2, 50), (4, 40), (4, 100)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_tree_attention_wide_teams_late_node_not_finite_gpu(G, N, bad):
+    """An infinity or NaN in V of a node behind the first 32: its descendants have it, the
+    others keep their bits."""
+    c = _case(4, 8, G, N, 4096, 0, seed=49, kind="tree")
+    for b in range(4):
+        c["par"][b] = torch.tensor([-1] + [i // 2 for i in range(N - 1)])   # a full tree: all nodes valid
+    clean = _run(c)
+    c["dv"][1, :, 35, 3] = bad
+    out = _run(c)
+    hit = _sees(c["par"])[1, :, 35].cuda()
+    assert 1 <= int(hit.sum()) < N - 30
+    assert torch.equal(out[[0, 2, 3]], clean[[0, 2, 3]]) and torch.equal(out[1][:, ~hit], clean[1][:, ~hit])
+    assert not torch.isfinite(out[1, :, hit, 3]).any()
+    rest = torch.arange(128, device="cuda") != 3
+    assert torch.isfinite(out[1][:, hit][..., rest]).all()
