@@ -623,7 +623,8 @@ int64_t lq_tree_attn_workspace(int64_t n_seq, int64_t heads, int64_t n_nodes, in
  *   nothing, are seen by nothing, and their rows of out are zero.
  * q, out: query head kvh * group + g, token = node; group 1..16, n_nodes 1..256;
  * dtype LQ_F16 or LQ_BF16 of q, the drafts, the tail and out (products are fp16:
- * bf16 values outside fp16's range become infinities).  Scale 1 / sqrt(128).
+ * bf16 values beyond fp16's range become infinities, those below 2^-14 lose bits and
+ * below 2^-25 are zero).  Scale 1 / sqrt(128).
  * Tokens that a row does not see do not reach it, whatever their values.
  * Deterministic. */
 int lq_resident_tree_attention(const lq_resident *k, const lq_resident *v, int64_t t_prefix, const lq_rows *q,

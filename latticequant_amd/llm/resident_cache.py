@@ -293,7 +293,8 @@ class ResidentKVCache(DynamicCache):
     # -- beams --------------------------------------------------------------
     def reorder_cache(self, beam_idx: torch.Tensor) -> None:
         """Sequence i becomes sequence beam_idx[i] as it was, in place (-1: the last one;
-        what is out of range is clamped)."""
+        what is out of range is clamped).  Whole prefixes move, what the sequences share
+        too; the launches are a few whatever the number of chunks."""
         if not self.tail_k:
             return
         if beam_idx.dim() != 1 or beam_idx.numel() != self.tail_k[0].shape[0] or beam_idx.numel() > MAX_REORDER:
@@ -313,7 +314,9 @@ class ResidentKVCache(DynamicCache):
         """Keep the sequences indices[r], in that order (a sequence may stand several
         times; -1 is the last one, what is out of range is clamped); the others' resident
         blocks and exceptions are freed, once all layers' new ones are there: a selection
-        that finds no room leaves the cache as it was."""
+        that finds no room leaves the cache as it was.  At-rest chunks stay whole, with the
+        bitstreams of all sequences they were flushed with (their .rows say whose are the
+        cache's).  One host wait per prefix (K and V of each layer)."""
         if not self.tail_k:
             return
         self._no_draft()
@@ -408,7 +411,8 @@ class ResidentKVCache(DynamicCache):
     def compressed_bytes(self) -> int:
         """Bytes of the at-rest chunks as the reference counts them
         (bitstream + coset bits + fp16 scales, llm/compressed_kv_cache.py:113-119),
-        wherever they are held."""
+        wherever they are held; chunks are whole, also those of sequences that a selection
+        has dropped since."""
         return sum(e.reference_bytes() for ch in self.chunks for pair in ch for e in pair)
 
     def resident_bytes(self) -> int:

@@ -114,8 +114,9 @@ def resident_tree_attention(k: ResidentKV, v: ResidentKV, q: torch.Tensor, draft
     Any strides with a contiguous last dimension are read in place.  work:
     tree_attn_workspace, used until the call's work on the stream is done; out: where
     to write, of q's shape and type.  Returns (B, Hq, N, 128).  The products are
-    fp16: bf16 values beyond its range become infinities.  The same inputs give the
-    same bits."""
+    fp16: bf16 values beyond its range become infinities, those below 2^-14 lose bits and
+    below 2^-25 are zero.  The same inputs give the same bits, and tokens that a row does
+    not see do not change its."""
     lib = L.lib()
     dev = k.a.device
     if q.dim() != 4 or q.dtype not in _DTYPES or q.shape[3] != HD:
