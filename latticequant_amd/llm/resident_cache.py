@@ -64,6 +64,10 @@ class ResidentKVCache(DynamicCache):
             raise ValueError(f"tail_tokens must be a non-negative multiple of {RB}")
         self.bits = bits_per_dim
         self.tail_tokens = tail_tokens
+        self._empty()
+
+    # -- storage ----------------------------------------------------------
+    def _empty(self):
         self.res_k: List[Optional[ResidentKV]] = []
         self.res_v: List[Optional[ResidentKV]] = []
         self.tail_k: List[Optional[torch.Tensor]] = []
@@ -77,7 +81,6 @@ class ResidentKVCache(DynamicCache):
         self._room = {}                       # layer -> (K, V) buffers that the tails are the first tokens of
         self._tree_work = None
 
-    # -- storage ----------------------------------------------------------
     def _ensure(self, layer_idx: int):
         while len(self.res_k) <= layer_idx:
             self.res_k.append(None)
@@ -313,8 +316,10 @@ class ResidentKVCache(DynamicCache):
     def batch_select_indices(self, indices: torch.Tensor) -> None:
         """Keep the sequences indices[r], in that order (a sequence may stand several
         times; -1 is the last one, what is out of range is clamped); the others' resident
-        blocks and exceptions are freed, once all layers' new ones are there: a selection
-        that finds no room leaves the cache as it was.  At-rest chunks stay whole, with the
+        blocks and exceptions are freed.  A selection that finds no room for its result
+        leaves the cache as it was; of fewer sequences than there are (or as many) each
+        prefix is freed once its successor is there, and the cache is left empty if there is no
+        room for one after the first.  At-rest chunks stay whole, with the
         bitstreams of all sequences they were flushed with (their .rows say whose are the
         cache's).  One host wait per prefix (K and V of each layer)."""
         if not self.tail_k:
@@ -325,9 +330,23 @@ class ResidentKVCache(DynamicCache):
         if idx.dim() != 1 or idx.numel() < 1:
             raise ValueError("indices must be a list of sequences")
         idx = self._numbers(idx)
-        new = [None if r is None else r.select(idx, B, cap_tokens=r.cap_blocks * RB) for r in self.res_k + self.res_v]
-        tails = self._tails_of(idx)
-        self.res_k, self.res_v = new[:len(self.res_k)], new[len(self.res_k):]
+        tails, old, new = self._tails_of(idx), self.res_k + self.res_v, []
+        layers, fewer = len(self.res_k), idx.numel() <= B
+        if fewer:
+            self.res_k, self.res_v = [], []        # `old` alone holds them
+        try:
+            while len(new) < len(old):
+                i = len(new)
+                new.append(None if old[i] is None else old[i].select(idx, B, cap_tokens=old[i].cap_blocks * RB))
+                if fewer:
+                    old[i] = None
+        except BaseException:
+            if fewer and any(r is not None for r in new):
+                self._empty()
+            else:
+                self.res_k, self.res_v = old[:layers], old[layers:]
+            raise
+        self.res_k, self.res_v = new[:layers], new[layers:]
         self._continue_as(idx, tails)
 
     def batch_repeat_interleave(self, repeats: int) -> None:

@@ -515,3 +515,35 @@ def test_generate_with_beams_over_a_compressed_prefix_gpu():
     b = model.generate(ids, past_key_values=Copied(bits_per_dim=5, tail_tokens=16), **kw)
     assert max(n for n, _ in seen) >= 48 and any(moved for _, moved in seen)
     assert torch.equal(a.sequences, b.sequences) and torch.equal(a.sequences_scores, b.sequences_scores)
+
+
+@pytest.mark.parametrize("room", [0, 1, 3, 4])
+def test_a_selection_of_fewer_frees_as_it_goes(monkeypatch, room):
+    """Where sequences are dropped, a layer's prefix goes as soon as its successor is there, so
+    that little room is needed; without room for the first one the cache stays as it was,
+    and without room later on it is empty, never a mixture."""
+    import gc
+    import weakref
+    c, _ = _two_devices(monkeypatch)
+    old = [weakref.ref(r) for r in c.res_k + c.res_v]
+    before = list(map(id, c.res_k + c.res_v + c.tail_k + c.tail_v))
+    select, alive = _Stand.select, []
+
+    def counted(self, *a, **kw):
+        gc.collect()
+        alive.append(sum(r() is not None for r in old))
+        if len(alive) > room:
+            raise torch.OutOfMemoryError("no room")
+        return select(self, *a, **kw)
+    monkeypatch.setattr(_Stand, "select", counted)
+    if room < 4:
+        with pytest.raises(torch.OutOfMemoryError):
+            c.batch_select_indices(torch.tensor([1]))
+        if room == 0:
+            assert list(map(id, c.res_k + c.res_v + c.tail_k + c.tail_v)) == before
+        else:
+            assert len(c) == c.get_seq_length() == 0 and not c.res_k and not c.res_v and not c.chunks
+    else:
+        c.batch_select_indices(torch.tensor([1]))
+        assert [r.n_heads for r in c.res_k + c.res_v] == [2] * 4
+    assert alive == [4, 3, 2, 1][:room + 1]
