@@ -700,6 +700,73 @@ int lq_resident_select_exceptions(const lq_resident *src, int64_t n_seq, int64_t
                                   int64_t n_out, const int32_t *d_blocks, int64_t n_blocks, const lq_resident *dst,
                                   hipStream_t s);
 
+/* --------------------------------------------------- pages, serving ---- */
+
+/* A pool of pages is an lq_resident of one kv head per row: page p is block p of every
+ * head.  The same prefix form, its blocks read and written by number, so sequences of any
+ * lengths share one pool and may share pages. */
+
+/* Quantize x (n, heads, t_tokens, 128) (heads = r->n_heads, t_tokens a multiple of 16) into
+ * pages: token block j of row i goes to page d_pages[i * (t_tokens / 16) + j] of every
+ * head, with the scales d_scale32 / d_scale16 [i * heads + h], as lq_resident_quantize.  A
+ * number outside the pool moves nothing; one that stands twice leaves its page undefined.
+ * d_room: int32 [n_heads][cap_blocks], zeros at first: how many exception entries each
+ * page owns.  A page that needs more takes the next power of two at *n_exc.  Where the
+ * list is too short (*n_exc > exc_cap, LQ_RES_ST_EXC_OVERFLOW), lengthen it (its first
+ * exc_cap entries kept) and call again: no room is taken twice. */
+int lq_page_quantize(const void *d_x, int dtype, int64_t n, int64_t t_tokens, const float *d_scale32,
+                     const uint16_t *d_scale16, const lq_resident *r, const int32_t *d_pages, int32_t *d_room,
+                     hipStream_t s);
+
+/* Pages back to rows: out (n, heads, per * 16, 128) fp16 / bf16 / fp32 from d_pages (n, per), as
+ * lq_resident_dequant; zeros for numbers outside the pool. */
+int lq_page_dequant(const lq_resident *r, const int32_t *d_pages, int64_t n, int64_t per, void *d_out, int out_dtype,
+                    hipStream_t s);
+
+/* Workspace (bytes) of lq_paged_attention, 16-byte aligned; weights: whether d_weights is
+ * given.  Needs no initialisation; in use until the call's work on the stream is done. */
+int64_t lq_paged_attn_workspace(int64_t n_seq, int64_t heads, int group, int64_t max_pages, int64_t tail_cap, int weights);
+
+/* Attention of one new token of each of n_seq sequences over its pages and its tail:
+ * out[b, qh] = softmax(q[b, qh] . K^T / sqrt(128)) V, kv head qh / group, over pages
+ * d_pages[b * max_pages + j], j < d_n_pages[b], of pools k and v, then the first
+ * d_tail_len[b] (null: tail_cap) rows of the tail.  A sequence without any token has zeros.
+ * Counts are clamped to max_pages and tail_cap, page numbers outside the pool read its last
+ * page, numbers and rows past the counts are not read.
+ * d_weights (nullable; [n_seq][max_pages]): d_weights[b][j] = decay * d_weights[b][j] + the
+ * sum over the query heads of the softmax weight of page j's tokens, j < d_n_pages[b] (decay
+ * 0: that sum, whatever stood there).
+ * dtype LQ_F16 or LQ_BF16 of q, the tail and out, products fp16, as lq_resident_tree_attention.
+ * group 1..16; stride_t of q and out is not used.  Deterministic. */
+int lq_paged_attention(const lq_resident *k, const lq_resident *v, const lq_rows *q, int64_t n_seq, int group,
+                       const int32_t *d_pages, int64_t max_pages, const int32_t *d_n_pages, const lq_rows *tail_k,
+                       const lq_rows *tail_v, int64_t tail_cap, const int32_t *d_tail_len, float *d_weights, float decay,
+                       int dtype, void *d_work, int64_t work_bytes, const lq_rows *out, hipStream_t s);
+
+/* Each sequence's pages down to `keep` (>= sink + recent): the first `sink` and the last
+ * `recent` stay, and of the others those of most weight (NaN above all, the lower place of
+ * equal ones), in their order.  Tables and weights are [n_seq][max_pages]; those written
+ * are others than those read.  d_out_pages / d_out_weights: the d_out_n[b] kept, then -1 and
+ * 0; d_freed: the others' numbers in order, then -1. */
+int lq_evict_pages(const int32_t *d_pages, const int32_t *d_n_pages, const float *d_weights, int64_t n_seq,
+                   int64_t max_pages, int64_t keep, int64_t sink, int64_t recent, int32_t *d_out_pages, int32_t *d_out_n,
+                   float *d_out_weights, int32_t *d_freed, hipStream_t s);
+
+#define LQ_LOGPROBS_MAX_TOP 64
+
+/* Workspace (bytes) of lq_token_logprobs, 16-byte aligned, uninitialised. */
+int64_t lq_logprobs_workspace(int64_t rows, int64_t vocab, int top);
+
+/* Of each of `rows` rows of logits (element (r, v) at r * stride + v; rows of any alignment,
+ * vocab < 2^31): d_logprob[r] = log softmax at d_tokens[r] (0 for a negative token or without
+ * d_tokens, NaN for one past the vocabulary), d_entropy[r] = -sum p log p, and the `top`
+ * (0..64, at most vocab) largest logits' places d_ids[r][k] and log probabilities d_top[r][k],
+ * in order (equal logits by place, NaN above all).  Logits of -inf weigh nothing; a row of
+ * nothing else, with a NaN or with +inf has NaN. */
+int lq_token_logprobs(const void *d_logits, int dtype, int64_t stride, int64_t rows, int64_t vocab,
+                      const int64_t *d_tokens, int top, void *d_work, int64_t work_bytes, float *d_logprob,
+                      float *d_entropy, int64_t *d_ids, float *d_top, hipStream_t s);
+
 #ifdef __cplusplus
 }
 #endif

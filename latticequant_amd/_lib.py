@@ -106,6 +106,14 @@ _SIGS = {
     "lq_select_total": ([_P, _P], _INT),
     "lq_resident_select": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _P], _INT),
     "lq_resident_select_exceptions": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P], _INT),
+    "lq_page_quantize": ([_P, _INT, _I64, _I64] + [_P] * 6, _INT),
+    "lq_page_dequant": ([_P, _P, _I64, _I64, _P, _INT, _P], _INT),
+    "lq_paged_attn_workspace": ([_I64, _I64, _INT, _I64, _I64, _INT], _I64),
+    "lq_paged_attention": ([_P, _P, _P, _I64, _INT, _P, _I64, _P, _P, _P, _I64, _P, _P, ctypes.c_float, _INT, _P, _I64] +
+                           [_P] * 2, _INT),
+    "lq_evict_pages": ([_P] * 3 + [_I64] * 5 + [_P] * 5, _INT),
+    "lq_logprobs_workspace": ([_I64, _I64, _INT], _I64),
+    "lq_token_logprobs": ([_P, _INT, _I64, _I64, _I64, _P, _INT, _P, _I64] + [_P] * 5, _INT),
     "lq_tree_attn_workspace": ([_I64, _I64, _I64, _INT, _I64, _I64], _I64),
     "lq_resident_tree_attention": ([_P, _P, _I64] + [_P] * 4 + [_I64, _I64, _INT, _P, _P, _I64, _P, _P, _INT, _P, _I64] +
                                    [_P] * 2, _INT),
@@ -136,6 +144,7 @@ class Rows(ctypes.Structure):
 
 LQ_RES_ST_EXC_OVERFLOW = 1
 LQ_TREE_MAX_NODES = 256
+LQ_LOGPROBS_MAX_TOP = 64
 
 
 def exported_symbols():

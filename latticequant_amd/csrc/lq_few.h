@@ -303,9 +303,11 @@ struct FewState {
     float m, l;      // reference (base 2), the lane's part of the sum
     f4_t o[8];       // O^T: column lane % 16; o[mm][i]: dimension 8 (4 (lane / 16) + i) + mm
 };
-__device__ __forceinline__ void few_attend(f4_t s[2], uint32_t word, bool every, const uint32_t vp[4][8], int lane,
-                                           FewState& st) {
-    const float c0 = 1.4426950408889634f / 11.313708498984761f;   // log2(e) / sqrt(128)
+constexpr float kScale2 = 1.4426950408889634f / 11.313708498984761f;   // log2(e) / sqrt(128)
+
+// Scores that the row does not see to -inf, and the row's reference raised where they pass
+// it; returns what is added to a score times kScale2 for the logarithm of its weight.
+__device__ __forceinline__ float few_reference(f4_t s[2], uint32_t word, bool every, int lane, FewState& st) {
     if (!every) {
         const uint32_t own = word >> (8 * (lane >> 4));
 #pragma unroll
@@ -316,7 +318,7 @@ __device__ __forceinline__ void few_attend(f4_t s[2], uint32_t word, bool every,
     float mx = s[0][0];
 #pragma unroll
     for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[i >> 2][i & 3]);
-    const float mn = quarters_max(mx) * c0;
+    const float mn = quarters_max(mx) * kScale2;
     if (__any(mn > st.m + kLazy)) {
         const float up = mn > st.m + kLazy ? mn : st.m;   // as in products
         const float al = up == st.m ? 1.f : __builtin_amdgcn_exp2f(st.m - up);
@@ -327,15 +329,22 @@ __device__ __forceinline__ void few_attend(f4_t s[2], uint32_t word, bool every,
             for (int i = 0; i < 4; i++) st.o[mm][i] *= al;
         st.m = up;
     }
-    const float off = (st.m == -INFINITY ? 0.f : -st.m) + kPShift;
-    uint32_t p[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) p[i] = weights(s[0][i], s[1][i], c0, off, st.l);   // in the order of the tokens
+    return (st.m == -INFINITY ? 0.f : -st.m) + kPShift;
+}
+__device__ __forceinline__ void few_products(const uint32_t p[4], const uint32_t vp[4][8], FewState& st) {
     const h8_t pb = as_h8(p[0], p[1], p[2], p[3]);
 #pragma unroll
     for (int mm = 0; mm < 8; mm++)
         st.o[mm] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(vp[0][mm], vp[1][mm], vp[2][mm], vp[3][mm]), pb, st.o[mm],
                                                           0, 0, 0);
+}
+__device__ __forceinline__ void few_attend(f4_t s[2], uint32_t word, bool every, const uint32_t vp[4][8], int lane,
+                                           FewState& st) {
+    const float off = few_reference(s, word, every, lane, st);
+    uint32_t p[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = weights(s[0][i], s[1][i], kScale2, off, st.l);   // in the order of the tokens
+    few_products(p, vp, st);
 }
 
 }  // namespace lq

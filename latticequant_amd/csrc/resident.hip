@@ -78,21 +78,19 @@ __device__ __forceinline__ int res_point(const void* x, int dtype, int64_t T, in
     return e8_nearest_fast(tv, ic);
 }
 
-// grid (t_tokens / 16, n_heads), 256 threads: wave = group, lane = slot
-__global__ __launch_bounds__(256) void k_res_quant(const void* __restrict__ x, int dtype, int64_t T,
-                                                   const float* __restrict__ scale32,
-                                                   const uint16_t* __restrict__ scale16, lq_resident r, int64_t h0,
-                                                   int64_t blk0, uint32_t* __restrict__ cnt) {
+// Block bb of head hh of x to resident block rb; its exceptions' number is returned to
+// thread 0.  256 threads: wave = group, lane = slot
+__device__ __forceinline__ int quant_block(const void* __restrict__ x, int dtype, int64_t T,
+                                           const float* __restrict__ scale32, const uint16_t* __restrict__ scale16,
+                                           const lq_resident& r, int64_t hh, int64_t bb, int64_t rb) {
     __shared__ unsigned long long wm[4];
     const int tid = threadIdx.x, grp = tid >> 6, slot = tid & 63;
-    const int64_t bb = blockIdx.x, hh = blockIdx.y;
     const int64_t t = bb * kRB + (slot & 15);
     const int g = 4 * grp + (slot >> 4);
     float ic[8];
     const int cs = res_point(x, dtype, T, hh, t, g, scale32[hh], ic);
     uint32_t a, b;
     const bool ok = rec_encode(ic, cs, &a, &b);
-    const int64_t rb = (h0 + hh) * r.cap_blocks + blk0 + bb;
     r.a[rb * 256 + grp * 64 + slot] = a;
     r.b[rb * 256 + grp * 64 + slot] = (uint8_t)b;
     const unsigned long long m = __ballot(!ok);
@@ -100,12 +98,12 @@ __global__ __launch_bounds__(256) void k_res_quant(const void* __restrict__ x, i
         r.mask[rb * 4 + grp] = m;
         wm[grp] = m;
     }
-    if (grp == 0 && slot < kRB) r.scale[(h0 + hh) * r.cap_blocks * kRB + (blk0 + bb) * kRB + slot] = scale16[hh];
+    if (grp == 0 && slot < kRB) r.scale[rb * kRB + slot] = scale16[hh];
     __syncthreads();
+    int n = 0;
     if (tid == 0) {
         // header: count and the first seven exceptions in (group, slot) order
         uint64_t hdr = 0;
-        int n = 0;
         for (int c = 0; c < 4; c++) {
             unsigned long long mm = wm[c];
             while (mm) {
@@ -119,8 +117,18 @@ __global__ __launch_bounds__(256) void k_res_quant(const void* __restrict__ x, i
         r.meta[rb * 4 + 0] = (uint32_t)hdr;
         r.meta[rb * 4 + 1] = (uint32_t)(hdr >> 32);
         r.meta[rb * 4 + 3] = (uint32_t)n;
-        cnt[hh * gridDim.x + bb] = (uint32_t)n;
     }
+    return n;
+}
+
+// grid (t_tokens / 16, n_heads)
+__global__ __launch_bounds__(256) void k_res_quant(const void* __restrict__ x, int dtype, int64_t T,
+                                                   const float* __restrict__ scale32,
+                                                   const uint16_t* __restrict__ scale16, lq_resident r, int64_t h0,
+                                                   int64_t blk0, uint32_t* __restrict__ cnt) {
+    const int64_t bb = blockIdx.x, hh = blockIdx.y;
+    const int n = quant_block(x, dtype, T, scale32, scale16, r, hh, bb, (h0 + hh) * r.cap_blocks + blk0 + bb);
+    if (threadIdx.x == 0) cnt[hh * gridDim.x + bb] = (uint32_t)n;
 }
 
 // exclusive scan of the per-block exception counts (one workgroup) -> base,
@@ -153,13 +161,11 @@ __global__ __launch_bounds__(256) void k_res_scan(const uint32_t* __restrict__ c
     if (tid == 255) *r.n_exc = (int32_t)(start + part[255]);
 }
 
-// exception entries: the vectors flagged by k_res_quant, recomputed
-__global__ __launch_bounds__(256) void k_res_fill(const void* __restrict__ x, int dtype, int64_t T,
-                                                  const float* __restrict__ scale32, lq_resident r, int64_t h0,
-                                                  int64_t blk0) {
+// exception entries: the vectors flagged by quant_block, recomputed
+__device__ __forceinline__ void fill_block(const void* __restrict__ x, int dtype, int64_t T,
+                                           const float* __restrict__ scale32, const lq_resident& r, int64_t hh,
+                                           int64_t bb, int64_t rb) {
     const int tid = threadIdx.x, grp = tid >> 6, slot = tid & 63;
-    const int64_t bb = blockIdx.x, hh = blockIdx.y;
-    const int64_t rb = (h0 + hh) * r.cap_blocks + blk0 + bb;
     const unsigned long long m0 = r.mask[rb * 4 + 0], m1 = r.mask[rb * 4 + 1], m2 = r.mask[rb * 4 + 2],
                              m3 = r.mask[rb * 4 + 3];
     if ((m0 | m1 | m2 | m3) == 0ull) return;
@@ -191,12 +197,17 @@ __global__ __launch_bounds__(256) void k_res_fill(const void* __restrict__ x, in
     reinterpret_cast<uint4*>(r.exc)[idx] = w;
 }
 
-// grid (n_blocks, n_heads), 256 threads: one record per thread
-__global__ __launch_bounds__(256) void k_res_dequant(lq_resident r, int64_t h0, int64_t blk0, int64_t nblk_call,
-                                                     void* __restrict__ out, int out_dtype) {
-    const int tid = threadIdx.x, grp = tid >> 6, slot = tid & 63;
+__global__ __launch_bounds__(256) void k_res_fill(const void* __restrict__ x, int dtype, int64_t T,
+                                                  const float* __restrict__ scale32, lq_resident r, int64_t h0,
+                                                  int64_t blk0) {
     const int64_t bb = blockIdx.x, hh = blockIdx.y;
-    const int64_t rb = (h0 + hh) * r.cap_blocks + blk0 + bb;
+    fill_block(x, dtype, T, scale32, r, hh, bb, (h0 + hh) * r.cap_blocks + blk0 + bb);
+}
+
+// Resident block rb to block bb of nblk_call of head hh of out, a record per thread
+__device__ __forceinline__ void dequant_block(const lq_resident& r, int64_t hh, int64_t bb, int64_t rb,
+                                              int64_t nblk_call, void* __restrict__ out, int out_dtype) {
+    const int tid = threadIdx.x, grp = tid >> 6, slot = tid & 63;
     const int64_t tok = bb * kRB + (slot & 15);
     const int g = 4 * grp + (slot >> 4);
     const unsigned long long m = r.mask[rb * 4 + grp];
@@ -222,11 +233,89 @@ __global__ __launch_bounds__(256) void k_res_dequant(lq_resident r, int64_t h0, 
             v2[2 * i + 1] = (int)((float)h[1] * 2.0f) - 1056;
         }
     }
-    const float s = h2f(r.scale[(h0 + hh) * r.cap_blocks * kRB + (blk0 + bb) * kRB + (slot & 15)]);
+    const float s = h2f(r.scale[rb * kRB + (slot & 15)]);
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) y[i] = ((float)v2[i] * 0.5f) * s;
     store8(out, out_dtype, (hh * nblk_call * kRB + tok) * (kHd / 8) + g, y);
+}
+
+// grid (n_blocks, n_heads)
+__global__ __launch_bounds__(256) void k_res_dequant(lq_resident r, int64_t h0, int64_t blk0, int64_t nblk_call,
+                                                     void* __restrict__ out, int out_dtype) {
+    const int64_t bb = blockIdx.x, hh = blockIdx.y;
+    dequant_block(r, hh, bb, (h0 + hh) * r.cap_blocks + blk0 + bb, nblk_call, out, out_dtype);
+}
+
+// ---------------------------------------------------------------- pages --
+//
+// Blocks by number: unit (i, h, j) of x (n, heads, t_tokens, 128) goes to block
+// pages[i][j] of head h; a number outside the pool moves nothing.
+struct PageMap {
+    const int32_t* pages;
+    int64_t heads, per;                        // of the pool; blocks of a row
+    __device__ __forceinline__ int64_t block(const lq_resident& r, int64_t hh, int64_t bb) const {
+        const int64_t p = pages[hh / heads * per + bb];
+        return p >= 0 && p < r.cap_blocks ? hh % heads * r.cap_blocks + p : -1;
+    }
+};
+
+__global__ __launch_bounds__(256) void k_page_quant(const void* __restrict__ x, int dtype, PageMap P,
+                                                    const float* __restrict__ scale32,
+                                                    const uint16_t* __restrict__ scale16, lq_resident r) {
+    const int64_t hh = blockIdx.x / (uint32_t)P.per, bb = blockIdx.x % (uint32_t)P.per, rb = P.block(r, hh, bb);
+    if (rb >= 0) quant_block(x, dtype, P.per * kRB, scale32, scale16, r, hh, bb, rb);
+}
+
+// Room for the exceptions of written pages: a page keeps the entries it had, where they
+// suffice, else it takes as many as the next power of two at the list's end.  A page's
+// rooms together are under twice its largest, however often it is written.
+__global__ __launch_bounds__(1024) void k_page_rooms(PageMap P, int64_t units, lq_resident r, int32_t* __restrict__ room) {
+    __shared__ uint32_t part[16];
+    __shared__ uint32_t s_run;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t run = (uint32_t)*r.n_exc;
+    for (int64_t i0 = 0; i0 < units; i0 += 1024) {
+        const int64_t i = i0 + tid, rb = i < units ? P.block(r, i / P.per, i % P.per) : -1;
+        uint32_t need = 0;
+        if (rb >= 0) {
+            const uint32_t n = r.meta[rb * 4 + 3];
+            if (n > (uint32_t)room[rb]) need = n < 2 ? n : 1u << (32 - __clz((int)(n - 1)));
+        }
+        uint32_t upto = need;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t v = __shfl_up(upto, o, 64);
+            upto += lane >= o ? v : 0u;
+        }
+        if (lane == 63) part[wave] = upto;
+        __syncthreads();
+        for (int w = 0; w < wave; w++) upto += part[w];
+        if (need) {
+            r.meta[rb * 4 + 2] = run + upto - need;
+            room[rb] = (int32_t)need;
+        }
+        if (tid == 1023) s_run = run + upto;
+        __syncthreads();
+        run = s_run;
+    }
+    if (tid == 0) *r.n_exc = (int32_t)run;
+}
+
+__global__ __launch_bounds__(256) void k_page_fill(const void* __restrict__ x, int dtype, PageMap P,
+                                                   const float* __restrict__ scale32, lq_resident r) {
+    const int64_t hh = blockIdx.x / (uint32_t)P.per, bb = blockIdx.x % (uint32_t)P.per, rb = P.block(r, hh, bb);
+    if (rb >= 0) fill_block(x, dtype, P.per * kRB, scale32, r, hh, bb, rb);
+}
+
+__global__ __launch_bounds__(256) void k_page_dequant(lq_resident r, PageMap P, void* __restrict__ out, int out_dtype) {
+    const int64_t hh = blockIdx.x / (uint32_t)P.per, bb = blockIdx.x % (uint32_t)P.per, rb = P.block(r, hh, bb);
+    if (rb >= 0) {
+        dequant_block(r, hh, bb, rb, P.per, out, out_dtype);
+    } else {
+        const float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        store8(out, out_dtype, (hh * P.per + bb) * 256 + threadIdx.x, y);
+    }
 }
 
 // ----------------------------------------------------------- attention --
@@ -967,6 +1056,32 @@ int lq_resident_dequant(const lq_resident* r, int64_t h0, int64_t n_heads, int64
         return LQ_ERR_ARG;
     hipLaunchKernelGGL(k_res_dequant, dim3((unsigned)n_blocks, (unsigned)n_heads), dim3(256), 0, s, *r, h0, blk0,
                        n_blocks, d_out, out_dtype);
+    return launch_status();
+}
+
+int lq_page_quantize(const void *d_x, int dtype, int64_t n, int64_t t_tokens, const float *d_scale32,
+                     const uint16_t *d_scale16, const lq_resident *r, const int32_t *d_pages, int32_t *d_room,
+                     hipStream_t s) {
+    if (!d_x || !d_scale32 || !d_scale16 || !res_ok(r) || !d_pages || !d_room || dtype < 0 || dtype > 2 || n < 1 ||
+        t_tokens <= 0 || t_tokens % kRB)
+        return LQ_ERR_ARG;
+    const int64_t per = t_tokens / kRB;
+    if (n > INT_MAX / per || n * per > INT_MAX / r->n_heads) return LQ_ERR_ARG;
+    const int64_t units = n * r->n_heads * per;
+    const PageMap P = {d_pages, r->n_heads, per};
+    hipLaunchKernelGGL(k_page_quant, dim3((unsigned)units), dim3(256), 0, s, d_x, dtype, P, d_scale32, d_scale16, *r);
+    hipLaunchKernelGGL(k_page_rooms, dim3(1), dim3(1024), 0, s, P, units, *r, d_room);
+    hipLaunchKernelGGL(k_page_fill, dim3((unsigned)units), dim3(256), 0, s, d_x, dtype, P, d_scale32, *r);
+    return launch_status();
+}
+
+int lq_page_dequant(const lq_resident *r, const int32_t *d_pages, int64_t n, int64_t per, void *d_out, int out_dtype,
+                    hipStream_t s) {
+    if (!res_ok(r) || !d_pages || !d_out || out_dtype < 0 || out_dtype > 2 || n < 1 || per < 1 || n > INT_MAX / per ||
+        n * per > INT_MAX / r->n_heads)
+        return LQ_ERR_ARG;
+    const PageMap P = {d_pages, r->n_heads, per};
+    hipLaunchKernelGGL(k_page_dequant, dim3((unsigned)(n * r->n_heads * per)), dim3(256), 0, s, *r, P, d_out, out_dtype);
     return launch_status();
 }
 

@@ -150,39 +150,46 @@ class ResidentKV:
                                              work.data_ptr(), L.stream_ptr(self.device)), "lq_resident_quantize")
 
         with torch.cuda.device(self.device):
-            if n_new <= self.ASYNC_MAX_VECTORS:
-                if self._exc_read is not None and self._exc_read[1].query():
-                    host, _, after = self._exc_read
-                    self._exc_known, self._exc_since, self._exc_read = int(host[0]), after, None
-                need = self._exc_known + self._exc_since + n_new
-                if need > self.exc_cap:
-                    self._grow_exc(max(2 * self.exc_cap, need), self.exc_cap)
-                launch()
-                self._exc_since += n_new
-                if self._exc_read is not None:
-                    host, ev, after = self._exc_read
-                    self._exc_read = (host, ev, after + n_new)
-                else:
-                    host = torch.empty(1, dtype=torch.int32, pin_memory=True)
-                    host.copy_(self.n_exc, non_blocking=True)
-                    ev = torch.cuda.Event()
-                    ev.record(torch.cuda.current_stream(self.device))
-                    self._exc_read = (host, ev, 0)
-            else:
-                n0 = int(self.n_exc.item())
-                for attempt in range(2):
-                    launch()
-                    n1 = int(self.n_exc.item())
-                    if n1 <= self.exc_cap:
-                        break
-                    # grow the exception list to the exact need and redo this append
-                    self._grow_exc(max(n1, 2 * self.exc_cap), n0)
-                    self.n_exc.fill_(n0)
-                    self.status.zero_()
-                self._exc_known, self._exc_since, self._exc_read = n1, 0, None
+            self._with_exceptions(n_new, launch, anew=True)
         if B != self.n_seq:
             self.n_seq = None if self.n_tokens else B
         self.n_tokens += T
+
+    def _with_exceptions(self, n_new: int, launch, anew: bool) -> None:
+        """launch(), which may add n_new exception entries, with room for them.  anew: where
+        the list was too short and launch runs again, its entries are numbered again (else
+        those that have numbers keep them)."""
+        if n_new <= self.ASYNC_MAX_VECTORS:
+            if self._exc_read is not None and self._exc_read[1].query():
+                host, _, after = self._exc_read
+                self._exc_known, self._exc_since, self._exc_read = int(host[0]), after, None
+            need = self._exc_known + self._exc_since + n_new
+            if need > self.exc_cap:
+                self._grow_exc(max(2 * self.exc_cap, need), self.exc_cap)
+            launch()
+            self._exc_since += n_new
+            if self._exc_read is not None:
+                host, ev, after = self._exc_read
+                self._exc_read = (host, ev, after + n_new)
+            else:
+                host = torch.empty(1, dtype=torch.int32, pin_memory=True)
+                host.copy_(self.n_exc, non_blocking=True)
+                ev = torch.cuda.Event()
+                ev.record(torch.cuda.current_stream(self.device))
+                self._exc_read = (host, ev, 0)
+        else:
+            n0 = int(self.n_exc.item())
+            for attempt in range(2):
+                launch()
+                n1 = int(self.n_exc.item())
+                if n1 <= self.exc_cap:
+                    break
+                # grow the exception list to the exact need and launch again
+                self._grow_exc(max(n1, 2 * self.exc_cap), n0 if anew else self.exc_cap)
+                if anew:
+                    self.n_exc.fill_(n0)
+                self.status.zero_()
+            self._exc_known, self._exc_since, self._exc_read = n1, 0, None
 
     def _grow_exc(self, cap: int, keep: int) -> None:
         """A longer exception list holding the first `keep` entries."""

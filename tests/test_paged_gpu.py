@@ -1,0 +1,456 @@
+"""One pool of resident pages for many sequences: writes and reads by page, attention of one
+new token with page weights, eviction by them, against plain computations in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from latticequant_amd.llm.paged import (PAGE, Eviction, PagedKV, evict_pages, paged_attn_workspace,
+                                        paged_decode_attention)
+from latticequant_amd.llm.resident import ResidentKV
+
+pytestmark = pytest.mark.gpu
+HD = 128
+HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}      # half a step
+
+
+def _rows(n, h, t, seed, loud=2, dtype=torch.float16):
+    """Rows with `loud` outlier channels (exceptions), and scales of 4 bits a dimension."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(n, h, t, HD, generator=g, device="cuda")
+    x[..., :loud] *= 5.0
+    s = 0.2 + 0.1 * torch.rand(n, h, generator=g, device="cuda")
+    return x.to(dtype), s
+
+
+def _pool(h, n, seed, loud=2):
+    p = PagedKV(h, n, device="cuda")
+    x, s = _rows(n, h, PAGE, seed, loud)
+    p.write(x, torch.arange(n, device="cuda")[:, None], s, s.half())
+    return p
+
+
+def _table(counts, n, width, seed, fill=-1):
+    rng = np.random.RandomState(seed)
+    order = rng.permutation(n)
+    tab = np.full((len(counts), width), fill, np.int32)
+    at = 0
+    for b, c in enumerate(counts):
+        tab[b, :c] = order[np.arange(at, at + c) % n]
+        at += c
+    return torch.from_numpy(tab).cuda()
+
+
+def _reference(k, v, q, tab, counts, tk, tv, tails):
+    """(out, tolerance of it, page weights, relative tolerance of those): 64 bits, from the rows
+    that the pages stand for.
+
+    P is rounded to fp16 (half a step 2^-11) in the sum over V and in the row's sum alike, so
+    a row is off by at most 2 x 2^-11 times its sum of p |v|.  A score is a sum of 128 products
+    in fp32: off by at most 130 x 2^-24 of the sum of their sizes (and, where bf16 values
+    below 2^-14 lose bits as fp16 operands, by 2^-25 of the other's sizes), a weight relatively
+    by that much twice (its own and the row's sum), once more for exp2 and the rounding of
+    its argument (z below 2^7: 2^-17).  Weights below 2^-35 of the row's largest may vanish."""
+    B, Hq = q.shape[:2]
+    H, G, W = k.n_heads, Hq // k.n_heads, tab.shape[1]
+    rk, rv = (p.read(torch.arange(p.n_pages, device="cuda")[:, None]).double() for p in (k, v))
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(out)
+    w = torch.zeros(B, W, dtype=torch.float64, device="cuda")
+    wtol = 0.0
+    half = HALF[q.dtype]
+    for b in range(B):
+        c, t = counts[b], tails[b]
+        if c * PAGE + t == 0:
+            continue
+        at = tab[b, :c].long().clamp(0, k.n_pages - 1)
+        for h in range(H):
+            kk = rk[at, h].reshape(-1, HD)
+            vv = rv[at, h].reshape(-1, HD)
+            if t:
+                kk = torch.cat([kk, tk[b, h, :t].double()])
+                vv = torch.cat([vv, tv[b, h, :t].double()])
+            qq = q[b, h * G:(h + 1) * G, 0].double()
+            size = (qq.abs() @ kk.abs().t().contiguous()).amax(1)
+            es = (130 * 2.0 ** -24 * size + 2.0 ** -25 * (qq.abs().sum(1) + kk.abs().sum(1).max())) / math.sqrt(HD)
+            p = torch.softmax(qq @ kk.t().contiguous() / math.sqrt(HD), 1)
+            rel = 2 * es + 2.0 ** -16
+            out[b, h * G:(h + 1) * G, 0] = p @ vv
+            a = p @ vv.abs()
+            tol[b, h * G:(h + 1) * G, 0] = (a * (2.0 ** -10 + rel[:, None]) + half * (p @ vv).abs() * (1 + 2.0 ** -9) +
+                                            len(vv) * 2.0 ** -35 * vv.abs().max() + 2.0 ** -24)
+            if c:
+                w[b, :c] += p[:, :c * PAGE].reshape(G, c, PAGE).sum((0, 2))
+            wtol = max(wtol, float(rel.max()))
+    return out, tol, w, wtol
+
+
+def _case(B, H, G, counts, tails, dtype, seed, cap=None, width=None, loud=2):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = max(1, sum(counts)) + 3
+    k, v = _pool(H, n, seed, loud), _pool(H, n, seed + 1, 1 if loud else 0)
+    width = max(counts) if width is None else width
+    tab = _table(counts, n, width, seed)
+    cap = max(tails) if cap is None else cap
+    q = torch.randn(B, H * G, 1, HD, generator=g, device="cuda").to(dtype)
+    tk, tv = (torch.randn(B, H, cap, HD, generator=g, device="cuda").to(dtype) for _ in range(2))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    return k, v, q, tab, i32(counts), tk, tv, i32(tails)
+
+
+SHAPES = [
+    # B, H, G, pages, tail rows
+    (1, 1, 1, [0], [1]),
+    (1, 1, 1, [1], [0]),
+    (1, 8, 4, [31], [5]),
+    (1, 2, 16, [3], [33]),
+    (2, 4, 7, [5, 0], [0, 64]),
+    (3, 1, 3, [1, 2, 3], [16, 1, 0]),
+    (4, 2, 2, [130, 1, 0, 65], [7, 0, 0, 16]),
+    (5, 8, 1, [64, 63, 62, 1, 0], [1, 31, 32, 33, 0]),
+    (300, 1, 2, [i % 3 for i in range(300)], [(i * 7) % 5 for i in range(300)]),
+    (2, 8, 4, [600, 257], [16, 3]),
+    (1, 1, 8, [2100], [1]),
+    (33, 4, 5, [(11 * i) % 40 for i in range(33)], [(5 * i) % 17 for i in range(33)]),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: f"{s[0]}x{s[1]}x{s[2]}-{max(s[3])}")
+def test_attention_and_weights(shape, dtype):
+    B, H, G, counts, tails = shape
+    k, v, q, tab, cnt, tk, tv, tl = _case(B, H, G, counts, tails, dtype, 100 + B + H)
+    want, tol, w, wtol = _reference(k, v, q, tab, counts, tk, tv, tails)
+    got = paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl)
+    assert got.dtype is dtype and got.shape == q.shape
+    bad = (got.double() - want).abs() > tol
+    assert not bool(bad.any()), f"{int(bad.sum())} of {bad.numel()} values off, worst {float((got.double() - want).abs().max())}"
+    if not tab.shape[1]:
+        return
+    old = torch.rand(tab.shape, device="cuda")
+    acc = old.clone()
+    again = paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl, weights=acc, decay=0.75)
+    assert torch.equal(again.isnan(), got.isnan())
+    assert bool(((again.double() - want).abs() <= tol).all())
+    on = torch.arange(tab.shape[1], device="cuda") < cnt[:, None]
+    assert torch.equal(acc[~on], old[~on]), "places past the count changed"
+    exp = 0.75 * old.double() + w
+    # the sum over the heads and one fma: (rows + 2) roundings of 2^-24
+    assert bool(((acc.double() - exp).abs() <= w * (wtol + (H * G + 2) * 2.0 ** -24) + exp * 2.0 ** -23 + 1e-30)[on].all())
+    acc.fill_(float("nan"))
+    paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl, weights=acc, decay=0.0)
+    assert bool(((acc.double() - w).abs() <= w * (wtol + (H * G + 2) * 2.0 ** -24) + 1e-30)[on].all())
+    assert bool(acc[~on].isnan().all())
+
+
+def test_weights_sum_to_the_heads():
+    k, v, q, tab, cnt, *_ = _case(3, 4, 4, [40, 7, 129], [0, 0, 0], torch.float16, 3, cap=0)
+    acc = torch.zeros(tab.shape, device="cuda")
+    for _ in range(3):
+        paged_decode_attention(k, v, q, tab, cnt, weights=acc)
+    # 3 steps x 16 heads; every weight off relatively by 2^-15 at most (see _reference, |q||k| below 2^10)
+    assert torch.allclose(acc.double().sum(1), torch.full((3,), 48.0, dtype=torch.float64, device="cuda"), rtol=2 ** -10)
+
+
+def test_no_pages_at_all_and_no_tail():
+    k, v, q, tab, cnt, tk, tv, tl = _case(2, 2, 2, [0, 0], [3, 0], torch.float16, 5, width=0)
+    got = paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl)
+    want, tol, *_ = _reference(k, v, q, tab, [0, 0], tk, tv, [3, 0])
+    assert bool(((got.double() - want).abs() <= tol).all()) and not bool(got[1].any())
+    got = paged_decode_attention(k, v, q, tab, cnt, weights=torch.zeros(2, 0, device="cuda"))
+    assert not bool(got.any())
+
+
+def test_counts_and_numbers_are_clamped():
+    counts, tails = [4, 3], [2, 5]
+    k, v, q, tab, cnt, tk, tv, tl = _case(2, 2, 4, counts, tails, torch.float16, 6, width=4)
+    wild = tab.clone()
+    wild[1, 1] = 10 ** 9
+    wild[1, 2] = -7
+    want, tol, *_ = _reference(k, v, q, torch.where(wild < 0, 10 ** 9, wild), counts, tk, tv, tails)
+    got = paged_decode_attention(k, v, q, wild, cnt, tk, tv, tail_len=tl)
+    assert bool(((got.double() - want).abs() <= tol).all())
+    over = torch.tensor([99, -3], dtype=torch.int32, device="cuda")
+    got = paged_decode_attention(k, v, q, tab, over, tk, tv, tail_len=torch.tensor([10 ** 6, -1], device="cuda"))
+    want, tol, *_ = _reference(k, v, q, tab, [4, 0], tk, tv, [5, 0])
+    assert bool(((got.double() - want).abs() <= tol).all()) and not bool(got[1].any())
+
+
+def test_what_is_not_read_does_not_matter():
+    counts, tails = [5, 2], [3, 1]
+    k, v, q, tab, cnt, tk, tv, tl = _case(2, 2, 4, counts, tails, torch.bfloat16, 7, cap=40, width=9)
+    a = paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl)
+    for t in (tk, tv):
+        t[0, :, 3:], t[1, :, 1:] = float("nan"), float("inf")
+    used = set(tab[0, :5].tolist() + tab[1, :2].tolist())
+    free = torch.tensor([i for i in range(k.n_pages) if i not in used], device="cuda")
+    for p in (k, v):
+        s = torch.full((len(free), 2), 3.0e4, device="cuda")
+        p.write(torch.full((len(free), 2, PAGE, HD), 6.0e4, device="cuda"), free[:, None], s, s.half())
+    tab[0, 5:], tab[1, 2:] = 2 ** 31 - 1, -2 ** 31
+    b = paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl)
+    assert torch.equal(a, b)
+
+
+def test_tail_values_that_are_not_finite_reach_their_sequence_only():
+    k, v, q, tab, cnt, tk, tv, tl = _case(3, 2, 2, [3, 3, 3], [4, 4, 4], torch.float16, 8)
+    a = paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl)
+    tk[1, 0, 2, 5] = float("nan")
+    b = paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[2], b[2]) and torch.equal(a[1, 2:], b[1, 2:])
+    assert bool(b[1, :2].isnan().all())
+
+
+@pytest.mark.parametrize("layout", ["heads_last", "odd_stride", "unaligned", "expanded"])
+def test_strides(layout):
+    counts, tails = [9, 4], [6, 20]
+    k, v, q, tab, cnt, tk, tv, tl = _case(2, 4, 4, counts, tails, torch.float16, 9)
+    want = paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl)
+    if layout == "heads_last":
+        f = lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)
+    elif layout == "odd_stride":
+        f = lambda t: torch.zeros(*t.shape[:3], HD + 3, dtype=t.dtype, device="cuda")[..., :HD].copy_(t)
+    elif layout == "unaligned":
+        f = lambda t: torch.zeros(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)
+    else:
+        q = q[:1].expand(2, -1, -1, -1)
+        tk, tv = (t[:1].expand(2, -1, -1, -1) for t in (tk, tv))
+        want = paged_decode_attention(k, v, q.contiguous(), tab, cnt, tk.contiguous(), tv.contiguous(), tail_len=tl)
+        f = lambda t: t
+    out = torch.empty(2, 1, 16, HD, dtype=torch.float16, device="cuda").transpose(1, 2)
+    got = paged_decode_attention(k, v, f(q), tab.long(), cnt.long(), f(tk), f(tv), tail_len=tl.long(), out=out)
+    assert got is out and torch.equal(got, want)
+
+
+def test_shared_pages_and_a_table_of_one_sequence():
+    k, v, q, tab, cnt, *_ = _case(2, 2, 4, [40, 40], [0, 0], torch.float16, 10, cap=0)
+    tab[1] = tab[0]
+    q[1] = q[0]
+    got = paged_decode_attention(k, v, q, tab, cnt)
+    one = paged_decode_attention(k, v, q[:1], tab[:1], cnt[:1])
+    # another division of the work, another order of the joins: both within a step of the same value
+    assert bool(((got[0].float() - one[0].float()).abs() <= 2.0 ** -9 * one[0].float().abs() + 2.0 ** -10).all())
+    assert torch.equal(got[0], paged_decode_attention(k, v, q, tab, cnt)[0])
+
+
+def test_against_the_contiguous_prefix():
+    """The same points at the same scales as a ResidentKV's, bit for bit."""
+    x, s = _rows(1, 4, 96, 11)
+    r = ResidentKV(4, 96, device="cuda")
+    r.append(x, s, s.half())
+    p = PagedKV(4, 9, device="cuda")
+    at = torch.tensor([[7, 2, 0, 8, 3, 5]], device="cuda")
+    p.write(x, at, s, s.half())
+    for dt in (torch.float16, torch.float32, torch.bfloat16):
+        assert torch.equal(p.read(at, dt)[0], r.dequant(dt))
+    assert not bool(p.read(torch.tensor([[1]], device="cuda")).any())     # never written
+    assert not bool(p.read(torch.tensor([[9, -1]], device="cuda")).any())  # outside
+    p.write(x, at, bits=4)                                                # scales of its own
+    err = (p.read(at)[0].float() - x[0].float()).square().mean() / x.float().square().mean()
+    assert float(err) < 0.02
+
+
+def test_pages_written_again_keep_their_room():
+    p = PagedKV(2, 8, device="cuda")
+    at = torch.arange(8, device="cuda")[:, None]
+    seen = []
+    for i in range(12):
+        x, s = _rows(8, 2, PAGE, 20 + i, loud=1 + i % 4)
+        p.write(x, at, s, s.half())
+        r = ResidentKV(16, PAGE, device="cuda")
+        r.append(x.reshape(1, 16, PAGE, HD), s.view(-1), s.view(-1).half())
+        assert torch.equal(p.read(at).reshape(16, PAGE, HD), r.dequant())
+        seen.append(int(p.pool.n_exc))
+    before = p.read(at)
+    for _ in range(3):                                     # as many exceptions again: no more room
+        p.write(x, at, s, s.half())
+    assert int(p.pool.n_exc) == seen[-1] and torch.equal(p.read(at), before)
+    assert seen[-1] <= 2 * 16 * int(p._room.max()) and int(p.pool.status) == 0
+    assert int(p._room.max()) <= 256
+
+
+def test_many_exceptions_lengthen_the_list():
+    """Every vector an exception, more of them than the list has room for; neighbours keep
+    theirs."""
+    p = PagedKV(1, 40, device="cuda", exc_cap=4)
+    x, s = _rows(2, 1, PAGE, 30)
+    p.write(x, torch.tensor([[0], [39]], device="cuda"), s, s.half())
+    first = p.read(torch.tensor([[0], [39]], device="cuda"))
+    y = torch.randn(38, 1, PAGE, HD, device="cuda") * 100
+    t = torch.full((38, 1), 0.25, device="cuda")
+    p.write(y, torch.arange(1, 39, device="cuda")[:, None], t, t.half())
+    assert int(p.pool.n_exc) >= 38 * 250 and p.exc_cap >= int(p.pool.n_exc) and int(p.pool.status) == 0
+    assert torch.equal(p.read(torch.tensor([[0], [39]], device="cuda")), first)
+    r = ResidentKV(38, PAGE, device="cuda")
+    r.append(y.reshape(1, 38, PAGE, HD), t.view(-1), t.view(-1).half())
+    assert torch.equal(p.read(torch.arange(1, 39, device="cuda")[:, None]).reshape(38, PAGE, HD), r.dequant())
+    # attention over pages that are nothing but exceptions
+    q = torch.randn(1, 3, 1, HD, device="cuda").half() * 0.01
+    tab = torch.arange(40, dtype=torch.int32, device="cuda")[None]
+    cnt = torch.tensor([40], dtype=torch.int32, device="cuda")
+    want, tol, *_ = _reference(p, p, q, tab, [40], None, None, [0])
+    assert bool(((paged_decode_attention(p, p, q, tab, cnt).double() - want).abs() <= tol).all())
+
+
+def test_dropped_entries_are_zero():
+    """A list shortened behind the pool's back: entries past it count as zero vectors."""
+    p = _pool(2, 12, 40)
+    tab, cnt = _table([12], 12, 12, 1), torch.tensor([12], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 4, 1, HD, device="cuda").half()
+    p.pool.exc = p.pool.exc[:8 * 20].clone()
+    p.pool._st = None
+    want, tol, *_ = _reference(p, p, q, tab, [12], None, None, [0])    # read() has them as zeros too
+    assert bool(((paged_decode_attention(p, p, q, tab, cnt).double() - want).abs() <= tol).all())
+
+
+def test_pool_beyond_four_gibibytes():
+    """Byte offsets past 32 bits: a pool of 4.3 million pages, the last ones in use."""
+    n = (1 << 22) + 70
+    k, v = PagedKV(1, n, device="cuda", exc_cap=65536), PagedKV(1, n, device="cuda", exc_cap=65536)
+    at = torch.tensor([[0, n - 1, 1 << 21, n - 3, (1 << 22) - 1, 1 << 22, 5]], device="cuda")
+    rows = {}
+    for name, p, seed in (("k", k, 1), ("v", v, 2)):
+        x, s = _rows(1, 1, 7 * PAGE, 50 + seed)
+        p.write(x, at, s, s.half())
+        small = PagedKV(1, 7, device="cuda")
+        small.write(x, torch.arange(7, device="cuda")[None], s, s.half())
+        rows[name] = small
+        assert torch.equal(p.read(at), small.read(torch.arange(7, device="cuda")[None]))
+    q = torch.randn(1, 5, 1, HD, device="cuda").bfloat16()
+    cnt = torch.tensor([7], dtype=torch.int32, device="cuda")
+    order = torch.arange(7, dtype=torch.int32, device="cuda")[None]
+    a, b = torch.zeros(1, 7, device="cuda"), torch.zeros(1, 7, device="cuda")
+    assert torch.equal(paged_decode_attention(k, v, q, at, cnt), paged_decode_attention(rows["k"], rows["v"], q, order, cnt))
+    paged_decode_attention(k, v, q, at, cnt, weights=a)
+    paged_decode_attention(rows["k"], rows["v"], q, order, cnt, weights=b)
+    assert torch.equal(a, b)
+
+
+def test_one_workspace_calls_of_other_sizes_and_other_streams():
+    cases = [_case(2, 4, 4, [50, 3], [6, 1], torch.float16, 60), _case(5, 4, 4, [1, 0, 9, 200, 4], [1] * 5, torch.float16, 61)]
+    work = torch.empty(max(paged_attn_workspace(c[2].shape[0], 4, 4, c[3].shape[1], c[5].shape[2], True).numel()
+                           for c in cases), dtype=torch.uint8, device="cuda").fill_(255)
+    want = [paged_decode_attention(*c[:7], tail_len=c[7]) for c in cases]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for i in (0, 1, 1, 0):
+        acc = torch.zeros(cases[i][3].shape, device="cuda")
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = paged_decode_attention(*cases[i][:7], tail_len=cases[i][7], work=work, weights=acc)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        assert torch.allclose(got.float(), want[i].float(), rtol=2.0 ** -9, atol=2.0 ** -10)
+
+
+def test_captured_step():
+    """Attention with weights, eviction and lengths that change between replays, in one graph,
+    beside eager work; two graphs share the workspace."""
+    counts = [30, 12, 0]
+    k, v, q, tab, cnt, tk, tv, tl = _case(3, 4, 4, counts, [5, 1, 9], torch.float16, 70, cap=16, width=32)
+    work = paged_attn_workspace(3, 4, 4, 32, 16, weights=True, device="cuda")
+    acc, out = torch.zeros(3, 32, device="cuda"), torch.empty_like(q)
+    ev = evict_pages(tab, cnt, acc, 8, 1, 2)
+    graphs = []
+    for _ in range(2):
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl, weights=acc, decay=0.5, work=work, out=out)
+            evict_pages(tab, cnt, acc, 8, 1, 2, out=ev)
+        graphs.append(g)
+    acc.zero_()
+    exp = acc.clone()
+    for step in range(6):
+        q.copy_(torch.randn(q.shape, device="cuda"))
+        cnt.copy_(torch.tensor([30 - step, 12, step], device="cuda"))
+        if step:
+            tab[2, step - 1] = tab[0, step]
+        want = paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl, weights=exp, decay=0.5)
+        chosen = evict_pages(tab, cnt, exp, 8, 1, 2)
+        out.fill_(7.0)
+        graphs[step % 2].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(acc, exp)
+        for a, b in zip(ev, chosen):
+            assert torch.equal(a, b)
+
+
+def test_refusals_on_the_device():
+    k, v, q, tab, cnt, tk, tv, tl = _case(2, 2, 4, [4, 3], [2, 5], torch.float16, 80)
+    with pytest.raises(ValueError, match="workspace too small"):
+        paged_decode_attention(k, v, q, tab, cnt, tk, tv, work=torch.empty(64, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(ValueError, match="out must be like q"):
+        paged_decode_attention(k, v, q, tab, cnt, tk, tv, out=torch.empty(2, 8, 1, HD, device="cuda"))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        paged_decode_attention(k, v, q.float().requires_grad_().half(), tab, cnt, tk, tv)
+    ev = evict_pages(tab, cnt, torch.zeros(2, 4, device="cuda"), 2)
+    with pytest.raises(ValueError, match="apart"):
+        evict_pages(ev.pages, ev.n_pages, ev.weights, 1, out=ev)
+    with pytest.raises(ValueError, match="stands twice"):
+        k.write(torch.zeros(1, 2, 32, HD, device="cuda"), torch.tensor([[1, 1]]))
+    x = torch.zeros(1, 2, 16, HD, device="cuda", dtype=torch.float16)
+    at = torch.tensor([[1]], device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="captured"):
+            k.write(x, at)
+    torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------ eviction --
+
+def _evicted(pages, count, weight, keep, sink, recent):
+    B, W = pages.shape
+    out = Eviction(np.full((B, W), -1, np.int32), np.zeros(B, np.int32), np.zeros((B, W), np.float32),
+                   np.full((B, W), -1, np.int32))
+    for b in range(B):
+        n = int(count[b])
+        lo = min(sink, n)
+        hi = max(lo, n - recent)
+        w = weight[b, lo:hi].astype(np.float64)
+        w = np.where(np.isnan(w), np.inf, np.where(np.isposinf(w), 1e300, w))
+        some = lo + np.lexsort((np.arange(hi - lo), -w))[:max(0, keep - lo - (n - hi))]
+        kept = np.arange(n) if n <= keep else np.sort(np.concatenate([np.arange(lo), some, np.arange(hi, n)])).astype(int)
+        gone = np.setdiff1d(np.arange(n), kept)
+        out.n_pages[b] = len(kept)
+        out.pages[b, :len(kept)], out.weights[b, :len(kept)] = pages[b, kept], weight[b, kept]
+        out.freed[b, :len(gone)] = pages[b, gone]
+    return out
+
+
+@pytest.mark.parametrize("W", [1, 2, 63, 64, 65, 1000, 1024, 1025, 4097, 20011, 70001])
+@pytest.mark.parametrize("kind", ["spread", "ties", "odd"])
+def test_eviction(W, kind):
+    rng = np.random.RandomState(W)
+    B = 5 if W < 5000 else 2
+    count = rng.randint(0, W + 1, B).astype(np.int32)
+    count[0] = W
+    pages = rng.randint(0, 2 ** 31 - 1, (B, W)).astype(np.int32)
+    if kind == "spread":
+        weight = np.exp(3 * rng.randn(B, W)).astype(np.float32)
+    elif kind == "ties":
+        weight = rng.randint(0, 3, (B, W)).astype(np.float32) * np.float32(0.1)
+    else:
+        weight = rng.choice(np.array([0.0, -0.0, np.nan, np.inf, 1e-42, -1.0, 5.0, -np.inf], np.float32), (B, W))
+    dev = [torch.from_numpy(x).cuda() for x in (pages, count, weight)]
+    for keep, sink, recent in [(0, 0, 0), (1, 0, 0), (W // 2, 0, 0), (W // 3 + 8, 3, 5), (W - 1, 0, 0), (W, 0, 0),
+                               (W + 5, 2, 3), (W // 4 + 2 * W, W, W), (2, 1, 1)]:
+        if keep < sink + recent:
+            continue
+        got = evict_pages(*dev, keep, sink, recent)
+        want = _evicted(pages, count, weight, keep, sink, recent)
+        for name, a, b in zip(Eviction._fields, got, want):
+            assert np.array_equal(a.cpu().numpy(), b, equal_nan=name == "weights"), (name, keep, sink, recent)
+
+
+def test_eviction_of_strided_inputs_and_counts_out_of_range():
+    w = torch.rand(4, 64, device="cuda")
+    pages = torch.arange(256, device="cuda").reshape(4, 64)
+    cnt = torch.tensor([70, -2, 64, 10], device="cuda")
+    got = evict_pages(pages[:, ::2], cnt, w[:, ::2], 7, 1, 1)
+    want = _evicted(pages[:, ::2].cpu().numpy(), cnt.clamp(0, 32).cpu().numpy(), w[:, ::2].cpu().numpy(), 7, 1, 1)
+    for a, b in zip(got, want):
+        assert np.array_equal(a.cpu().numpy(), b)

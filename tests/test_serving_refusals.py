@@ -1,0 +1,121 @@
+"""CPU tier: what paged attention, eviction and log probabilities refuse, before any GPU work."""
+import ctypes
+
+import pytest
+import torch
+
+from latticequant_amd import _lib as L
+from latticequant_amd.llm.logprobs import token_logprobs
+from latticequant_amd.llm.paged import PagedKV, evict_pages, paged_decode_attention, paged_workspace_size
+
+
+def _args(B=2, H=2, G=4, W=3, cap=5, dtype=torch.float16):
+    k, v = PagedKV(H, 4, device="cpu"), PagedKV(H, 4, device="cpu")
+    return dict(k=k, v=v, q=torch.zeros(B, H * G, 1, 128, dtype=dtype), pages=torch.zeros(B, W, dtype=torch.int32),
+                n_pages=torch.zeros(B, dtype=torch.int32), tail_k=torch.zeros(B, H, cap, 128, dtype=dtype),
+                tail_v=torch.zeros(B, H, cap, 128, dtype=dtype))
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(q=torch.zeros(2, 8, 2, 128).half()), "q must be"),
+    (dict(q=torch.zeros(2, 8, 1, 64).half()), "q must be"),
+    (dict(q=torch.zeros(2, 8, 1, 128)), "q must be"),
+    (dict(q=torch.zeros(2, 7, 1, 128).half()), "times the pools' heads"),
+    (dict(q=torch.zeros(2, 34, 1, 128).half()), "times the pools' heads"),
+    (dict(v=PagedKV(2, 5, device="cpu")), "same heads, pages"),
+    (dict(v=PagedKV(1, 4, device="cpu")), "same heads, pages"),
+    (dict(pages=torch.zeros(3, 3, dtype=torch.int32)), "pages must be"),
+    (dict(pages=torch.zeros(6, dtype=torch.int32)), "pages must be"),
+    (dict(tail_v=None), "go together"),
+    (dict(tail_k=None, tail_v=None, tail_len=torch.zeros(2, dtype=torch.int32)), "without a tail"),
+    (dict(tail_v=torch.zeros(2, 2, 4, 128).half()), "tail K / V"),
+    (dict(tail_k=torch.zeros(2, 2, 5, 128).bfloat16()), "one type"),
+    (dict(weights=torch.zeros(2, 4)), "weights must be"),
+    (dict(weights=torch.zeros(2, 3).half()), "weights must be"),
+    (dict(weights=torch.zeros(3, 2).t()), "weights must be"),
+    (dict(out=torch.zeros(2, 8, 1, 128)), "out must be"),
+    (dict(out=torch.zeros(1, 8, 1, 128).half().expand(2, -1, -1, -1)), "out must be"),
+])
+def test_attention(change, message):
+    with pytest.raises(ValueError, match=message):
+        paged_decode_attention(**{**_args(), **change})
+
+
+def test_attention_has_no_gradient():
+    a = _args()
+    a["q"].requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        paged_decode_attention(**a)
+
+
+def test_pools():
+    for h, n in ((0, 4), (4, 0), (65536, 65536)):
+        with pytest.raises(ValueError):
+            PagedKV(h, n, device="cpu")
+    p = PagedKV(2, 4, device="cpu")
+    x = torch.zeros(1, 2, 32, 128)
+    for bad, pages in ((x[:, :1], [[0, 1]]), (x[..., :64], [[0, 1]]), (x[:, :, :20], [[0]]), (x, [[0]]), (x, [[0, 4]]),
+                       (x, [[-1, 0]]), (x, [[2, 2]]), (x.double(), [[0, 1]])):
+        with pytest.raises(ValueError):
+            p.write(bad, torch.tensor(pages))
+    with pytest.raises(ValueError, match="int32 or int64"):
+        p.write(x, torch.tensor([[0.0, 1.0]]))
+    with pytest.raises(ValueError, match="go together"):
+        p.write(x, torch.tensor([[0, 1]]), scale32=torch.ones(2))
+    with pytest.raises(ValueError):
+        p.read(torch.tensor([0, 1]))
+
+
+def test_geometry():
+    assert paged_workspace_size(4, 8, 4, 100, 16) % 16 == 0
+    assert paged_workspace_size(4, 8, 4, 100, 16, True) > paged_workspace_size(4, 8, 4, 100, 16)
+    for bad in ((0, 8, 4, 1, 1), (1, 0, 4, 1, 1), (1, 8, 0, 1, 1), (1, 8, 17, 1, 1), (1, 8, 4, -1, 1), (1, 8, 4, 1, -1),
+                (60000, 64, 4, 1 << 20, 0)):
+        with pytest.raises(ValueError):
+            paged_workspace_size(*bad)
+    lib = L.load()
+    for bad in ((0, 10, 0), (1, 0, 0), (1, 10, -1), (1, 10, 11), (1, 100, 65), (1, 2 ** 31, 0)):
+        assert lib.lq_logprobs_workspace(*bad) < 0
+    assert lib.lq_logprobs_workspace(1, 128256, 64) > 0
+
+
+def test_c_entries_refuse_null_and_bad_sizes():
+    lib = L.load()
+    res = L.Resident(a=16, b=16, mask=16, meta=16, exc=16, scale=16, n_exc=16, status=16, n_heads=2, cap_blocks=4, exc_cap=1)
+    rows = L.Rows(p=16, stride_b=128, stride_h=128, stride_t=128)
+    odd = L.Rows(p=16, stride_b=129, stride_h=128, stride_t=128)
+    r, q = ctypes.addressof(res), ctypes.addressof(rows)
+
+    def attend(k=r, v=r, qq=q, n=2, g=4, pages=16, width=3, counts=16, tk=q, tv=q, cap=4, work=16, nbytes=1 << 40, out=q, dt=0):
+        return lib.lq_paged_attention(k, v, qq, n, g, pages, width, counts, tk, tv, cap, None, None, 1.0, dt, work, nbytes,
+                                      out, None)
+    for bad in (dict(k=None), dict(v=None), dict(qq=None), dict(qq=ctypes.addressof(odd)), dict(n=0), dict(g=0), dict(g=17),
+                dict(pages=None), dict(counts=None), dict(tk=None), dict(cap=-1), dict(work=None), dict(work=24),
+                dict(nbytes=0), dict(out=None), dict(dt=2), dict(width=-1)):
+        assert attend(**bad) == L.LQ_ERR_ARG, bad
+    assert lib.lq_page_quantize(None, 0, 1, 16, 16, 16, r, 16, 16, None) == L.LQ_ERR_ARG
+    assert lib.lq_page_quantize(16, 0, 1, 17, 16, 16, r, 16, 16, None) == L.LQ_ERR_ARG
+    assert lib.lq_page_dequant(r, None, 1, 1, 16, 0, None) == L.LQ_ERR_ARG
+    ev = [16, 16, 16, 1, 4, 2, 1, 1, 16, 16, 16, 16, None]
+    for i, x in ((0, None), (3, 0), (4, 0), (5, 1), (6, -1), (7, -1), (11, None)):
+        bad = list(ev)
+        bad[i] = x
+        assert lib.lq_evict_pages(*bad) == L.LQ_ERR_ARG
+    lp = [16, 0, 10, 1, 10, None, 0, 16, 1 << 20, 16, 16, None, None, None]
+    for i, x in ((0, None), (1, 3), (2, -1), (3, 0), (4, 0), (6, 11), (7, None), (7, 8), (8, 0), (9, None), (10, None), (6, 2)):
+        bad = list(lp)
+        bad[i] = x
+        assert lib.lq_token_logprobs(*bad) == L.LQ_ERR_ARG
+
+
+def test_eviction_and_logprobs_need_the_gpu_and_sound_arguments():
+    w, p, n = torch.zeros(2, 3), torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for a, kw in (((p, n, w, 1), {}), ((p, n, w.half(), 1), {}), ((p, n, w[0], 1), {}), ((p, n, w, 1), dict(sink=1, recent=1)),
+                  ((p, n, w, -1), {}), ((p, n, w, 2), dict(sink=-1))):
+        with pytest.raises(ValueError):
+            evict_pages(*a, **kw)
+    x = torch.zeros(2, 5)
+    for a, kw in (((x,), {}), ((x.double(),), {}), ((x, torch.zeros(3, dtype=torch.int64)), {}), ((x,), dict(top=6)),
+                  ((x,), dict(top=-1)), ((x[:, :0],), {})):
+        with pytest.raises(ValueError):
+            token_logprobs(*a, **kw)
