@@ -754,18 +754,15 @@ int lq_evict_pages(const int32_t *d_pages, const int32_t *d_n_pages, const float
 
 #define LQ_LOGPROBS_MAX_TOP 64
 
-/* Workspace (bytes) of lq_token_logprobs, 16-byte aligned, uninitialised. */
-int64_t lq_logprobs_workspace(int64_t rows, int64_t vocab, int top);
-
 /* Of each of `rows` rows of logits (element (r, v) at r * stride + v; rows of any alignment,
- * vocab < 2^31): d_logprob[r] = log softmax at d_tokens[r] (0 for a negative token or without
+ * rows and vocab below 2^31): d_logprob[r] = log softmax at d_tokens[r] (0 for a negative token or without
  * d_tokens, NaN for one past the vocabulary), d_entropy[r] = -sum p log p, and the `top`
  * (0..64, at most vocab) largest logits' places d_ids[r][k] and log probabilities d_top[r][k],
  * in order (equal logits by place, NaN above all).  Logits of -inf weigh nothing; a row of
  * nothing else, with a NaN or with +inf has NaN. */
 int lq_token_logprobs(const void *d_logits, int dtype, int64_t stride, int64_t rows, int64_t vocab,
-                      const int64_t *d_tokens, int top, void *d_work, int64_t work_bytes, float *d_logprob,
-                      float *d_entropy, int64_t *d_ids, float *d_top, hipStream_t s);
+                      const int64_t *d_tokens, int top, float *d_logprob, float *d_entropy, int64_t *d_ids, float *d_top,
+                      hipStream_t s);
 
 #ifdef __cplusplus
 }

@@ -112,8 +112,7 @@ _SIGS = {
     "lq_paged_attention": ([_P, _P, _P, _I64, _INT, _P, _I64, _P, _P, _P, _I64, _P, _P, ctypes.c_float, _INT, _P, _I64] +
                            [_P] * 2, _INT),
     "lq_evict_pages": ([_P] * 3 + [_I64] * 5 + [_P] * 5, _INT),
-    "lq_logprobs_workspace": ([_I64, _I64, _INT], _I64),
-    "lq_token_logprobs": ([_P, _INT, _I64, _I64, _I64, _P, _INT, _P, _I64] + [_P] * 5, _INT),
+    "lq_token_logprobs": ([_P, _INT, _I64, _I64, _I64, _P, _INT] + [_P] * 5, _INT),
     "lq_tree_attn_workspace": ([_I64, _I64, _I64, _INT, _I64, _I64], _I64),
     "lq_resident_tree_attention": ([_P, _P, _I64] + [_P] * 4 + [_I64, _I64, _INT, _P, _P, _I64, _P, _P, _INT, _P, _I64] +
                                    [_P] * 2, _INT),

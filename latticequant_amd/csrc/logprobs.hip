@@ -4,9 +4,13 @@
 // a = sum 2^z z:
 //   log p(t) = ln 2 (z_t - log2 l),    H = ln 2 (log2 l - a / l),
 // in one pass over the logits: each lane has a reference r of its own, raised (l and a
-// rescaled) once a logit passes it by more than kLazy.  The `top` largest are kept as a
-// sorted list a wave, an entry a lane; a logit not above the list's last is passed over by
-// the same comparison that guards the reference.
+// rescaled) once the sums show that a logit is far beyond it.
+// The `top` largest are a sorted list a wave, an entry a lane.  A lane's vector of logits none
+// of which passes the list's last is passed over by one comparison; the others gather in
+// LDS, are looked at a logit a lane, and what passes gathers again and goes into the list 64 at
+// a time (sorted by a bitonic network, then merged), few of them one by one.  A first bound comes from the workgroup's first vectors: of the four
+// largest of the lanes' maxima of every wave the top-th largest, which `top` logits reach.
+// Few logits of a row pass it, and most waves need no list.
 #include <climits>
 #include <cmath>
 
@@ -19,23 +23,21 @@ namespace {
 inline int launch_status() { return hipGetLastError() == hipSuccess ? LQ_OK : LQ_ERR_LAUNCH; }
 
 constexpr int kTop = LQ_LOGPROBS_MAX_TOP;
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLazy = 8.0f;
+constexpr float kBig = 1e12f;                  // sums beyond it: the reference is too low
 constexpr float kHuge = 1e37f;                 // beyond it c x can leave fp32's range
+constexpr int kUnroll = 4;                     // vectors of 16 bytes a lane has in flight
 
 struct LogArgs {
     const char* logits;
-    int64_t stride, vocab, part;               // elements
+    int64_t stride, vocab;                     // elements
     const int64_t* tokens;
-    int top, parts;
+    int top;
     float* logprob;
     float* entropy;
     int64_t* ids;
     float* tops;
-    float4* stat;                              // [row][part]: m, l, a
-    uint64_t* keys;                            // [row][part][top]
 };
 
 // A logit and its place as one number: the larger value first (NaN above all; -0 as 0),
@@ -82,59 +84,195 @@ __device__ __forceinline__ void raise(Stat& s, float to) {
     s.l *= f;
     s.m = to;
 }
-__device__ __forceinline__ Stat join(Stat a, Stat b) {
-    const float m = fmaxf(a.m, b.m);
-    raise(a, m);
-    raise(b, m);
-    return {m, a.l + b.l, a.a + b.a};
-}
-
-// N logits; FAR where the reference is beyond kHuge.  A sum that is no number says that
-// one of them is none.
+// N logits; FAR where the reference is beyond kHuge.  Returns their sum: a NaN says that one
+// of them is none.
 template <bool FAR, int N>
-__device__ __forceinline__ float add(Stat& s, const float x[N]) {
+__device__ __forceinline__ float add(Stat& s, const float* x) {
     const float m = s.m == -INFINITY ? 0.f : s.m;
     const float r = -(m * kLog2e);
-    float l = 0.f, a = 0.f;
+    float l = 0.f;
 #pragma unroll
     for (int i = 0; i < N; i++) {
         // 2^-200 is 0, as 2^-inf, but 0 times -200 is 0 (and the maximum with a NaN is one)
         const float z = __builtin_elementwise_maximum(FAR ? z_of<true>(x[i], m) : __builtin_fmaf(x[i], kLog2e, r), -200.f);
         const float e = __builtin_amdgcn_exp2f(z);
         l += e;
-        a = __builtin_fmaf(e, z, a);
+        s.a = __builtin_fmaf(e, z, s.a);
     }
     s.l += l;
-    s.a += a;
     return l;
 }
+template <int N>
+__device__ __forceinline__ float max_of(const float* x) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i + 1 < N; i += 2) m = fmaxf(fmaxf(m, x[i]), x[i + 1]);   // v_max3
+    return N % 2 ? m : fmaxf(m, x[N - 1]);
+}
 
-// The wave's sorted list: lane i has the i-th largest key, 0 where there is none yet.
+// ---- sorted lists: lane i has the i-th largest of 64 keys, 0 for none
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp(uint64_t v) {
+    return (uint64_t)dpp<CTRL>((uint32_t)(v >> 32)) << 32 | dpp<CTRL>((uint32_t)v);
+}
+// the key of lane ^ X
+template <int X>
+__device__ __forceinline__ uint64_t of_lane_xor(uint64_t k, int lane) {
+    if constexpr (X == 1) return dpp<0xB1>(k);           // quad_perm
+    if constexpr (X == 2) return dpp<0x4E>(k);
+    if constexpr (X == 3) return dpp<0x1B>(k);
+    if constexpr (X == 4) return dpp<0x1B>(dpp<0x141>(k));   // row_half_mirror, then each quad reversed
+    if constexpr (X == 7) return dpp<0x141>(k);
+    if constexpr (X == 8) return dpp<0x128>(k);          // row_ror:8
+    if constexpr (X == 15) return dpp<0x140>(k);         // row_mirror
+    if constexpr (X == 31) return of_lane_xor<16>(dpp<0x140>(k), lane);
+    if constexpr (X == 63) return of_lane_xor<32>(of_lane_xor<31>(k, lane), lane);
+    if constexpr (X == 16 || X == 32) {                  // rows (halves) of two registers exchanged
+        const uint32_t hi = (uint32_t)(k >> 32), lo = (uint32_t)k;
+        if constexpr (X == 16) {
+            const auto h = __builtin_amdgcn_permlane16_swap(hi, hi, false, false), l = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+            return lane & 16 ? (uint64_t)h[0] << 32 | l[0] : (uint64_t)h[1] << 32 | l[1];
+        } else {
+            const auto h = __builtin_amdgcn_permlane32_swap(hi, hi, false, false), l = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+            return lane & 32 ? (uint64_t)h[0] << 32 | l[0] : (uint64_t)h[1] << 32 | l[1];
+        }
+    }
+    return 0;
+}
+// the larger of the keys of lane and lane ^ X in the lower lane
+template <int X>
+__device__ __forceinline__ uint64_t exchange(uint64_t k, int lane) {
+    constexpr int bit = X & ~(X >> 1);                   // X's highest bit
+    const uint64_t p = of_lane_xor<X>(k, lane);
+    return (p > k) != ((lane & bit) != 0) ? p : k;
+}
+__device__ __forceinline__ uint64_t halves(uint64_t k, int lane) {   // a bitonic sequence sorted
+    k = exchange<32>(k, lane);
+    k = exchange<16>(k, lane);
+    k = exchange<8>(k, lane);
+    k = exchange<4>(k, lane);
+    k = exchange<2>(k, lane);
+    return exchange<1>(k, lane);
+}
+__device__ __forceinline__ uint64_t sorted(uint64_t k, int lane) {
+    k = exchange<1>(k, lane);
+    k = exchange<3>(k, lane);
+    k = exchange<1>(k, lane);
+    k = exchange<7>(k, lane);
+    k = exchange<2>(k, lane);
+    k = exchange<1>(k, lane);
+    k = exchange<15>(k, lane);
+    k = exchange<4>(k, lane);
+    k = exchange<2>(k, lane);
+    k = exchange<1>(k, lane);
+    k = exchange<31>(k, lane);
+    k = exchange<8>(k, lane);
+    k = exchange<4>(k, lane);
+    k = exchange<2>(k, lane);
+    k = exchange<1>(k, lane);
+    k = exchange<63>(k, lane);
+    k = exchange<16>(k, lane);
+    k = exchange<8>(k, lane);
+    k = exchange<4>(k, lane);
+    k = exchange<2>(k, lane);
+    return exchange<1>(k, lane);
+}
+// the 64 largest of a sorted list and another, reversed one
+__device__ __forceinline__ uint64_t merged(uint64_t a, uint64_t reversed, int lane) {
+    return halves(a > reversed ? a : reversed, lane);
+}
+
+// the top-th largest of 64 numbers, one a lane, none of them a NaN
+template <int X>
+__device__ __forceinline__ float exchange(float v, int lane) {
+    constexpr int bit = X & ~(X >> 1);
+    const float p = __uint_as_float((uint32_t)of_lane_xor<X>((uint64_t)__float_as_uint(v), lane));
+    return lane & bit ? fminf(v, p) : fmaxf(v, p);
+}
+__device__ __forceinline__ float nth_largest(float v, int n, int lane) {
+    v = exchange<1>(v, lane);
+    v = exchange<3>(v, lane);
+    v = exchange<1>(v, lane);
+    v = exchange<7>(v, lane);
+    v = exchange<2>(v, lane);
+    v = exchange<1>(v, lane);
+    v = exchange<15>(v, lane);
+    v = exchange<4>(v, lane);
+    v = exchange<2>(v, lane);
+    v = exchange<1>(v, lane);
+    v = exchange<31>(v, lane);
+    v = exchange<8>(v, lane);
+    v = exchange<4>(v, lane);
+    v = exchange<2>(v, lane);
+    v = exchange<1>(v, lane);
+    v = exchange<63>(v, lane);
+    v = exchange<16>(v, lane);
+    v = exchange<8>(v, lane);
+    v = exchange<4>(v, lane);
+    v = exchange<2>(v, lane);
+    v = exchange<1>(v, lane);
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), n - 1));
+}
+
 struct List {
-    uint64_t key;
-    float last;                                // value of entry top - 1; NaN while there is none
+    uint64_t key, least;                       // least: entry top - 1
+    float bound;                               // no smaller logit is among the `top` largest
+    float last;                                // least's value; the bound where there is none yet
+    uint64_t* buf;                             // keys that passed, count of them
+    int count;
+    bool any;                                  // whether the list has any
 };
-__device__ __forceinline__ uint64_t lane_key(uint64_t k, int lane) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), lane) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, lane);
+__device__ __forceinline__ void settle(List& t, int top) {
+    t.least = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(t.key >> 32), top - 1) << 32 |
+              (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)t.key, top - 1);
+    t.last = t.least ? key_value(t.least) : t.bound;
 }
-__device__ __forceinline__ void insert(List& t, uint64_t k, int top, int lane) {   // k: wave-uniform
-    const int at = __builtin_popcountll(__ballot(t.key > k));
-    const uint64_t up = (uint64_t)__shfl_up((unsigned long long)t.key, 1, 64);
-    t.key = lane < at ? t.key : lane == at ? k : up;
-    const uint64_t l = lane_key(t.key, top - 1);
-    t.last = l ? key_value(l) : NAN;
+__device__ __forceinline__ void wave_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-// one key a lane, 0 for none
-__device__ __forceinline__ void insert_all(List& t, uint64_t k, int top, int lane) {
-    for (;;) {
-        const uint64_t hit = __ballot(k > lane_key(t.key, top - 1));
-        if (!hit) return;
-        const int from = __ffsll((long long)hit) - 1;
-        insert(t, lane_key(k, from), top, lane);
-        if (lane == from) k = 0;
+// n keys, one a lane and 0 in the others, into the list
+__device__ __forceinline__ void take(List& t, uint64_t k, int n, int lane) {
+    if (n > 16) {
+        t.key = merged(t.key, of_lane_xor<63>(sorted(k, lane), lane), lane);
+    } else {
+        for (int i = 0; i < n; i++) {
+            const uint64_t c = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), i) << 32 |
+                               (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, i);
+            const int at = __builtin_popcountll(__ballot(t.key > c));
+            const uint64_t up = dpp<0x138>(t.key);       // wave_shr:1
+            t.key = lane < at ? t.key : lane == at ? c : up;
+        }
     }
 }
+__device__ __forceinline__ void flush(List& t, int top, int lane) {   // the buffer's last 64
+    const int n = min(t.count, 64);
+    t.count -= n;
+    wave_lds_sync();
+    const uint64_t k = lane < n ? t.buf[t.count + lane] : 0ull;
+    wave_lds_sync();
+    take(t, k, n, lane);
+    settle(t, top);
+    t.any = true;
+}
+// one logit a lane, of those that have one, to the buffer
+__device__ __forceinline__ void offer(List& t, float x, uint32_t at, bool mine, int lane) {
+    const bool in = mine && !(x < t.last);
+    if (!__ballot(in)) return;
+    const uint64_t k = key_of(x, at);
+    const bool c = in && k > t.least;
+    const uint64_t m = __ballot(c);
+    if (c) t.buf[t.count + __builtin_popcountll(m & ((1ull << lane) - 1ull))] = k;
+    t.count += __builtin_popcountll(m);
+}
+constexpr int kBuffer = 128;                   // keys left from before and those of an offer
+constexpr int kJoint = 512;                    // keys of all waves that go into one list
 
 // (r's rounding is in z and l alike; what it leaves is at most 0 for p = 1, not above)
 __device__ __forceinline__ float log_prob(float x, const Stat& s) {
@@ -143,166 +281,251 @@ __device__ __forceinline__ float log_prob(float x, const Stat& s) {
     return p > 0.f ? 0.f : p;
 }
 
-template <int DT>
-__device__ __forceinline__ void finish(const LogArgs& A, int64_t row, const Stat& s, uint64_t key, int lane) {
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, __uint_as_float(dpp<0xB1>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(dpp<0x4E>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(dpp<0x141>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(dpp<0x140>(__float_as_uint(v))));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v += __uint_as_float(dpp<0xB1>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x4E>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x141>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x140>(__float_as_uint(v)));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+__device__ __forceinline__ Stat wave_join(Stat s) {
+    raise(s, wave_max(s.m));
+    return {s.m, wave_sum(s.l), wave_sum(s.a)};
+}
+
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+
+// A row a workgroup.
+template <int DT, bool TOP, int NW>
+__global__ __launch_bounds__(NW * 64) void k_logprobs(LogArgs A) {
+    constexpr int E = DT == LQ_F32 ? 4 : 2, V = 16 / E, U = kUnroll, T = NW * 64;
+    __shared__ Stat s_stat[NW];
+    __shared__ float s_max[64];
+    __shared__ int s_count[NW];
+    constexpr int M = 64 / V, Q = M + U * 64;  // vectors looked at together, and a wave's queue of them
+    __shared__ uint64_t s_key[NW][TOP ? kBuffer : 1], s_joint[TOP ? kJoint : 1];
+    __shared__ u4_t s_vec[NW][TOP ? Q : 1];
+    __shared__ uint32_t s_at[NW][TOP ? Q : 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t row = blockIdx.x, n = A.vocab;
+    const char* base = A.logits + row * A.stride * E;
+    const int64_t tok = A.tokens ? A.tokens[row] : -1;
+    Stat s = {-INFINITY, 0.f, 0.f};
+    List t = {0ull, 0ull, -INFINITY, -INFINITY, s_key[wave], 0, false};
+    // rows need no alignment: what lies before the first 16-byte boundary and behind the last goes one by one
+    const int64_t head = min(n, (int64_t)((16 - ((uintptr_t)base & 15)) & 15) / E);
+    const int64_t nv = (n - head) / V, tail = head + nv * V;
+    if (wave == 0 && (head || tail < n)) {
+        const int64_t i = lane < V ? lane : tail + lane - V;
+        const bool mine = lane < V ? i < head : lane < 2 * V && i < n;
+        const float x = mine ? logit<DT>(base, i) : -INFINITY;
+        raise(s, fmaxf(s.m, x));
+        if (mine) {
+            if (far_of(s.m)) add<true, 1>(s, &x);
+            else add<false, 1>(s, &x);
+        }
+        if (TOP) offer(t, x, (uint32_t)i, mine, lane);
+    }
+    int queued = 0;
+    auto drain = [&]() __attribute__((always_inline)) {
+        wave_lds_sync();
+        while (queued) {
+            const int m = min(queued, M), at = queued - m + lane / V;
+            queued -= m;
+            const bool mine = lane / V < m;
+            const float x = mine ? logit<DT>(reinterpret_cast<const char*>(&s_vec[wave][at]), lane % V) : 0.f;
+            offer(t, x, (uint32_t)head + (mine ? s_at[wave][at] : 0u) * V + lane % V, mine, lane);
+            if (t.count >= 64) flush(t, A.top, lane);
+        }
+        wave_lds_sync();
+    };
+    u4_t next[U];
+    // past the row -inf, which weighs nothing
+    constexpr uint32_t none = DT == LQ_F32 ? 0xff800000u : DT == LQ_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+    auto fetch = [&](int64_t j0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t j = j0 + u * T + lane;
+            next[u] = u4_t{none, none, none, none};
+            if (j < nv) next[u] = __builtin_nontemporal_load(reinterpret_cast<const u4_t*>(base + head * E) + j);
+        }
+    };
+    fetch(wave * 64);
+    bool first = TOP;
+    for (int64_t j0 = wave * 64; first || j0 < nv; j0 += U * T) {
+        u4_t w[U];
+        float mx[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) w[u] = next[u];
+        fetch(j0 + U * T);
+        auto unpack = [&](const u4_t& v, float* x) __attribute__((always_inline)) {
+            if constexpr (DT == LQ_F32) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = __uint_as_float(v[e]);
+            } else {
+                unpack8(make_uint4(v[0], v[1], v[2], v[3]), DT, x);
+            }
+        };
+        // Without a look at the largest logit and at -inf first: where the sums show that the
+        // reference was too low, or a logit -inf, they are taken again with both.
+        float l = 0.f, a = NAN;
+        if (j0 >= T) {                         // there is a reference
+            const float r = -(s.m * kLog2e);
+            a = 0.f;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float x[V];
+                unpack(w[u], x);
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    const float z = __builtin_fmaf(x[e], kLog2e, r), p = __builtin_amdgcn_exp2f(z);
+                    l += p;
+                    a = __builtin_fmaf(p, z, a);
+                }
+            }
+        }
+        if (TOP) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float x[V];
+                unpack(w[u], x);
+                mx[u] = max_of<V>(x);
+            }
+        }
+        bool odd = false;                      // a logit is a NaN (or the sum is none for another reason)
+        if (__any(!(l < kBig) || a != a)) {
+            float x[U * V];
+#pragma unroll
+            for (int u = 0; u < U; u++) unpack(w[u], x + u * V);
+            const float all = max_of<U * V>(x);
+            if (all > s.m + kLazy || (s.m == -INFINITY && all > -INFINITY)) raise(s, all);
+            l = far_of(s.m) ? add<true, U * V>(s, x) : add<false, U * V>(s, x);
+            odd = l != l;
+        } else {
+            s.l += l;
+            s.a += a;
+        }
+        if (!TOP) continue;
+        if (first) {
+            first = false;
+            constexpr int J = 64 / NW;         // a wave's part of the 64 maxima
+            float v = max_of<U>(mx), own = -INFINITY;
+            v = v == v ? v : -INFINITY;
+            for (int i = 0; i < min(J, A.top); i++) {
+                const float b = wave_max(v);
+                const int at = __ffsll((long long)__ballot(v == b)) - 1;
+                v = lane == at ? -INFINITY : v;
+                own = lane == i ? b : own;
+            }
+            if (lane < J) s_max[wave * J + lane] = own;
+            __syncthreads();
+            v = s_max[lane];
+            if (A.top > 6) {
+                t.bound = nth_largest(v, A.top, lane);
+            } else {
+                for (int i = 0; i < A.top; i++) {
+                    t.bound = wave_max(v);
+                    const int at = __ffsll((long long)__ballot(v == t.bound)) - 1;
+                    v = lane == at ? -INFINITY : v;
+                }
+            }
+            if (!t.least) t.last = t.bound;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t j = j0 + u * T + lane;
+            const bool hit = j < nv && (odd || mx[u] >= t.last);
+            const uint64_t m = __ballot(hit);
+            if (!m) continue;
+            if (hit) {
+                const int to = queued + __builtin_popcountll(m & ((1ull << lane) - 1ull));
+                s_vec[wave][to] = w[u];
+                s_at[wave][to] = (uint32_t)j;
+            }
+            queued += __builtin_popcountll(m);
+        }
+        if (queued >= M) drain();
+    }
+    if (TOP && queued) drain();
+    s = wave_join(s);
+    if (lane == 0) s_stat[wave] = s;
+    if (TOP) {
+        if (t.any && t.count) flush(t, A.top, lane);
+        if (lane == 0) s_count[wave] = t.any ? -1 : t.count;
+    }
+    __syncthreads();
+    int all_n = 0, before = 0;                 // keys of waves without a list
+    if (TOP) {
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const int c = max(s_count[w], 0);
+            before += w < wave ? c : 0;
+            all_n += c;
+        }
+        const bool lists = all_n > kJoint;     // too many: lists of all waves
+        if (lists && !t.any) flush(t, A.top, lane);
+        all_n = lists ? 0 : all_n;
+        if (t.any) s_key[wave][lane] = t.key;
+        else if (lane < t.count) s_joint[before + lane] = t.buf[lane];
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll 1
+            for (int w = 1; w < NW; w++)
+                if (lists || s_count[w] < 0) t.key = merged(t.key, s_key[w][63 - lane], lane);
+#pragma unroll 1
+            for (int i = 0; i < all_n; i += 64)
+                take(t, i + lane < all_n ? s_joint[i + lane] : 0ull, min(64, all_n - i), lane);
+        }
+    }
+    if (wave) return;
+    s = wave_join(lane < NW ? s_stat[lane] : Stat{-INFINITY, 0.f, 0.f});
     if (lane == 0) {
-        const int64_t t = A.tokens ? A.tokens[row] : -1;
-        A.logprob[row] = t < 0 ? 0.f : t >= A.vocab ? NAN
-                               : log_prob(logit<DT>(A.logits, row * A.stride + t), s);
+        A.logprob[row] = tok < 0 ? 0.f : tok >= n ? NAN : log_prob(logit<DT>(base, tok), s);
         const float h = kLn2 * (__builtin_amdgcn_logf(s.l) - s.a / s.l);
         A.entropy[row] = h < 0.f ? 0.f : h;
     }
-    if (lane < A.top) {
-        A.ids[row * A.top + lane] = (int64_t)(0xffffffffu - (uint32_t)key);
-        A.tops[row * A.top + lane] = log_prob(key_value(key), s);
+    if (TOP && lane < A.top) {
+        A.ids[row * A.top + lane] = (int64_t)(0xffffffffu - (uint32_t)t.key);
+        A.tops[row * A.top + lane] = log_prob(key_value(t.key), s);
     }
 }
 
-// A part of a row a workgroup.
-template <int DT, bool TOP>
-__global__ __launch_bounds__(kThreads) void k_logprobs(LogArgs A) {
-    constexpr int E = DT == LQ_F32 ? 4 : 2, V = 16 / E;
-    __shared__ Stat s_stat[kWaves];
-    __shared__ uint64_t s_key[kWaves][TOP ? kTop : 1];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t row = blockIdx.x / (uint32_t)A.parts, part = blockIdx.x % (uint32_t)A.parts;
-    const int64_t lo = part * A.part, hi = min(lo + A.part, A.vocab);
-    const char* base = A.logits + row * A.stride * E;
-    Stat s = {-INFINITY, 0.f, 0.f};
-    List t = {0ull, NAN};
-    // rows need no alignment: what lies before the first 16-byte boundary and behind the last goes one by one
-    const int64_t head = min(hi, lo + (int64_t)((16 - ((uintptr_t)(base + lo * E) & 15)) & 15) / E);
-    const int64_t nv = (hi - head) / V, tail = head + nv * V;
-    // places grow in a lane's and a wave's order: of equal logits the list keeps the first
-    auto single = [&](int64_t i, bool mine) __attribute__((always_inline)) {
-        const float x[1] = {mine ? logit<DT>(base, i) : -INFINITY};
-        raise(s, fmaxf(s.m, x[0]));
-        if (mine) {
-            if (far_of(s.m)) add<true, 1>(s, x);
-            else add<false, 1>(s, x);
-        }
-        if (TOP) insert_all(t, mine ? key_of(x[0], (uint32_t)i) : 0ull, A.top, lane);
-    };
-    if (head > lo) single(lo + tid, lo + tid < head);
-    for (int64_t j0 = 0; j0 < nv; j0 += kThreads) {
-        const int64_t j = j0 + tid, i = head + j * V;
-        const bool mine = j < nv;
-        const uint4 w = *reinterpret_cast<const uint4*>(base + (mine ? i : head) * E);
-        float x[8];
-        if constexpr (DT == LQ_F32) {
-            x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
-        } else {
-            unpack8(w, DT, x);
-        }
-        float mx = x[0];
-#pragma unroll
-        for (int e = 1; e < V; e++) mx = fmaxf(mx, x[e]);
-        float l = 0.f;
-        if (mine) {
-            if (mx > s.m + kLazy || (s.m == -INFINITY && mx > -INFINITY)) raise(s, mx);
-            l = far_of(s.m) ? add<true, V>(s, x) : add<false, V>(s, x);
-        }
-        // an equal logit loses to those of earlier rounds, not to all of this one
-        const float last = t.last;
-        if (TOP && __any(mine && (!(mx <= last) || l != l))) {
-#pragma unroll
-            for (int e = 0; e < V; e++)
-                insert_all(t, mine && !(x[e] <= last) ? key_of(x[e], (uint32_t)(i + e)) : 0ull, A.top, lane);
-        }
-    }
-    if (tail < hi) single(tail + tid, tail + tid < hi);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        s = join(s, {__shfl_xor(s.m, o, 64), __shfl_xor(s.l, o, 64), __shfl_xor(s.a, o, 64)});
-    if (lane == 0) s_stat[wave] = s;
-    if (TOP && lane < A.top) s_key[wave][lane] = t.key;
-    __syncthreads();
-    if (wave) return;
-#pragma unroll
-    for (int w = 1; w < kWaves; w++) {
-        s = join(s, s_stat[w]);
-        if (TOP) insert_all(t, lane < A.top ? s_key[w][lane] : 0ull, A.top, lane);
-    }
-    if (A.parts == 1) {
-        finish<DT>(A, row, s, t.key, lane);
-        return;
-    }
-    const int64_t at = row * A.parts + part;
-    if (lane == 0) A.stat[at] = make_float4(s.m, s.l, s.a, 0.f);
-    if (TOP && lane < A.top) A.keys[at * A.top + lane] = t.key;
+template <int DT, int NW>
+void launch(const LogArgs& A, int64_t rows, hipStream_t s) {
+    if (A.top) hipLaunchKernelGGL((k_logprobs<DT, true, NW>), dim3((unsigned)rows), dim3(NW * 64), 0, s, A);
+    else hipLaunchKernelGGL((k_logprobs<DT, false, NW>), dim3((unsigned)rows), dim3(NW * 64), 0, s, A);
 }
-
-// A wave per row: its parts joined.
-template <int DT, bool TOP>
-__global__ __launch_bounds__(64) void k_logprobs_join(LogArgs A) {
-    const int lane = threadIdx.x;
-    const int64_t row = blockIdx.x;
-    Stat s = {-INFINITY, 0.f, 0.f};
-    for (int p = lane; p < A.parts; p += 64) {
-        const float4 x = A.stat[row * A.parts + p];
-        s = join(s, {x.x, x.y, x.z});
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        s = join(s, {__shfl_xor(s.m, o, 64), __shfl_xor(s.l, o, 64), __shfl_xor(s.a, o, 64)});
-    List t = {0ull, NAN};
-    if (TOP) {
-        const int n = A.parts * A.top;
-        for (int i = lane; i - lane < n; i += 64)
-            insert_all(t, i < n ? A.keys[row * n + i] : 0ull, A.top, lane);
-    }
-    finish<DT>(A, row, s, t.key, lane);
-}
-
-// Parts of a row: enough that all rows' fill the chip, of 8192 logits at least.
-int64_t parts_of(int64_t rows, int64_t vocab) {
-    const int64_t want = (1024 + rows - 1) / rows, most = (vocab + 8191) / 8192;
-    return want < most ? want : most;
-}
-
 template <int DT>
 void launch(const LogArgs& A, int64_t rows, hipStream_t s) {
-    const dim3 grid((unsigned)(rows * A.parts));
-    if (A.top) {
-        hipLaunchKernelGGL((k_logprobs<DT, true>), grid, dim3(kThreads), 0, s, A);
-        if (A.parts > 1) hipLaunchKernelGGL((k_logprobs_join<DT, true>), dim3((unsigned)rows), dim3(64), 0, s, A);
-    } else {
-        hipLaunchKernelGGL((k_logprobs<DT, false>), grid, dim3(kThreads), 0, s, A);
-        if (A.parts > 1) hipLaunchKernelGGL((k_logprobs_join<DT, false>), dim3((unsigned)rows), dim3(64), 0, s, A);
-    }
+    // few rows: a compute unit reads its row as fast as sixteen waves ask for it
+    if (rows < 1024 && A.vocab > 4096) launch<DT, 16>(A, rows, s);
+    else launch<DT, 4>(A, rows, s);
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t lq_logprobs_workspace(int64_t rows, int64_t vocab, int top) {
-    if (rows < 1 || rows > INT_MAX / 1024 || vocab < 1 || vocab > INT_MAX || top < 0 || top > kTop || top > vocab) return -1;
-    const int64_t parts = parts_of(rows, vocab);
-    return parts > 1 ? rows * parts * (16 + 8 * (int64_t)top) : 16;
-}
-
 int lq_token_logprobs(const void *d_logits, int dtype, int64_t stride, int64_t rows, int64_t vocab,
-                      const int64_t *d_tokens, int top, void *d_work, int64_t work_bytes, float *d_logprob,
-                      float *d_entropy, int64_t *d_ids, float *d_top, hipStream_t s) {
-    const int64_t need = lq_logprobs_workspace(rows, vocab, top);
-    if (!d_logits || dtype < 0 || dtype > 2 || stride < 0 || need < 0 || !d_work || ((uintptr_t)d_work & 15) ||
-        work_bytes < need || !d_logprob || !d_entropy || (top && (!d_ids || !d_top)))
+                      const int64_t *d_tokens, int top, float *d_logprob, float *d_entropy, int64_t *d_ids, float *d_top,
+                      hipStream_t s) {
+    if (!d_logits || dtype < 0 || dtype > 2 || stride < 0 || rows < 1 || rows > INT_MAX || vocab < 1 || vocab > INT_MAX ||
+        top < 0 || top > kTop || top > vocab || !d_logprob || !d_entropy || (top && (!d_ids || !d_top)))
         return LQ_ERR_ARG;
-    LogArgs A{};
-    A.logits = static_cast<const char*>(d_logits);
-    A.stride = stride;
-    A.vocab = vocab;
-    A.parts = (int)parts_of(rows, vocab);
-    A.part = (vocab + A.parts - 1) / A.parts;
-    A.tokens = d_tokens;
-    A.top = top;
-    A.logprob = d_logprob;
-    A.entropy = d_entropy;
-    A.ids = d_ids;
-    A.tops = d_top;
-    A.stat = static_cast<float4*>(d_work);
-    A.keys = reinterpret_cast<uint64_t*>(A.stat + rows * A.parts);
+    const LogArgs A = {static_cast<const char*>(d_logits), stride, vocab, d_tokens, top, d_logprob, d_entropy, d_ids, d_top};
     if (dtype == LQ_F32) launch<LQ_F32>(A, rows, s);
     else if (dtype == LQ_BF16) launch<LQ_BF16>(A, rows, s);
     else launch<LQ_F16>(A, rows, s);

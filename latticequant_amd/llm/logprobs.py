@@ -24,23 +24,14 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: Optional[torch.Tensor]   # (..., top) fp32
 
 
-def logprobs_workspace(rows: int, vocab: int, top: int = 0, device=None) -> torch.Tensor:
-    """Workspace of token_logprobs, uninitialised."""
-    n = L.load().lq_logprobs_workspace(rows, vocab, top)
-    if n < 0:
-        raise ValueError("bad log probability geometry")
-    return torch.empty(n, dtype=torch.uint8, device=device)
-
-
-def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0,
-                   work: Optional[torch.Tensor] = None) -> TokenLogprobs:
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
     """logits: (..., V) fp16, bf16 or fp32, rows of any strides with a contiguous last
     dimension (others are copied); tokens: (...) int64 or None (log probabilities 0 then);
     top: 0..64 alternatives, at most V.  Natural logarithms.
     A negative token names none: its log probability is 0; one of V or more gives NaN.
     Logits of -inf weigh nothing; a row of nothing else, or with a NaN or +inf, is NaN.
     Alternatives are in order of their logits, the lower id first of equal ones, NaN above
-    all.  work: logprobs_workspace, used until the call's work on the stream is done."""
+    all.  Nothing waits for the device."""
     if logits.dim() < 1 or logits.dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise ValueError("logits must be (..., V) fp16, bf16 or fp32")
     dev = logits.device
@@ -66,17 +57,9 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
             ids = torch.empty(shape + (top,), dtype=torch.int64, device=dev)
             tops = torch.empty(shape + (top,), dtype=torch.float32, device=dev)
         if n:
-            need = lib.lq_logprobs_workspace(n, V, top)
-            if need < 0:
-                raise ValueError("too many rows or too large a vocabulary")
-            if work is None:
-                work = torch.empty(need, dtype=torch.uint8, device=dev)
-            elif work.device != dev or not work.is_contiguous() or work.numel() * work.element_size() < need:
-                raise ValueError("the workspace must be logprobs_workspace bytes or more, on the logits' device")
             tok = None if tokens is None else tokens.contiguous()
             at = both.data_ptr()
             L.check(lib.lq_token_logprobs(x.data_ptr(), L.dtype_code(x.dtype), x.stride(0), n, V,
-                                          None if tok is None else tok.data_ptr(), top, work.data_ptr(),
-                                          work.numel() * work.element_size(), at, at + 4 * n, L.ptr(ids), L.ptr(tops),
-                                          L.raw_stream(dev)), "lq_token_logprobs")
+                                          None if tok is None else tok.data_ptr(), top, at, at + 4 * n, L.ptr(ids),
+                                          L.ptr(tops), L.raw_stream(dev)), "lq_token_logprobs")
     return TokenLogprobs(both[0], both[1], ids, tops)

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from latticequant_amd.llm.logprobs import logprobs_workspace, token_logprobs
+from latticequant_amd.llm.logprobs import token_logprobs
 
 pytestmark = pytest.mark.gpu
 DT = [torch.bfloat16, torch.float16, torch.float32]
@@ -144,12 +144,11 @@ def test_offsets_past_32_bits():
 def test_captured_and_other_streams():
     x = torch.randn(3, 60000, device="cuda").bfloat16()
     tok = torch.randint(0, 60000, (3,), device="cuda")
-    work = logprobs_workspace(3, 60000, 7, device="cuda")
     want = token_logprobs(x, tok, 7)
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
-        got = token_logprobs(x, tok, 7, work=work)
+        got = token_logprobs(x, tok, 7)
     for i in range(4):
         x.copy_(torch.randn(3, 60000, device="cuda"))
         g.replay()
@@ -170,5 +169,3 @@ def test_refusals():
     x = torch.randn(2, 50, device="cuda")
     with pytest.raises(RuntimeError, match="no gradient"):
         token_logprobs(x.clone().requires_grad_())
-    with pytest.raises(ValueError, match="workspace"):
-        token_logprobs(torch.randn(2, 50000, device="cuda"), work=torch.empty(16, dtype=torch.uint8, device="cuda"))
