@@ -14,7 +14,10 @@
 // the sequences' tiles and takes an equal share of the list, every wave an equal part of
 // that, so lengths of any mix load the chip evenly.  A (sequence, head) that lies within
 // a wave is written out by it; the pieces of one that several waves share are joined in
-// LDS, those that several workgroups share by k_paged_join, in the order of the list.
+// LDS, those that several workgroups share by k_paged_join, in the order of the list.  (The
+// last of the workgroups joining them itself, by a counter per unit, was no faster: its
+// device-scope stores, release and acquire took the 4 to 5 us of the second launch with 136
+// tiles, and 9 us more than it with 8200.)
 #include <climits>
 #include <cmath>
 
@@ -52,7 +55,7 @@ struct PagedArgs {
     Rows q, tk, tv;
     uint16_t* out;
     int64_t ob, oh;
-    int n_seq, heads, group, per;              // per: sequences of a thread's sum
+    int n_seq, heads, group, per;              // per: sequences of a lane's sum
     float* rec;                                // [2 workgroup + (0: of an earlier one's, 1: begun here)][row][kRecF]
     Desc* desc;
     float* lse;                                // [unit][row]: m + log2(l32), with the weights' factor 2^kPShift
@@ -186,12 +189,22 @@ __device__ __forceinline__ void put8(const PagedArgs& A, int unit, int row, int 
     *reinterpret_cast<uint4*>(A.out + b * A.ob + (int64_t)(h * A.group + row) * A.oh + d) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The lengths of up to 64 sequences, one a lane (per == 1), or from memory.
+struct Lens {
+    int pages, tail;
+};
+__device__ __forceinline__ Len len_at(const PagedArgs& A, const Lens& mine, int b) {
+    if (A.per > 1) return len_of(A, b);
+    Len l;
+    l.pages = __builtin_amdgcn_readlane(mine.pages, b);
+    l.tail = __builtin_amdgcn_readlane(mine.tail, b);
+    l.page_tiles = (l.pages + 1) >> 1;
+    l.tiles = l.page_tiles + ((l.tail + 31) >> 5);
+    return l;
+}
 template <bool BF16, bool SUMS, bool BIG>
 __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
     extern __shared__ __align__(16) char s_dyn[];
-    __shared__ uint32_t s_sum[kWaves];
-    __shared__ int s_b[kWaves];
-    __shared__ uint32_t s_rem[kWaves];
     // pieces in the order of the list: wave w's first (2 w), which ends its unit there, and its last (2 w + 1)
     __shared__ int s_unit[2 * kWaves], s_begins[2 * kWaves];
     __shared__ uint32_t s_end;                 // where the list's unit that is begun here and not ended ends
@@ -202,27 +215,25 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
     char* mine = s_dyn + wave * stride;        // exceptions, then the wave's last piece; behind it its first
     u32x4_t* area = reinterpret_cast<u32x4_t*>(mine);
 
-    // ---- the workgroup's share of the list
-    const int b0 = tid * A.per, b1 = min(b0 + A.per, A.n_seq);
+    // ---- the workgroup's share of the list, found by every wave for itself
+    Lens lens = {0, 0};
     uint32_t own = 0;
-    for (int b = b0; b < b1; b++) own += (uint32_t)len_of(A, b).tiles * A.heads;
+    for (int b = lane * A.per; b < min((lane + 1) * A.per, A.n_seq); b++) {
+        const Len l = len_of(A, b);
+        lens = {l.pages, l.tail};
+        own += (uint32_t)l.tiles * A.heads;
+    }
     uint32_t upto = own;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const uint32_t x = __shfl_up(upto, o, 64);
         upto += lane >= o ? x : 0u;
     }
-    if (lane == 63) s_sum[wave] = upto;
+    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63), before = upto - own;
     if (tid < 2 * kWaves) s_unit[tid] = -1;
     __syncthreads();
-    uint32_t total = 0, before = upto - own;
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) {
-        before += w < wave ? s_sum[w] : 0u;
-        total += s_sum[w];
-    }
     for (int b = blockIdx.x; b < A.n_seq; b += gridDim.x)
-        if (len_of(A, b).tiles == 0) zero_out(A, b, tid);
+        if (len_at(A, lens, b).tiles == 0) zero_out(A, b, tid);
     const uint32_t groups = max(1u, min((uint32_t)gridDim.x, (total + kWaves - 1) / kWaves));
     const uint32_t me = blockIdx.x;
     if (me >= groups) {
@@ -230,34 +241,23 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
         return;
     }
     const uint32_t lo = (uint32_t)((uint64_t)me * total / groups), hi = (uint32_t)((uint64_t)(me + 1) * total / groups);
-    for (int w = 0; w < kWaves; w++) {
-        const uint32_t p = lo + (uint32_t)((uint64_t)(hi - lo) * w / kWaves);
-        if (p >= before && p < before + own) {
-            uint32_t rem = p - before;
-            int b = b0;
-            for (;;) {
-                const uint32_t n = (uint32_t)len_of(A, b).tiles * A.heads;
-                if (rem < n || b + 1 >= b1) break;
-                rem -= n;
-                b++;
-            }
-            s_b[w] = b;
-            s_rem[w] = rem;
-        }
-    }
-    __syncthreads();
     uint32_t pos = lo + (uint32_t)((uint64_t)(hi - lo) * wave / kWaves);
     const uint32_t end = lo + (uint32_t)((uint64_t)(hi - lo) * (wave + 1) / kWaves);
 
     if (pos < end) {
-        int b = __builtin_amdgcn_readfirstlane(s_b[wave]);
-        Len L = len_of(A, b);
-        int h, t;
-        {
-            const uint32_t rem = (uint32_t)__builtin_amdgcn_readfirstlane((int)s_rem[wave]);
-            h = (int)(rem / (uint32_t)max(L.tiles, 1));
-            t = (int)(rem % (uint32_t)max(L.tiles, 1));
+        const uint64_t there = __ballot(pos >= before && pos - before < own);
+        const int from = __ffsll((long long)there) - 1;
+        uint32_t rem = pos - (uint32_t)__builtin_amdgcn_readlane((int)before, from);
+        int b = from * A.per;
+        Len L = len_at(A, lens, b);
+        for (int k = 1; k < A.per; k++) {
+            const uint32_t n = (uint32_t)L.tiles * A.heads;
+            if (rem < n || b + 1 >= A.n_seq) break;
+            rem -= n;
+            L = len_of(A, ++b);
         }
+        const uint32_t tiles = (uint32_t)max(L.tiles, 1);
+        int h = (int)(rem / tiles), t = (int)(rem % tiles);
         for (;;) {
             const int unit = b * A.heads + h;
             const int n = (int)min((uint32_t)(L.tiles - t), end - pos);
@@ -423,7 +423,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                 h = 0;
                 do {
                     if (++b >= A.n_seq) break;
-                    L = len_of(A, b);
+                    L = len_at(A, lens, b);
                 } while (L.tiles == 0);
                 if (b >= A.n_seq) break;
             }
@@ -551,18 +551,35 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs A) {
 }
 
 // weights[b][j] = decay * weights[b][j] + the page's weight of this step (decay 0: that
-// alone), a thread a page.
+// alone), a lane a page, the heads dealt to four waves whose sums are joined in order.
+template <int G4>   // whole rows of four, or 0 for any group
 __global__ __launch_bounds__(256) void k_page_weights(PagedArgs A, float* __restrict__ w, float decay) {
-    const int b = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
+    __shared__ float s_sum[4][64];
+    const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.x * 64 + lane;
     const int n = min(max(A.n_pages[b], 0), (int)A.width);
-    if (j >= n) return;
+    if ((int)blockIdx.x * 64 >= n) return;
     float sum = 0.f;
-    for (int h = 0; h < A.heads; h++) {
-        const int64_t unit = (int64_t)b * A.heads + h;
-        const float* z = A.z + (unit * A.width + j) * A.group;
-        const float* lse = A.lse + unit * A.group;
-        for (int r = 0; r < A.group; r++) sum += __builtin_amdgcn_exp2f(z[r] - lse[r]);
+    if (j < n) {
+        for (int h = wave; h < A.heads; h += 4) {
+            const int64_t unit = (int64_t)b * A.heads + h;
+            const float* z = A.z + (unit * A.width + j) * A.group;
+            const float* lse = A.lse + unit * A.group;
+            if constexpr (G4) {
+#pragma unroll
+                for (int r = 0; r < 4 * G4; r += 4) {
+                    const f4_t x = *reinterpret_cast<const f4_t*>(z + r);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sum += __builtin_amdgcn_exp2f(x[i] - lse[r + i]);
+                }
+            } else {
+                for (int r = 0; r < A.group; r++) sum += __builtin_amdgcn_exp2f(z[r] - lse[r]);
+            }
+        }
     }
+    s_sum[wave][lane] = sum;
+    __syncthreads();
+    if (wave || j >= n) return;
+    sum = (s_sum[0][lane] + s_sum[1][lane]) + (s_sum[2][lane] + s_sum[3][lane]);
     float* to = w + b * A.width + j;
     *to = decay == 0.f ? sum : __builtin_fmaf(decay, *to, sum);
 }
@@ -766,7 +783,7 @@ int lq_paged_attention(const lq_resident *k, const lq_resident *v, const lq_rows
     A.n_seq = (int)n_seq;
     A.heads = (int)k->n_heads;
     A.group = group;
-    A.per = (int)((n_seq + kThreads - 1) / kThreads);
+    A.per = (int)((n_seq + 63) / 64);
     char* w = static_cast<char*>(d_work);
     A.rec = reinterpret_cast<float*>(w + p.rec);
     A.desc = reinterpret_cast<Desc*>(w + p.desc);
@@ -780,9 +797,12 @@ int lq_paged_attention(const lq_resident *k, const lq_resident *v, const lq_rows
         if (d_weights) paged_launch<false, true>(A, p.grid, big, s);
         else paged_launch<false, false>(A, p.grid, big, s);
     }
-    if (d_weights && max_pages > 0)
-        hipLaunchKernelGGL(k_page_weights, dim3((unsigned)((max_pages + 255) / 256), (unsigned)n_seq), dim3(256), 0, s, A,
-                           d_weights, decay);
+    if (d_weights && max_pages > 0) {
+        const dim3 wg((unsigned)((max_pages + 63) / 64), (unsigned)n_seq);
+        if (group == 4) hipLaunchKernelGGL(k_page_weights<1>, wg, dim3(256), 0, s, A, d_weights, decay);
+        else if (group == 8) hipLaunchKernelGGL(k_page_weights<2>, wg, dim3(256), 0, s, A, d_weights, decay);
+        else hipLaunchKernelGGL(k_page_weights<0>, wg, dim3(256), 0, s, A, d_weights, decay);
+    }
     return launch_status();
 }
 
