@@ -702,25 +702,30 @@ int lq_resident_select_exceptions(const lq_resident *src, int64_t n_seq, int64_t
 
 /* --------------------------------------------------- pages, serving ---- */
 
-/* A pool of pages is an lq_resident of one kv head per row: page p is block p of every
- * head.  The same prefix form, its blocks read and written by number, so sequences of any
- * lengths share one pool and may share pages. */
+/* A pool of pages: a resident form of one head per kv head, whose blocks are read and
+ * written by number (page p is block p of every head), so sequences of any lengths share it
+ * and may share pages.  A vector with an exception entry has the record of the zero vector.
+ * Beside the form, which record an entry stands for, and how many entries each page owns (zeros
+ * at first). */
+typedef struct {
+    lq_resident r;
+    int32_t *room;           /* [n_heads][cap_blocks] */
+    uint8_t *rec;            /* [exc_cap]: 64 * group + slot */
+} lq_pages;
 
-/* Quantize x (n, heads, t_tokens, 128) (heads = r->n_heads, t_tokens a multiple of 16) into
+/* Quantize x (n, heads, t_tokens, 128) (heads = p->r.n_heads, t_tokens a multiple of 16) into
  * pages: token block j of row i goes to page d_pages[i * (t_tokens / 16) + j] of every
  * head, with the scales d_scale32 / d_scale16 [i * heads + h], as lq_resident_quantize.  A
  * number outside the pool moves nothing; one that stands twice leaves its page undefined.
- * d_room: int32 [n_heads][cap_blocks], zeros at first: how many exception entries each
- * page owns.  A page that needs more takes the next power of two at *n_exc.  Where the
- * list is too short (*n_exc > exc_cap, LQ_RES_ST_EXC_OVERFLOW), lengthen it (its first
- * exc_cap entries kept) and call again: no room is taken twice. */
+ * A page that needs more exception entries than it owns takes the next power of two at
+ * *n_exc.  Where the list is too short (*n_exc > exc_cap, LQ_RES_ST_EXC_OVERFLOW), lengthen it
+ * (its first exc_cap entries and their rec kept) and call again: no room is taken twice. */
 int lq_page_quantize(const void *d_x, int dtype, int64_t n, int64_t t_tokens, const float *d_scale32,
-                     const uint16_t *d_scale16, const lq_resident *r, const int32_t *d_pages, int32_t *d_room,
-                     hipStream_t s);
+                     const uint16_t *d_scale16, const lq_pages *p, const int32_t *d_pages, hipStream_t s);
 
 /* Pages back to rows: out (n, heads, per * 16, 128) fp16 / bf16 / fp32 from d_pages (n, per), as
  * lq_resident_dequant; zeros for numbers outside the pool. */
-int lq_page_dequant(const lq_resident *r, const int32_t *d_pages, int64_t n, int64_t per, void *d_out, int out_dtype,
+int lq_page_dequant(const lq_pages *p, const int32_t *d_pages, int64_t n, int64_t per, void *d_out, int out_dtype,
                     hipStream_t s);
 
 /* Workspace (bytes) of lq_paged_attention, 16-byte aligned; weights: whether d_weights is
@@ -736,9 +741,12 @@ int64_t lq_paged_attn_workspace(int64_t n_seq, int64_t heads, int group, int64_t
  * d_weights (nullable; [n_seq][max_pages]): d_weights[b][j] = decay * d_weights[b][j] + the
  * sum over the query heads of the softmax weight of page j's tokens, j < d_n_pages[b] (decay
  * 0: that sum, whatever stood there).
- * dtype LQ_F16 or LQ_BF16 of q, the tail and out, products fp16, as lq_resident_tree_attention.
+ * dtype LQ_F16 or LQ_BF16 of q, the tail and out, products fp16, as lq_resident_tree_attention
+ * (bf16 beyond fp16's range becomes infinite, below 2^-14 it loses bits).  A page's value is its
+ * lattice coordinate times its scale: V's unrounded, K's rounded to fp16 with d_weights, as
+ * lq_page_dequant rounds it, and unrounded without.
  * group 1..16; stride_t of q and out is not used.  Deterministic. */
-int lq_paged_attention(const lq_resident *k, const lq_resident *v, const lq_rows *q, int64_t n_seq, int group,
+int lq_paged_attention(const lq_pages *k, const lq_pages *v, const lq_rows *q, int64_t n_seq, int group,
                        const int32_t *d_pages, int64_t max_pages, const int32_t *d_n_pages, const lq_rows *tail_k,
                        const lq_rows *tail_v, int64_t tail_cap, const int32_t *d_tail_len, float *d_weights, float decay,
                        int dtype, void *d_work, int64_t work_bytes, const lq_rows *out, hipStream_t s);

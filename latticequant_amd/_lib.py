@@ -106,7 +106,7 @@ _SIGS = {
     "lq_select_total": ([_P, _P], _INT),
     "lq_resident_select": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _P], _INT),
     "lq_resident_select_exceptions": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P], _INT),
-    "lq_page_quantize": ([_P, _INT, _I64, _I64] + [_P] * 6, _INT),
+    "lq_page_quantize": ([_P, _INT, _I64, _I64] + [_P] * 5, _INT),
     "lq_page_dequant": ([_P, _P, _I64, _I64, _P, _INT, _P], _INT),
     "lq_paged_attn_workspace": ([_I64, _I64, _INT, _I64, _I64, _INT], _I64),
     "lq_paged_attention": ([_P, _P, _P, _I64, _INT, _P, _I64, _P, _P, _P, _I64, _P, _P, ctypes.c_float, _INT, _P, _I64] +
@@ -134,6 +134,11 @@ class Resident(ctypes.Structure):
     """lq_resident: device pointers + geometry of a resident (fixed-width) KV prefix."""
     _fields_ = [("a", _P), ("b", _P), ("mask", _P), ("meta", _P), ("exc", _P), ("scale", _P), ("n_exc", _P),
                 ("status", _P), ("n_heads", _I64), ("cap_blocks", _I64), ("exc_cap", _I64)]
+
+
+class Pages(ctypes.Structure):
+    """lq_pages: a resident form read and written by block number."""
+    _fields_ = [("r", Resident), ("room", _P), ("rec", _P)]
 
 
 class Rows(ctypes.Structure):

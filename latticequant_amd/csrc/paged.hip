@@ -47,7 +47,7 @@ struct Desc {                                  // the (sequence, head) that a wo
 };
 
 struct PagedArgs {
-    lq_resident k, v;
+    lq_pages k, v;
     const int32_t* pages;
     const int32_t* n_pages;
     const int32_t* tail_len;
@@ -88,53 +88,120 @@ __device__ __forceinline__ T at(const void* base, O bytes) {
     return *reinterpret_cast<const T*>(static_cast<const char*>(base) + bytes);
 }
 
-// K's records as k_tree_few's (KFew), b0 and b1 the tile's blocks
-template <bool BIG>
-__device__ __forceinline__ void load_k(const lq_resident& r, uint32_t b0, uint32_t b1, uint32_t lane, KFew& d) {
+// Records of a tile's blocks b0 and b1: of K, pairs of tokens 8 g + 2 i, + 1 (lane % 16 =
+// 4 g + i) of vectors 4 c + lane / 16; of V, vector lane % 16 of tokens 8 (lane / 16) .. + 7.
+struct Recs {
+    uint2 ka[4];
+    uint32_t kb[4];
+    uint4 va[2];
+    uint2 vb;
+    uint4 vs;                                  // scales of the lane's tokens of V ..
+    uint4 ks;                                  // .. and of K's, where the products come out; or
+    uint32_t kp;                               // of K's, where the records lie
+};
+struct Meta2 {
+    uint32_t base, count;                      // exceptions of block lane / 32
+};
+template <bool BIG, bool ROUND>
+__device__ __forceinline__ void load_recs(const PagedArgs& A, uint32_t b0, uint32_t b1, uint32_t lane, Recs& d) {
     typedef typename Off<BIG>::type O;
-    const uint32_t row = lane & 15, blk = row & 8 ? b1 : b0;
-    const uint32_t tok = 8 * ((row >> 2) & 1) + 2 * (row & 3), rec = 16 * (lane >> 4) + tok;
-    const O a = (O)blk * 1024 + rec * 4, b = (O)blk * 256 + rec;
+    const uint32_t row = lane & 15, kblk = row & 8 ? b1 : b0, vblk = lane & 32 ? b1 : b0;
+    const uint32_t tok = 8 * ((row >> 2) & 1) + 2 * (row & 3), krec = 16 * (lane >> 4) + tok;
+    const uint32_t half = (lane >> 4) & 1, vrec = 16 * row + 8 * half;
+    const O ka = (O)kblk * 1024 + krec * 4, kb = (O)kblk * 256 + krec;
+    const O va = (O)vblk * 1024 + vrec * 4, s = (O)vblk * 32 + half * 16;
 #pragma unroll
     for (int c = 0; c < 4; c++) {
-        d.a[c] = at<uint2>(r.a, a + 256 * c);
-        d.b[c] = at<uint16_t>(r.b, b + 64 * c);
+        d.ka[c] = at<uint2>(A.k.r.a, ka + 256 * c);
+        d.kb[c] = at<uint16_t>(A.k.r.b, kb + 64 * c);
     }
-    d.s = at<uint32_t>(r.scale, (O)blk * 32 + tok * 2);
-    d.mask = at<uint2>(r.mask, (O)(lane & 4 ? b1 : b0) * 32 + (lane & 3) * 8);
-}
-// V's: vector lane % 16 of tokens 8 (lane / 16) .. + 7
-template <bool BIG>
-__device__ __forceinline__ void load_v(const lq_resident& r, uint32_t b0, uint32_t b1, uint32_t lane, Raw& d) {
-    typedef typename Off<BIG>::type O;
-    const uint32_t blk = lane & 32 ? b1 : b0, rec = 16 * (lane & 15) + 8 * ((lane >> 4) & 1);
-    const O a = (O)blk * 1024 + rec * 4;
-    d.a[0] = at<uint4>(r.a, a);
-    d.a[1] = at<uint4>(r.a, a + 16);
-    const uint2 b = at<uint2>(r.b, (O)blk * 256 + rec);
-    const uint4 s = at<uint4>(r.scale, (O)blk * 32 + (rec & 15) * 2);
-    d.b[0] = b.x;
-    d.b[1] = b.y;
-    d.s[0] = make_uint2(s.x, s.y);
-    d.s[1] = make_uint2(s.z, s.w);
-    d.mask[0] = at<uint2>(r.mask, (O)blk * 32 + (rec >> 6) * 8);
+    if constexpr (ROUND) d.kp = at<uint32_t>(A.k.r.scale, (O)kblk * 32 + tok * 2);
+    else d.ks = at<uint4>(A.k.r.scale, s);
+    d.va[0] = at<uint4>(A.v.r.a, va);
+    d.va[1] = at<uint4>(A.v.r.a, va + 16);
+    d.vb = at<uint2>(A.v.r.b, (O)vblk * 256 + vrec);
+    d.vs = at<uint4>(A.v.r.scale, s);
 }
 template <bool BIG>
-__device__ __forceinline__ Meta load_meta(const lq_resident& r, uint32_t b0, uint32_t b1, uint32_t lane) {
+__device__ __forceinline__ Meta2 load_meta(const lq_pages& p, uint32_t b0, uint32_t b1, uint32_t lane) {
     typedef typename Off<BIG>::type O;
-    const uint4 w = at<uint4>(r.meta, (O)(lane & 32 ? b1 : b0) * 16);
-    return {w.x, w.y, w.z, w.w};
+    const uint2 w = at<uint2>(p.r.meta, (O)(lane & 32 ? b1 : b0) * 16 + 8);
+    return {w.x, w.y};
+}
+// The first 32 exceptions of each block, one a lane, with the number of its record.
+struct Entry {
+    uint4 v;
+    uint32_t rec;
+};
+__device__ __forceinline__ Entry load_entry(const lq_pages& p, const Meta2& m, uint32_t e) {
+    const int64_t i = (int64_t)m.base + e, from = e < m.count && i < p.r.exc_cap ? i : 0;
+    return {reinterpret_cast<const uint4*>(p.r.exc)[from], p.rec[from]};
+}
+__device__ __forceinline__ uint32_t most_of(const Meta2& m) {   // wave-uniform
+    return max((uint32_t)__builtin_amdgcn_readlane((int)m.count, 0), (uint32_t)__builtin_amdgcn_readlane((int)m.count, 32));
+}
+// put(rec, v): the lane's entry over record rec of block lane / 32, for all of a tile, 32 of
+// a block at a time (in the place of one that the list had no room for stands the zero vector)
+template <typename P>
+__device__ __forceinline__ void each_entry(const lq_pages& p, const Meta2& m, Entry e, uint32_t most, int lane, P put) {
+#pragma unroll 1
+    for (uint32_t r0 = 0; r0 < most; r0 += 32) {
+        const uint32_t k = r0 + (lane & 31);
+        if (r0) e = load_entry(p, m, k);
+        if (k < m.count && (int64_t)m.base + k < p.r.exc_cap) put(e.rec, e.v);
+    }
+}
+
+// Without the record's bias: as a pair of fp16 numbers 2^-24 w, w = 2 c + 32, whole and
+// below 64 for a record.  What is multiplied by them needs neither the 32 taken off nor the
+// scale: both go into the other operand's sum and into the product (see attend below).
+__device__ __forceinline__ void raw_pairs(uint32_t a, uint32_t b, uint32_t p[4]) {
+    const uint32_t kc = __builtin_amdgcn_perm(0u, a, 0x0c000c00u) & 0x00010001u;
+    p[0] = (a & kFieldMask) | kc;
+    p[1] = ((a >> 5) & kFieldMask) | kc;
+    p[2] = ((a >> 10) & kFieldMask) | kc;
+    const uint32_t c7h = ((b >> 5) & 7u) | ((a >> 13) & 8u);
+    const uint32_t par = ((uint32_t)__builtin_popcount(a & kLsbMask) + b) & 1u;
+    p[3] = kc | ((b & 31u) << 1) | (((c7h << 1) | par) << 17);
+}
+__device__ __forceinline__ void raw_pairs_tok(uint32_t a0, uint32_t b0, uint32_t a1, uint32_t b1, uint32_t p[8]) {
+    const uint32_t lo = __builtin_amdgcn_perm(a1, a0, 0x05040100u);
+    const uint32_t hi = __builtin_amdgcn_perm(a1, a0, 0x07060302u);
+    const uint32_t kc = lo & 0x00010001u;
+    p[0] = (lo & kFieldMask) | kc;
+    p[2] = ((lo >> 5) & kFieldMask) | kc;
+    p[4] = ((lo >> 10) & kFieldMask) | kc;
+    p[1] = (hi & kFieldMask) | kc;
+    p[3] = ((hi >> 5) & kFieldMask) | kc;
+    p[5] = ((hi >> 10) & kFieldMask) | kc;
+    const uint32_t h0 = ((b0 >> 5) & 7u) | ((a0 >> 13) & 8u);
+    const uint32_t h1 = ((b1 >> 5) & 7u) | ((a1 >> 13) & 8u);
+    const uint32_t q0 = ((uint32_t)__builtin_popcount(a0 & kLsbMask) + b0) & 1u;
+    const uint32_t q1 = ((uint32_t)__builtin_popcount(a1 & kLsbMask) + b1) & 1u;
+    p[6] = kc | ((b0 & 31u) << 1) | ((b1 & 31u) << 17);
+    p[7] = kc | (((h0 << 1) | q0) << 1) | (((h1 << 1) | q1) << 17);
+}
+// an entry's eight values 2c so (beyond 2048 they lose bits, as fp16 does), and as c
+__device__ __forceinline__ void raw_entry(const uint4& w, uint32_t p[4]) {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    const h2_t tiny = __builtin_bit_cast(h2_t, 0x00010001u), bias = __builtin_bit_cast(h2_t, 0x00200020u);   // 2^-24, 2^-19
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const h2_t h = {(_Float16)(int16_t)(x[i] & 0xffffu), (_Float16)(int16_t)(x[i] >> 16)};
+        p[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(h, tiny, bias));
+    }
 }
 
 // Page numbers of a wave's tiles, 64 a register: those of tiles 32 g .. + 31 and of the 32
 // behind.  A number outside the pool reads its last page.
-struct Pages {
-    int32_t near, far, g;
+struct Table {
+    int32_t near, far;
+    int g;
 };
 __device__ __forceinline__ int32_t load_pages(const int32_t* row, int n, uint32_t cap, int g, int lane) {
     return (int32_t)min((uint32_t)row[min(64 * g + lane, n - 1)], cap - 1);
 }
-__device__ __forceinline__ uint32_t page_of(const Pages& p, int j) {   // j: the page's place, within the two
+__device__ __forceinline__ uint32_t page_of(const Table& p, int j) {   // j: the page's place, within the two
     const int at = j & 63;
     return (uint32_t)((j >> 6) == p.g ? __builtin_amdgcn_readlane(p.near, at) : __builtin_amdgcn_readlane(p.far, at));
 }
@@ -144,31 +211,109 @@ __device__ __forceinline__ float pair_sum(float v) {   // of lane and lane ^ 16
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// few_attend; with SUMS also the logarithm (base 2) of the sum of the lane's page (lanes
-// 0..31 hold the first page's tokens, 32..63 the second's), and the row's sum l32, both of
-// the weights in 32 bits, as they are before they are rounded for P V.
-template <bool SUMS>
-__device__ __forceinline__ float attend(f4_t s[2], uint32_t word, bool every, const uint32_t vp[4][8], int lane,
-                                        FewState& st, float& l32) {
-    if constexpr (!SUMS) {
-        few_attend(s, word, every, vp, lane, st);
-        return 0.f;
+// State of a row over a unit's pages.  K's and V's values are c times their token's scale,
+// and enter the products as 2^-24 (2 c + 32):
+//   z   = kScale2 2^23 s_k (sum_i q_i k_i - 2^-19 sum_i q_i)
+//   o   = 2^23 (sum_t P_t v_t - 2^-19 sum_t P_t),   P_t = 2^(z_t - m) s_v 2^shift in fp16
+// so a record is decoded by bit operations alone.  The correction of z starts the product's
+// accumulator; that of o is taken off every 32 tiles, so that the sums stay near their result
+// (N tokens of like weights: the result falls as sqrt(N) beside them).  ROUND: K's values
+// are rounded to fp16 as the cache's readers see them, for weights that agree with a dense
+// attention's in 32 bits: c's own pairs, times the scale.
+struct PageState {
+    float m, l, sum;                           // reference, sum of 2^(z - m + shift), of P_t since the last correction
+    float shift;                               // P stays in fp16's range: 2^(shift + kLazy) times the largest scale
+    f4_t o[8];
+};
+constexpr float kUnit = 8388608.0f;            // 2^23
+__device__ __forceinline__ void rescale(PageState& st, float f) {
+    st.l *= f;
+    st.sum *= f;
+#pragma unroll
+    for (int mm = 0; mm < 8; mm++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) st.o[mm][i] *= f;
+}
+// sum over the lanes that hold a row
+__device__ __forceinline__ float quarters_sum(float v) {
+    v = pair_sum(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ void correct(PageState& st) {
+    const float c = quarters_sum(st.sum) * (-0x1p-19f);
+#pragma unroll
+    for (int mm = 0; mm < 8; mm++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) st.o[mm][i] += c;
+    st.sum = 0.f;
+}
+// the largest of eight fp16 numbers that are not negative, over the wave
+__device__ __forceinline__ float wave_scale(const uint4& w) {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; i++) top = max(top, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
+    return quarters_max(h2f((uint16_t)top));   // the 16 lanes of a quarter have the same tokens
+}
+// the least e with 2^e >= s (0 for a scale of 0), and whether a scale passes 2^e
+__device__ __forceinline__ int scale_exp(float s) {
+    const uint32_t u = __float_as_uint(s);
+    return s == 0.f ? 0 : (int)((u + 0x7fffffu) >> 23) - 127;
+}
+__device__ __forceinline__ float scale_limit(float s) { return __builtin_amdgcn_ldexpf(1.f, scale_exp(s)); }
+__device__ __forceinline__ bool above(const uint4& w, float limit) {
+    const h2_t a = __builtin_elementwise_max(__builtin_bit_cast(h2_t, w.x), __builtin_bit_cast(h2_t, w.y));
+    const h2_t b = __builtin_elementwise_max(__builtin_bit_cast(h2_t, w.z), __builtin_bit_cast(h2_t, w.w));
+    const h2_t c = __builtin_elementwise_max(a, b);
+    return fmaxf((float)c[0], (float)c[1]) > limit;
+}
+__device__ __forceinline__ float half_of(const uint4& w, int i) {
+    const uint32_t x = i < 2 ? w.x : i < 4 ? w.y : i < 6 ? w.z : w.w;
+    return (float)__builtin_bit_cast(h2_t, x)[i & 1];
+}
+
+// One tile: scores s[y][i] of token 8 (lane / 16) + 2 i + y (without their scales, or with
+// them where ROUND), raw V.  With SUMS the logarithm (base 2) of the sum of the lane's page
+// (lanes 0..31 hold the first page's tokens, 32..63 the second's).
+template <bool SUMS, bool ROUND>
+__device__ __forceinline__ float attend(f4_t s[2], const uint4& ks, const uint4& vs, uint32_t word,
+                                        const uint32_t vp[4][8], int lane, PageState& st) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        y[i] = s[i & 1][i >> 1] * (ROUND ? kScale2 : half_of(ks, i) * (kScale2 * kUnit));
+    if (word != ~0u) {
+        const uint32_t own = word >> (8 * (lane >> 4));
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = (own >> i) & 1u ? y[i] : -INFINITY;
     }
-    const float was = st.m, off = few_reference(s, word, every, lane, st);
-    if (was != st.m) l32 *= __builtin_amdgcn_exp2f(was - st.m);
+    float mx = fmaxf(y[0], y[1]);
+#pragma unroll
+    for (int i = 2; i < 8; i += 2) mx = fmaxf(fmaxf(mx, y[i]), y[i + 1]);
+    const float mn = quarters_max(mx);
+    if (__any(mn > st.m + kLazy)) {
+        const float up = mn > st.m + kLazy ? mn : st.m;
+        rescale(st, up == st.m ? 1.f : __builtin_amdgcn_exp2f(st.m - up));
+        st.m = up;
+    }
+    const float off = (st.m == -INFINITY ? 0.f : -st.m) + st.shift;
     uint32_t p[4];
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], kScale2, off));
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][i], kScale2, off));
-        p[i] = pair_h(x, y);
-        st.l = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, p[i]), h2_t{(_Float16)1.f, (_Float16)1.f}, st.l, false);
-        sum += x + y;
+        const float u = __builtin_amdgcn_exp2f(y[2 * i] + off), v = __builtin_amdgcn_exp2f(y[2 * i + 1] + off);
+        sum += u + v;
+        p[i] = pair_h(u * half_of(vs, 2 * i), v * half_of(vs, 2 * i + 1));
+        st.sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, p[i]), h2_t{(_Float16)1.f, (_Float16)1.f}, st.sum, false);
     }
-    few_products(p, vp, st);
-    l32 += sum;
-    return __builtin_amdgcn_logf(pair_sum(sum)) - off + kPShift;
+    st.l += sum;
+    const h8_t pb = as_h8(p[0], p[1], p[2], p[3]);
+#pragma unroll
+    for (int mm = 0; mm < 8; mm++)
+        st.o[mm] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(vp[0][mm], vp[1][mm], vp[2][mm], vp[3][mm]), pb, st.o[mm],
+                                                          0, 0, 0);
+    return SUMS ? __builtin_amdgcn_logf(pair_sum(sum)) - off + kPShift : 0.f;
 }
 
 __device__ __forceinline__ void zero_out(const PagedArgs& A, int b, int tid) {
@@ -204,6 +349,7 @@ __device__ __forceinline__ Len len_at(const PagedArgs& A, const Lens& mine, int 
 }
 template <bool BF16, bool SUMS, bool BIG>
 __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
+    constexpr bool ROUND = SUMS;
     extern __shared__ __align__(16) char s_dyn[];
     // pieces in the order of the list: wave w's first (2 w), which ends its unit there, and its last (2 w + 1)
     __shared__ int s_unit[2 * kWaves], s_begins[2 * kWaves];
@@ -271,7 +417,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
             FewState st;
             st.m = -INFINITY;
             st.l = 0.f;
-            float l32 = 0.f;
+            float l32 = 0.f;                   // the sum in 32 bits throughout
 #pragma unroll
             for (int mm = 0; mm < 8; mm++) st.o[mm] = f4_t{0.f, 0.f, 0.f, 0.f};
 
@@ -279,77 +425,160 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
             const int pe = min(t + n, L.page_tiles);
             if (t < pe) {
                 const int32_t* row = A.pages + b * A.width;
-                const uint32_t cap = (uint32_t)A.k.cap_blocks, hb = (uint32_t)h * cap, hbv = (uint32_t)h * (uint32_t)A.v.cap_blocks;
-                Pages pg;
+                const uint32_t cap = (uint32_t)A.k.r.cap_blocks, hb = (uint32_t)h * cap;
+                Table pg;
                 pg.g = t >> 5;
                 pg.near = load_pages(row, L.pages, cap, pg.g, lane);
                 pg.far = load_pages(row, L.pages, cap, pg.g + 1, lane);
-                KFew kr;
-                Raw vr;
-                Meta mk, mv, nk, nv;
-                uint4 ek, ev;
-                const auto blocks = [&](int tile, uint32_t& x, uint32_t& y) __attribute__((always_inline)) {
-                    const int j = 2 * min(tile, pe - 1);
-                    x = page_of(pg, j);
-                    y = page_of(pg, min(j + 1, L.pages - 1));
-                };
-                {
-                    uint32_t x, y;
-                    blocks(t, x, y);
-                    mk = load_meta<BIG>(A.k, hb + x, hb + y, lane);
-                    mv = load_meta<BIG>(A.v, hbv + x, hbv + y, lane);
-                    load_k<BIG>(A.k, hb + x, hb + y, lane, kr);
-                    load_v<BIG>(A.v, hbv + x, hbv + y, lane, vr);
-                    blocks(t + 1, x, y);
-                    nk = load_meta<BIG>(A.k, hb + x, hb + y, lane);
-                    nv = load_meta<BIG>(A.v, hbv + x, hbv + y, lane);
-                    ek = load_entry(A.k, mk, lane);
-                    ev = load_entry(A.v, mv, lane);
+                f4_t s0 = {0.f, 0.f, 0.f, 0.f};
+                if (!ROUND) {                  // -2^-19 sum_i q_i
+                    float x = 0.f;
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) x += (float)q[c][i];
+                    x = quarters_sum(x) * (-0x1p-19f);
+                    s0 = f4_t{x, x, x, x};
                 }
+                PageState ps;
+                ps.m = -INFINITY;
+                ps.l = ps.sum = 0.f;
+#pragma unroll
+                for (int mm = 0; mm < 8; mm++) ps.o[mm] = f4_t{0.f, 0.f, 0.f, 0.f};
+                Recs rd;
+                Meta2 mk, mv, nk, nv;
+                Entry ek, ev;
+                uint32_t x1, y1;               // blocks of the next tile; past the end the last again
+                const auto blocks = [&](int tile) __attribute__((always_inline)) {
+                    const int j = 2 * min(tile, pe - 1);
+                    x1 = hb + page_of(pg, j);
+                    y1 = hb + page_of(pg, min(j + 1, L.pages - 1));
+                };
+                blocks(t);
+                mk = load_meta<BIG>(A.k, x1, y1, lane);
+                mv = load_meta<BIG>(A.v, x1, y1, lane);
+                load_recs<BIG, ROUND>(A, x1, y1, lane, rd);
+                blocks(t + 1);
+                nk = load_meta<BIG>(A.k, x1, y1, lane);
+                nv = load_meta<BIG>(A.v, x1, y1, lane);
+                ek = load_entry(A.k, mk, lane & 31);
+                ev = load_entry(A.v, mv, lane & 31);
+                float top = wave_scale(rd.vs);         // 2^shift times it lies within (2^(kPShift - 1), 2^kPShift]
+                ps.shift = kPShift - (float)scale_exp(top);
+                float limit = scale_limit(top);
                 for (int tile = t; tile < pe; tile++) {
                     const uint32_t word = 2 * tile + 1 < L.pages ? ~0u : 0xffffu;
-                    f4_t s[2] = {f4_t{0.f, 0.f, 0.f, 0.f}, f4_t{0.f, 0.f, 0.f, 0.f}};
+                    f4_t s[2] = {s0, s0};
                     uint32_t vp[4][8], p[8][4];
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        rec_pairs(j & 1 ? kr.a[j >> 1].y : kr.a[j >> 1].x, (kr.b[j >> 1] >> (8 * (j & 1))) & 0xffu, p[j]);
+                        const uint32_t ra = j & 1 ? rd.ka[j >> 1].y : rd.ka[j >> 1].x, rb = (rd.kb[j >> 1] >> (8 * (j & 1))) & 0xffu;
+                        if constexpr (ROUND) {
+                            rec_pairs(ra, rb, p[j]);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) p[j][i] = unbias(p[j][i]);
+                            for (int i = 0; i < 4; i++) p[j][i] = unbias(p[j][i]);
+                        } else {
+                            raw_pairs(ra, rb, p[j]);
+                        }
                     }
-                    if (const uint32_t most = most_of(mk)) patch_k(A.k, kr, mk, ek, most, lane, area, p);
+                    if (const uint32_t most = most_of(mk)) {
+                        // through 8 KB of LDS of the wave's own, the lanes with entries write over their records
+#pragma unroll
+                        for (int j = 0; j < 8; j++) area[64 * j + lane] = u32x4_t{p[j][0], p[j][1], p[j][2], p[j][3]};
+                        wave_lds_sync();
+                        each_entry(A.k, mk, ek, most, lane, [&](uint32_t rec, const uint4& w) __attribute__((always_inline)) {
+                            uint32_t e[4];
+                            if constexpr (ROUND) exc_pairs(w, e);
+                            else raw_entry(w, e);
+                            area[64 * (2 * (rec >> 6) + (rec & 1)) + 16 * ((rec >> 4) & 3) + 8 * (lane >> 5) + ((rec & 15) >> 1)] =
+                                u32x4_t{e[0], e[1], e[2], e[3]};
+                        });
+                        wave_lds_sync();
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const u32x4_t w = area[64 * j + lane];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) p[j][i] = w[i];
+                        }
+                        wave_lds_sync();
+                    }
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        mul_pairs<4>(p[j], __builtin_amdgcn_perm(0u, kr.s, j & 1 ? 0x03020302u : 0x01000100u));
+                        if constexpr (ROUND) mul_pairs<4>(p[j], __builtin_amdgcn_perm(0u, rd.kp, j & 1 ? 0x03020302u : 0x01000100u));
                         s[j & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(p[j][0], p[j][1], p[j][2], p[j][3]), q[j >> 1],
                                                                           s[j & 1], 0, 0, 0);
                     }
-                    decode_v(vr, vp);
-                    if (const uint32_t most = most_of(mv)) patch_v(A.v, vr, mv, ev, most, lane, area, vp);
-                    scale_v(vr, word, lane, vp);
+                    {
+                        const uint32_t aw[8] = {rd.va[0].x, rd.va[0].y, rd.va[0].z, rd.va[0].w,
+                                                rd.va[1].x, rd.va[1].y, rd.va[1].z, rd.va[1].w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t w = k < 2 ? rd.vb.x : rd.vb.y;
+                            raw_pairs_tok(aw[2 * k], w >> (16 * (k & 1)), aw[2 * k + 1], w >> (16 * (k & 1) + 8), vp[k]);
+                        }
+                    }
+                    if (const uint32_t most = most_of(mv)) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            area[64 * j + lane] = u32x4_t{vp[j >> 1][4 * (j & 1)], vp[j >> 1][4 * (j & 1) + 1],
+                                                          vp[j >> 1][4 * (j & 1) + 2], vp[j >> 1][4 * (j & 1) + 3]};
+                        wave_lds_sync();
+                        each_entry(A.v, mv, ev, most, lane, [&](uint32_t rec, const uint4& v) __attribute__((always_inline)) {
+                            uint32_t e[4];
+                            raw_entry(v, e);
+                            const uint32_t tok = 16 * (lane >> 5) + (rec & 15);   // pair (tok / 2) % 4 of lane vector + 16 (tok / 8)
+                            uint16_t* w = reinterpret_cast<uint16_t*>(area + 64 * (tok & 6) + 16 * (tok >> 3) + (rec >> 4)) + (tok & 1);
+#pragma unroll
+                            for (int i = 0; i < 8; i++) w[(i & 4) * 128 + (i & 3) * 2] = (uint16_t)(i & 1 ? e[i >> 1] >> 16 : e[i >> 1]);
+                        });
+                        wave_lds_sync();
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const u32x4_t w = area[64 * j + lane];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) vp[j >> 1][4 * (j & 1) + i] = w[i];
+                        }
+                        wave_lds_sync();
+                    }
+                    if (__any(above(rd.vs, limit))) {    // a larger scale than any before: P's range moves
+                        top = wave_scale(rd.vs);
+                        const float shift = kPShift - (float)scale_exp(top);
+                        rescale(ps, __builtin_amdgcn_exp2f(shift - ps.shift));
+                        ps.shift = shift;
+                        limit = scale_limit(top);
+                    }
+                    const uint4 ks = ROUND ? make_uint4(0u, 0u, 0u, 0u) : rd.ks, vs = rd.vs;
                     __builtin_amdgcn_sched_barrier(0);   // every use of the records before their reload
-                    // the next tile's records and the bases of the one behind; past the end the last again
-                    ek = load_entry(A.k, nk, lane);
-                    ev = load_entry(A.v, nv, lane);
+                    // the next tile's records and the bases of the one behind
+                    ek = load_entry(A.k, nk, lane & 31);
+                    ev = load_entry(A.v, nv, lane & 31);
                     mk = nk;
                     mv = nv;
-                    uint32_t x, y;
-                    if (((tile + 1) >> 5) != pg.g) {
+                    load_recs<BIG, ROUND>(A, x1, y1, lane, rd);
+                    if (((tile + 2) >> 5) == pg.g + 2) {
                         pg.g++;
                         pg.near = pg.far;
                         pg.far = load_pages(row, L.pages, cap, pg.g + 1, lane);
+                        correct(ps);           // with the sums of the tiles before this one
                     }
-                    blocks(tile + 1, x, y);
-                    load_k<BIG>(A.k, hb + x, hb + y, lane, kr);
-                    load_v<BIG>(A.v, hbv + x, hbv + y, lane, vr);
-                    blocks(tile + 2, x, y);
-                    nk = load_meta<BIG>(A.k, hb + x, hb + y, lane);
-                    nv = load_meta<BIG>(A.v, hbv + x, hbv + y, lane);
-                    const float z = attend<SUMS>(s, word, word == ~0u, vp, lane, st, l32);
+                    blocks(tile + 2);
+                    nk = load_meta<BIG>(A.k, x1, y1, lane);
+                    nv = load_meta<BIG>(A.v, x1, y1, lane);
+                    const float z = attend<SUMS, ROUND>(s, ks, vs, word, vp, lane, ps);
                     if (SUMS) {
                         const int j = 2 * tile + (lane >> 5);
                         if (!(g & 1) && col < G && j < L.pages) A.z[((int64_t)unit * A.width + j) * G + col] = z;
                     }
                 }
+                // on as the tail's rows are taken
+                correct(ps);
+                const float f = __builtin_amdgcn_exp2f(kPShift - ps.shift);
+                st.m = ps.m;
+                st.l = l32 = ps.l * f;
+#pragma unroll
+                for (int mm = 0; mm < 8; mm++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) st.o[mm][i] = ps.o[mm][i] * (f * kUnit);
             }
             // ---- the tail's
             for (int tile = max(t, L.page_tiles); tile < t + n; tile++) {
@@ -373,7 +602,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                     for (int c = 0; c < 4; c++)
                         s[y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                             __builtin_bit_cast(h8_t, BF16 ? bf_to_h(w[y][c]) : w[y][c]), q[c], s[y], 0, 0, 0);
-                attend<SUMS>(s, word, word == ~0u, vp, lane, st, l32);
+                const float was = st.m;
+                few_attend(s, word, word == ~0u, vp, lane, st);
+                if (SUMS) {                    // few_attend's sum is of the rounded weights: these few again
+                    if (was != st.m) l32 *= __builtin_amdgcn_exp2f(was - st.m);
+                    const float off = (st.m == -INFINITY ? 0.f : -st.m) + kPShift;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) l32 += __builtin_amdgcn_exp2f(__builtin_fmaf(s[i & 1][i >> 1], kScale2, off));
+                }
             }
             // ---- the unit is written out, or its piece kept
             float l = st.l + __shfl_xor(st.l, 16, 64);
@@ -725,9 +961,10 @@ bool plan(int64_t n_seq, int64_t heads, int64_t group, int64_t width, int64_t ta
     return true;
 }
 
-bool pool_ok(const lq_resident* r) {
+bool pool_ok(const lq_pages* p) {
+    const lq_resident* r = p ? &p->r : nullptr;
     return r && r->a && r->b && r->mask && r->meta && r->scale && r->n_heads > 0 && r->cap_blocks > 0 && r->exc_cap >= 0 &&
-           r->cap_blocks <= INT_MAX / r->n_heads;
+           r->cap_blocks <= INT_MAX / r->n_heads && (r->exc_cap == 0 || (r->exc && p->rec));
 }
 bool rows_ok(const lq_rows* r) {
     return r && r->p && ((uintptr_t)r->p & 15) == 0 && r->stride_b % 8 == 0 && r->stride_h % 8 == 0 && r->stride_t % 8 == 0;
@@ -752,24 +989,27 @@ int64_t lq_paged_attn_workspace(int64_t n_seq, int64_t heads, int group, int64_t
     return plan(n_seq, heads, group, max_pages, tail_cap, weights != 0, &p) ? p.bytes : -1;
 }
 
-int lq_paged_attention(const lq_resident *k, const lq_resident *v, const lq_rows *q, int64_t n_seq, int group,
+int lq_paged_attention(const lq_pages *k, const lq_pages *v, const lq_rows *q, int64_t n_seq, int group,
                        const int32_t *d_pages, int64_t max_pages, const int32_t *d_n_pages, const lq_rows *tail_k,
                        const lq_rows *tail_v, int64_t tail_cap, const int32_t *d_tail_len, float *d_weights, float decay,
                        int dtype, void *d_work, int64_t work_bytes, const lq_rows *out, hipStream_t s) {
-    if (!pool_ok(k) || !pool_ok(v) || k->n_heads != v->n_heads || k->cap_blocks != v->cap_blocks || !rows_ok(q) ||
+    if (!pool_ok(k) || !pool_ok(v) || k->r.n_heads != v->r.n_heads || k->r.cap_blocks != v->r.cap_blocks || !rows_ok(q) ||
         !rows_ok(out) || !d_n_pages || (max_pages > 0 && !d_pages) || !d_work || ((uintptr_t)d_work & 15) ||
         (dtype != LQ_F16 && dtype != LQ_BF16))
         return LQ_ERR_ARG;
     if (tail_cap > 0 && (!rows_ok(tail_k) || !rows_ok(tail_v))) return LQ_ERR_ARG;
     Plan p;
-    if (!plan(n_seq, k->n_heads, group, max_pages, tail_cap, d_weights != nullptr, &p) || work_bytes < p.bytes)
+    if (!plan(n_seq, k->r.n_heads, group, max_pages, tail_cap, d_weights != nullptr, &p) || work_bytes < p.bytes)
         return LQ_ERR_ARG;
     PagedArgs A{};
     A.k = *k;
     A.v = *v;
     // an empty exception list is read at its first entry and the value not used
-    if (!A.k.exc || A.k.exc_cap == 0) A.k.exc = reinterpret_cast<int16_t*>(A.k.a);
-    if (!A.v.exc || A.v.exc_cap == 0) A.v.exc = reinterpret_cast<int16_t*>(A.v.a);
+    for (lq_pages* p : {&A.k, &A.v}) {
+        if (p->r.exc_cap) continue;
+        p->r.exc = reinterpret_cast<int16_t*>(p->r.a);
+        p->rec = p->r.b;
+    }
     A.pages = d_pages;
     A.n_pages = d_n_pages;
     A.tail_len = d_tail_len;
@@ -781,7 +1021,7 @@ int lq_paged_attention(const lq_resident *k, const lq_resident *v, const lq_rows
     A.ob = out->stride_b;
     A.oh = out->stride_h;
     A.n_seq = (int)n_seq;
-    A.heads = (int)k->n_heads;
+    A.heads = (int)k->r.n_heads;
     A.group = group;
     A.per = (int)((n_seq + 63) / 64);
     char* w = static_cast<char*>(d_work);
@@ -789,7 +1029,7 @@ int lq_paged_attention(const lq_resident *k, const lq_resident *v, const lq_rows
     A.desc = reinterpret_cast<Desc*>(w + p.desc);
     A.lse = reinterpret_cast<float*>(w + p.lse);
     A.z = reinterpret_cast<float*>(w + p.z);
-    const bool big = k->n_heads * k->cap_blocks > (int64_t)(UINT32_MAX / 1024);
+    const bool big = k->r.n_heads * k->r.cap_blocks > (int64_t)(UINT32_MAX / 1024);
     if (dtype == LQ_BF16) {
         if (d_weights) paged_launch<true, true>(A, p.grid, big, s);
         else paged_launch<true, false>(A, p.grid, big, s);

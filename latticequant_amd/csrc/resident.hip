@@ -78,8 +78,12 @@ __device__ __forceinline__ int res_point(const void* x, int dtype, int64_t T, in
     return e8_nearest_fast(tv, ic);
 }
 
+// record of c = 0: every u is 16
+constexpr uint32_t kZeroA = (16u << 1) | (16u << 6) | (16u << 11) | (1u << 16) | (16u << 17) | (16u << 22) | (16u << 27), kZeroB = 16u;
+
 // Block bb of head hh of x to resident block rb; its exceptions' number is returned to
 // thread 0.  256 threads: wave = group, lane = slot
+template <bool PAGE>
 __device__ __forceinline__ int quant_block(const void* __restrict__ x, int dtype, int64_t T,
                                            const float* __restrict__ scale32, const uint16_t* __restrict__ scale16,
                                            const lq_resident& r, int64_t hh, int64_t bb, int64_t rb) {
@@ -91,6 +95,10 @@ __device__ __forceinline__ int quant_block(const void* __restrict__ x, int dtype
     const int cs = res_point(x, dtype, T, hh, t, g, scale32[hh], ic);
     uint32_t a, b;
     const bool ok = rec_encode(ic, cs, &a, &b);
+    if (PAGE && !ok) {                         // the zero vector: what a dropped entry stands for
+        a = kZeroA;
+        b = kZeroB;
+    }
     r.a[rb * 256 + grp * 64 + slot] = a;
     r.b[rb * 256 + grp * 64 + slot] = (uint8_t)b;
     const unsigned long long m = __ballot(!ok);
@@ -127,7 +135,7 @@ __global__ __launch_bounds__(256) void k_res_quant(const void* __restrict__ x, i
                                                    const uint16_t* __restrict__ scale16, lq_resident r, int64_t h0,
                                                    int64_t blk0, uint32_t* __restrict__ cnt) {
     const int64_t bb = blockIdx.x, hh = blockIdx.y;
-    const int n = quant_block(x, dtype, T, scale32, scale16, r, hh, bb, (h0 + hh) * r.cap_blocks + blk0 + bb);
+    const int n = quant_block<false>(x, dtype, T, scale32, scale16, r, hh, bb, (h0 + hh) * r.cap_blocks + blk0 + bb);
     if (threadIdx.x == 0) cnt[hh * gridDim.x + bb] = (uint32_t)n;
 }
 
@@ -164,7 +172,7 @@ __global__ __launch_bounds__(256) void k_res_scan(const uint32_t* __restrict__ c
 // exception entries: the vectors flagged by quant_block, recomputed
 __device__ __forceinline__ void fill_block(const void* __restrict__ x, int dtype, int64_t T,
                                            const float* __restrict__ scale32, const lq_resident& r, int64_t hh,
-                                           int64_t bb, int64_t rb) {
+                                           int64_t bb, int64_t rb, uint8_t* __restrict__ rec = nullptr) {
     const int tid = threadIdx.x, grp = tid >> 6, slot = tid & 63;
     const unsigned long long m0 = r.mask[rb * 4 + 0], m1 = r.mask[rb * 4 + 1], m2 = r.mask[rb * 4 + 2],
                              m3 = r.mask[rb * 4 + 3];
@@ -195,6 +203,7 @@ __device__ __forceinline__ void fill_block(const void* __restrict__ x, int dtype
     w.z = (uint16_t)e[4] | ((uint32_t)(uint16_t)e[5] << 16);
     w.w = (uint16_t)e[6] | ((uint32_t)(uint16_t)e[7] << 16);
     reinterpret_cast<uint4*>(r.exc)[idx] = w;
+    if (rec) rec[idx] = (uint8_t)tid;
 }
 
 __global__ __launch_bounds__(256) void k_res_fill(const void* __restrict__ x, int dtype, int64_t T,
@@ -264,7 +273,7 @@ __global__ __launch_bounds__(256) void k_page_quant(const void* __restrict__ x, 
                                                     const float* __restrict__ scale32,
                                                     const uint16_t* __restrict__ scale16, lq_resident r) {
     const int64_t hh = blockIdx.x / (uint32_t)P.per, bb = blockIdx.x % (uint32_t)P.per, rb = P.block(r, hh, bb);
-    if (rb >= 0) quant_block(x, dtype, P.per * kRB, scale32, scale16, r, hh, bb, rb);
+    if (rb >= 0) quant_block<true>(x, dtype, P.per * kRB, scale32, scale16, r, hh, bb, rb);
 }
 
 // Room for the exceptions of written pages: a page keeps the entries it had, where they
@@ -303,9 +312,10 @@ __global__ __launch_bounds__(1024) void k_page_rooms(PageMap P, int64_t units, l
 }
 
 __global__ __launch_bounds__(256) void k_page_fill(const void* __restrict__ x, int dtype, PageMap P,
-                                                   const float* __restrict__ scale32, lq_resident r) {
+                                                   const float* __restrict__ scale32, lq_resident r,
+                                                   uint8_t* __restrict__ rec) {
     const int64_t hh = blockIdx.x / (uint32_t)P.per, bb = blockIdx.x % (uint32_t)P.per, rb = P.block(r, hh, bb);
-    if (rb >= 0) fill_block(x, dtype, P.per * kRB, scale32, r, hh, bb, rb);
+    if (rb >= 0) fill_block(x, dtype, P.per * kRB, scale32, r, hh, bb, rb, rec);
 }
 
 __global__ __launch_bounds__(256) void k_page_dequant(lq_resident r, PageMap P, void* __restrict__ out, int out_dtype) {
@@ -1060,28 +1070,28 @@ int lq_resident_dequant(const lq_resident* r, int64_t h0, int64_t n_heads, int64
 }
 
 int lq_page_quantize(const void *d_x, int dtype, int64_t n, int64_t t_tokens, const float *d_scale32,
-                     const uint16_t *d_scale16, const lq_resident *r, const int32_t *d_pages, int32_t *d_room,
-                     hipStream_t s) {
-    if (!d_x || !d_scale32 || !d_scale16 || !res_ok(r) || !d_pages || !d_room || dtype < 0 || dtype > 2 || n < 1 ||
-        t_tokens <= 0 || t_tokens % kRB)
+                     const uint16_t *d_scale16, const lq_pages *p, const int32_t *d_pages, hipStream_t s) {
+    if (!d_x || !d_scale32 || !d_scale16 || !p || !res_ok(&p->r) || !p->room || !p->rec || !d_pages || dtype < 0 ||
+        dtype > 2 || n < 1 || t_tokens <= 0 || t_tokens % kRB)
         return LQ_ERR_ARG;
+    const lq_resident& r = p->r;
     const int64_t per = t_tokens / kRB;
-    if (n > INT_MAX / per || n * per > INT_MAX / r->n_heads) return LQ_ERR_ARG;
-    const int64_t units = n * r->n_heads * per;
-    const PageMap P = {d_pages, r->n_heads, per};
-    hipLaunchKernelGGL(k_page_quant, dim3((unsigned)units), dim3(256), 0, s, d_x, dtype, P, d_scale32, d_scale16, *r);
-    hipLaunchKernelGGL(k_page_rooms, dim3(1), dim3(1024), 0, s, P, units, *r, d_room);
-    hipLaunchKernelGGL(k_page_fill, dim3((unsigned)units), dim3(256), 0, s, d_x, dtype, P, d_scale32, *r);
+    if (n > INT_MAX / per || n * per > INT_MAX / r.n_heads) return LQ_ERR_ARG;
+    const int64_t units = n * r.n_heads * per;
+    const PageMap P = {d_pages, r.n_heads, per};
+    hipLaunchKernelGGL(k_page_quant, dim3((unsigned)units), dim3(256), 0, s, d_x, dtype, P, d_scale32, d_scale16, r);
+    hipLaunchKernelGGL(k_page_rooms, dim3(1), dim3(1024), 0, s, P, units, r, p->room);
+    hipLaunchKernelGGL(k_page_fill, dim3((unsigned)units), dim3(256), 0, s, d_x, dtype, P, d_scale32, r, p->rec);
     return launch_status();
 }
 
-int lq_page_dequant(const lq_resident *r, const int32_t *d_pages, int64_t n, int64_t per, void *d_out, int out_dtype,
+int lq_page_dequant(const lq_pages *p, const int32_t *d_pages, int64_t n, int64_t per, void *d_out, int out_dtype,
                     hipStream_t s) {
-    if (!res_ok(r) || !d_pages || !d_out || out_dtype < 0 || out_dtype > 2 || n < 1 || per < 1 || n > INT_MAX / per ||
-        n * per > INT_MAX / r->n_heads)
+    if (!p || !res_ok(&p->r) || !d_pages || !d_out || out_dtype < 0 || out_dtype > 2 || n < 1 || per < 1 ||
+        n > INT_MAX / per || n * per > INT_MAX / p->r.n_heads)
         return LQ_ERR_ARG;
-    const PageMap P = {d_pages, r->n_heads, per};
-    hipLaunchKernelGGL(k_page_dequant, dim3((unsigned)(n * r->n_heads * per)), dim3(256), 0, s, *r, P, d_out, out_dtype);
+    const PageMap P = {d_pages, p->r.n_heads, per};
+    hipLaunchKernelGGL(k_page_dequant, dim3((unsigned)(n * p->r.n_heads * per)), dim3(256), 0, s, p->r, P, d_out, out_dtype);
     return launch_status();
 }
 

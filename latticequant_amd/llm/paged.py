@@ -34,6 +34,29 @@ def _no_grad(what: str, *ts) -> None:
         raise RuntimeError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 
+class _Pool(ResidentKV):
+    """The resident form behind a PagedKV: its exception list has the entries' records beside it."""
+
+    def __init__(self, n_heads: int, n_pages: int, device, exc_cap: int):
+        super().__init__(n_heads, n_pages * PAGE, device=device, exc_cap=exc_cap)
+        self.n_tokens = n_pages * PAGE
+        self.room = torch.zeros(n_heads * n_pages, dtype=torch.int32, device=self.a.device)
+        self.rec = torch.zeros(exc_cap, dtype=torch.uint8, device=self.a.device)
+        self._pages = None
+
+    def _grow_exc(self, cap: int, keep: int) -> None:
+        super()._grow_exc(cap, keep)
+        grown = torch.zeros(cap, dtype=torch.uint8, device=self.device)
+        grown[:keep] = self.rec[:keep]
+        self.rec = grown
+
+    def pages(self) -> L.Pages:
+        """The buffers as the C ABI's lq_pages (cached as struct() is)."""
+        if self._st is None or self._pages is None:
+            self._pages = L.Pages(r=self.struct(), room=self.room.data_ptr(), rec=self.rec.data_ptr())
+        return self._pages
+
+
 class PagedKV:
     """A pool of n_pages pages of n_heads kv heads (K or V of a layer).
 
@@ -49,17 +72,15 @@ class PagedKV:
             raise ValueError("a pool has fewer than 2^31 pages in all its heads")
         if exc_cap is None:
             exc_cap = max(4096, 8 * n_heads * n_pages)
-        self.pool = ResidentKV(n_heads, n_pages * PAGE, device=device, exc_cap=exc_cap)
-        self.pool.n_tokens = n_pages * PAGE
+        self.pool = _Pool(n_heads, n_pages, device, exc_cap)
         self.n_heads, self.n_pages, self.device = int(n_heads), int(n_pages), self.pool.a.device
-        self._room = torch.zeros(n_heads * n_pages, dtype=torch.int32, device=self.device)
 
     @property
     def exc_cap(self) -> int:
         return self.pool.exc_cap
 
-    def struct(self) -> L.Resident:
-        return self.pool.struct()
+    def struct(self) -> L.Pages:
+        return self.pool.pages()
 
     def _numbers(self, pages: torch.Tensor, shape, write: bool) -> torch.Tensor:
         if not isinstance(pages, torch.Tensor) or pages.dtype not in (torch.int32, torch.int64):
@@ -111,8 +132,8 @@ class PagedKV:
 
             def launch():
                 L.check(lib.lq_page_quantize(xc.data_ptr(), L.dtype_code(xc.dtype), n, T, s32.data_ptr(), s16.data_ptr(),
-                                             ctypes.addressof(r.struct()), num.data_ptr(), self._room.data_ptr(),
-                                             L.raw_stream(self.device)), "lq_page_quantize")
+                                             ctypes.addressof(r.pages()), num.data_ptr(), L.raw_stream(self.device)),
+                        "lq_page_quantize")
             r._with_exceptions(n * H * T * (HD // 8), launch, anew=False)
 
     def read(self, pages: torch.Tensor, out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
@@ -165,8 +186,10 @@ def paged_decode_attention(k: PagedKV, v: PagedKV, q: torch.Tensor, pages: torch
     alone, whatever stood there); places past n_pages[b] stay as they are.
     Any strides with a contiguous last dimension are read in place.  work:
     paged_attn_workspace, used until the call's work on the stream is done; out: where to
-    write, of q's shape and type.  Returns (B, Hq, 1, 128).  The products are fp16, as
-    resident_tree_attention's.  The same inputs give the same bits."""
+    write, of q's shape and type.  Returns (B, Hq, 1, 128).  The products are fp16 as
+    resident_tree_attention's are; a page's value is its lattice coordinate times its scale,
+    V's unrounded, K's rounded to fp16 (as ``read`` rounds it) with weights and unrounded
+    without.  The same inputs give the same bits."""
     dev = k.device
     if q.dim() != 4 or q.dtype not in _DTYPES or q.shape[2] != 1 or q.shape[3] != HD:
         raise ValueError("q must be (B, Hq, 1, 128) fp16 or bf16")

@@ -42,19 +42,28 @@ def _table(counts, n, width, seed, fill=-1):
     return torch.from_numpy(tab).cuda()
 
 
-def _reference(k, v, q, tab, counts, tk, tv, tails):
-    """(out, tolerance of it, page weights, relative tolerance of those): 64 bits, from the rows
-    that the pages stand for.
+def _scales(p, at, h):
+    """Scales of the tokens of pages `at` of head h."""
+    return p.pool.scale.view(p.n_heads, p.n_pages, PAGE)[h, at].double().reshape(-1)
 
-    P is rounded to fp16 (half a step 2^-11) in the sum over V and in the row's sum alike, so
-    a row is off by at most 2 x 2^-11 times its sum of p |v|.  A score is a sum of 128 products
-    in fp32: off by at most 130 x 2^-24 of the sum of their sizes (and, where bf16 values
-    below 2^-14 lose bits as fp16 operands, by 2^-25 of the other's sizes), a weight relatively
-    by that much twice (its own and the row's sum), once more for exp2 and the rounding of
-    its argument (z below 2^7: 2^-17).  Weights below 2^-35 of the row's largest may vanish."""
+
+def _reference(k, v, q, tab, counts, tk, tv, tails, rounded=False):
+    """(out, tolerance of it, page weights, relative tolerance of those): 64 bits, from the
+    lattice points times their scales (K's rounded to fp16 with page weights).
+
+    P is rounded to fp16 (half a step, 2^-11), and so are V's coordinates beyond 1008 (2 c + 32
+    beyond 2048): a row is off by at most 2 x 2^-11 times its sum of p |v| (rows of the tail
+    have the sum of the rounded P instead of V's rounding).  A score is a sum of 128
+    products of q and c + 16 in fp32, less 16 sum q: off by at most 130 x 2^-24 of the sum of their
+    sizes, by 2^-11 of those with such a coordinate, and, where bf16 values below 2^-14 lose
+    bits, by 2^-25 of the other's sizes; a weight relatively by that much twice (its own
+    and the row's sum), once more for exp2 and the rounding of its argument (z below
+    2^7: 2^-17).  The sums of P (c + 16) over 32 tiles: 34 roundings of at most 32 times the
+    largest scale, twice.  Weights below 2^-34 of the row's largest may vanish."""
     B, Hq = q.shape[:2]
     H, G, W = k.n_heads, Hq // k.n_heads, tab.shape[1]
-    rk, rv = (p.read(torch.arange(p.n_pages, device="cuda")[:, None]).double() for p in (k, v))
+    every = torch.arange(k.n_pages, device="cuda")[:, None]
+    rk, rv = k.read(every, torch.float16 if rounded else torch.float32).double(), v.read(every, torch.float32).double()
     out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
     tol = torch.zeros_like(out)
     w = torch.zeros(B, W, dtype=torch.float64, device="cuda")
@@ -64,22 +73,31 @@ def _reference(k, v, q, tab, counts, tk, tv, tails):
         c, t = counts[b], tails[b]
         if c * PAGE + t == 0:
             continue
-        at = tab[b, :c].long().clamp(0, k.n_pages - 1)
+        at = tab[b, :c].long()
+        at = torch.where((at < 0) | (at >= k.n_pages), k.n_pages - 1, at)
         for h in range(H):
             kk = rk[at, h].reshape(-1, HD)
             vv = rv[at, h].reshape(-1, HD)
+            sk, sv = _scales(k, at, h)[:, None], _scales(v, at, h)
+            big = torch.where((2 * kk / sk).abs() > 2016, kk.abs(), 0.0)
+            bias = 16 * float(sk.max()) if c else 0.0
+            vmax = (float(vv.abs().max()) + 32 * float(sv.max())) if c else 0.0
             if t:
                 kk = torch.cat([kk, tk[b, h, :t].double()])
                 vv = torch.cat([vv, tv[b, h, :t].double()])
             qq = q[b, h * G:(h + 1) * G, 0].double()
-            size = (qq.abs() @ kk.abs().t().contiguous()).amax(1)
-            es = (130 * 2.0 ** -24 * size + 2.0 ** -25 * (qq.abs().sum(1) + kk.abs().sum(1).max())) / math.sqrt(HD)
+            size = (qq.abs() @ kk.abs().t().contiguous()).amax(1) + bias * qq.abs().sum(1)
+            es = 130 * 2.0 ** -24 * size + 2.0 ** -25 * (qq.abs().sum(1) + kk.abs().sum(1).max())
+            if c:
+                es = es + 2.0 ** -11 * (qq.abs() @ big.t().contiguous()).amax(1)
+            es = es / math.sqrt(HD)
             p = torch.softmax(qq @ kk.t().contiguous() / math.sqrt(HD), 1)
             rel = 2 * es + 2.0 ** -16
             out[b, h * G:(h + 1) * G, 0] = p @ vv
             a = p @ vv.abs()
             tol[b, h * G:(h + 1) * G, 0] = (a * (2.0 ** -10 + rel[:, None]) + half * (p @ vv).abs() * (1 + 2.0 ** -9) +
-                                            len(vv) * 2.0 ** -35 * vv.abs().max() + 2.0 ** -24)
+                                            len(vv) * 2.0 ** -34 * max(vmax, float(vv.abs().max())) +
+                                            34 * 2.0 ** -23 * vmax + 2.0 ** -24)
             if c:
                 w[b, :c] += p[:, :c * PAGE].reshape(G, c, PAGE).sum((0, 2))
             wtol = max(wtol, float(rel.max()))
@@ -128,6 +146,7 @@ def test_attention_and_weights(shape, dtype):
     assert not bool(bad.any()), f"{int(bad.sum())} of {bad.numel()} values off, worst {float((got.double() - want).abs().max())}"
     if not tab.shape[1]:
         return
+    want, tol, w, wtol = _reference(k, v, q, tab, counts, tk, tv, tails, rounded=True)
     old = torch.rand(tab.shape, device="cuda")
     acc = old.clone()
     again = paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl, weights=acc, decay=0.75)
@@ -168,7 +187,7 @@ def test_counts_and_numbers_are_clamped():
     wild = tab.clone()
     wild[1, 1] = 10 ** 9
     wild[1, 2] = -7
-    want, tol, *_ = _reference(k, v, q, torch.where(wild < 0, 10 ** 9, wild), counts, tk, tv, tails)
+    want, tol, *_ = _reference(k, v, q, wild, counts, tk, tv, tails)
     got = paged_decode_attention(k, v, q, wild, cnt, tk, tv, tail_len=tl)
     assert bool(((got.double() - want).abs() <= tol).all())
     over = torch.tensor([99, -3], dtype=torch.int32, device="cuda")
@@ -266,8 +285,8 @@ def test_pages_written_again_keep_their_room():
     for _ in range(3):                                     # as many exceptions again: no more room
         p.write(x, at, s, s.half())
     assert int(p.pool.n_exc) == seen[-1] and torch.equal(p.read(at), before)
-    assert seen[-1] <= 2 * 16 * int(p._room.max()) and int(p.pool.status) == 0
-    assert int(p._room.max()) <= 256
+    assert seen[-1] <= 2 * 16 * int(p.pool.room.max()) and int(p.pool.status) == 0
+    assert int(p.pool.room.max()) <= 256
 
 
 def test_many_exceptions_lengthen_the_list():

@@ -80,7 +80,8 @@ def test_c_entries_refuse_null_and_bad_sizes():
     res = L.Resident(a=16, b=16, mask=16, meta=16, exc=16, scale=16, n_exc=16, status=16, n_heads=2, cap_blocks=4, exc_cap=1)
     rows = L.Rows(p=16, stride_b=128, stride_h=128, stride_t=128)
     odd = L.Rows(p=16, stride_b=129, stride_h=128, stride_t=128)
-    r, q = ctypes.addressof(res), ctypes.addressof(rows)
+    pool = L.Pages(r=res, room=16, rec=16)
+    r, q = ctypes.addressof(pool), ctypes.addressof(rows)
 
     def attend(k=r, v=r, qq=q, n=2, g=4, pages=16, width=3, counts=16, tk=q, tv=q, cap=4, work=16, nbytes=1 << 40, out=q, dt=0):
         return lib.lq_paged_attention(k, v, qq, n, g, pages, width, counts, tk, tv, cap, None, None, 1.0, dt, work, nbytes,
@@ -89,8 +90,8 @@ def test_c_entries_refuse_null_and_bad_sizes():
                 dict(pages=None), dict(counts=None), dict(tk=None), dict(cap=-1), dict(work=None), dict(work=24),
                 dict(nbytes=0), dict(out=None), dict(dt=2), dict(width=-1)):
         assert attend(**bad) == L.LQ_ERR_ARG, bad
-    assert lib.lq_page_quantize(None, 0, 1, 16, 16, 16, r, 16, 16, None) == L.LQ_ERR_ARG
-    assert lib.lq_page_quantize(16, 0, 1, 17, 16, 16, r, 16, 16, None) == L.LQ_ERR_ARG
+    assert lib.lq_page_quantize(None, 0, 1, 16, 16, 16, r, 16, None) == L.LQ_ERR_ARG
+    assert lib.lq_page_quantize(16, 0, 1, 17, 16, 16, r, 16, None) == L.LQ_ERR_ARG
     assert lib.lq_page_dequant(r, None, 1, 1, 16, 0, None) == L.LQ_ERR_ARG
     ev = [16, 16, 16, 1, 4, 2, 1, 1, 16, 16, 16, 16, None]
     for i, x in ((0, None), (3, 0), (4, 0), (5, 1), (6, -1), (7, -1), (11, None)):
