@@ -90,37 +90,64 @@ __device__ __forceinline__ T at(const void* base, O bytes) {
 
 // Records of a tile's blocks b0 and b1: of K, pairs of tokens 8 g + 2 i, + 1 (lane % 16 =
 // 4 g + i) of vectors 4 c + lane / 16; of V, vector lane % 16 of tokens 8 (lane / 16) .. + 7.
+// A copy that is made here: where a register's next value is being loaded, the compiler
+// would copy the loaded one at the loop's end instead, and wait for it there.
+__device__ __forceinline__ uint32_t copied(uint32_t x) {
+    uint32_t y;
+    asm volatile("v_mov_b32 %0, %1" : "=v"(y) : "v"(x));
+    return y;
+}
 struct Recs {
     uint2 ka[4];
     uint32_t kb[4];
     uint4 va[2];
     uint2 vb;
-    uint4 vs;                                  // scales of the lane's tokens of V ..
-    uint4 ks;                                  // .. and of K's, where the products come out; or
-    uint32_t kp;                               // of K's, where the records lie
+    uint32_t vs[4], ks[4];                     // scales of V and K of the tokens that the lane weighs, pairs
+    uint32_t kp;                               // of K where the records lie, where they are multiplied there
 };
+// The lanes of a quarter (16) hold the scores of eight tokens of 16 rows, but a group has
+// mostly fewer: with NR row slots lane r + NR a of a quarter weighs row r's tokens
+// (NR / 2) a .. + NR / 2 - 1.  Pairs of tokens a lane weighs, and their scales:
+template <int NR>
+constexpr int kPairs = NR / 4;
+template <int NR, typename O>
+__device__ __forceinline__ void load_scales(const uint16_t* scale, O at_block, uint32_t lane, uint32_t s[4]) {
+    const O from = at_block + (lane & 16) + (lane & 15) / NR * (NR / 4) * 4;
+    if constexpr (NR == 16) {
+        const uint4 w = at<uint4>(scale, from);
+        s[0] = w.x; s[1] = w.y; s[2] = w.z; s[3] = w.w;
+    } else if constexpr (NR == 8) {
+        const uint2 w = at<uint2>(scale, from);
+        s[0] = w.x; s[1] = w.y;
+    } else {
+        s[0] = at<uint32_t>(scale, from);
+    }
+}
 struct Meta2 {
     uint32_t base, count;                      // exceptions of block lane / 32
 };
-template <bool BIG, bool ROUND>
-__device__ __forceinline__ void load_recs(const PagedArgs& A, uint32_t b0, uint32_t b1, uint32_t lane, Recs& d) {
+template <bool BIG, bool ROUND, int NR>
+__device__ __forceinline__ void load_k(const PagedArgs& A, uint32_t b0, uint32_t b1, uint32_t lane, Recs& d) {
     typedef typename Off<BIG>::type O;
-    const uint32_t row = lane & 15, kblk = row & 8 ? b1 : b0, vblk = lane & 32 ? b1 : b0;
-    const uint32_t tok = 8 * ((row >> 2) & 1) + 2 * (row & 3), krec = 16 * (lane >> 4) + tok;
-    const uint32_t half = (lane >> 4) & 1, vrec = 16 * row + 8 * half;
-    const O ka = (O)kblk * 1024 + krec * 4, kb = (O)kblk * 256 + krec;
-    const O va = (O)vblk * 1024 + vrec * 4, s = (O)vblk * 32 + half * 16;
+    const uint32_t row = lane & 15, blk = row & 8 ? b1 : b0, tok = 8 * ((row >> 2) & 1) + 2 * (row & 3), rec = 16 * (lane >> 4) + tok;
+    const O a = (O)blk * 1024 + rec * 4, b = (O)blk * 256 + rec;
 #pragma unroll
     for (int c = 0; c < 4; c++) {
-        d.ka[c] = at<uint2>(A.k.r.a, ka + 256 * c);
-        d.kb[c] = at<uint16_t>(A.k.r.b, kb + 64 * c);
+        d.ka[c] = at<uint2>(A.k.r.a, a + 256 * c);
+        d.kb[c] = at<uint16_t>(A.k.r.b, b + 64 * c);
     }
-    if constexpr (ROUND) d.kp = at<uint32_t>(A.k.r.scale, (O)kblk * 32 + tok * 2);
-    else d.ks = at<uint4>(A.k.r.scale, s);
-    d.va[0] = at<uint4>(A.v.r.a, va);
-    d.va[1] = at<uint4>(A.v.r.a, va + 16);
-    d.vb = at<uint2>(A.v.r.b, (O)vblk * 256 + vrec);
-    d.vs = at<uint4>(A.v.r.scale, s);
+    if constexpr (ROUND) d.kp = at<uint32_t>(A.k.r.scale, (O)blk * 32 + tok * 2);
+    else load_scales<NR>(A.k.r.scale, (O)(lane & 32 ? b1 : b0) * 32, lane, d.ks);
+}
+template <bool BIG, int NR>
+__device__ __forceinline__ void load_v(const PagedArgs& A, uint32_t b0, uint32_t b1, uint32_t lane, Recs& d) {
+    typedef typename Off<BIG>::type O;
+    const uint32_t blk = lane & 32 ? b1 : b0, rec = 16 * (lane & 15) + (lane & 16 ? 8 : 0);
+    const O a = (O)blk * 1024 + rec * 4;
+    d.va[0] = at<uint4>(A.v.r.a, a);
+    d.va[1] = at<uint4>(A.v.r.a, a + 16);
+    d.vb = at<uint2>(A.v.r.b, (O)blk * 256 + rec);
+    load_scales<NR>(A.v.r.scale, (O)blk * 32, lane, d.vs);
 }
 template <bool BIG>
 __device__ __forceinline__ Meta2 load_meta(const lq_pages& p, uint32_t b0, uint32_t b1, uint32_t lane) {
@@ -133,38 +160,42 @@ struct Entry {
     uint4 v;
     uint32_t rec;
 };
+template <bool BIG>
 __device__ __forceinline__ Entry load_entry(const lq_pages& p, const Meta2& m, uint32_t e) {
-    const int64_t i = (int64_t)m.base + e, from = e < m.count && i < p.r.exc_cap ? i : 0;
-    return {reinterpret_cast<const uint4*>(p.r.exc)[from], p.rec[from]};
+    typedef typename Off<BIG>::type O;
+    const uint32_t i = m.base + e, from = e < m.count && i < (uint32_t)p.r.exc_cap ? i : 0u;
+    return {at<uint4>(p.r.exc, (O)from * 16), at<uint8_t>(p.rec, from)};
 }
 __device__ __forceinline__ uint32_t most_of(const Meta2& m) {   // wave-uniform
     return max((uint32_t)__builtin_amdgcn_readlane((int)m.count, 0), (uint32_t)__builtin_amdgcn_readlane((int)m.count, 32));
 }
 // put(rec, v): the lane's entry over record rec of block lane / 32, for all of a tile, 32 of
 // a block at a time (in the place of one that the list had no room for stands the zero vector)
-template <typename P>
+template <bool BIG, typename P>
 __device__ __forceinline__ void each_entry(const lq_pages& p, const Meta2& m, Entry e, uint32_t most, int lane, P put) {
 #pragma unroll 1
     for (uint32_t r0 = 0; r0 < most; r0 += 32) {
         const uint32_t k = r0 + (lane & 31);
-        if (r0) e = load_entry(p, m, k);
-        if (k < m.count && (int64_t)m.base + k < p.r.exc_cap) put(e.rec, e.v);
+        if (r0) e = load_entry<BIG>(p, m, k);
+        if (k < m.count && m.base + k < (uint32_t)p.r.exc_cap) put(e.rec, e.v);
     }
 }
 
 // Without the record's bias: as a pair of fp16 numbers 2^-24 w, w = 2 c + 32, whole and
 // below 64 for a record.  What is multiplied by them needs neither the 32 taken off nor the
 // scale: both go into the other operand's sum and into the product (see attend below).
+template <int SH>   // b's byte from bit SH on
 __device__ __forceinline__ void raw_pairs(uint32_t a, uint32_t b, uint32_t p[4]) {
     const uint32_t kc = __builtin_amdgcn_perm(0u, a, 0x0c000c00u) & 0x00010001u;
     p[0] = (a & kFieldMask) | kc;
     p[1] = ((a >> 5) & kFieldMask) | kc;
     p[2] = ((a >> 10) & kFieldMask) | kc;
-    const uint32_t c7h = ((b >> 5) & 7u) | ((a >> 13) & 8u);
-    const uint32_t par = ((uint32_t)__builtin_popcount(a & kLsbMask) + b) & 1u;
-    p[3] = kc | ((b & 31u) << 1) | (((c7h << 1) | par) << 17);
+    const uint32_t u6 = (b >> SH) & 31u, c7h = ((b >> (SH + 5)) & 7u) | ((a >> 13) & 8u);
+    const uint32_t par = ((uint32_t)__builtin_popcount(a & kLsbMask) + u6) & 1u;
+    p[3] = kc | (u6 << 1) | (((c7h << 1) | par) << 17);
 }
-__device__ __forceinline__ void raw_pairs_tok(uint32_t a0, uint32_t b0, uint32_t a1, uint32_t b1, uint32_t p[8]) {
+template <int SH>   // both bytes, from bits SH and SH + 8 on
+__device__ __forceinline__ void raw_pairs_tok(uint32_t a0, uint32_t a1, uint32_t b, uint32_t p[8]) {
     const uint32_t lo = __builtin_amdgcn_perm(a1, a0, 0x05040100u);
     const uint32_t hi = __builtin_amdgcn_perm(a1, a0, 0x07060302u);
     const uint32_t kc = lo & 0x00010001u;
@@ -174,11 +205,12 @@ __device__ __forceinline__ void raw_pairs_tok(uint32_t a0, uint32_t b0, uint32_t
     p[1] = (hi & kFieldMask) | kc;
     p[3] = ((hi >> 5) & kFieldMask) | kc;
     p[5] = ((hi >> 10) & kFieldMask) | kc;
-    const uint32_t h0 = ((b0 >> 5) & 7u) | ((a0 >> 13) & 8u);
-    const uint32_t h1 = ((b1 >> 5) & 7u) | ((a1 >> 13) & 8u);
-    const uint32_t q0 = ((uint32_t)__builtin_popcount(a0 & kLsbMask) + b0) & 1u;
-    const uint32_t q1 = ((uint32_t)__builtin_popcount(a1 & kLsbMask) + b1) & 1u;
-    p[6] = kc | ((b0 & 31u) << 1) | ((b1 & 31u) << 17);
+    const uint32_t u0 = (b >> SH) & 31u, u1 = (b >> (SH + 8)) & 31u;
+    const uint32_t h0 = ((b >> (SH + 5)) & 7u) | ((a0 >> 13) & 8u);
+    const uint32_t h1 = ((b >> (SH + 13)) & 7u) | ((a1 >> 13) & 8u);
+    const uint32_t q0 = ((uint32_t)__builtin_popcount(a0 & kLsbMask) + u0) & 1u;
+    const uint32_t q1 = ((uint32_t)__builtin_popcount(a1 & kLsbMask) + u1) & 1u;
+    p[6] = kc | (u0 << 1) | (u1 << 17);
     p[7] = kc | (((h0 << 1) | q0) << 1) | (((h1 << 1) | q1) << 17);
 }
 // an entry's eight values 2c so (beyond 2048 they lose bits, as fp16 does), and as c
@@ -214,7 +246,7 @@ __device__ __forceinline__ float pair_sum(float v) {   // of lane and lane ^ 16
 // State of a row over a unit's pages.  K's and V's values are c times their token's scale,
 // and enter the products as 2^-24 (2 c + 32):
 //   z   = kScale2 2^23 s_k (sum_i q_i k_i - 2^-19 sum_i q_i)
-//   o   = 2^23 (sum_t P_t v_t - 2^-19 sum_t P_t),   P_t = 2^(z_t - m) s_v 2^shift in fp16
+//   o   = 2^23 (sum_t P_t v_t - 2^-19 sum_t P_t),   P_t = fp16(fp16(2^(z_t - m + shift)) s_v)
 // so a record is decoded by bit operations alone.  The correction of z starts the product's
 // accumulator; that of o is taken off every 32 tiles, so that the sums stay near their result
 // (N tokens of like weights: the result falls as sqrt(N) beside them).  ROUND: K's values
@@ -222,7 +254,8 @@ __device__ __forceinline__ float pair_sum(float v) {   // of lane and lane ^ 16
 // attention's in 32 bits: c's own pairs, times the scale.
 struct PageState {
     float m, l, sum;                           // reference, sum of 2^(z - m + shift), of P_t since the last correction
-    float shift;                               // P stays in fp16's range: 2^(shift + kLazy) times the largest scale
+    float shift;                               // kPShift, less where a scale is above 1 (P stays in fp16's range)
+    float limit;                               // a logarithm of a weight beyond it raises the reference
     f4_t o[8];
 };
 constexpr float kUnit = 8388608.0f;            // 2^23
@@ -234,86 +267,128 @@ __device__ __forceinline__ void rescale(PageState& st, float f) {
 #pragma unroll
         for (int i = 0; i < 4; i++) st.o[mm][i] *= f;
 }
-// sum over the lanes that hold a row
+template <int CTRL>
+__device__ __forceinline__ float dppf(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+// sum and maximum over the lanes that hold a row
 __device__ __forceinline__ float quarters_sum(float v) {
     v = pair_sum(v);
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+template <int NR>
+__device__ __forceinline__ float shares_sum(float v) {   // within a quarter
+    if (NR <= 8) v += dppf<0x128>(v);          // row_ror:8
+    if (NR <= 4) v += dppf<0x124>(v);          // row_ror:4
+    return v;
+}
+template <int NR>
+__device__ __forceinline__ float row_sum(float v) { return quarters_sum(shares_sum<NR>(v)); }
+template <int NR>
+__device__ __forceinline__ float row_max(float v) {
+    if (NR <= 8) v = fmaxf(v, dppf<0x128>(v));
+    if (NR <= 4) v = fmaxf(v, dppf<0x124>(v));
+    return quarters_max(v);
+}
+template <int NR>
 __device__ __forceinline__ void correct(PageState& st) {
-    const float c = quarters_sum(st.sum) * (-0x1p-19f);
+    const float c = row_sum<NR>(st.sum) * (-0x1p-19f);
 #pragma unroll
     for (int mm = 0; mm < 8; mm++)
 #pragma unroll
         for (int i = 0; i < 4; i++) st.o[mm][i] += c;
     st.sum = 0.f;
 }
-// the largest of eight fp16 numbers that are not negative, over the wave
-__device__ __forceinline__ float wave_scale(const uint4& w) {
-    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-    uint32_t top = 0u;
+// the largest of the lane's scales, and the least e with 2^e >= every one of the wave's, 0 at least
+template <int NR>
+__device__ __forceinline__ float lane_scale(const uint32_t s[4]) {
+    h2_t m = __builtin_bit_cast(h2_t, s[0]);
 #pragma unroll
-    for (int i = 0; i < 4; i++) top = max(top, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
-    return quarters_max(h2f((uint16_t)top));   // the 16 lanes of a quarter have the same tokens
+    for (int i = 1; i < kPairs<NR>; i++) m = __builtin_elementwise_max(m, __builtin_bit_cast(h2_t, s[i]));
+    return fmaxf((float)m[0], (float)m[1]);
 }
-// the least e with 2^e >= s (0 for a scale of 0), and whether a scale passes 2^e
-__device__ __forceinline__ int scale_exp(float s) {
-    const uint32_t u = __float_as_uint(s);
-    return s == 0.f ? 0 : (int)((u + 0x7fffffu) >> 23) - 127;
-}
-__device__ __forceinline__ float scale_limit(float s) { return __builtin_amdgcn_ldexpf(1.f, scale_exp(s)); }
-__device__ __forceinline__ bool above(const uint4& w, float limit) {
-    const h2_t a = __builtin_elementwise_max(__builtin_bit_cast(h2_t, w.x), __builtin_bit_cast(h2_t, w.y));
-    const h2_t b = __builtin_elementwise_max(__builtin_bit_cast(h2_t, w.z), __builtin_bit_cast(h2_t, w.w));
-    const h2_t c = __builtin_elementwise_max(a, b);
-    return fmaxf((float)c[0], (float)c[1]) > limit;
-}
-__device__ __forceinline__ float half_of(const uint4& w, int i) {
-    const uint32_t x = i < 2 ? w.x : i < 4 ? w.y : i < 6 ? w.z : w.w;
-    return (float)__builtin_bit_cast(h2_t, x)[i & 1];
+template <int NR>
+__device__ __forceinline__ float scale_log(const uint32_t s[4]) {
+    const float m = row_max<NR>(lane_scale<NR>(s));   // the lanes of a quarter have the same tokens
+    return fmaxf((float)((int)((__float_as_uint(m) + 0x7fffffu) >> 23) - 127), 0.f);
 }
 
 // One tile: scores s[y][i] of token 8 (lane / 16) + 2 i + y (without their scales, or with
 // them where ROUND), raw V.  With SUMS the logarithm (base 2) of the sum of the lane's page
 // (lanes 0..31 hold the first page's tokens, 32..63 the second's).
-template <bool SUMS, bool ROUND>
-__device__ __forceinline__ float attend(f4_t s[2], const uint4& ks, const uint4& vs, uint32_t word,
+template <bool SUMS, bool ROUND, int NR>
+__device__ __forceinline__ float attend(const f4_t s[2], const uint32_t ks[4], const uint32_t vs[4], uint32_t word,
                                         const uint32_t vp[4][8], int lane, PageState& st) {
-    float y[8];
+    constexpr int N = 2 * kPairs<NR>;          // tokens that the lane weighs
+    float z[N];
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        y[i] = s[i & 1][i >> 1] * (ROUND ? kScale2 : half_of(ks, i) * (kScale2 * kUnit));
+    for (int i = 0; i < N; i++) {              // from the lane that has them, r of the quarter, a share at a time
+        int x = __float_as_int(s[i & 1][i >> 1]);
+#define LQ_SHARE(A) x = __builtin_amdgcn_update_dpp(x, __float_as_int(s[i & 1][(i >> 1) + (A) * kPairs<NR>]), \
+                                                    0x110 + (A) * NR, 0xf, NR == 8 ? 0xc : 1 << (A), false)   // row_shr
+        if constexpr (NR <= 8) LQ_SHARE(1);
+        if constexpr (NR == 4) {
+            LQ_SHARE(2);
+            LQ_SHARE(3);
+        }
+#undef LQ_SHARE
+        z[i] = __int_as_float(x);
+    }
+    float off = (st.m == -INFINITY ? 0.f : -st.m) + st.shift;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        z[i] = ROUND ? __builtin_fmaf(z[i], kScale2, off)
+                     : __builtin_fmaf((float)__builtin_bit_cast(h2_t, ks[i >> 1])[i & 1], z[i] * (kScale2 * kUnit), off);
     if (word != ~0u) {
-        const uint32_t own = word >> (8 * (lane >> 4));
+        const uint32_t own = word >> (8 * (lane >> 4) + (lane & 15) / NR * N);
 #pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = (own >> i) & 1u ? y[i] : -INFINITY;
+        for (int i = 0; i < N; i++) z[i] = (own >> i) & 1u ? z[i] : -INFINITY;
     }
-    float mx = fmaxf(y[0], y[1]);
+    float mx = fmaxf(z[0], z[1]);
 #pragma unroll
-    for (int i = 2; i < 8; i += 2) mx = fmaxf(fmaxf(mx, y[i]), y[i + 1]);
-    const float mn = quarters_max(mx);
-    if (__any(mn > st.m + kLazy)) {
-        const float up = mn > st.m + kLazy ? mn : st.m;
-        rescale(st, up == st.m ? 1.f : __builtin_amdgcn_exp2f(st.m - up));
-        st.m = up;
+    for (int i = 2; i < N; i += 2) mx = fmaxf(fmaxf(mx, z[i]), z[i + 1]);
+    if (__any(mx > st.limit)) {                // rare after the first tile
+        const float mn = row_max<NR>(mx);      // what the reference is raised by, in the rows that pass it
+        const bool up = mn > st.limit;
+        const float by = up ? mn - st.shift : 0.f;
+        rescale(st, st.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(-by));   // nothing has been summed without one
+        if (up) st.m = (st.m == -INFINITY ? 0.f : st.m) + by;
+        st.limit = st.m == -INFINITY ? -INFINITY : st.shift + kLazy;
+#pragma unroll
+        for (int i = 0; i < N; i++) z[i] -= by;
+        off -= by;
     }
-    const float off = (st.m == -INFINITY ? 0.f : -st.m) + st.shift;
     uint32_t p[4];
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float u = __builtin_amdgcn_exp2f(y[2 * i] + off), v = __builtin_amdgcn_exp2f(y[2 * i + 1] + off);
-        sum += u + v;
-        p[i] = pair_h(u * half_of(vs, 2 * i), v * half_of(vs, 2 * i + 1));
-        st.sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, p[i]), h2_t{(_Float16)1.f, (_Float16)1.f}, st.sum, false);
+    for (int i = 0; i < N / 2; i++) {
+        const float u = __builtin_amdgcn_exp2f(z[2 * i]), v = __builtin_amdgcn_exp2f(z[2 * i + 1]);
+        const h2_t h = __builtin_bit_cast(h2_t, pair_h(u, v)), one = {(_Float16)1.f, (_Float16)1.f};
+        if (SUMS) sum += u + v;
+        else st.l = __builtin_amdgcn_fdot2(h, one, st.l, false);
+        const h2_t w = h * __builtin_bit_cast(h2_t, vs[i]);
+        p[i] = __builtin_bit_cast(uint32_t, w);
+        st.sum = __builtin_amdgcn_fdot2(w, one, st.sum, false);
     }
-    st.l += sum;
+    if (SUMS) st.l += sum;
+    // back to lane r, which has row r's eight tokens in the product (what the others have goes
+    // into columns that are not read)
+    if constexpr (NR == 8) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) p[2 + i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)p[i], 0x108, 0xf, 0xf, false);   // row_shl
+    }
+    if constexpr (NR == 4) {
+        p[1] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)p[0], 0x104, 0xf, 0xf, false);
+        p[2] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)p[0], 0x108, 0xf, 0xf, false);
+        p[3] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)p[0], 0x10c, 0xf, 0xf, false);
+    }
     const h8_t pb = as_h8(p[0], p[1], p[2], p[3]);
 #pragma unroll
     for (int mm = 0; mm < 8; mm++)
         st.o[mm] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(vp[0][mm], vp[1][mm], vp[2][mm], vp[3][mm]), pb, st.o[mm],
                                                           0, 0, 0);
-    return SUMS ? __builtin_amdgcn_logf(pair_sum(sum)) - off + kPShift : 0.f;
+    return SUMS ? __builtin_amdgcn_logf(pair_sum(shares_sum<NR>(sum))) - off + kPShift : 0.f;
 }
 
 __device__ __forceinline__ void zero_out(const PagedArgs& A, int b, int tid) {
@@ -347,7 +422,7 @@ __device__ __forceinline__ Len len_at(const PagedArgs& A, const Lens& mine, int 
     l.tiles = l.page_tiles + ((l.tail + 31) >> 5);
     return l;
 }
-template <bool BF16, bool SUMS, bool BIG>
+template <bool BF16, bool SUMS, bool BIG, int NR>
 __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
     constexpr bool ROUND = SUMS;
     extern __shared__ __align__(16) char s_dyn[];
@@ -443,6 +518,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                 PageState ps;
                 ps.m = -INFINITY;
                 ps.l = ps.sum = 0.f;
+                ps.shift = kPShift;
+                ps.limit = -INFINITY;
+                float largest = 1.f;           // no scale has been above it
 #pragma unroll
                 for (int mm = 0; mm < 8; mm++) ps.o[mm] = f4_t{0.f, 0.f, 0.f, 0.f};
                 Recs rd;
@@ -457,28 +535,28 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                 blocks(t);
                 mk = load_meta<BIG>(A.k, x1, y1, lane);
                 mv = load_meta<BIG>(A.v, x1, y1, lane);
-                load_recs<BIG, ROUND>(A, x1, y1, lane, rd);
+                load_k<BIG, ROUND, NR>(A, x1, y1, lane, rd);
+                load_v<BIG, NR>(A, x1, y1, lane, rd);
                 blocks(t + 1);
                 nk = load_meta<BIG>(A.k, x1, y1, lane);
                 nv = load_meta<BIG>(A.v, x1, y1, lane);
-                ek = load_entry(A.k, mk, lane & 31);
-                ev = load_entry(A.v, mv, lane & 31);
-                float top = wave_scale(rd.vs);         // 2^shift times it lies within (2^(kPShift - 1), 2^kPShift]
-                ps.shift = kPShift - (float)scale_exp(top);
-                float limit = scale_limit(top);
+                ek = load_entry<BIG>(A.k, mk, lane & 31);
+                ev = load_entry<BIG>(A.v, mv, lane & 31);
                 for (int tile = t; tile < pe; tile++) {
                     const uint32_t word = 2 * tile + 1 < L.pages ? ~0u : 0xffffu;
                     f4_t s[2] = {s0, s0};
                     uint32_t vp[4][8], p[8][4];
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        const uint32_t ra = j & 1 ? rd.ka[j >> 1].y : rd.ka[j >> 1].x, rb = (rd.kb[j >> 1] >> (8 * (j & 1))) & 0xffu;
+                        const uint32_t ra = j & 1 ? rd.ka[j >> 1].y : rd.ka[j >> 1].x, rb = rd.kb[j >> 1];
                         if constexpr (ROUND) {
-                            rec_pairs(ra, rb, p[j]);
+                            rec_pairs(ra, (rb >> (8 * (j & 1))) & 0xffu, p[j]);
 #pragma unroll
                             for (int i = 0; i < 4; i++) p[j][i] = unbias(p[j][i]);
+                        } else if (j & 1) {
+                            raw_pairs<8>(ra, rb, p[j]);
                         } else {
-                            raw_pairs(ra, rb, p[j]);
+                            raw_pairs<0>(ra, rb, p[j]);
                         }
                     }
                     if (const uint32_t most = most_of(mk)) {
@@ -486,7 +564,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
 #pragma unroll
                         for (int j = 0; j < 8; j++) area[64 * j + lane] = u32x4_t{p[j][0], p[j][1], p[j][2], p[j][3]};
                         wave_lds_sync();
-                        each_entry(A.k, mk, ek, most, lane, [&](uint32_t rec, const uint4& w) __attribute__((always_inline)) {
+                        each_entry<BIG>(A.k, mk, ek, most, lane, [&](uint32_t rec, const uint4& w) __attribute__((always_inline)) {
                             uint32_t e[4];
                             if constexpr (ROUND) exc_pairs(w, e);
                             else raw_entry(w, e);
@@ -508,14 +586,24 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                         s[j & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(p[j][0], p[j][1], p[j][2], p[j][3]), q[j >> 1],
                                                                           s[j & 1], 0, 0, 0);
                     }
+                    // The next tile's records, as soon as these are used (every use scheduled before the
+                    // reload), and the bases of the one behind; past the end the last tile's again.
+                    uint32_t ks[4], vs[4];
+                    if (!ROUND) {
+#pragma unroll
+                        for (int i = 0; i < kPairs<NR>; i++) ks[i] = copied(rd.ks[i]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    ek = load_entry<BIG>(A.k, nk, lane & 31);
+                    mk = {copied(nk.base), copied(nk.count)};
+                    load_k<BIG, ROUND, NR>(A, x1, y1, lane, rd);
                     {
                         const uint32_t aw[8] = {rd.va[0].x, rd.va[0].y, rd.va[0].z, rd.va[0].w,
                                                 rd.va[1].x, rd.va[1].y, rd.va[1].z, rd.va[1].w};
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint32_t w = k < 2 ? rd.vb.x : rd.vb.y;
-                            raw_pairs_tok(aw[2 * k], w >> (16 * (k & 1)), aw[2 * k + 1], w >> (16 * (k & 1) + 8), vp[k]);
-                        }
+                        raw_pairs_tok<0>(aw[0], aw[1], rd.vb.x, vp[0]);
+                        raw_pairs_tok<16>(aw[2], aw[3], rd.vb.x, vp[1]);
+                        raw_pairs_tok<0>(aw[4], aw[5], rd.vb.y, vp[2]);
+                        raw_pairs_tok<16>(aw[6], aw[7], rd.vb.y, vp[3]);
                     }
                     if (const uint32_t most = most_of(mv)) {
 #pragma unroll
@@ -523,7 +611,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                             area[64 * j + lane] = u32x4_t{vp[j >> 1][4 * (j & 1)], vp[j >> 1][4 * (j & 1) + 1],
                                                           vp[j >> 1][4 * (j & 1) + 2], vp[j >> 1][4 * (j & 1) + 3]};
                         wave_lds_sync();
-                        each_entry(A.v, mv, ev, most, lane, [&](uint32_t rec, const uint4& v) __attribute__((always_inline)) {
+                        each_entry<BIG>(A.v, mv, ev, most, lane, [&](uint32_t rec, const uint4& v) __attribute__((always_inline)) {
                             uint32_t e[4];
                             raw_entry(v, e);
                             const uint32_t tok = 16 * (lane >> 5) + (rec & 15);   // pair (tok / 2) % 4 of lane vector + 16 (tok / 8)
@@ -540,41 +628,39 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                         }
                         wave_lds_sync();
                     }
-                    if (__any(above(rd.vs, limit))) {    // a larger scale than any before: P's range moves
-                        top = wave_scale(rd.vs);
-                        const float shift = kPShift - (float)scale_exp(top);
-                        rescale(ps, __builtin_amdgcn_exp2f(shift - ps.shift));
-                        ps.shift = shift;
-                        limit = scale_limit(top);
+                    if (__any(lane_scale<NR>(rd.vs) > largest)) {
+                        const float e = scale_log<NR>(rd.vs), by = kPShift - e - ps.shift;
+                        rescale(ps, __builtin_amdgcn_exp2f(by));
+                        ps.shift += by;
+                        ps.limit += by;
+                        largest = __builtin_amdgcn_exp2f(e);
                     }
-                    const uint4 ks = ROUND ? make_uint4(0u, 0u, 0u, 0u) : rd.ks, vs = rd.vs;
-                    __builtin_amdgcn_sched_barrier(0);   // every use of the records before their reload
-                    // the next tile's records and the bases of the one behind
-                    ek = load_entry(A.k, nk, lane & 31);
-                    ev = load_entry(A.v, nv, lane & 31);
-                    mk = nk;
-                    mv = nv;
-                    load_recs<BIG, ROUND>(A, x1, y1, lane, rd);
+#pragma unroll
+                    for (int i = 0; i < kPairs<NR>; i++) vs[i] = copied(rd.vs[i]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    ev = load_entry<BIG>(A.v, nv, lane & 31);
+                    mv = {copied(nv.base), copied(nv.count)};
+                    load_v<BIG, NR>(A, x1, y1, lane, rd);
                     if (((tile + 2) >> 5) == pg.g + 2) {
                         pg.g++;
                         pg.near = pg.far;
                         pg.far = load_pages(row, L.pages, cap, pg.g + 1, lane);
-                        correct(ps);           // with the sums of the tiles before this one
+                        correct<NR>(ps);           // with the sums of the tiles before this one
                     }
                     blocks(tile + 2);
                     nk = load_meta<BIG>(A.k, x1, y1, lane);
                     nv = load_meta<BIG>(A.v, x1, y1, lane);
-                    const float z = attend<SUMS, ROUND>(s, ks, vs, word, vp, lane, ps);
+                    const float z = attend<SUMS, ROUND, NR>(s, ks, vs, word, vp, lane, ps);
                     if (SUMS) {
                         const int j = 2 * tile + (lane >> 5);
                         if (!(g & 1) && col < G && j < L.pages) A.z[((int64_t)unit * A.width + j) * G + col] = z;
                     }
                 }
                 // on as the tail's rows are taken
-                correct(ps);
+                correct<NR>(ps);
                 const float f = __builtin_amdgcn_exp2f(kPShift - ps.shift);
                 st.m = ps.m;
-                st.l = l32 = ps.l * f;
+                st.l = l32 = shares_sum<NR>(ps.l) * f;
 #pragma unroll
                 for (int mm = 0; mm < 8; mm++)
 #pragma unroll
@@ -595,13 +681,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                         const int tok = min(8 * (col >> 2) + 2 * (col & 3) + y, have - 1);
                         w[y][c] = *reinterpret_cast<const uint4*>(p + (t0 + tok) * A.tk.st + 32 * c + 8 * g);
                     }
-                rows_v<BF16>(A.tv.p + b * A.tv.sb + h * A.tv.sh, A.tv.st, t0, have, word, lane, vp);
 #pragma unroll
                 for (int y = 0; y < 2; y++)
 #pragma unroll
                     for (int c = 0; c < 4; c++)
                         s[y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                             __builtin_bit_cast(h8_t, BF16 ? bf_to_h(w[y][c]) : w[y][c]), q[c], s[y], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);       // K's rows leave their registers before V's come
+                rows_v<BF16>(A.tv.p + b * A.tv.sb + h * A.tv.sh, A.tv.st, t0, have, word, lane, vp);
                 const float was = st.m;
                 few_attend(s, word, word == ~0u, vp, lane, st);
                 if (SUMS) {                    // few_attend's sum is of the rounded weights: these few again
@@ -964,20 +1051,27 @@ bool plan(int64_t n_seq, int64_t heads, int64_t group, int64_t width, int64_t ta
 bool pool_ok(const lq_pages* p) {
     const lq_resident* r = p ? &p->r : nullptr;
     return r && r->a && r->b && r->mask && r->meta && r->scale && r->n_heads > 0 && r->cap_blocks > 0 && r->exc_cap >= 0 &&
-           r->cap_blocks <= INT_MAX / r->n_heads && (r->exc_cap == 0 || (r->exc && p->rec));
+           r->exc_cap <= INT_MAX && r->cap_blocks <= INT_MAX / r->n_heads && (r->exc_cap == 0 || (r->exc && p->rec));
 }
 bool rows_ok(const lq_rows* r) {
     return r && r->p && ((uintptr_t)r->p & 15) == 0 && r->stride_b % 8 == 0 && r->stride_h % 8 == 0 && r->stride_t % 8 == 0;
 }
 Rows rows_of(const lq_rows* r) { return {static_cast<const uint16_t*>(r->p), r->stride_b, r->stride_h, r->stride_t}; }
 
-template <bool BF16, bool SUMS>
-void paged_launch(const PagedArgs& A, int grid, bool big, hipStream_t s) {
+template <bool BF16, bool SUMS, bool BIG>
+void paged_launch(const PagedArgs& A, int grid, hipStream_t s) {
     const int slot = A.group * kMRow * 4;
     const size_t lds = (size_t)kWaves * ((slot > kPatch ? slot : kPatch) + slot);
-    if (big) hipLaunchKernelGGL((k_paged<BF16, SUMS, true>), dim3((unsigned)grid), dim3(kThreads), lds, s, A);
-    else hipLaunchKernelGGL((k_paged<BF16, SUMS, false>), dim3((unsigned)grid), dim3(kThreads), lds, s, A);
+    const dim3 g((unsigned)grid), wg(kThreads);
+    if (A.group <= 4) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 4>), g, wg, lds, s, A);
+    else if (A.group <= 8) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 8>), g, wg, lds, s, A);
+    else hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 16>), g, wg, lds, s, A);
     if (grid > 1) hipLaunchKernelGGL((k_paged_join<BF16, SUMS>), dim3((unsigned)grid, (unsigned)A.group), dim3(256), 0, s, A);
+}
+template <bool BF16, bool SUMS>
+void paged_launch(const PagedArgs& A, int grid, bool big, hipStream_t s) {
+    if (big) paged_launch<BF16, SUMS, true>(A, grid, s);
+    else paged_launch<BF16, SUMS, false>(A, grid, s);
 }
 
 }  // namespace
@@ -1029,7 +1123,8 @@ int lq_paged_attention(const lq_pages *k, const lq_pages *v, const lq_rows *q, i
     A.desc = reinterpret_cast<Desc*>(w + p.desc);
     A.lse = reinterpret_cast<float*>(w + p.lse);
     A.z = reinterpret_cast<float*>(w + p.z);
-    const bool big = k->r.n_heads * k->r.cap_blocks > (int64_t)(UINT32_MAX / 1024);
+    const bool big = k->r.n_heads * k->r.cap_blocks > (int64_t)(UINT32_MAX / 1024) ||
+                     (k->r.exc_cap > v->r.exc_cap ? k->r.exc_cap : v->r.exc_cap) > (int64_t)(UINT32_MAX / 16);
     if (dtype == LQ_BF16) {
         if (d_weights) paged_launch<true, true>(A, p.grid, big, s);
         else paged_launch<true, false>(A, p.grid, big, s);
