@@ -20,6 +20,7 @@
 // tiles, and 9 us more than it with 8200.)
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "lq_device.h"
 #include "lq_few.h"
@@ -929,29 +930,92 @@ __device__ __forceinline__ uint32_t weight_key(float v) {
 
 constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64, kBins = 2048;
 
-// A sequence a workgroup: the room-th largest weight of the pages that may go, by a radix
-// search of 11, 11 and 10 bits, then one pass in the order of the pages, each wave a part.
-__global__ __launch_bounds__(kEvictThreads) void k_evict(EvictArgs A) {
+// The room-th largest weight of a sequence's pages that may go, by a radix search of 11, 11
+// and 10 bits (that ends where all of a bin stay), then one pass in the order of the pages,
+// each wave a part of them.  A sequence of up to 16384 pages is a workgroup's, N of them a
+// lane in registers, read once.  Longer ones (N = 0) are searched by `parts` workgroups each
+// of which looks at all of it and writes its part: the search is repeated on compute units
+// that would idle (4 sequences of 65536 pages, alone in its workgroup each: 80 us).
+// Bound by latency with few pages, by instructions with many.
+template <int N>
+__global__ __launch_bounds__(kEvictThreads) void k_evict(EvictArgs A, int parts) {
     __shared__ uint32_t s_bin[kBins];
-    __shared__ uint32_t s_part[kEvictWaves];
-    __shared__ uint32_t s_pick, s_left;
+    __shared__ uint32_t s_part[kEvictWaves], s_tie[2][kEvictWaves], s_sure[2][kEvictWaves];
+    __shared__ uint32_t s_pick, s_left, s_in;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t at = blockIdx.x * A.width;
-    const int n = min(max(A.n_pages[blockIdx.x], 0), (int)A.width);
+    const int b = N ? blockIdx.x : blockIdx.x / parts, part = N ? 0 : blockIdx.x % parts;
+    const float* weights = A.weights + b * A.width;
+    const int32_t* pages = A.pages + b * A.width;
+    const int n = min(max(A.n_pages[b], 0), (int)A.width);
     const int lo = min(A.sink, n), hi = max(lo, n - A.recent);
     const bool all = n <= A.keep;
     uint32_t room = all ? 0u : (uint32_t)max(0, A.keep - lo - (n - hi));
     const uint32_t kept_n = all ? (uint32_t)n : (uint32_t)lo + (uint32_t)(n - hi) + room;
-    uint32_t prefix = 0;                       // the bits found so far
-    if (!all && room) {
+    const bool some = room > 0;
+    // steps of 64 pages: those before the workgroup's part, and the wave's of the part
+    const int tiles = (n + 63) / 64, t0 = N ? 0 : (int)((int64_t)tiles * part / parts), t1 = N ? tiles : (int)((int64_t)tiles * (part + 1) / parts);
+    const int per = (t1 - t0 + kEvictWaves - 1) / kEvictWaves, mine = t0 + wave * per, steps = max(0, min(per, t1 - mine));
+    constexpr int C = N > 0 && N < 8 ? N : 8;  // steps whose loads go out together
+    constexpr int R = N ? N : 1;
+    float w[R];
+    auto weight = [&](int t) __attribute__((always_inline)) { return weights[min(64 * t + lane, n - 1)]; };
+    if (N) {
+#pragma unroll
+        for (int i = 0; i < R; i++) w[i] = i < steps ? weight(mine + i) : 0.f;
+    }
+    // f(page's place, weight, open: may go, in: there is such a page, its number where PAGES)
+    // for `count` steps from `first` on, `stride` apart
+    auto chunk = [&](auto numbers, int t, int stride, int count, const float* x, auto f) __attribute__((always_inline)) {
+        int32_t page[C];
+#pragma unroll
+        for (int i = 0; i < C; i++)
+            page[i] = decltype(numbers)::value && i < count ? pages[min(64 * (t + i * stride) + lane, n - 1)] : 0;
+#pragma unroll
+        for (int i = 0; i < C; i++) {
+            if (i >= count) break;
+            const int j = 64 * (t + i * stride) + lane;
+            f(j, x[i], j >= lo && j < hi, j < n, page[i]);
+        }
+    };
+    auto from_memory = [&](auto numbers, int first, int stride, int count, auto f) __attribute__((always_inline)) {
+        float x[C];
+        int i0 = 0;
+        for (; i0 + C <= count; i0 += C) {
+#pragma unroll
+            for (int i = 0; i < C; i++) x[i] = weight(first + (i0 + i) * stride);
+            chunk(numbers, first + i0 * stride, stride, C, x, f);
+        }
+        if (i0 < count) {
+#pragma unroll
+            for (int i = 0; i < C; i++) x[i] = weight(min(first + (i0 + i) * stride, tiles - 1));
+            chunk(numbers, first + i0 * stride, stride, count - i0, x, f);
+        }
+    };
+    auto each = [&](auto numbers, auto f) __attribute__((always_inline)) {   // of the wave's part
+        if constexpr (N > 0) {
+#pragma unroll
+            for (int i = 0; i < N; i += C)
+                if (i < steps) chunk(numbers, mine + i, 1, steps - i, w + i, f);
+        } else {
+            from_memory(numbers, mine, 1, steps, f);
+        }
+    };
+    const std::false_type no;
+    const std::true_type yes;
+    uint32_t prefix = 0;                       // the bits found so far, those from `shift` on
+    int shift = 32;
+    if (some) {
         for (int digit = 0; digit < 3; digit++) {
-            const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
+            const int bits = digit == 2 ? 10 : 11, up = shift;
+            shift -= bits;
             for (int i = tid; i < kBins; i += kEvictThreads) s_bin[i] = 0u;
             __syncthreads();
-            for (int j = lo + tid; j < hi; j += kEvictThreads) {
-                const uint32_t k = weight_key(A.weights[at + j]);
-                if (digit == 0 || k >> (shift + bits) == prefix) atomicAdd(&s_bin[(k >> shift) & ((1u << bits) - 1u)], 1u);
-            }
+            auto count = [&](int, float x, bool open, bool, int32_t) __attribute__((always_inline)) {
+                const uint32_t k = weight_key(x);
+                if (open && (digit == 0 || k >> up == prefix)) atomicAdd(&s_bin[(k >> shift) & ((1u << bits) - 1u)], 1u);
+            };
+            if constexpr (N > 0) each(no, count);
+            else from_memory(no, wave, kEvictWaves, (tiles - wave + kEvictWaves - 1) / kEvictWaves, count);
             __syncthreads();
             // bins from the largest down, two a thread
             const uint32_t c0 = s_bin[kBins - 1 - 2 * tid], c1 = s_bin[kBins - 2 - 2 * tid];
@@ -963,66 +1027,77 @@ __global__ __launch_bounds__(kEvictThreads) void k_evict(EvictArgs A) {
             }
             if (lane == 63) s_part[wave] = upto;
             __syncthreads();
-            for (int w = 0; w < wave; w++) upto += s_part[w];
+            for (int v = 0; v < wave; v++) upto += s_part[v];
             const uint32_t before = upto - c0 - c1;
             if (before < room && room <= upto) {
                 const bool second = room > before + c0;
                 s_pick = (uint32_t)(kBins - 1 - 2 * tid - (second ? 1 : 0));
                 s_left = room - before - (second ? c0 : 0u);
+                s_in = second ? c1 : c0;
             }
             __syncthreads();
             prefix = prefix << bits | s_pick;
             room = s_left;
+            if (room == s_in) break;           // the same in all threads
             __syncthreads();
         }
     }
-    // kept: the protected, what is above the key, and the first `room` of those equal to it
-    const int seg = ((n + 63) / 64 + kEvictWaves - 1) / kEvictWaves * 64;
-    const int j0 = wave * seg, j1 = min(n, j0 + seg);
-    const bool some = !all && kept_n > (uint32_t)(lo + n - hi);
-    uint32_t ties = 0, above = 0;
-    for (int j = j0; j < j1; j += 64) {
-        const int i = j + lane;
-        const bool open = i >= lo && i < hi;
-        const uint32_t k = open && i < j1 ? weight_key(A.weights[at + i]) : 0u;
-        ties += __builtin_popcountll(__ballot(open && i < j1 && some && k == prefix));
-        above += __builtin_popcountll(__ballot(i < j1 && (all || !open || (some && k > prefix))));
-    }
+    if (!some) shift = 0;
+    // kept: the protected, what is above the bits, and the first `room` of those that have them
+    uint32_t ties = 0, sure = 0;
+    auto tally = [&](int, float x, bool open, bool in, int32_t) __attribute__((always_inline)) {
+        const uint32_t k = weight_key(x) >> shift;
+        ties += __builtin_popcountll(__ballot(open && some && k == prefix));
+        sure += __builtin_popcountll(__ballot(in && (all || !open || (some && k > prefix))));
+    };
+    if (!N && t0 > 0) from_memory(no, wave, kEvictWaves, max(0, (t0 - wave + kEvictWaves - 1) / kEvictWaves), tally);
     if (lane == 0) {
-        s_bin[wave] = ties;
-        s_bin[kEvictWaves + wave] = above;
+        s_tie[0][wave] = ties;
+        s_sure[0][wave] = sure;
+    }
+    ties = sure = 0;
+    each(no, tally);
+    if (lane == 0) {
+        s_tie[1][wave] = ties;
+        s_sure[1][wave] = sure;
     }
     __syncthreads();
-    uint32_t tie = 0, to = 0;                  // equal and kept ones before the wave's part
-    for (int w = 0; w < wave; w++) {
-        to += s_bin[kEvictWaves + w] + min(s_bin[w], tie < room ? room - tie : 0u);
-        tie += s_bin[w];
+    uint32_t tie = 0, to = 0;                  // of those with the bits, and of all kept, before the wave's part
+#pragma unroll
+    for (int v = 0; v < kEvictWaves; v++) {
+        tie += s_tie[0][v];
+        to += s_sure[0][v];
     }
-    for (int j = j0; j < j1; j += 64) {
-        const int i = j + lane;
-        const bool in = i < j1, open = i >= lo && i < hi;
-        const float w = in ? A.weights[at + i] : 0.f;
-        const int32_t page = in ? A.pages[at + i] : 0;
-        const uint32_t k = weight_key(w);
-        const uint64_t eq = __ballot(in && open && some && k == prefix), below = (1ull << lane) - 1ull;
+    to += min(tie, room);
+    for (int v = 0; v < wave; v++) {
+        to += s_sure[1][v] + min(s_tie[1][v], tie < room ? room - tie : 0u);
+        tie += s_tie[1][v];
+    }
+    int32_t* out_pages = A.out_pages + b * A.width;
+    float* out_weights = A.out_weights + b * A.width;
+    int32_t* freed = A.freed + b * A.width;
+    const uint64_t below = (1ull << lane) - 1ull;
+    each(yes, [&](int j, float x, bool open, bool in, int32_t page) __attribute__((always_inline)) {
+        const uint32_t k = weight_key(x) >> shift;
+        const uint64_t eq = __ballot(open && some && k == prefix);
         const bool keep = in && (all || !open || (some && (k > prefix || (k == prefix && tie + __builtin_popcountll(eq & below) < room))));
         const uint64_t kept = __ballot(keep);
         const uint32_t p = to + __builtin_popcountll(kept & below);
         if (keep) {
-            A.out_pages[at + p] = page;
-            A.out_weights[at + p] = w;
+            out_pages[p] = page;
+            out_weights[p] = x;
         } else if (in) {
-            A.freed[at + (uint32_t)i - p] = page;
+            freed[(uint32_t)j - p] = page;
         }
         tie += __builtin_popcountll(eq);
         to += __builtin_popcountll(kept);
+    });
+    for (int64_t j = (int64_t)kept_n + part * kEvictThreads + tid; j < A.width; j += (int64_t)kEvictThreads * parts) {
+        out_pages[j] = -1;
+        out_weights[j] = 0.f;
     }
-    for (int64_t j = kept_n + tid; j < A.width; j += kEvictThreads) {
-        A.out_pages[at + j] = -1;
-        A.out_weights[at + j] = 0.f;
-    }
-    for (int64_t j = n - kept_n + tid; j < A.width; j += kEvictThreads) A.freed[at + j] = -1;
-    if (tid == 0) A.out_n[blockIdx.x] = (int32_t)kept_n;
+    for (int64_t j = (int64_t)(n - kept_n) + part * kEvictThreads + tid; j < A.width; j += (int64_t)kEvictThreads * parts) freed[j] = -1;
+    if (tid == 0 && part == 0) A.out_n[b] = (int32_t)kept_n;
 }
 
 // ------------------------------------------------------------------- plan --
@@ -1150,7 +1225,19 @@ int lq_evict_pages(const int32_t *d_pages, const int32_t *d_n_pages, const float
         return LQ_ERR_ARG;
     const EvictArgs A = {d_pages, d_n_pages, d_weights, max_pages, (int)keep, (int)sink, (int)recent,
                          d_out_pages, d_out_n, d_out_weights, d_freed};
-    hipLaunchKernelGGL(k_evict, dim3((unsigned)n_seq), dim3(kEvictThreads), 0, s, A);
+    const dim3 grid((unsigned)n_seq), wg(kEvictThreads);
+    if (max_pages <= kEvictThreads) {
+        hipLaunchKernelGGL(k_evict<1>, grid, wg, 0, s, A, 1);
+    } else if (max_pages <= 4 * kEvictThreads) {
+        hipLaunchKernelGGL(k_evict<4>, grid, wg, 0, s, A, 1);
+    } else if (max_pages <= 16 * kEvictThreads) {
+        hipLaunchKernelGGL(k_evict<16>, grid, wg, 0, s, A, 1);
+    } else {
+        int64_t parts = max_pages / (4 * kEvictThreads);
+        if (parts > 256 / n_seq) parts = 256 / n_seq;
+        if (parts < 1) parts = 1;
+        hipLaunchKernelGGL(k_evict<0>, dim3((unsigned)(n_seq * parts)), wg, 0, s, A, (int)parts);
+    }
     return launch_status();
 }
 

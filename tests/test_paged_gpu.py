@@ -473,3 +473,22 @@ def test_eviction_of_strided_inputs_and_counts_out_of_range():
     want = _evicted(pages[:, ::2].cpu().numpy(), cnt.clamp(0, 32).cpu().numpy(), w[:, ::2].cpu().numpy(), 7, 1, 1)
     for a, b in zip(got, want):
         assert np.array_equal(a.cpu().numpy(), b)
+
+
+@pytest.mark.parametrize("W,B", [(16384, 2), (16385, 3), (40001, 4), (70001, 1), (20000, 130)])
+def test_eviction_of_long_tables(W, B):
+    """Tables that one or several workgroups a sequence work on, with counts from none to all,
+    ties across the workgroups' parts and protected ends longer than a part."""
+    rng = np.random.RandomState(B)
+    count = rng.randint(0, W + 1, B).astype(np.int32)
+    count[0] = W
+    if B > 2:
+        count[1:3] = 0, 65
+    pages = rng.randint(0, 2 ** 31 - 1, (B, W)).astype(np.int32)
+    weight = rng.randint(0, 4, (B, W)).astype(np.float32)
+    weight[B // 2] = np.exp(rng.randn(W))
+    dev = [torch.from_numpy(x).cuda() for x in (pages, count, weight)]
+    for keep, sink, recent in [(0, 0, 0), (W // 2, 4, 16), (W // 2, W // 3, 9), (W // 2, 9, W // 3), (W - 1, 0, 1)]:
+        got = evict_pages(*dev, keep, sink, recent)
+        for a, b in zip(got, _evicted(pages, count, weight, keep, sink, recent)):
+            assert np.array_equal(a.cpu().numpy(), b), (keep, sink, recent)
