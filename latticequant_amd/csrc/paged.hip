@@ -33,6 +33,13 @@ inline int launch_status() { return hipGetLastError() == hipSuccess ? LQ_OK : LQ
 
 constexpr int kWaves = 4;                      // of a workgroup
 constexpr int kGroups = 512;                   // workgroups at most
+// Where no (sequence, head) can have more than kWhole tiles and all fit on the chip at once, a
+// workgroup takes one as a whole and there is no second launch.  1 / 8 / 32 sequences of 8
+// heads, replayed from a graph, against equal shares: 4 tiles 8.0 / 8.2 / 8.4 us (9.1 / 9.7
+// / 9.8), 12 tiles 10.2 / 11.5 / 11.5 (11.4 / 11.9 / 16.0), 20 tiles 12.9 / 14.0 / 14.9
+// (11.5 / 13.2 / 18.2), the host's time for the launch not counted; 128 sequences, two
+// rounds: 20 tiles 35.5 (31.0).
+constexpr int kWhole = 20;
 constexpr int kMRow = kHd + 4;                 // floats of a piece's row in LDS: o[128], m, l, l32
 constexpr int kRecF = 4 + kHd;                 // floats of a record's row: m, l, l32, unused, o[128]
 constexpr int kPatch = 8 * 64 * 16;            // bytes of a wave's area for exceptions
@@ -57,6 +64,7 @@ struct PagedArgs {
     uint16_t* out;
     int64_t ob, oh;
     int n_seq, heads, group, per;              // per: sequences of a lane's sum
+    int whole;                                 // a workgroup a unit, instead of equal shares
     float* rec;                                // [2 workgroup + (0: of an earlier one's, 1: begun here)][row][kRecF]
     Desc* desc;
     float* lse;                                // [unit][row]: m + log2(l32), with the weights' factor 2^kPShift
@@ -456,13 +464,24 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
     __syncthreads();
     for (int b = blockIdx.x; b < A.n_seq; b += gridDim.x)
         if (len_at(A, lens, b).tiles == 0) zero_out(A, b, tid);
-    const uint32_t groups = max(1u, min((uint32_t)gridDim.x, (total + kWaves - 1) / kWaves));
     const uint32_t me = blockIdx.x;
-    if (me >= groups) {
-        if (tid == 0) A.desc[me] = {-1, 0};
-        return;
+    uint32_t groups = gridDim.x, lo, hi;
+    if (A.whole) {
+        const int b = (int)(me / (uint32_t)A.heads);
+        const uint32_t tiles = (uint32_t)len_at(A, lens, b).tiles;
+        lo = (uint32_t)__builtin_amdgcn_readlane((int)before, b / A.per);
+        for (int k = b / A.per * A.per; k < b; k++) lo += (uint32_t)len_at(A, lens, k).tiles * A.heads;
+        lo += (me - (uint32_t)b * A.heads) * tiles;
+        hi = lo + tiles;
+    } else {
+        groups = max(1u, min(groups, (total + kWaves - 1) / kWaves));
+        if (me >= groups) {
+            if (tid == 0) A.desc[me] = {-1, 0};
+            return;
+        }
+        lo = (uint32_t)((uint64_t)me * total / groups);
+        hi = (uint32_t)((uint64_t)(me + 1) * total / groups);
     }
-    const uint32_t lo = (uint32_t)((uint64_t)me * total / groups), hi = (uint32_t)((uint64_t)(me + 1) * total / groups);
     uint32_t pos = lo + (uint32_t)((uint64_t)(hi - lo) * wave / kWaves);
     const uint32_t end = lo + (uint32_t)((uint64_t)(hi - lo) * (wave + 1) / kWaves);
 
@@ -800,7 +819,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
             if (begins) left = {unit, (int32_t)(((uint64_t)s_end * groups - 1) / total - me)};
         }
     }
-    if (tid == 0) A.desc[me] = left;
+    if (tid == 0 && !A.whole) A.desc[me] = left;
 }
 
 // The records of a unit that several workgroups share, a workgroup per row: thread
@@ -1103,7 +1122,7 @@ __global__ __launch_bounds__(kEvictThreads) void k_evict(EvictArgs A, int parts)
 // ------------------------------------------------------------------- plan --
 
 struct Plan {
-    int grid;
+    int grid, whole;
     int64_t rec, desc, lse, z, bytes;          // bytes before each, and in all
 };
 bool plan(int64_t n_seq, int64_t heads, int64_t group, int64_t width, int64_t tail_cap, bool weights, Plan* p) {
@@ -1113,11 +1132,12 @@ bool plan(int64_t n_seq, int64_t heads, int64_t group, int64_t width, int64_t ta
     const int64_t tiles = (width + 1) / 2 + (tail_cap + 31) / 32;
     if (tiles > INT_MAX / (n_seq * heads)) return false;
     const int64_t most = (n_seq * heads * tiles + kWaves - 1) / kWaves;
-    p->grid = (int)(most < 1 ? 1 : most < kGroups ? most : kGroups);
+    p->whole = tiles <= kWhole && n_seq * heads <= kGroups;
+    p->grid = (int)(p->whole ? n_seq * heads : most < kGroups ? most : kGroups);
     const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     p->rec = 0;
-    p->desc = p->rec + up(2 * p->grid * group * kRecF * 4);
-    p->lse = p->desc + up(p->grid * (int64_t)sizeof(Desc));
+    p->desc = p->rec + (p->whole ? 256 : up(2 * p->grid * group * kRecF * 4));
+    p->lse = p->desc + up(p->whole ? 0 : p->grid * (int64_t)sizeof(Desc));
     p->z = p->lse + (weights ? up(n_seq * heads * group * 4) : 0);
     p->bytes = p->z + (weights ? up(n_seq * heads * group * width * 4) : 0);
     return true;
@@ -1141,7 +1161,7 @@ void paged_launch(const PagedArgs& A, int grid, hipStream_t s) {
     if (A.group <= 4) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 4>), g, wg, lds, s, A);
     else if (A.group <= 8) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 8>), g, wg, lds, s, A);
     else hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 16>), g, wg, lds, s, A);
-    if (grid > 1) hipLaunchKernelGGL((k_paged_join<BF16, SUMS>), dim3((unsigned)grid, (unsigned)A.group), dim3(256), 0, s, A);
+    if (!A.whole) hipLaunchKernelGGL((k_paged_join<BF16, SUMS>), dim3((unsigned)grid, (unsigned)A.group), dim3(256), 0, s, A);
 }
 template <bool BF16, bool SUMS>
 void paged_launch(const PagedArgs& A, int grid, bool big, hipStream_t s) {
@@ -1193,6 +1213,7 @@ int lq_paged_attention(const lq_pages *k, const lq_pages *v, const lq_rows *q, i
     A.heads = (int)k->r.n_heads;
     A.group = group;
     A.per = (int)((n_seq + 63) / 64);
+    A.whole = p.whole;
     char* w = static_cast<char*>(d_work);
     A.rec = reinterpret_cast<float*>(w + p.rec);
     A.desc = reinterpret_cast<Desc*>(w + p.desc);

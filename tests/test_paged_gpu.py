@@ -163,6 +163,26 @@ def test_attention_and_weights(shape, dtype):
     assert bool(acc[~on].isnan().all())
 
 
+@pytest.mark.parametrize("width", [0, 1, 64])
+@pytest.mark.parametrize("shape", SHAPES[:9] + [(128, 4, 2, [i % 5 for i in range(128)], [i % 4 for i in range(128)]),
+                                                (129, 4, 2, [i % 5 for i in range(129)], [i % 4 for i in range(129)])],
+                         ids=lambda s: f"{s[0]}x{s[1]}x{s[2]}-{max(s[3])}")
+def test_tables_wider_than_the_lengths(shape, width):
+    """Short sequences whose table and tail would hold more: a workgroup's equal share of
+    the list instead of a whole (sequence, head)."""
+    B, H, G, counts, tails = shape
+    k, v, q, tab, cnt, tk, tv, tl = _case(B, H, G, counts, tails, torch.float16, 7 + B + H, max(tails) + 9 * width,
+                                          max(counts) + width)
+    want, tol, w, wtol = _reference(k, v, q, tab, counts, tk, tv, tails)
+    got = paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl)
+    assert bool(((got.double() - want).abs() <= tol).all())
+    want, tol, w, wtol = _reference(k, v, q, tab, counts, tk, tv, tails, rounded=True)
+    acc = torch.zeros(tab.shape, device="cuda")
+    got = paged_decode_attention(k, v, q, tab, cnt, tk, tv, tail_len=tl, weights=acc)
+    assert bool(((got.double() - want).abs() <= tol).all())
+    assert bool(((acc.double() - w).abs() <= w * (wtol + (H * G + 2) * 2.0 ** -24) + 1e-30).all())
+
+
 def test_weights_sum_to_the_heads():
     k, v, q, tab, cnt, *_ = _case(3, 4, 4, [40, 7, 129], [0, 0, 0], torch.float16, 3, cap=0)
     acc = torch.zeros(tab.shape, device="cuda")
