@@ -203,24 +203,24 @@ __device__ __forceinline__ void raw_pairs(uint32_t a, uint32_t b, uint32_t p[4])
     const uint32_t par = ((uint32_t)__builtin_popcount(a & kLsbMask) + u6) & 1u;
     p[3] = kc | (u6 << 1) | (((c7h << 1) | par) << 17);
 }
-template <int SH>   // both bytes, from bits SH and SH + 8 on
-__device__ __forceinline__ void raw_pairs_tok(uint32_t a0, uint32_t a1, uint32_t b, uint32_t p[8]) {
+template <int SH, int K>   // both bytes, from bits SH and SH + 8 on, into each dimension's pair K
+__device__ __forceinline__ void raw_pairs_tok(uint32_t a0, uint32_t a1, uint32_t b, u32x4_t p[8]) {
     const uint32_t lo = __builtin_amdgcn_perm(a1, a0, 0x05040100u);
     const uint32_t hi = __builtin_amdgcn_perm(a1, a0, 0x07060302u);
     const uint32_t kc = lo & 0x00010001u;
-    p[0] = (lo & kFieldMask) | kc;
-    p[2] = ((lo >> 5) & kFieldMask) | kc;
-    p[4] = ((lo >> 10) & kFieldMask) | kc;
-    p[1] = (hi & kFieldMask) | kc;
-    p[3] = ((hi >> 5) & kFieldMask) | kc;
-    p[5] = ((hi >> 10) & kFieldMask) | kc;
+    p[0][K] = (lo & kFieldMask) | kc;
+    p[2][K] = ((lo >> 5) & kFieldMask) | kc;
+    p[4][K] = ((lo >> 10) & kFieldMask) | kc;
+    p[1][K] = (hi & kFieldMask) | kc;
+    p[3][K] = ((hi >> 5) & kFieldMask) | kc;
+    p[5][K] = ((hi >> 10) & kFieldMask) | kc;
     const uint32_t u0 = (b >> SH) & 31u, u1 = (b >> (SH + 8)) & 31u;
     const uint32_t h0 = ((b >> (SH + 5)) & 7u) | ((a0 >> 13) & 8u);
     const uint32_t h1 = ((b >> (SH + 13)) & 7u) | ((a1 >> 13) & 8u);
     const uint32_t q0 = ((uint32_t)__builtin_popcount(a0 & kLsbMask) + u0) & 1u;
     const uint32_t q1 = ((uint32_t)__builtin_popcount(a1 & kLsbMask) + u1) & 1u;
-    p[6] = kc | (u0 << 1) | (u1 << 17);
-    p[7] = kc | (((h0 << 1) | q0) << 1) | (((h1 << 1) | q1) << 17);
+    p[6][K] = kc | (u0 << 1) | (u1 << 17);
+    p[7][K] = kc | (((h0 << 1) | q0) << 1) | (((h1 << 1) | q1) << 17);
 }
 // an entry's eight values 2c so (beyond 2048 they lose bits, as fp16 does), and as c
 __device__ __forceinline__ void raw_entry(const uint4& w, uint32_t p[4]) {
@@ -328,7 +328,7 @@ __device__ __forceinline__ float scale_log(const uint32_t s[4]) {
 // (lanes 0..31 hold the first page's tokens, 32..63 the second's).
 template <bool SUMS, bool ROUND, int NR>
 __device__ __forceinline__ float attend(const f4_t s[2], const uint32_t ks[4], const uint32_t vs[4], uint32_t word,
-                                        const uint32_t vp[4][8], int lane, PageState& st) {
+                                        const u32x4_t vq[8], int lane, PageState& st) {
     constexpr int N = 2 * kPairs<NR>;          // tokens that the lane weighs
     float z[N];
 #pragma unroll
@@ -395,8 +395,7 @@ __device__ __forceinline__ float attend(const f4_t s[2], const uint32_t ks[4], c
     const h8_t pb = as_h8(p[0], p[1], p[2], p[3]);
 #pragma unroll
     for (int mm = 0; mm < 8; mm++)
-        st.o[mm] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(vp[0][mm], vp[1][mm], vp[2][mm], vp[3][mm]), pb, st.o[mm],
-                                                          0, 0, 0);
+        st.o[mm] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, vq[mm]), pb, st.o[mm], 0, 0, 0);
     return SUMS ? __builtin_amdgcn_logf(pair_sum(shares_sum<NR>(sum))) - off + kPShift : 0.f;
 }
 
@@ -565,7 +564,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                 for (int tile = t; tile < pe; tile++) {
                     const uint32_t word = 2 * tile + 1 < L.pages ? ~0u : 0xffffu;
                     f4_t s[2] = {s0, s0};
-                    uint32_t vp[4][8], p[8][4];
+                    uint32_t p[8][4];
+                    u32x4_t vq[8];             // of V: vector lane % 16's dimension, four pairs of tokens
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         const uint32_t ra = j & 1 ? rd.ka[j >> 1].y : rd.ka[j >> 1].x, rb = rd.kb[j >> 1];
@@ -620,32 +620,26 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                     {
                         const uint32_t aw[8] = {rd.va[0].x, rd.va[0].y, rd.va[0].z, rd.va[0].w,
                                                 rd.va[1].x, rd.va[1].y, rd.va[1].z, rd.va[1].w};
-                        raw_pairs_tok<0>(aw[0], aw[1], rd.vb.x, vp[0]);
-                        raw_pairs_tok<16>(aw[2], aw[3], rd.vb.x, vp[1]);
-                        raw_pairs_tok<0>(aw[4], aw[5], rd.vb.y, vp[2]);
-                        raw_pairs_tok<16>(aw[6], aw[7], rd.vb.y, vp[3]);
+                        raw_pairs_tok<0, 0>(aw[0], aw[1], rd.vb.x, vq);
+                        raw_pairs_tok<16, 1>(aw[2], aw[3], rd.vb.x, vq);
+                        raw_pairs_tok<0, 2>(aw[4], aw[5], rd.vb.y, vq);
+                        raw_pairs_tok<16, 3>(aw[6], aw[7], rd.vb.y, vq);
                     }
                     if (const uint32_t most = most_of(mv)) {
 #pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            area[64 * j + lane] = u32x4_t{vp[j >> 1][4 * (j & 1)], vp[j >> 1][4 * (j & 1) + 1],
-                                                          vp[j >> 1][4 * (j & 1) + 2], vp[j >> 1][4 * (j & 1) + 3]};
+                        for (int j = 0; j < 8; j++) area[64 * j + lane] = vq[j];
                         wave_lds_sync();
                         each_entry<BIG>(A.v, mv, ev, most, lane, [&](uint32_t rec, const uint4& v) __attribute__((always_inline)) {
                             uint32_t e[4];
                             raw_entry(v, e);
-                            const uint32_t tok = 16 * (lane >> 5) + (rec & 15);   // pair (tok / 2) % 4 of lane vector + 16 (tok / 8)
-                            uint16_t* w = reinterpret_cast<uint16_t*>(area + 64 * (tok & 6) + 16 * (tok >> 3) + (rec >> 4)) + (tok & 1);
+                            const uint32_t tok = 16 * (lane >> 5) + (rec & 15);
+                            uint16_t* w = reinterpret_cast<uint16_t*>(area + 16 * (tok >> 3) + (rec >> 4)) + (tok & 7);
 #pragma unroll
-                            for (int i = 0; i < 8; i++) w[(i & 4) * 128 + (i & 3) * 2] = (uint16_t)(i & 1 ? e[i >> 1] >> 16 : e[i >> 1]);
+                            for (int i = 0; i < 8; i++) w[512 * i] = (uint16_t)(i & 1 ? e[i >> 1] >> 16 : e[i >> 1]);
                         });
                         wave_lds_sync();
 #pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const u32x4_t w = area[64 * j + lane];
-#pragma unroll
-                            for (int i = 0; i < 4; i++) vp[j >> 1][4 * (j & 1) + i] = w[i];
-                        }
+                        for (int j = 0; j < 8; j++) vq[j] = area[64 * j + lane];
                         wave_lds_sync();
                     }
                     if (__any(lane_scale<NR>(rd.vs) > largest)) {
@@ -670,7 +664,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                     blocks(tile + 2);
                     nk = load_meta<BIG>(A.k, x1, y1, lane);
                     nv = load_meta<BIG>(A.v, x1, y1, lane);
-                    const float z = attend<SUMS, ROUND, NR>(s, ks, vs, word, vp, lane, ps);
+                    const float z = attend<SUMS, ROUND, NR>(s, ks, vs, word, vq, lane, ps);
                     if (SUMS) {
                         const int j = 2 * tile + (lane >> 5);
                         if (!(g & 1) && col < G && j < L.pages) A.z[((int64_t)unit * A.width + j) * G + col] = z;
@@ -701,14 +695,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                         const int tok = min(8 * (col >> 2) + 2 * (col & 3) + y, have - 1);
                         w[y][c] = *reinterpret_cast<const uint4*>(p + (t0 + tok) * A.tk.st + 32 * c + 8 * g);
                     }
+                __builtin_amdgcn_sched_barrier(0);
+                rows_v<BF16>(A.tv.p + b * A.tv.sb + h * A.tv.sh, A.tv.st, t0, have, word, lane, vp);
 #pragma unroll
                 for (int y = 0; y < 2; y++)
 #pragma unroll
                     for (int c = 0; c < 4; c++)
                         s[y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                             __builtin_bit_cast(h8_t, BF16 ? bf_to_h(w[y][c]) : w[y][c]), q[c], s[y], 0, 0, 0);
-                __builtin_amdgcn_sched_barrier(0);       // K's rows leave their registers before V's come
-                rows_v<BF16>(A.tv.p + b * A.tv.sb + h * A.tv.sh, A.tv.st, t0, have, word, lane, vp);
                 const float was = st.m;
                 few_attend(s, word, word == ~0u, vp, lane, st);
                 if (SUMS) {                    // few_attend's sum is of the rounded weights: these few again
