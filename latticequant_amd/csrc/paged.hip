@@ -40,6 +40,11 @@ constexpr int kGroups = 512;                   // workgroups at most
 // (11.5 / 13.2 / 18.2), the host's time for the launch not counted; 128 sequences, two
 // rounds: 20 tiles 35.5 (31.0).
 constexpr int kWhole = 20;
+// A unit's first tile waits for its page numbers, records and exceptions in turn and its tail
+// for its rows, which took about two tiles' time: the list has two places for that before each
+// unit's tiles.  32 sequences up to 2048 tokens 24.1 -> 21.6 us, 64 up to 8192 with weights
+// 112.7 -> 104.6 (one place: 22.2 and 106.8, four: 21.8 and 106.8).
+constexpr int kAhead = 2;
 constexpr int kMRow = kHd + 4;                 // floats of a piece's row in LDS: o[128], m, l, l32
 constexpr int kRecF = 4 + kHd;                 // floats of a record's row: m, l, l32, unused, o[128]
 constexpr int kPatch = 8 * 64 * 16;            // bytes of a wave's area for exceptions
@@ -65,6 +70,7 @@ struct PagedArgs {
     int64_t ob, oh;
     int n_seq, heads, group, per;              // per: sequences of a lane's sum
     int whole;                                 // a workgroup a unit, instead of equal shares
+    int ahead;                                 // places of the list that a unit has before its tiles'
     float* rec;                                // [2 workgroup + (0: of an earlier one's, 1: begun here)][row][kRecF]
     Desc* desc;
     float* lse;                                // [unit][row]: m + log2(l32), with the weights' factor 2^kPShift
@@ -73,6 +79,7 @@ struct PagedArgs {
 
 struct Len {
     int pages, tail, tiles, page_tiles;
+    uint32_t places;                           // of the list, for a head
 };
 __device__ __forceinline__ Len len_of(const PagedArgs& A, int b) {
     Len l;
@@ -80,6 +87,7 @@ __device__ __forceinline__ Len len_of(const PagedArgs& A, int b) {
     l.tail = A.tail_cap ? (A.tail_len ? min(max(A.tail_len[b], 0), (int)A.tail_cap) : (int)A.tail_cap) : 0;
     l.page_tiles = (l.pages + 1) >> 1;
     l.tiles = l.page_tiles + ((l.tail + 31) >> 5);
+    l.places = l.tiles ? (uint32_t)(l.tiles + A.ahead) : 0u;
     return l;
 }
 
@@ -428,6 +436,7 @@ __device__ __forceinline__ Len len_at(const PagedArgs& A, const Lens& mine, int 
     l.tail = __builtin_amdgcn_readlane(mine.tail, b);
     l.page_tiles = (l.pages + 1) >> 1;
     l.tiles = l.page_tiles + ((l.tail + 31) >> 5);
+    l.places = l.tiles ? (uint32_t)(l.tiles + A.ahead) : 0u;
     return l;
 }
 template <bool BF16, bool SUMS, bool BIG, int NR>
@@ -450,7 +459,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
     for (int b = lane * A.per; b < min((lane + 1) * A.per, A.n_seq); b++) {
         const Len l = len_of(A, b);
         lens = {l.pages, l.tail};
-        own += (uint32_t)l.tiles * A.heads;
+        own += l.places * A.heads;
     }
     uint32_t upto = own;
 #pragma unroll
@@ -464,25 +473,28 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
     for (int b = blockIdx.x; b < A.n_seq; b += gridDim.x)
         if (len_at(A, lens, b).tiles == 0) zero_out(A, b, tid);
     const uint32_t me = blockIdx.x;
-    uint32_t groups = gridDim.x, lo, hi;
+    uint32_t lo, hi, share = 0, longer = 0;    // the first `longer` workgroups have one place more
     if (A.whole) {
         const int b = (int)(me / (uint32_t)A.heads);
-        const uint32_t tiles = (uint32_t)len_at(A, lens, b).tiles;
+        const uint32_t places = len_at(A, lens, b).places;
         lo = (uint32_t)__builtin_amdgcn_readlane((int)before, b / A.per);
-        for (int k = b / A.per * A.per; k < b; k++) lo += (uint32_t)len_at(A, lens, k).tiles * A.heads;
-        lo += (me - (uint32_t)b * A.heads) * tiles;
-        hi = lo + tiles;
+        for (int k = b / A.per * A.per; k < b; k++) lo += len_at(A, lens, k).places * A.heads;
+        lo += (me - (uint32_t)b * A.heads) * places;
+        hi = lo + places;
     } else {
-        groups = max(1u, min(groups, (total + kWaves - 1) / kWaves));
+        const uint32_t groups = max(1u, min((uint32_t)gridDim.x, (total + kWaves - 1) / kWaves));
         if (me >= groups) {
             if (tid == 0) A.desc[me] = {-1, 0};
             return;
         }
-        lo = (uint32_t)((uint64_t)me * total / groups);
-        hi = (uint32_t)((uint64_t)(me + 1) * total / groups);
+        share = total / groups;
+        longer = total % groups;
+        lo = me * share + min(me, longer);
+        hi = lo + share + (me < longer ? 1u : 0u);
     }
-    uint32_t pos = lo + (uint32_t)((uint64_t)(hi - lo) * wave / kWaves);
-    const uint32_t end = lo + (uint32_t)((uint64_t)(hi - lo) * (wave + 1) / kWaves);
+    const uint32_t part = (hi - lo) / kWaves, rest = (hi - lo) % kWaves;
+    uint32_t pos = lo + wave * part + min((uint32_t)wave, rest);
+    const uint32_t end = pos + part + ((uint32_t)wave < rest ? 1u : 0u);
 
     if (pos < end) {
         const uint64_t there = __ballot(pos >= before && pos - before < own);
@@ -491,16 +503,19 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
         int b = from * A.per;
         Len L = len_at(A, lens, b);
         for (int k = 1; k < A.per; k++) {
-            const uint32_t n = (uint32_t)L.tiles * A.heads;
+            const uint32_t n = L.places * A.heads;
             if (rem < n || b + 1 >= A.n_seq) break;
             rem -= n;
             L = len_of(A, ++b);
         }
-        const uint32_t tiles = (uint32_t)max(L.tiles, 1);
-        int h = (int)(rem / tiles), t = (int)(rem % tiles);
+        const uint32_t places = max(L.places, 1u);
+        int h = (int)(rem / places);
+        uint32_t place = rem % places;         // within the unit
         for (;;) {
             const int unit = b * A.heads + h;
-            const int n = (int)min((uint32_t)(L.tiles - t), end - pos);
+            const uint32_t take = min(L.places - place, end - pos);
+            const int t = max((int)place - A.ahead, 0), n = max((int)(place + take) - A.ahead, 0) - t;
+            if (n == 0) break;                 // the share ends before the unit's tiles
             h8_t q[4];
 #pragma unroll
             for (int c = 0; c < 4; c++) {
@@ -750,12 +765,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                     const int i = 2 * wave + (ends ? 0 : 1);
                     s_unit[i] = unit;
                     s_begins[i] = t == 0;
-                    if (!ends && pos + n == hi) s_end = pos + (uint32_t)(L.tiles - t);
+                    if (!ends && pos + take == hi) s_end = pos + L.places - place;
                 }
             }
-            pos += n;
+            pos += take;
             if (pos == end) break;
-            t = 0;
+            place = 0;
             if (++h == A.heads) {
                 h = 0;
                 do {
@@ -810,7 +825,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                 *reinterpret_cast<f4_t*>(rec + 8 + d) = f4_t{x[4], x[5], x[6], x[7]};
                 if (d == 0) *reinterpret_cast<f4_t*>(rec) = f4_t{m, l, l32, 0.f};
             }
-            if (begins) left = {unit, (int32_t)(((uint64_t)s_end * groups - 1) / total - me)};
+            if (begins) {                      // the workgroup that has the unit's last place
+                const uint32_t at = s_end - 1, split = longer * (share + 1);
+                left = {unit, (int32_t)((at < split ? at / (share + 1) : longer + (at - split) / share) - me)};
+            }
         }
     }
     if (tid == 0 && !A.whole) A.desc[me] = left;
@@ -818,10 +836,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
 
 // The records of a unit that several workgroups share, a workgroup per row: thread
 // (sub, dq) sums dimensions 4 dq .. + 3 of records sub, sub + 8, .., then the eight sums
-// are joined in order.
+// are joined in order.  Most workgroups find no unit: within 64 registers all are resident
+// at once (2048 in two rounds, seven a compute unit: 8.0 us for 6.3).
 template <bool BF16, bool SUMS>
-__global__ __launch_bounds__(256) void k_paged_join(PagedArgs A) {
-    constexpr int kUp = 8;                     // records in flight per thread
+__global__ __launch_bounds__(256, 8) void k_paged_join(PagedArgs A) {
+    constexpr int kUp = 4;                     // records in flight per thread
     __shared__ __align__(16) f4_t s_o[8][32];
     __shared__ float s_m[8], s_l[8], s_l32[8];
     const int dq = threadIdx.x & 31, sub = threadIdx.x >> 5, row = blockIdx.y, wg = blockIdx.x;
@@ -871,7 +890,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs A) {
 #pragma unroll
     for (int k = 0; k < 8; k++) M = fmaxf(M, s_m[k]);
     float L = 0.f, L32 = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll 2
     for (int k = 0; k < 8; k++) {
         const float f = s_m[k] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[k] - M);
         const f4_t u = s_o[k][2 * lane], v = s_o[k][2 * lane + 1];
@@ -1124,7 +1143,7 @@ bool plan(int64_t n_seq, int64_t heads, int64_t group, int64_t width, int64_t ta
         tail_cap > INT_MAX / 64 || n_seq > 65535 || heads > 65535 || n_seq * heads > INT_MAX / 16)
         return false;
     const int64_t tiles = (width + 1) / 2 + (tail_cap + 31) / 32;
-    if (tiles > INT_MAX / (n_seq * heads)) return false;
+    if (tiles + kAhead > INT_MAX / (n_seq * heads)) return false;
     const int64_t most = (n_seq * heads * tiles + kWaves - 1) / kWaves;
     p->whole = tiles <= kWhole && n_seq * heads <= kGroups;
     p->grid = (int)(p->whole ? n_seq * heads : most < kGroups ? most : kGroups);
@@ -1208,6 +1227,7 @@ int lq_paged_attention(const lq_pages *k, const lq_pages *v, const lq_rows *q, i
     A.group = group;
     A.per = (int)((n_seq + 63) / 64);
     A.whole = p.whole;
+    A.ahead = p.whole ? 0 : kAhead;
     char* w = static_cast<char*>(d_work);
     A.rec = reinterpret_cast<float*>(w + p.rec);
     A.desc = reinterpret_cast<Desc*>(w + p.desc);
