@@ -52,14 +52,15 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
             x = x.reshape(-1, V)
         n = x.shape[0]
         both = torch.empty((2,) + shape, dtype=torch.float32, device=dev)
+        logprob, entropy = both.unbind()
         ids = tops = None
         if top:
             ids = torch.empty(shape + (top,), dtype=torch.int64, device=dev)
-            tops = torch.empty(shape + (top,), dtype=torch.float32, device=dev)
+            tops = both.new_empty(shape + (top,))
         if n:
             tok = None if tokens is None else tokens.contiguous()
             at = both.data_ptr()
             L.check(lib.lq_token_logprobs(x.data_ptr(), L.dtype_code(x.dtype), x.stride(0), n, V,
                                           None if tok is None else tok.data_ptr(), top, at, at + 4 * n, L.ptr(ids),
                                           L.ptr(tops), L.raw_stream(dev)), "lq_token_logprobs")
-    return TokenLogprobs(both[0], both[1], ids, tops)
+    return TokenLogprobs(logprob, entropy, ids, tops)
