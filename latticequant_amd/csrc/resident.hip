@@ -169,10 +169,10 @@ __global__ __launch_bounds__(256) void k_res_scan(const uint32_t* __restrict__ c
     if (tid == 255) *r.n_exc = (int32_t)(start + part[255]);
 }
 
-// exception entries: the vectors flagged by quant_block, recomputed
+// exception entries: the vectors flagged by quant_block, recomputed; `room` of them at most
 __device__ __forceinline__ void fill_block(const void* __restrict__ x, int dtype, int64_t T,
                                            const float* __restrict__ scale32, const lq_resident& r, int64_t hh,
-                                           int64_t bb, int64_t rb, uint8_t* __restrict__ rec = nullptr) {
+                                           int64_t bb, int64_t rb, int room = 256, uint8_t* __restrict__ rec = nullptr) {
     const int tid = threadIdx.x, grp = tid >> 6, slot = tid & 63;
     const unsigned long long m0 = r.mask[rb * 4 + 0], m1 = r.mask[rb * 4 + 1], m2 = r.mask[rb * 4 + 2],
                              m3 = r.mask[rb * 4 + 3];
@@ -184,6 +184,7 @@ __device__ __forceinline__ void fill_block(const void* __restrict__ x, int dtype
     if (grp > 1) before += __popcll(m1);
     if (grp > 2) before += __popcll(m2);
     before += __popcll(m & ((1ull << slot) - 1ull));
+    if (before >= room) return;
     const int64_t idx = (int64_t)r.meta[rb * 4 + 2] + before;
     if (idx >= r.exc_cap) {
         atomicOr(r.status, LQ_RES_ST_EXC_OVERFLOW);
@@ -308,14 +309,15 @@ __global__ __launch_bounds__(1024) void k_page_rooms(PageMap P, int64_t units, l
         __syncthreads();
         run = s_run;
     }
-    if (tid == 0) *r.n_exc = (int32_t)run;
+    if (tid == 0) *r.n_exc = (int32_t)min(run, (uint32_t)INT_MAX);
 }
 
 __global__ __launch_bounds__(256) void k_page_fill(const void* __restrict__ x, int dtype, PageMap P,
                                                    const float* __restrict__ scale32, lq_resident r,
-                                                   uint8_t* __restrict__ rec) {
+                                                   const int32_t* __restrict__ room, uint8_t* __restrict__ rec) {
     const int64_t hh = blockIdx.x / (uint32_t)P.per, bb = blockIdx.x % (uint32_t)P.per, rb = P.block(r, hh, bb);
-    if (rb >= 0) fill_block(x, dtype, P.per * kRB, scale32, r, hh, bb, rb, rec);
+    // (the masks of a page that stands twice may be of both, with more exceptions than either has)
+    if (rb >= 0) fill_block(x, dtype, P.per * kRB, scale32, r, hh, bb, rb, room[rb], rec);
 }
 
 __global__ __launch_bounds__(256) void k_page_dequant(lq_resident r, PageMap P, void* __restrict__ out, int out_dtype) {
@@ -1081,7 +1083,7 @@ int lq_page_quantize(const void *d_x, int dtype, int64_t n, int64_t t_tokens, co
     const PageMap P = {d_pages, r.n_heads, per};
     hipLaunchKernelGGL(k_page_quant, dim3((unsigned)units), dim3(256), 0, s, d_x, dtype, P, d_scale32, d_scale16, r);
     hipLaunchKernelGGL(k_page_rooms, dim3(1), dim3(1024), 0, s, P, units, r, p->room);
-    hipLaunchKernelGGL(k_page_fill, dim3((unsigned)units), dim3(256), 0, s, d_x, dtype, P, d_scale32, r, p->rec);
+    hipLaunchKernelGGL(k_page_fill, dim3((unsigned)units), dim3(256), 0, s, d_x, dtype, P, d_scale32, r, p->room, p->rec);
     return launch_status();
 }
 

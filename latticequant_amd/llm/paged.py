@@ -304,7 +304,8 @@ def evict_pages(pages: torch.Tensor, n_pages: torch.Tensor, weights: torch.Tenso
             for t, like in zip(out, (tab, cnt, w, tab)):
                 if t.shape != like.shape or t.dtype is not like.dtype or t.device != dev or not t.is_contiguous():
                     raise ValueError("out must be an Eviction of the same shapes and device")
-            if len({t.data_ptr() for t in (*out, tab, cnt, w)}) != 7 and W:
+            spans = sorted((t.data_ptr(), t.nbytes) for t in (*out, tab, cnt, w))
+            if any(at + size > behind for (at, size), (behind, _) in zip(spans, spans[1:])) and W:
                 raise ValueError("out must be apart from the inputs")
         if W == 0:
             out.n_pages.zero_()

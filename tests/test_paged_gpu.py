@@ -309,6 +309,28 @@ def test_pages_written_again_keep_their_room():
     assert int(p.pool.room.max()) <= 256
 
 
+@pytest.mark.parametrize("loud", [(1, 9), (3, 3), (40, 2)])
+def test_a_page_that_stands_twice_leaves_the_others(loud):
+    p = _pool(2, 12, 60, loud=3)
+    every = torch.arange(12, device="cuda")[:, None]
+    x, s = _rows(12, 2, PAGE, 61, loud=loud[0])
+    p.write(x, every, s, s.half())
+    before = p.read(every)
+    for i in range(3):
+        x, s = _rows(4, 2, PAGE, 62 + i, loud=loud[1])
+        x[1:, :, i::2] /= 8                                # exceptions in other places
+        p.write(x, torch.tensor([[7], [7], [7], [2]], device="cuda"), s, s.half())
+        after = p.read(every)
+        others = [j for j in range(12) if j != 7 and j != 2]
+        assert torch.equal(after[others], before[others])
+        fresh = PagedKV(2, 1, device="cuda")
+        fresh.write(x[3:], torch.zeros(1, 1, dtype=torch.int64, device="cuda"), s[3:], s[3:].half())
+        assert torch.equal(after[2], fresh.read(torch.zeros(1, 1, dtype=torch.int64, device="cuda"))[0])
+    p.write(x[:1], torch.tensor([[7]], device="cuda"), s[:1], s[:1].half())
+    fresh.write(x[:1], torch.zeros(1, 1, dtype=torch.int64, device="cuda"), s[:1], s[:1].half())
+    assert torch.equal(p.read(every)[7], fresh.read(torch.zeros(1, 1, dtype=torch.int64, device="cuda"))[0])
+
+
 def test_many_exceptions_lengthen_the_list():
     """Every vector an exception, more of them than the list has room for; neighbours keep
     theirs."""
@@ -427,6 +449,10 @@ def test_refusals_on_the_device():
     ev = evict_pages(tab, cnt, torch.zeros(2, 4, device="cuda"), 2)
     with pytest.raises(ValueError, match="apart"):
         evict_pages(ev.pages, ev.n_pages, ev.weights, 1, out=ev)
+    raw = torch.zeros(20, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="apart"):         # one after the other, overlapping
+        evict_pages(raw[2:10].view(2, 4), cnt, torch.zeros(2, 4, device="cuda"), 2,
+                    out=ev._replace(pages=raw[:8].view(2, 4)))
     with pytest.raises(ValueError, match="stands twice"):
         k.write(torch.zeros(1, 2, 32, HD, device="cuda"), torch.tensor([[1, 1]]))
     x = torch.zeros(1, 2, 16, HD, device="cuda", dtype=torch.float16)
