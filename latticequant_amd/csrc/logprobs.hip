@@ -510,8 +510,12 @@ void launch(const LogArgs& A, int64_t rows, hipStream_t s) {
 }
 template <int DT>
 void launch(const LogArgs& A, int64_t rows, hipStream_t s) {
-    // few rows: a compute unit reads its row as fast as sixteen waves ask for it
-    if (rows < 1024 && A.vocab > 4096) launch<DT, 16>(A, rows, s);
+    // Few rows: a compute unit reads its row as fast as sixteen waves ask for it; with
+    // alternatives only one row at a time, by what the waves' queues take of LDS.  bf16, sixteen waves
+    // against four, without / with 5 alternatives: 64 x 8192 5.3 / 11.1 us (4.3 / 7.5),
+    // 64 x 32000 5.6 / 11.2 (7.8 / 13.0), 256 x 128256 16.3 / 23.3 (23.4 / 36.0), 512 x 128256
+    // 25.3 / 42.6 (27.1 / 39.7), 2048 x 128256 88 / 155 (87 / 102).
+    if (A.vocab > 16384 && rows <= (A.top ? 256 : 1024)) launch<DT, 16>(A, rows, s);
     else launch<DT, 4>(A, rows, s);
 }
 

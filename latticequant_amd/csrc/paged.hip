@@ -964,11 +964,13 @@ constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64, kBins = 20
 
 // The room-th largest weight of a sequence's pages that may go, by a radix search of 11, 11
 // and 10 bits (that ends where all of a bin stay), then one pass in the order of the pages,
-// each wave a part of them.  A sequence of up to 16384 pages is a workgroup's, N of them a
+// each wave a part of them.  A sequence of up to 8192 pages is a workgroup's, N of them a
 // lane in registers, read once.  Longer ones (N = 0) are searched by `parts` workgroups each
 // of which looks at all of it and writes its part: the search is repeated on compute units
-// that would idle (4 sequences of 65536 pages, alone in its workgroup each: 80 us).
-// Bound by latency with few pages, by instructions with many.
+// that would idle (4 sequences of 65536 pages: 41 us, one workgroup each 80).  1 / 64 / 256
+// tables of 8192 pages 13.8 / 17.0 / 19.5 us (N = 0: 15.7 / 16.9 / 20.4), of 16384 with 16 a
+// lane 21.2 / 26.0 / 29.6 (20.9 / 23.0 / 31.0).  Bound by latency with few pages (1024: 5.4 us),
+// by instructions with many.
 template <int N>
 __global__ __launch_bounds__(kEvictThreads) void k_evict(EvictArgs A, int parts) {
     __shared__ uint32_t s_bin[kBins];
@@ -1265,8 +1267,8 @@ int lq_evict_pages(const int32_t *d_pages, const int32_t *d_n_pages, const float
         hipLaunchKernelGGL(k_evict<1>, grid, wg, 0, s, A, 1);
     } else if (max_pages <= 4 * kEvictThreads) {
         hipLaunchKernelGGL(k_evict<4>, grid, wg, 0, s, A, 1);
-    } else if (max_pages <= 16 * kEvictThreads) {
-        hipLaunchKernelGGL(k_evict<16>, grid, wg, 0, s, A, 1);
+    } else if (max_pages <= 8 * kEvictThreads) {
+        hipLaunchKernelGGL(k_evict<8>, grid, wg, 0, s, A, 1);
     } else {
         int64_t parts = max_pages / (4 * kEvictThreads);
         if (parts > 256 / n_seq) parts = 256 / n_seq;

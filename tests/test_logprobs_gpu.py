@@ -44,7 +44,8 @@ def _check(x, tok, top, got):
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (1, 2, 0), (3, 7, 7), (2, 64, 64), (5, 65, 20), (1, 8191, 5),
                                             (4, 8193, 1), (1, 32000, 5), (37, 50021, 3), (1, 200003, 64), (7, 4096, 33),
-                                            (300, 1000, 10), (1030, 513, 2), (2, 131072, 0)])
+                                            (300, 1000, 10), (1030, 513, 2), (2, 131072, 0), (256, 16400, 7), (257, 16400, 3),
+                                            (300, 20000, 0), (1025, 16387, 0)])
 def test_rows(rows, vocab, top, dtype):
     g = torch.Generator(device="cuda").manual_seed(rows * 7 + vocab)
     x = (torch.randn(rows, vocab, generator=g, device="cuda") * 4).to(dtype)
@@ -63,10 +64,11 @@ def test_orders(order, dtype):
     _check(x, tok, 64, token_logprobs(x, tok, 64))
 
 
+@pytest.mark.parametrize("vocab", [3001, 40009])
 @pytest.mark.parametrize("dtype", DT)
-def test_masks_and_values_that_are_not_finite(dtype):
+def test_masks_and_values_that_are_not_finite(dtype, vocab):
     low = torch.finfo(dtype).min
-    x = torch.randn(9, 3001, device="cuda").to(dtype)
+    x = torch.randn(9, vocab, device="cuda").to(dtype)
     x[0, 10:] = -float("inf")
     x[1] = -float("inf")
     x[2, 5] = float("nan")
@@ -75,8 +77,8 @@ def test_masks_and_values_that_are_not_finite(dtype):
     x[5] = low
     x[6] = -low
     x[7, 3] = -low
-    x[8, :3000] = -float("inf")
-    tok = torch.tensor([3, 3, 3, 3, 200, 5, 5, 3, 3000], device="cuda")
+    x[8, :-1] = -float("inf")
+    tok = torch.tensor([3, 3, 3, 3, 200, 5, 5, 3, vocab - 1], device="cuda")
     got = token_logprobs(x, tok, 12)
     for r in (0, 1, 2, 5, 6, 8):
         _check(x[r:r + 1], tok[r:r + 1], 12, type(got)(*(t[r:r + 1] for t in got)))
