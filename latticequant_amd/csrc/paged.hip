@@ -55,8 +55,11 @@ struct Rows {
     int64_t sb, sh, st;
 };
 
-struct Desc {                                  // the (sequence, head) that a workgroup leaves unfinished
-    int32_t unit, more;                        // -1: none; the workgroups that follow it there
+// A unit: the sequence's number and the head's (of at most 65535 each), none: ~0.
+__device__ __forceinline__ uint32_t unit_of(int b, int h) { return (uint32_t)b << 16 | (uint32_t)h; }
+struct Desc {                                  // the unit that a workgroup leaves unfinished
+    uint32_t unit;
+    int32_t more;                              // the workgroups that follow it there
 };
 
 struct PagedArgs {
@@ -414,15 +417,19 @@ __device__ __forceinline__ void zero_out(const PagedArgs& A, int b, int tid) {
 }
 
 template <bool BF16>
-__device__ __forceinline__ void put8(const PagedArgs& A, int unit, int row, int d, const float x[8], float inv) {
+__device__ __forceinline__ void put8(const PagedArgs& A, uint32_t unit, int row, int d, const float x[8], float inv) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float u = x[2 * i] * inv, v = x[2 * i + 1] * inv;
         w[i] = BF16 ? (uint32_t)f2bf(u) | ((uint32_t)f2bf(v) << 16) : pair_h(u, v);
     }
-    const int b = unit / A.heads, h = unit % A.heads;
+    const int b = (int)(unit >> 16), h = (int)(unit & 0xffffu);
     *reinterpret_cast<uint4*>(A.out + b * A.ob + (int64_t)(h * A.group + row) * A.oh + d) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ int64_t lse_at(const PagedArgs& A, uint32_t unit, int row) {
+    return ((int64_t)(unit >> 16) * A.heads + (unit & 0xffffu)) * A.group + row;
 }
 
 // The lengths of up to 64 sequences, one a lane (per == 1), or from memory.
@@ -444,7 +451,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
     constexpr bool ROUND = SUMS;
     extern __shared__ __align__(16) char s_dyn[];
     // pieces in the order of the list: wave w's first (2 w), which ends its unit there, and its last (2 w + 1)
-    __shared__ int s_unit[2 * kWaves], s_begins[2 * kWaves];
+    __shared__ uint32_t s_unit[2 * kWaves];
+    __shared__ int s_begins[2 * kWaves];
     __shared__ uint32_t s_end;                 // where the list's unit that is begun here and not ended ends
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4, G = A.group;
@@ -453,38 +461,40 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
     char* mine = s_dyn + wave * stride;        // exceptions, then the wave's last piece; behind it its first
     u32x4_t* area = reinterpret_cast<u32x4_t*>(mine);
 
+    if (tid < 2 * kWaves) s_unit[tid] = ~0u;
     // ---- the workgroup's share of the list, found by every wave for itself
-    Lens lens = {0, 0};
-    uint32_t own = 0;
-    for (int b = lane * A.per; b < min((lane + 1) * A.per, A.n_seq); b++) {
-        const Len l = len_of(A, b);
-        lens = {l.pages, l.tail};
-        own += l.places * A.heads;
-    }
-    uint32_t upto = own;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t x = __shfl_up(upto, o, 64);
-        upto += lane >= o ? x : 0u;
-    }
-    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63), before = upto - own;
-    if (tid < 2 * kWaves) s_unit[tid] = -1;
-    __syncthreads();
-    for (int b = blockIdx.x; b < A.n_seq; b += gridDim.x)
-        if (len_at(A, lens, b).tiles == 0) zero_out(A, b, tid);
-    const uint32_t me = blockIdx.x;
     uint32_t lo, hi, share = 0, longer = 0;    // the first `longer` workgroups have one place more
+    Lens lens = {0, 0};
+    uint32_t own = 0, before = 0;
+    int b = 0, h = 0;
+    Len L;
+    const uint32_t me = blockIdx.x;
     if (A.whole) {
-        const int b = (int)(me / (uint32_t)A.heads);
-        const uint32_t places = len_at(A, lens, b).places;
-        lo = (uint32_t)__builtin_amdgcn_readlane((int)before, b / A.per);
-        for (int k = b / A.per * A.per; k < b; k++) lo += len_at(A, lens, k).places * A.heads;
-        lo += (me - (uint32_t)b * A.heads) * places;
-        hi = lo + places;
+        b = blockIdx.y;
+        h = blockIdx.x;
+        L = len_of(A, b);
+        lo = 0;
+        hi = L.places;
+        if (hi == 0 && h == 0) zero_out(A, b, tid);
     } else {
+        for (int i = lane * A.per; i < min((lane + 1) * A.per, A.n_seq); i++) {
+            const Len l = len_of(A, i);
+            lens = {l.pages, l.tail};
+            own += l.places * A.heads;
+        }
+        uint32_t upto = own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t x = __shfl_up(upto, o, 64);
+            upto += lane >= o ? x : 0u;
+        }
+        const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+        before = upto - own;
+        for (int i = blockIdx.x; i < A.n_seq; i += gridDim.x)
+            if (len_at(A, lens, i).tiles == 0) zero_out(A, i, tid);
         const uint32_t groups = max(1u, min((uint32_t)gridDim.x, (total + kWaves - 1) / kWaves));
         if (me >= groups) {
-            if (tid == 0) A.desc[me] = {-1, 0};
+            if (tid == 0) A.desc[me] = {~0u, 0};
             return;
         }
         share = total / groups;
@@ -492,27 +502,31 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
         lo = me * share + min(me, longer);
         hi = lo + share + (me < longer ? 1u : 0u);
     }
+    __syncthreads();
     const uint32_t part = (hi - lo) / kWaves, rest = (hi - lo) % kWaves;
     uint32_t pos = lo + wave * part + min((uint32_t)wave, rest);
     const uint32_t end = pos + part + ((uint32_t)wave < rest ? 1u : 0u);
 
     if (pos < end) {
-        const uint64_t there = __ballot(pos >= before && pos - before < own);
-        const int from = __ffsll((long long)there) - 1;
-        uint32_t rem = pos - (uint32_t)__builtin_amdgcn_readlane((int)before, from);
-        int b = from * A.per;
-        Len L = len_at(A, lens, b);
-        for (int k = 1; k < A.per; k++) {
-            const uint32_t n = L.places * A.heads;
-            if (rem < n || b + 1 >= A.n_seq) break;
-            rem -= n;
-            L = len_of(A, ++b);
+        uint32_t place = pos;                  // within the unit
+        if (!A.whole) {
+            const uint64_t there = __ballot(pos >= before && pos - before < own);
+            const int from = __ffsll((long long)there) - 1;
+            uint32_t rem = pos - (uint32_t)__builtin_amdgcn_readlane((int)before, from);
+            b = from * A.per;
+            L = len_at(A, lens, b);
+            for (int k = 1; k < A.per; k++) {
+                const uint32_t n = L.places * A.heads;
+                if (rem < n || b + 1 >= A.n_seq) break;
+                rem -= n;
+                L = len_of(A, ++b);
+            }
+            const uint32_t places = max(L.places, 1u);
+            h = (int)(rem / places);
+            place = rem % places;
         }
-        const uint32_t places = max(L.places, 1u);
-        int h = (int)(rem / places);
-        uint32_t place = rem % places;         // within the unit
         for (;;) {
-            const int unit = b * A.heads + h;
+            const uint32_t unit = unit_of(b, h);
             const uint32_t take = min(L.places - place, end - pos);
             const int t = max((int)place - A.ahead, 0), n = max((int)(place + take) - A.ahead, 0) - t;
             if (n == 0) break;                 // the share ends before the unit's tiles
@@ -682,7 +696,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                     const float z = attend<SUMS, ROUND, NR>(s, ks, vs, word, vq, lane, ps);
                     if (SUMS) {
                         const int j = 2 * tile + (lane >> 5);
-                        if (!(g & 1) && col < G && j < L.pages) A.z[((int64_t)unit * A.width + j) * G + col] = z;
+                        if (!(g & 1) && col < G && j < L.pages) A.z[(((int64_t)b * A.heads + h) * A.width + j) * G + col] = z;
                     }
                 }
                 // on as the tail's rows are taken
@@ -728,12 +742,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                 }
             }
             // ---- the unit is written out, or its piece kept
-            float l = st.l + __shfl_xor(st.l, 16, 64);
-            l += __shfl_xor(l, 32, 64);
-            if (SUMS) {
-                l32 += __shfl_xor(l32, 16, 64);
-                l32 += __shfl_xor(l32, 32, 64);
-            }
+            const float l = quarters_sum(st.l);
+            if (SUMS) l32 = quarters_sum(l32);
             const bool ends = t + n == L.tiles;
             if (t == 0 && ends) {
                 if (col < G) {
@@ -744,7 +754,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
                                             st.o[4][i], st.o[5][i], st.o[6][i], st.o[7][i]};
                         put8<BF16>(A, unit, col, 8 * (4 * g + i), x, inv);
                     }
-                    if (SUMS && g == 0) A.lse[(int64_t)unit * G + col] = st.m + __builtin_amdgcn_logf(l32);
+                    if (SUMS && g == 0) A.lse[lse_at(A, unit, col)] = st.m + __builtin_amdgcn_logf(l32);
                 }
             } else {
                 float* to = reinterpret_cast<float*>(mine + (ends ? last_area : 0)) + col * kMRow;
@@ -783,52 +793,59 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
     }
     __syncthreads();
 
-    // ---- pieces joined: 16 lanes a row, eight dimensions a lane
-    Desc left = {-1, 0};
+    // ---- pieces joined, unit by unit, a wave's at most: 16 lanes a row, eight dimensions a lane
+    Desc left = {~0u, 0};
     const int row = tid >> 4, d = 8 * (tid & 15);
-    for (int i = 0; i < 2 * kWaves;) {
-        const int unit = s_unit[i];
-        if (unit < 0) {
-            i++;
-            continue;
-        }
-        const bool begins = s_begins[i] != 0;
-        bool ends = false;
-        float m = -INFINITY, l = 0.f, l32 = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (; i < 2 * kWaves && (s_unit[i] == unit || s_unit[i] < 0); i++) {
-            if (s_unit[i] < 0) continue;
-            ends = !(i & 1);
-            if (row >= G) continue;
-            const float* p = reinterpret_cast<const float*>(s_dyn + (i >> 1) * stride + (ends ? last_area : 0)) + row * kMRow;
-            const float pm = p[kHd], M = fmaxf(m, pm);
-            const float f0 = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - M);
-            const float f1 = pm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(pm - M);
-            l = l * f0 + p[kHd + 1] * f1;
-            if (SUMS) l32 = l32 * f0 + p[kHd + 2] * f1;
-            const f4_t u = *reinterpret_cast<const f4_t*>(p + d), v = *reinterpret_cast<const f4_t*>(p + d + 4);
+    const uint32_t units = lane < 2 * kWaves ? s_unit[lane] : ~0u;
+    const uint32_t begun = (uint32_t)__ballot(lane < 2 * kWaves && s_begins[lane & (2 * kWaves - 1)] != 0);
+    for (uint32_t open = (uint32_t)__ballot(units != ~0u); open;) {
+        const int at = __ffs((int)open) - 1;
+        const uint32_t unit = (uint32_t)__builtin_amdgcn_readlane((int)units, at), its = (uint32_t)__ballot(units == unit);
+        open &= ~its;
+        const bool begins = (begun >> at) & 1u, ends = (its & 0x55555555u) != 0u;
+        if (row < G) {
+            float pm[kWaves], pl[kWaves], p32[kWaves];
+            f4_t u[kWaves], v[kWaves];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[e] = x[e] * f0 + u[e] * f1;
-                x[4 + e] = x[4 + e] * f0 + v[e] * f1;
+            for (int w = 0; w < kWaves; w++) {
+                pm[w] = -INFINITY;
+                pl[w] = p32[w] = 0.f;
+                u[w] = v[w] = f4_t{0.f, 0.f, 0.f, 0.f};
+                if (!((its >> (2 * w)) & 3u)) continue;
+                const float* p = reinterpret_cast<const float*>(s_dyn + w * stride + ((its >> (2 * w)) & 1u ? last_area : 0)) + row * kMRow;
+                pm[w] = p[kHd];
+                pl[w] = p[kHd + 1];
+                if (SUMS) p32[w] = p[kHd + 2];
+                u[w] = *reinterpret_cast<const f4_t*>(p + d);
+                v[w] = *reinterpret_cast<const f4_t*>(p + d + 4);
             }
-            m = M;
-        }
-        if (begins && ends) {
-            if (row < G) {
+            float m = -INFINITY, l = 0.f, l32 = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) m = fmaxf(m, pm[w]);
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                const float f = pm[w] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(pm[w] - m);
+                l = __builtin_fmaf(pl[w], f, l);
+                if (SUMS) l32 = __builtin_fmaf(p32[w], f, l32);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[e] = __builtin_fmaf(u[w][e], f, x[e]);
+                    x[4 + e] = __builtin_fmaf(v[w][e], f, x[4 + e]);
+                }
+            }
+            if (begins && ends) {
                 put8<BF16>(A, unit, row, d, x, 1.f / l);
-                if (SUMS && d == 0) A.lse[(int64_t)unit * G + row] = m + __builtin_amdgcn_logf(l32);
-            }
-        } else {
-            if (row < G) {
+                if (SUMS && d == 0) A.lse[lse_at(A, unit, row)] = m + __builtin_amdgcn_logf(l32);
+            } else {
                 float* rec = A.rec + ((int64_t)(2 * me + (begins ? 1 : 0)) * G + row) * kRecF;
                 *reinterpret_cast<f4_t*>(rec + 4 + d) = f4_t{x[0], x[1], x[2], x[3]};
                 *reinterpret_cast<f4_t*>(rec + 8 + d) = f4_t{x[4], x[5], x[6], x[7]};
                 if (d == 0) *reinterpret_cast<f4_t*>(rec) = f4_t{m, l, l32, 0.f};
             }
-            if (begins) {                      // the workgroup that has the unit's last place
-                const uint32_t at = s_end - 1, split = longer * (share + 1);
-                left = {unit, (int32_t)((at < split ? at / (share + 1) : longer + (at - split) / share) - me)};
-            }
+        }
+        if (begins && !ends) {                 // the workgroup that has the unit's last place
+            const uint32_t last = s_end - 1, split = longer * (share + 1);
+            left = {unit, (int32_t)((last < split ? last / (share + 1) : longer + (last - split) / share) - me)};
         }
     }
     if (tid == 0 && !A.whole) A.desc[me] = left;
@@ -845,7 +862,7 @@ __global__ __launch_bounds__(256, 8) void k_paged_join(PagedArgs A) {
     __shared__ float s_m[8], s_l[8], s_l32[8];
     const int dq = threadIdx.x & 31, sub = threadIdx.x >> 5, row = blockIdx.y, wg = blockIdx.x;
     const Desc D = A.desc[wg];
-    if (D.unit < 0) return;
+    if (D.unit == ~0u) return;
     const int n = 1 + D.more;
     float m = -INFINITY, l = 0.f, l32 = 0.f;
     f4_t o = {0.f, 0.f, 0.f, 0.f};
@@ -903,7 +920,7 @@ __global__ __launch_bounds__(256, 8) void k_paged_join(PagedArgs A) {
         }
     }
     put8<BF16>(A, D.unit, row, 8 * lane, x, 1.f / L);
-    if (SUMS && lane == 0) A.lse[(int64_t)D.unit * A.group + row] = M + __builtin_amdgcn_logf(L32);
+    if (SUMS && lane == 0) A.lse[lse_at(A, D.unit, row)] = M + __builtin_amdgcn_logf(L32);
 }
 
 // weights[b][j] = decay * weights[b][j] + the page's weight of this step (decay 0: that
@@ -1172,7 +1189,7 @@ template <bool BF16, bool SUMS, bool BIG>
 void paged_launch(const PagedArgs& A, int grid, hipStream_t s) {
     const int slot = A.group * kMRow * 4;
     const size_t lds = (size_t)kWaves * ((slot > kPatch ? slot : kPatch) + slot);
-    const dim3 g((unsigned)grid), wg(kThreads);
+    const dim3 g(A.whole ? (unsigned)A.heads : (unsigned)grid, A.whole ? (unsigned)A.n_seq : 1u), wg(kThreads);
     if (A.group <= 4) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 4>), g, wg, lds, s, A);
     else if (A.group <= 8) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 8>), g, wg, lds, s, A);
     else hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 16>), g, wg, lds, s, A);

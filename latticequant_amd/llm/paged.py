@@ -242,7 +242,7 @@ def paged_decode_attention(k: PagedKV, v: PagedKV, q: torch.Tensor, pages: torch
         elif work.device != dev or not work.is_contiguous():
             raise ValueError("the attention workspace must be contiguous, on the pools' device")
         if out is None:
-            out = torch.empty(q.shape, dtype=dt, device=dev)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         keep, flat = [], []                    # the copies stay until the launch; four lq_rows
         for t in given:
             t, r = _rows(t)
@@ -299,7 +299,7 @@ def evict_pages(pages: torch.Tensor, n_pages: torch.Tensor, weights: torch.Tenso
         cnt = _ints(n_pages, (B,), "n_pages", dev)
         w = weights.contiguous()
         if out is None:
-            out = Eviction(tab.new_empty((B, W)), tab.new_empty(B), w.new_empty((B, W)), tab.new_empty((B, W)))
+            out = Eviction(torch.empty_like(tab), torch.empty_like(cnt), torch.empty_like(w), torch.empty_like(tab))
         else:
             for t, like in zip(out, (tab, cnt, w, tab)):
                 if t.shape != like.shape or t.dtype is not like.dtype or t.device != dev or not t.is_contiguous():
