@@ -31,15 +31,16 @@ namespace {
 
 inline int launch_status() { return hipGetLastError() == hipSuccess ? LQ_OK : LQ_ERR_LAUNCH; }
 
-constexpr int kWaves = 4;                      // of a workgroup
+constexpr int kWaves = 4;                      // of a workgroup that takes a share
+constexpr int kWholeWaves = 8;                 // of one that takes a unit, where each has a compute unit
 constexpr int kGroups = 512;                   // workgroups at most
 // Where no (sequence, head) can have more than kWhole tiles and all fit on the chip at once, a
-// workgroup takes one as a whole and there is no second launch.  1 / 8 / 32 sequences of 8
-// heads, replayed from a graph, against equal shares: 4 tiles 8.0 / 8.2 / 8.4 us (9.1 / 9.7
-// / 9.8), 12 tiles 10.2 / 11.5 / 11.5 (11.4 / 11.9 / 16.0), 20 tiles 12.9 / 14.0 / 14.9
-// (11.5 / 13.2 / 18.2), the host's time for the launch not counted; 128 sequences, two
-// rounds: 20 tiles 35.5 (31.0).
-constexpr int kWhole = 20;
+// workgroup takes one as a whole, of eight waves where each finds a compute unit, and there is
+// no second launch.  1 / 8 / 32 sequences of 8 heads, replayed from a graph, against equal
+// shares: 4 tiles 6.5 / 6.7 / 6.9 us (9.1 / 9.7 / 9.8), 20 tiles 10.1 / 10.8 / 11.1 (11.5 / 13.2 /
+// 18.2), 32 tiles 13.4 / 13.8 / 15.4 (11.5 / 14.0 / 20.7), the host's 3 us for a launch not
+// counted; 48 tiles 17.0 / 17.9 / 19.0 (11.9 / 15.3 / 23.5), and lengths may differ.
+constexpr int kWhole = 32;
 // A unit's first tile waits for its page numbers, records and exceptions in turn and its tail
 // for its rows, which took about two tiles' time: the list has two places for that before each
 // unit's tiles.  32 sequences up to 2048 tokens 24.1 -> 21.6 us, 64 up to 8192 with weights
@@ -48,7 +49,6 @@ constexpr int kAhead = 2;
 constexpr int kMRow = kHd + 4;                 // floats of a piece's row in LDS: o[128], m, l, l32
 constexpr int kRecF = 4 + kHd;                 // floats of a record's row: m, l, l32, unused, o[128]
 constexpr int kPatch = 8 * 64 * 16;            // bytes of a wave's area for exceptions
-constexpr int kThreads = kWaves * 64;
 
 struct Rows {
     const uint16_t* p;
@@ -410,9 +410,9 @@ __device__ __forceinline__ float attend(const f4_t s[2], const uint32_t ks[4], c
     return SUMS ? __builtin_amdgcn_logf(pair_sum(shares_sum<NR>(sum))) - off + kPShift : 0.f;
 }
 
-__device__ __forceinline__ void zero_out(const PagedArgs& A, int b, int tid) {
+__device__ __forceinline__ void zero_out(const PagedArgs& A, int b, int tid, int threads) {
     const int n = A.heads * A.group * (kHd / 8);
-    for (int i = tid; i < n; i += kThreads)
+    for (int i = tid; i < n; i += threads)
         *reinterpret_cast<uint4*>(A.out + b * A.ob + (i >> 4) * A.oh + 8 * (i & 15)) = make_uint4(0u, 0u, 0u, 0u);
 }
 
@@ -446,13 +446,13 @@ __device__ __forceinline__ Len len_at(const PagedArgs& A, const Lens& mine, int 
     l.places = l.tiles ? (uint32_t)(l.tiles + A.ahead) : 0u;
     return l;
 }
-template <bool BF16, bool SUMS, bool BIG, int NR>
-__global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
+template <bool BF16, bool SUMS, bool BIG, int NR, int W>
+__global__ __launch_bounds__(W * 64, 2) void k_paged(PagedArgs A) {
     constexpr bool ROUND = SUMS;
     extern __shared__ __align__(16) char s_dyn[];
     // pieces in the order of the list: wave w's first (2 w), which ends its unit there, and its last (2 w + 1)
-    __shared__ uint32_t s_unit[2 * kWaves];
-    __shared__ int s_begins[2 * kWaves];
+    __shared__ uint32_t s_unit[2 * W];
+    __shared__ int s_begins[2 * W];
     __shared__ uint32_t s_end;                 // where the list's unit that is begun here and not ended ends
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4, G = A.group;
@@ -461,7 +461,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
     char* mine = s_dyn + wave * stride;        // exceptions, then the wave's last piece; behind it its first
     u32x4_t* area = reinterpret_cast<u32x4_t*>(mine);
 
-    if (tid < 2 * kWaves) s_unit[tid] = ~0u;
+    if (tid < 2 * W) s_unit[tid] = ~0u;
     // ---- the workgroup's share of the list, found by every wave for itself
     uint32_t lo, hi, share = 0, longer = 0;    // the first `longer` workgroups have one place more
     Lens lens = {0, 0};
@@ -475,24 +475,28 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
         L = len_of(A, b);
         lo = 0;
         hi = L.places;
-        if (hi == 0 && h == 0) zero_out(A, b, tid);
+        if (hi == 0 && h == 0) zero_out(A, b, tid, W * 64);
     } else {
         for (int i = lane * A.per; i < min((lane + 1) * A.per, A.n_seq); i++) {
             const Len l = len_of(A, i);
             lens = {l.pages, l.tail};
             own += l.places * A.heads;
         }
+        // the sums up to each lane: of the lanes of a row, then of the rows
         uint32_t upto = own;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t x = __shfl_up(upto, o, 64);
-            upto += lane >= o ? x : 0u;
-        }
+#define LQ_UPTO(CTRL, ROWS) upto += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)upto, CTRL, ROWS, 0xf, false)
+        LQ_UPTO(0x111, 0xf);                   // row_shr:1, 2, 4, 8
+        LQ_UPTO(0x112, 0xf);
+        LQ_UPTO(0x114, 0xf);
+        LQ_UPTO(0x118, 0xf);
+        LQ_UPTO(0x142, 0xa);                   // row_bcast:15 to the second and fourth
+        LQ_UPTO(0x143, 0xc);                   // row_bcast:31 to the last two
+#undef LQ_UPTO
         const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
         before = upto - own;
         for (int i = blockIdx.x; i < A.n_seq; i += gridDim.x)
-            if (len_at(A, lens, i).tiles == 0) zero_out(A, i, tid);
-        const uint32_t groups = max(1u, min((uint32_t)gridDim.x, (total + kWaves - 1) / kWaves));
+            if (len_at(A, lens, i).tiles == 0) zero_out(A, i, tid, W * 64);
+        const uint32_t groups = max(1u, min((uint32_t)gridDim.x, (total + W - 1) / W));
         if (me >= groups) {
             if (tid == 0) A.desc[me] = {~0u, 0};
             return;
@@ -503,7 +507,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
         hi = lo + share + (me < longer ? 1u : 0u);
     }
     __syncthreads();
-    const uint32_t part = (hi - lo) / kWaves, rest = (hi - lo) % kWaves;
+    const uint32_t part = (hi - lo) / W, rest = (hi - lo) % W;
     uint32_t pos = lo + wave * part + min((uint32_t)wave, rest);
     const uint32_t end = pos + part + ((uint32_t)wave < rest ? 1u : 0u);
 
@@ -796,18 +800,18 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
     // ---- pieces joined, unit by unit, a wave's at most: 16 lanes a row, eight dimensions a lane
     Desc left = {~0u, 0};
     const int row = tid >> 4, d = 8 * (tid & 15);
-    const uint32_t units = lane < 2 * kWaves ? s_unit[lane] : ~0u;
-    const uint32_t begun = (uint32_t)__ballot(lane < 2 * kWaves && s_begins[lane & (2 * kWaves - 1)] != 0);
+    const uint32_t units = lane < 2 * W ? s_unit[lane] : ~0u;
+    const uint32_t begun = (uint32_t)__ballot(lane < 2 * W && s_begins[lane & (2 * W - 1)] != 0);
     for (uint32_t open = (uint32_t)__ballot(units != ~0u); open;) {
         const int at = __ffs((int)open) - 1;
         const uint32_t unit = (uint32_t)__builtin_amdgcn_readlane((int)units, at), its = (uint32_t)__ballot(units == unit);
         open &= ~its;
         const bool begins = (begun >> at) & 1u, ends = (its & 0x55555555u) != 0u;
         if (row < G) {
-            float pm[kWaves], pl[kWaves], p32[kWaves];
-            f4_t u[kWaves], v[kWaves];
+            float pm[W], pl[W], p32[W];
+            f4_t u[W], v[W];
 #pragma unroll
-            for (int w = 0; w < kWaves; w++) {
+            for (int w = 0; w < W; w++) {
                 pm[w] = -INFINITY;
                 pl[w] = p32[w] = 0.f;
                 u[w] = v[w] = f4_t{0.f, 0.f, 0.f, 0.f};
@@ -821,9 +825,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_paged(PagedArgs A) {
             }
             float m = -INFINITY, l = 0.f, l32 = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < kWaves; w++) m = fmaxf(m, pm[w]);
+            for (int w = 0; w < W; w++) m = fmaxf(m, pm[w]);
 #pragma unroll
-            for (int w = 0; w < kWaves; w++) {
+            for (int w = 0; w < W; w++) {
                 const float f = pm[w] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(pm[w] - m);
                 l = __builtin_fmaf(pl[w], f, l);
                 if (SUMS) l32 = __builtin_fmaf(p32[w], f, l32);
@@ -1185,14 +1189,20 @@ bool rows_ok(const lq_rows* r) {
 }
 Rows rows_of(const lq_rows* r) { return {static_cast<const uint16_t*>(r->p), r->stride_b, r->stride_h, r->stride_t}; }
 
+template <bool BF16, bool SUMS, bool BIG, int W>
+void paged_launch(const PagedArgs& A, const dim3& g, hipStream_t s) {
+    const int slot = A.group * kMRow * 4;
+    const size_t lds = (size_t)W * ((slot > kPatch ? slot : kPatch) + slot);
+    const dim3 wg(W * 64);
+    if (A.group <= 4) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 4, W>), g, wg, lds, s, A);
+    else if (A.group <= 8) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 8, W>), g, wg, lds, s, A);
+    else hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 16, W>), g, wg, lds, s, A);
+}
 template <bool BF16, bool SUMS, bool BIG>
 void paged_launch(const PagedArgs& A, int grid, hipStream_t s) {
-    const int slot = A.group * kMRow * 4;
-    const size_t lds = (size_t)kWaves * ((slot > kPatch ? slot : kPatch) + slot);
-    const dim3 g(A.whole ? (unsigned)A.heads : (unsigned)grid, A.whole ? (unsigned)A.n_seq : 1u), wg(kThreads);
-    if (A.group <= 4) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 4>), g, wg, lds, s, A);
-    else if (A.group <= 8) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 8>), g, wg, lds, s, A);
-    else hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 16>), g, wg, lds, s, A);
+    const dim3 g(A.whole ? (unsigned)A.heads : (unsigned)grid, A.whole ? (unsigned)A.n_seq : 1u);
+    if (A.whole && grid <= kGroups / 2) paged_launch<BF16, SUMS, BIG, kWholeWaves>(A, g, s);
+    else paged_launch<BF16, SUMS, BIG, kWaves>(A, g, s);
     if (!A.whole) hipLaunchKernelGGL((k_paged_join<BF16, SUMS>), dim3((unsigned)grid, (unsigned)A.group), dim3(256), 0, s, A);
 }
 template <bool BF16, bool SUMS>
