@@ -266,7 +266,7 @@ __device__ __forceinline__ float pair_sum(float v) {   // of lane and lane ^ 16
 // State of a row over a unit's pages.  K's and V's values are c times their token's scale,
 // and enter the products as 2^-24 (2 c + 32):
 //   z   = kScale2 2^23 s_k (sum_i q_i k_i - 2^-19 sum_i q_i)
-//   o   = 2^23 (sum_t P_t v_t - 2^-19 sum_t P_t),   P_t = fp16(fp16(2^(z_t - m + shift)) s_v)
+//   o   = 2^23 (sum_t P_t v_t - 2^-19 sum_t P_t),   P_t = fp16(2^(z_t - m + shift) s_v)
 // so a record is decoded by bit operations alone.  The correction of z starts the product's
 // accumulator; that of o is taken off every 32 tiles, so that the sums stay near their result
 // (N tokens of like weights: the result falls as sqrt(N) beside them).  ROUND: K's values
@@ -384,14 +384,12 @@ __device__ __forceinline__ float attend(const f4_t s[2], const uint32_t ks[4], c
 #pragma unroll
     for (int i = 0; i < N / 2; i++) {
         const float u = __builtin_amdgcn_exp2f(z[2 * i]), v = __builtin_amdgcn_exp2f(z[2 * i + 1]);
-        const h2_t h = __builtin_bit_cast(h2_t, pair_h(u, v)), one = {(_Float16)1.f, (_Float16)1.f};
-        if (SUMS) sum += u + v;
-        else st.l = __builtin_amdgcn_fdot2(h, one, st.l, false);
-        const h2_t w = h * __builtin_bit_cast(h2_t, vs[i]);
-        p[i] = __builtin_bit_cast(uint32_t, w);
-        st.sum = __builtin_amdgcn_fdot2(w, one, st.sum, false);
+        const h2_t sv = __builtin_bit_cast(h2_t, vs[i]), one = {(_Float16)1.f, (_Float16)1.f};
+        sum += u + v;
+        p[i] = pair_h(u * (float)sv[0], v * (float)sv[1]);   // the product's operand: one rounding, 2^-11 of it at most
+        st.sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, p[i]), one, st.sum, false);
     }
-    if (SUMS) st.l += sum;
+    st.l += sum;
     // back to lane r, which has row r's eight tokens in the product (what the others have goes
     // into columns that are not read)
     if constexpr (NR == 8) {
