@@ -11,6 +11,9 @@
 // a time (sorted by a bitonic network, then merged), few of them one by one.  A first bound comes from the workgroup's first vectors: of the four
 // largest of the lanes' maxima of every wave the top-th largest, which `top` logits reach.
 // Few logits of a row pass it, and most waves need no list.
+// Bound by memory with many rows (2048 of 128256 bf16 logits: 82 to 89 us, 6.2 TB/s; with 20
+// alternatives 256 rows 23 us), by the latency of a row's loads, lists and sums with one (32000
+// logits with 5 alternatives: 9.8 us).
 #include <climits>
 #include <cmath>
 

@@ -18,6 +18,14 @@
 // last of the workgroups joining them itself, by a counter per unit, was no faster: its
 // device-scope stores, release and acquire took the 4 to 5 us of the second launch with 136
 // tiles, and 9 us more than it with 8200.)
+//
+// Long ones are bound by instructions and memory alike: 480 vector instructions a tile (decode
+// of K and V about 310, K's exceptions through LDS and back 60, softmax of a lane's two
+// tokens and both products' rest 110) at two waves a SIMD, one tile in flight beside the
+// one that is worked on; 2 sequences of 131072 tokens, 8 heads, 4 rows, 8 % of K's vectors
+// exceptions: 86 us, 4.2 TB/s (three waves a SIMD 105, two tiles in flight 139: both spill).
+// Short ones by latency: lengths, table, records and exceptions are loaded in turn, and a tile
+// takes a lone wave 4200 cycles; 1 sequence of 500 tokens 11.1 us.
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -926,7 +934,9 @@ __global__ __launch_bounds__(256, 8) void k_paged_join(PagedArgs A) {
 }
 
 // weights[b][j] = decay * weights[b][j] + the page's weight of this step (decay 0: that
-// alone), a lane a page, the heads dealt to four waves whose sums are joined in order.
+// alone), a lane a page, the heads dealt to four waves whose sums are joined in order.  Bound
+// by the latency of a wave's loads: 64 sequences of up to 512 pages, 8 heads, 4 rows 4.9 us (a
+// wave for all heads 8.0).
 template <int G4>   // whole rows of four, or 0 for any group
 __global__ __launch_bounds__(256) void k_page_weights(PagedArgs A, float* __restrict__ w, float decay) {
     __shared__ float s_sum[4][64];
