@@ -131,6 +131,8 @@ SHAPES = [
     (2, 8, 4, [600, 257], [16, 3]),
     (1, 1, 8, [2100], [1]),
     (33, 4, 5, [(11 * i) % 40 for i in range(33)], [(5 * i) % 17 for i in range(33)]),
+    (2, 2, 4, [0, 3], [1000, 700]),
+    (1500, 1, 2, [(i * i) % 4 if i % 5 else 0 for i in range(1500)], [i % 3 for i in range(1500)]),
 ]
 
 
