@@ -17,6 +17,9 @@ merge / decode-attention step, as hand-written HIP kernels behind a C ABI
   latticequant_amd.llm.resident             (decode step over its resident fixed-width form;
                                              sequences reordered, selected, forked)
   latticequant_amd.llm.tree                 (drafted trees over it: attention, acceptance)
+  latticequant_amd.llm.paged                (many sequences over one pool of its pages: attention,
+                                             page weights, eviction)
+  latticequant_amd.llm.logprobs             (log probabilities of a step)
   latticequant_amd.llm.resident_cache       (HF cache and attention of the resident form)
 """
 __version__ = "0.1.0"

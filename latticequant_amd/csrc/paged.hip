@@ -25,7 +25,7 @@
 // one that is worked on; 2 sequences of 131072 tokens, 8 heads, 4 rows, 8 % of K's vectors
 // exceptions: 86 us, 4.2 TB/s (three waves a SIMD 105, two tiles in flight 139: both spill).
 // Short ones by latency: lengths, table, records and exceptions are loaded in turn, and a tile
-// takes a lone wave 4200 cycles; 1 sequence of 500 tokens 11.1 us.
+// takes a lone wave 4200 cycles; 1 sequence of 500 tokens 10.4 us.
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -45,9 +45,12 @@ constexpr int kGroups = 512;                   // workgroups at most
 // Where no (sequence, head) can have more than kWhole tiles and all fit on the chip at once, a
 // workgroup takes one as a whole, of eight waves where each finds a compute unit, and there is
 // no second launch.  1 / 8 / 32 sequences of 8 heads, replayed from a graph, against equal
-// shares: 4 tiles 6.5 / 6.7 / 6.9 us (9.1 / 9.7 / 9.8), 20 tiles 10.1 / 10.8 / 11.1 (11.5 / 13.2 /
-// 18.2), 32 tiles 13.4 / 13.8 / 15.4 (11.5 / 14.0 / 20.7), the host's 3 us for a launch not
-// counted; 48 tiles 17.0 / 17.9 / 19.0 (11.9 / 15.3 / 23.5), and lengths may differ.
+// shares: 4 tiles 5.9 / 6.0 / 6.1 us (9.1 / 9.7 / 9.8), 20 tiles 9.5 / 10.0 / 10.2 (11.5 / 13.2 /
+// 18.2), 32 tiles 11.9 / 12.8 / 14.7 (11.5 / 14.0 / 20.7), the host's 3 us for a launch not
+// counted; 48 tiles 17.0 / 17.9 / 19.0 (11.9 / 15.3 / 23.5), and lengths may differ.  64
+// sequences, with four waves so that all are there at once: 2 / 16 / 32 tiles 5.9 / 13.9 / 21.6
+// (shares 8.6 / 18.5 / 25.6, eight waves 9.8 / 18.9 / 26.3).  A kernel of its own, without what
+// finds shares: code that is only branched around cost 0.9 us (11.1 for 10.3 with 17 tiles).
 constexpr int kWhole = 32;
 // A unit's first tile waits for its page numbers, records and exceptions in turn and its tail
 // for its rows, which took about two tiles' time: the list has two places for that before each
@@ -80,7 +83,6 @@ struct PagedArgs {
     uint16_t* out;
     int64_t ob, oh;
     int n_seq, heads, group, per;              // per: sequences of a lane's sum
-    int whole;                                 // a workgroup a unit, instead of equal shares
     int ahead;                                 // places of the list that a unit has before its tiles'
     float* rec;                                // [2 workgroup + (0: of an earlier one's, 1: begun here)][row][kRecF]
     Desc* desc;
@@ -452,7 +454,7 @@ __device__ __forceinline__ Len len_at(const PagedArgs& A, const Lens& mine, int 
     l.places = l.tiles ? (uint32_t)(l.tiles + A.ahead) : 0u;
     return l;
 }
-template <bool BF16, bool SUMS, bool BIG, int NR, int W>
+template <bool BF16, bool SUMS, bool BIG, int NR, int W, bool WHOLE>
 __global__ __launch_bounds__(W * 64, 2) void k_paged(PagedArgs A) {
     constexpr bool ROUND = SUMS;
     extern __shared__ __align__(16) char s_dyn[];
@@ -475,7 +477,7 @@ __global__ __launch_bounds__(W * 64, 2) void k_paged(PagedArgs A) {
     int b = 0, h = 0;
     Len L;
     const uint32_t me = blockIdx.x;
-    if (A.whole) {
+    if (WHOLE) {
         b = blockIdx.y;
         h = blockIdx.x;
         L = len_of(A, b);
@@ -519,7 +521,7 @@ __global__ __launch_bounds__(W * 64, 2) void k_paged(PagedArgs A) {
 
     if (pos < end) {
         uint32_t place = pos;                  // within the unit
-        if (!A.whole) {
+        if (!WHOLE) {
             const uint64_t there = __ballot(pos >= before && pos - before < own);
             const int from = __ffsll((long long)there) - 1;
             uint32_t rem = pos - (uint32_t)__builtin_amdgcn_readlane((int)before, from);
@@ -789,7 +791,7 @@ __global__ __launch_bounds__(W * 64, 2) void k_paged(PagedArgs A) {
                 }
             }
             pos += take;
-            if (pos == end) break;
+            if (WHOLE || pos == end) break;
             place = 0;
             if (++h == A.heads) {
                 h = 0;
@@ -858,7 +860,7 @@ __global__ __launch_bounds__(W * 64, 2) void k_paged(PagedArgs A) {
             left = {unit, (int32_t)((last < split ? last / (share + 1) : longer + (last - split) / share) - me)};
         }
     }
-    if (tid == 0 && !A.whole) A.desc[me] = left;
+    if (tid == 0 && !WHOLE) A.desc[me] = left;
 }
 
 // The records of a unit that several workgroups share, a workgroup per row: thread
@@ -1166,7 +1168,8 @@ __global__ __launch_bounds__(kEvictThreads) void k_evict(EvictArgs A, int parts)
 // ------------------------------------------------------------------- plan --
 
 struct Plan {
-    int grid, whole;
+    int grid;
+    bool whole;                                // a workgroup a unit, instead of equal shares
     int64_t rec, desc, lse, z, bytes;          // bytes before each, and in all
 };
 bool plan(int64_t n_seq, int64_t heads, int64_t group, int64_t width, int64_t tail_cap, bool weights, Plan* p) {
@@ -1197,26 +1200,30 @@ bool rows_ok(const lq_rows* r) {
 }
 Rows rows_of(const lq_rows* r) { return {static_cast<const uint16_t*>(r->p), r->stride_b, r->stride_h, r->stride_t}; }
 
-template <bool BF16, bool SUMS, bool BIG, int W>
+template <bool BF16, bool SUMS, bool BIG, int W, bool WHOLE>
 void paged_launch(const PagedArgs& A, const dim3& g, hipStream_t s) {
     const int slot = A.group * kMRow * 4;
     const size_t lds = (size_t)W * ((slot > kPatch ? slot : kPatch) + slot);
     const dim3 wg(W * 64);
-    if (A.group <= 4) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 4, W>), g, wg, lds, s, A);
-    else if (A.group <= 8) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 8, W>), g, wg, lds, s, A);
-    else hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 16, W>), g, wg, lds, s, A);
+    if (A.group <= 4) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 4, W, WHOLE>), g, wg, lds, s, A);
+    else if (A.group <= 8) hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 8, W, WHOLE>), g, wg, lds, s, A);
+    else hipLaunchKernelGGL((k_paged<BF16, SUMS, BIG, 16, W, WHOLE>), g, wg, lds, s, A);
 }
 template <bool BF16, bool SUMS, bool BIG>
-void paged_launch(const PagedArgs& A, int grid, hipStream_t s) {
-    const dim3 g(A.whole ? (unsigned)A.heads : (unsigned)grid, A.whole ? (unsigned)A.n_seq : 1u);
-    if (A.whole && grid <= kGroups / 2) paged_launch<BF16, SUMS, BIG, kWholeWaves>(A, g, s);
-    else paged_launch<BF16, SUMS, BIG, kWaves>(A, g, s);
-    if (!A.whole) hipLaunchKernelGGL((k_paged_join<BF16, SUMS>), dim3((unsigned)grid, (unsigned)A.group), dim3(256), 0, s, A);
+void paged_launch(const PagedArgs& A, bool whole, int grid, hipStream_t s) {
+    if (whole) {
+        const dim3 g((unsigned)A.heads, (unsigned)A.n_seq);
+        if (grid <= kGroups / 2) paged_launch<BF16, SUMS, BIG, kWholeWaves, true>(A, g, s);
+        else paged_launch<BF16, SUMS, BIG, kWaves, true>(A, g, s);
+        return;
+    }
+    paged_launch<BF16, SUMS, BIG, kWaves, false>(A, dim3((unsigned)grid), s);
+    hipLaunchKernelGGL((k_paged_join<BF16, SUMS>), dim3((unsigned)grid, (unsigned)A.group), dim3(256), 0, s, A);
 }
 template <bool BF16, bool SUMS>
-void paged_launch(const PagedArgs& A, int grid, bool big, hipStream_t s) {
-    if (big) paged_launch<BF16, SUMS, true>(A, grid, s);
-    else paged_launch<BF16, SUMS, false>(A, grid, s);
+void paged_launch(const PagedArgs& A, const Plan& p, bool big, hipStream_t s) {
+    if (big) paged_launch<BF16, SUMS, true>(A, p.whole, p.grid, s);
+    else paged_launch<BF16, SUMS, false>(A, p.whole, p.grid, s);
 }
 
 }  // namespace
@@ -1263,7 +1270,6 @@ int lq_paged_attention(const lq_pages *k, const lq_pages *v, const lq_rows *q, i
     A.heads = (int)k->r.n_heads;
     A.group = group;
     A.per = (int)((n_seq + 63) / 64);
-    A.whole = p.whole;
     A.ahead = p.whole ? 0 : kAhead;
     char* w = static_cast<char*>(d_work);
     A.rec = reinterpret_cast<float*>(w + p.rec);
@@ -1273,11 +1279,11 @@ int lq_paged_attention(const lq_pages *k, const lq_pages *v, const lq_rows *q, i
     const bool big = k->r.n_heads * k->r.cap_blocks > (int64_t)(UINT32_MAX / 1024) ||
                      (k->r.exc_cap > v->r.exc_cap ? k->r.exc_cap : v->r.exc_cap) > (int64_t)(UINT32_MAX / 16);
     if (dtype == LQ_BF16) {
-        if (d_weights) paged_launch<true, true>(A, p.grid, big, s);
-        else paged_launch<true, false>(A, p.grid, big, s);
+        if (d_weights) paged_launch<true, true>(A, p, big, s);
+        else paged_launch<true, false>(A, p, big, s);
     } else {
-        if (d_weights) paged_launch<false, true>(A, p.grid, big, s);
-        else paged_launch<false, false>(A, p.grid, big, s);
+        if (d_weights) paged_launch<false, true>(A, p, big, s);
+        else paged_launch<false, false>(A, p, big, s);
     }
     if (d_weights && max_pages > 0) {
         const dim3 wg((unsigned)((max_pages + 63) / 64), (unsigned)n_seq);
