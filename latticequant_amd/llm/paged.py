@@ -30,8 +30,10 @@ PAGE = RB        # tokens of a page
 
 
 def _no_grad(what: str, *ts) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 
 class _Pool(ResidentKV):
@@ -191,24 +193,26 @@ def paged_decode_attention(k: PagedKV, v: PagedKV, q: torch.Tensor, pages: torch
     V's unrounded, K's rounded to fp16 (as ``read`` rounds it) with weights and unrounded
     without.  The same inputs give the same bits."""
     dev = k.device
-    if q.dim() != 4 or q.dtype not in _DTYPES or q.shape[2] != 1 or q.shape[3] != HD:
+    dt, shape = q.dtype, q.shape
+    if len(shape) != 4 or dt not in _DTYPES or shape[2] != 1 or shape[3] != HD:
         raise ValueError("q must be (B, Hq, 1, 128) fp16 or bf16")
-    dt = q.dtype
-    B, Hq = q.shape[0], q.shape[1]
+    B, Hq, _, _ = shape
     H = k.n_heads
     if v.n_heads != H or v.n_pages != k.n_pages or v.device != dev:
         raise ValueError("the K and V pools must have the same heads, pages and device")
     if B < 1 or Hq < 1 or Hq % H or Hq // H > 16:
         raise ValueError("query heads must be 1..16 times the pools' heads")
-    if pages.dim() != 2 or pages.shape[0] != B:
+    wide = pages.shape
+    if len(wide) != 2 or wide[0] != B:
         raise ValueError("pages must be (B, W) whole numbers")
-    W = pages.shape[1]
+    W = wide[1]
     given = [q]
     cap = 0
     if tail_k is not None and tail_v is not None:
-        if tail_k.dim() != 4 or tail_k.shape != tail_v.shape or tail_k.shape[:2] != (B, H) or tail_k.shape[3] != HD:
+        rows = tail_k.shape
+        if len(rows) != 4 or rows != tail_v.shape or rows[0] != B or rows[1] != H or rows[3] != HD:
             raise ValueError("tail K / V must be (B, n_heads, cap, 128)")
-        cap = tail_k.shape[2]
+        cap = rows[2]
         if cap:
             given += [tail_k, tail_v]
     elif tail_k is not None or tail_v is not None:
@@ -228,7 +232,7 @@ def paged_decode_attention(k: PagedKV, v: PagedKV, q: torch.Tensor, pages: torch
         raise ValueError("out must be like q, its rows 16-byte aligned and apart")
     lib = L.lib()
     with L.on_device(dev):
-        tab = _ints(pages, (B, W), "pages", dev)
+        tab = _ints(pages, wide, "pages", dev)
         cnt = _ints(n_pages, (B,), "n_pages", dev)
         tl = None if tail_len is None else _ints(tail_len, (B,), "tail_len", dev)
         if L.debug_checks():
