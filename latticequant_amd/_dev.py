@@ -16,5 +16,14 @@ def to_gpu(t: torch.Tensor, dtype=None) -> torch.Tensor:
     return t.contiguous()
 
 
+def int32_on(t: torch.Tensor, device) -> torch.Tensor:
+    """Whole numbers as a contiguous int32 tensor on the device, those beyond 32 bits as the nearest
+    that has them: a number outside a range stays outside on its side, where narrowing alone
+    would wrap 2^32 + 5 to 5."""
+    if t.dtype is torch.int64:
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
+    return t.to(device=device, dtype=torch.int32).contiguous()
+
+
 def back(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
     return t if like.is_cuda else t.to(like.device)

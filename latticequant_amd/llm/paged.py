@@ -23,6 +23,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from .. import _lib as L
+from .._dev import int32_on
 from .resident import HD, RB, ResidentKV
 from .tree import _DTYPES, _ints, _rows
 
@@ -94,7 +95,7 @@ class PagedKV:
                 raise ValueError("page number outside the pool")
             if write and pages.unique().numel() != pages.numel():
                 raise ValueError("a page stands twice")
-        return pages.to(device=self.device, dtype=torch.int32).contiguous()
+        return int32_on(pages, self.device)
 
     def write(self, x: torch.Tensor, pages: torch.Tensor, scale32: Optional[torch.Tensor] = None,
               scale16: Optional[torch.Tensor] = None, bits: int = 4) -> None:

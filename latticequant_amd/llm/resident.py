@@ -25,6 +25,7 @@ from typing import Optional, Sequence
 import torch
 
 from .. import _lib as L
+from .._dev import int32_on
 
 RB = 16          # tokens per resident block
 HD = 128
@@ -254,8 +255,8 @@ class ResidentKV:
         with L.on_device(dev):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a selection reads its exception count back: not while a graph is captured")
-            idx = index.to(device=dev, dtype=torch.int32).contiguous()
-            blk = None if blocks is None else blocks.to(device=dev, dtype=torch.int32).contiguous()
+            idx = int32_on(index, dev)
+            blk = None if blocks is None else int32_on(blocks, dev)
             work, n_exc, status = idx.new_empty(need + 3 >> 2), self.n_exc.new_empty(1), self.status.new_empty(1)
             stream = L.raw_stream(dev)
             args = (ctypes.addressof(self.struct()), n_seq, used, idx.data_ptr(), R, L.ptr(blk), nb)
@@ -349,7 +350,7 @@ def reorder_sequences(residents: Sequence[ResidentKV], index: torch.Tensor, t_fr
         return
     lib = L.lib()
     with L.on_device(dev):
-        idx = index.to(device=dev, dtype=torch.int32).contiguous()
+        idx = int32_on(index, dev)
         if L.debug_checks() and (bool((idx < 0).any()) or bool((idx >= B).any())):
             raise ValueError("sequence out of range")
         table = b"".join([r.struct() for r in residents])   # lq_resident[]

@@ -46,6 +46,7 @@ import torch
 from transformers.cache_utils import DynamicCache
 
 from .. import codec
+from .._dev import int32_on
 from .resident import MAX_REORDER, RB, ResidentKV, attn_workspace, reorder_sequences, resident_decode_attention
 from .tree import (MAX_NODES, accept_drafts, append_accepted, gather_tails, node_depths, resident_tree_attention,
                    tree_workspace_size)
@@ -201,8 +202,8 @@ class ResidentKVCache(DynamicCache):
         st = None if start is None else torch.as_tensor(start)
         if st is not None and (st.shape != (B,) or st.dtype not in (torch.int32, torch.int64)):
             raise ValueError("start must be (B,) whole numbers")
-        self._parents = par.to(device=dev, dtype=torch.int32).contiguous()
-        self._start = None if st is None else st.to(device=dev, dtype=torch.int32)
+        self._parents = int32_on(par, dev)
+        self._start = None if st is None else int32_on(st, dev)
         self._drafts = {}
 
     def draft_positions(self) -> torch.Tensor:

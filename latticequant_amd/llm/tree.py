@@ -24,6 +24,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from .. import _lib as L
+from .._dev import int32_on
 from .resident import HD, RB, ResidentKV
 
 MAX_NODES = L.LQ_TREE_MAX_NODES
@@ -44,14 +45,14 @@ def _rows(t: torch.Tensor):
 
 
 def _ints(t, shape, name: str, dev) -> torch.Tensor:
-    """Whole numbers of the given shape as a contiguous int32 tensor on dev."""
+    """Whole numbers of the given shape as a contiguous int32 tensor on dev (int32_on)."""
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be an int32 or int64 tensor")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
     if t.dtype is torch.int32 and t.device == dev and t.is_contiguous():
         return t
-    return t.to(device=dev, dtype=torch.int32).contiguous()
+    return int32_on(t, dev)
 
 
 def _parents(parents, B: int, N: int, dev) -> torch.Tensor:

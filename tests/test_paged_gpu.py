@@ -540,3 +540,35 @@ def test_eviction_of_long_tables(W, B):
         got = evict_pages(*dev, keep, sink, recent)
         for a, b in zip(got, _evicted(pages, count, weight, keep, sink, recent)):
             assert np.array_equal(a.cpu().numpy(), b), (keep, sink, recent)
+
+
+# ------------------------------------------------------------------ numbers --
+
+BEYOND = [2 ** 32, 2 ** 32 + 5, -2 ** 32 + 1, 2 ** 63 - 1, -2 ** 63, 2 ** 31]
+
+
+def test_page_numbers_beyond_32_bits_are_outside_the_pool():
+    p = _pool(2, 8, 90)
+    every = torch.arange(8, device="cuda")[:, None]
+    before = p.read(every)
+    x, s = _rows(6, 2, PAGE, 91, loud=5)
+    p.write(x, torch.tensor(BEYOND, device="cuda")[:, None], s, s.half())
+    assert torch.equal(p.read(every), before)
+    assert not bool(p.read(torch.tensor([BEYOND], device="cuda")).any())
+
+
+def test_counts_and_numbers_beyond_32_bits_are_clamped():
+    k, v, q, tab, cnt, tk, tv, tl = _case(2, 2, 4, [6, 6], [3, 3], torch.float16, 92, cap=5)
+    wild = tab.long()
+    wild[0, :len(BEYOND)] = torch.tensor(BEYOND, device="cuda")
+    clamped = wild.clone()
+    clamped[0, :len(BEYOND)] = k.n_pages - 1
+    got = paged_decode_attention(k, v, q, wild, torch.tensor([2 ** 32 + 1, -2 ** 32 + 3], device="cuda"), tk, tv,
+                                 tail_len=torch.tensor([2 ** 40, -2 ** 40 + 2], device="cuda"))
+    want = paged_decode_attention(k, v, q, clamped, torch.tensor([6, 0], device="cuda"), tk, tv,
+                                  tail_len=torch.tensor([5, 0], device="cuda"))
+    assert torch.equal(got, want) and not bool(got[1].any()) and bool(got[0].any())
+    w = torch.rand(2, 6, device="cuda")
+    for a, b in zip(evict_pages(tab, torch.tensor([2 ** 33 + 2, -2 ** 33 + 2], device="cuda"), w, 3),
+                    evict_pages(tab, torch.tensor([6, 0], device="cuda"), w, 3)):
+        assert torch.equal(a, b)

@@ -504,3 +504,24 @@ def test_row_moves_of_unaligned_sources_gpu():
     d = torch.randn(3, 5, 128, 1, device="cuda").half().movedim(3, 0)   # a length of one whose stride is 1
     assert d.stride(0) == 1
     assert torch.equal(gather_tails([d], torch.tensor([0, 0]))[0], d[[0, 0]])
+
+
+@gpu
+def test_numbers_beyond_32_bits_are_clamped_or_left():
+    """Sequences and blocks by 64-bit numbers that 32 bits do not have: clamped in a selection,
+    no move in a reorder."""
+    from latticequant_amd.llm.resident import ResidentKV
+
+    def fresh():
+        r = ResidentKV(6, 64, device="cuda", n_seq=3)
+        g = torch.Generator(device="cuda").manual_seed(5)
+        r.append(torch.randn(3, 2, 64, 128, generator=g, device="cuda"), torch.full((6,), 0.25, device="cuda"),
+                 torch.full((6,), 0.25, device="cuda").half())
+        return r
+    i64 = lambda x: torch.tensor(x, device="cuda")
+    r = fresh()
+    far = r.select(i64([2 ** 32, -2 ** 32 + 1, 1]), blocks=i64([[2 ** 32 + 1, 0], [-2 ** 63, 2 ** 63 - 1], [2, 3]]))
+    near = r.select(i64([2, 0, 1]), blocks=i64([[3, 0], [0, 3], [2, 3]]))
+    assert torch.equal(far.dequant(), near.dequant())
+    r.reorder(i64([2 ** 32 + 1, -2 ** 32 + 2, 2]))
+    assert torch.equal(r.dequant(), fresh().dequant())

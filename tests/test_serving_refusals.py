@@ -5,8 +5,10 @@ import pytest
 import torch
 
 from latticequant_amd import _lib as L
+from latticequant_amd._dev import int32_on
 from latticequant_amd.llm.logprobs import token_logprobs
 from latticequant_amd.llm.paged import PagedKV, evict_pages, paged_decode_attention, paged_workspace_size
+from latticequant_amd.llm.tree import _ints
 
 
 def _args(B=2, H=2, G=4, W=3, cap=5, dtype=torch.float16):
@@ -117,3 +119,19 @@ def test_eviction_and_logprobs_need_the_gpu_and_sound_arguments():
                   ((x,), dict(top=-1)), ((x[:, :0],), {})):
         with pytest.raises(ValueError):
             token_logprobs(*a, **kw)
+
+
+def test_numbers_beyond_32_bits_stay_out_of_range():
+    """Tables, counts and indices of 64 bits become 32-bit ones without wrapping into a range."""
+    t = torch.tensor([2 ** 32, 2 ** 32 + 5, -2 ** 32 + 1, 2 ** 63 - 1, -2 ** 63, 2 ** 31, 7, -7])
+    want = [2 ** 31 - 1, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 7, -7]
+    assert int32_on(t, "cpu").tolist() == want and _ints(t, (8,), "t", t.device).tolist() == want
+    assert int32_on(t.int(), "cpu").tolist() == t.int().tolist()
+
+
+def test_a_pool_checks_page_numbers_of_64_bits(monkeypatch):
+    monkeypatch.setenv("LQ_DEBUG_CHECKS", "1")
+    p = PagedKV(1, 4, device="cpu")
+    for bad in (2 ** 32, -2 ** 32, 2 ** 63 - 1):
+        with pytest.raises(ValueError, match="outside the pool"):
+            p._numbers(torch.tensor([[bad]]), None, False)
