@@ -30,6 +30,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLazy = 8.0f;
 constexpr float kBig = 1e12f;                  // sums beyond it: the reference is too low
 constexpr float kHuge = 1e37f;                 // beyond it c x can leave fp32's range
+constexpr float kFar = 0x1p20f;                // references beyond it are taken off before the product
 constexpr int kUnroll = 4;                     // vectors of 16 bytes a lane has in flight
 
 struct LogArgs {
@@ -62,8 +63,10 @@ __device__ __forceinline__ float logit(const char* p, int64_t i) {
     return DT == LQ_F16 ? h2f(u) : bf2f(u);
 }
 
-// z of a logit: where c x or r would leave fp32's range (a mask of the type's lowest value,
-// a row of nothing else) from the difference, else by one fma
+// z of a logit by one fma, r = c m rounded: off by that rounding, which all of a row share, so
+// it drops out, as long as it is small beside the range of 2^z: 2^-4 at kFar, but 2^9 at a mask of
+// -10^10, whose lanes had sums of infinity or 0.  FAR: from the difference (of a
+// reference beyond kFar; c x may leave fp32's range), without that rounding
 template <bool FAR>
 __device__ __forceinline__ float z_of(float x, float m) {
     return FAR ? (x - m) * kLog2e : __builtin_fmaf(x, kLog2e, -(m * kLog2e));
@@ -72,9 +75,10 @@ __device__ __forceinline__ float z_of(float x, float m) {
 struct Stat {
     float m, l, a;                             // reference (of x), sum, sum of 2^z z
 };
-__device__ __forceinline__ bool far_of(float m) { return fabsf(m) > kHuge && fabsf(m) < INFINITY; }
-__device__ __forceinline__ float gap(float m, float to) {   // z of one reference from another
-    return far_of(m) || far_of(to) ? z_of<true>(m, to) : m * kLog2e - to * kLog2e;
+__device__ __forceinline__ bool far_of(float m) { return fabsf(m) > kFar && fabsf(m) < INFINITY; }
+__device__ __forceinline__ float gap(float m, float to) {   // z of one reference from another, as their logits have it
+    if (far_of(to)) return far_of(m) ? z_of<true>(m, to) : -__builtin_fmaf(to, kLog2e, -(m * kLog2e));
+    return far_of(m) ? z_of<false>(m, to) : m * kLog2e - to * kLog2e;
 }
 __device__ __forceinline__ void raise(Stat& s, float to) {
     if (s.m == to) return;
@@ -87,7 +91,7 @@ __device__ __forceinline__ void raise(Stat& s, float to) {
     s.l *= f;
     s.m = to;
 }
-// N logits; FAR where the reference is beyond kHuge.  Returns their sum: a NaN says that one
+// N logits; FAR where the reference is beyond kFar.  Returns their sum: a NaN says that one
 // of them is none.
 template <bool FAR, int N>
 __device__ __forceinline__ float add(Stat& s, const float* x) {
@@ -280,7 +284,8 @@ constexpr int kJoint = 512;                    // keys of all waves that go into
 // (r's rounding is in z and l alike; what it leaves is at most 0 for p = 1, not above)
 __device__ __forceinline__ float log_prob(float x, const Stat& s) {
     const float l = __builtin_amdgcn_logf(s.l);
-    const float p = far_of(x) || far_of(s.m) ? (x - s.m) - kLn2 * l : kLn2 * (z_of<false>(x, s.m) - l);
+    const bool diff = far_of(s.m) || (fabsf(x) > kHuge && fabsf(x) < INFINITY);
+    const float p = diff ? (x - s.m) - kLn2 * l : kLn2 * (z_of<false>(x, s.m) - l);
     return p > 0.f ? 0.f : p;
 }
 
@@ -383,11 +388,11 @@ __global__ __launch_bounds__(NW * 64) void k_logprobs(LogArgs A) {
             }
         };
         // Without a look at the largest logit and at -inf first: where the sums show that the
-        // reference was too low, or a logit -inf, they are taken again with both.
+        // reference was too low or is far, or a logit -inf, they are taken again with both.
         float l = 0.f, a = NAN;
         if (j0 >= T) {                         // there is a reference
             const float r = -(s.m * kLog2e);
-            a = 0.f;
+            a = fabsf(s.m) > kFar ? NAN : 0.f;
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 float x[V];

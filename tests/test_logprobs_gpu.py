@@ -171,3 +171,41 @@ def test_refusals():
     x = torch.randn(2, 50, device="cuda")
     with pytest.raises(RuntimeError, match="no gradient"):
         token_logprobs(x.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("vocab", [3001, 40009])
+@pytest.mark.parametrize("value", [1e5, 1e6, 3e6, 1e7, 1e8, 1e9, 1e10, 1e12, 1e20, 1e30, 1e36, 2e38])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_masks_of_any_finite_value(dtype, value, vocab):
+    """Logits masked with -value: a run of the row, all but a few, all of them, all but lesser ones
+    of like size; and logits of the size itself. (A reference of that size is off by more
+    than the logits differ where c x is rounded.)"""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    low = torch.tensor(-value, device="cuda").to(dtype)
+    x = (torch.randn(7, vocab, generator=g, device="cuda") * 3).to(dtype)
+    x[0, vocab // 3:] = low
+    x[1, 10:] = low
+    x[2] = low
+    x[3] = low
+    x[3, ::7] = low * 1.5
+    x[4, :-1] = low
+    x[5] = -low
+    x[5, 5:] = x[6, 5:]
+    x[6] = (value + value / 64 * torch.randn(vocab, generator=g, device="cuda").clamp(-8, 8)).to(dtype)
+    tok = torch.tensor([3, 3, 3, 3, vocab - 1, 2, 11], device="cuda")
+    _check(x, tok, 12, token_logprobs(x, tok, 12))
+    _check(x, None, 0, token_logprobs(x))
+    masked = torch.full((7,), vocab // 2, device="cuda")
+    got = token_logprobs(x, masked).logprob.double()
+    want = torch.log_softmax(x.double(), 1).gather(1, masked[:, None])[:, 0]
+    # c x, c m and ln 2 z: four roundings of the result's size
+    assert bool(((got - want).abs() <= 2.0 ** -22 * want.abs() + 2.0 ** -17).all())
+
+
+@pytest.mark.parametrize("vocab", [3001, 40009])
+@pytest.mark.parametrize("centre", [2.0 ** 20, -2.0 ** 20, 2.0 ** 17, -2.0 ** 22])
+def test_logits_of_large_size_and_small_differences(centre, vocab):
+    """fp32 logits that differ by a few units far from zero: of every lane its own reference."""
+    x = torch.randn(4, vocab, device="cuda") * 4 + centre
+    tok = torch.randint(0, vocab, (4,), device="cuda")
+    _check(x, tok, 20, token_logprobs(x, tok, 20))
