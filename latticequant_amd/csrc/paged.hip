@@ -284,7 +284,7 @@ __device__ __forceinline__ float pair_sum(float v) {   // of lane and lane ^ 16
 // attention's in 32 bits: c's own pairs, times the scale.
 struct PageState {
     float m, l, sum;                           // reference, sum of 2^(z - m + shift), of P_t since the last correction
-    float shift;                               // kPShift, less where a scale is above 1 (P stays in fp16's range)
+    float shift;                               // kPShift less the exponent of V's largest scale so far: P's range is that of a scale of 1
     float limit;                               // a logarithm of a weight beyond it raises the reference
     f4_t o[8];
 };
@@ -330,7 +330,7 @@ __device__ __forceinline__ void correct(PageState& st) {
         for (int i = 0; i < 4; i++) st.o[mm][i] += c;
     st.sum = 0.f;
 }
-// the largest of the lane's scales, and the least e with 2^e >= every one of the wave's, 0 at least
+// the largest of the lane's scales, and the least e with 2^e >= every one of the wave's (fp16's: -24 at least)
 template <int NR>
 __device__ __forceinline__ float lane_scale(const uint32_t s[4]) {
     h2_t m = __builtin_bit_cast(h2_t, s[0]);
@@ -341,7 +341,7 @@ __device__ __forceinline__ float lane_scale(const uint32_t s[4]) {
 template <int NR>
 __device__ __forceinline__ float scale_log(const uint32_t s[4]) {
     const float m = row_max<NR>(lane_scale<NR>(s));   // the lanes of a quarter have the same tokens
-    return fmaxf((float)((int)((__float_as_uint(m) + 0x7fffffu) >> 23) - 127), 0.f);
+    return fmaxf((float)((int)((__float_as_uint(m) + 0x7fffffu) >> 23) - 127), -24.f);
 }
 
 // One tile: scores s[y][i] of token 8 (lane / 16) + 2 i + y (without their scales, or with
@@ -580,7 +580,7 @@ __global__ __launch_bounds__(W * 64, 2) void k_paged(PagedArgs A) {
                 ps.l = ps.sum = 0.f;
                 ps.shift = kPShift;
                 ps.limit = -INFINITY;
-                float largest = 1.f;           // no scale has been above it
+                float largest = 0.f;           // no scale has been above it
 #pragma unroll
                 for (int mm = 0; mm < 8; mm++) ps.o[mm] = f4_t{0.f, 0.f, 0.f, 0.f};
                 Recs rd;

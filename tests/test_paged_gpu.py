@@ -572,3 +572,81 @@ def test_counts_and_numbers_beyond_32_bits_are_clamped():
     for a, b in zip(evict_pages(tab, torch.tensor([2 ** 33 + 2, -2 ** 33 + 2], device="cuda"), w, 3),
                     evict_pages(tab, torch.tensor([6, 0], device="cuda"), w, 3)):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------- scales --
+
+def _scaled(h, n, seed, scales, loud=0):
+    """A pool whose page j has rows of about three times scales[j], head by head a little apart."""
+    p = PagedKV(h, n, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    s = torch.tensor([scales[j % len(scales)] for j in range(n)], device="cuda")[:, None].repeat(1, h)
+    s[:, 1::2] *= 0.75
+    s = s.half().float()
+    x = torch.randn(n, h, PAGE, HD, generator=g, device="cuda") * 3 * s[:, :, None, None]
+    x[..., :loud] *= 9.0
+    p.write(x, torch.arange(n, device="cuda")[:, None], s, s.half())
+    return p
+
+
+SCALES = {"rising": [2.0 ** (i / 4 - 10) for i in range(68)], "falling": [2.0 ** (7 - i / 4) for i in range(68)],
+          "mixed": [0.25, 100.0, 2.0 ** -10, 1.0, 2.0, 0.5, 1.0009765625, 2.0 ** -14, 64.0],
+          "late": [0.25] * 37 + [1.5] + [0.3] * 41 + [2.0] + [0.3] * 50 + [40.0]}
+
+
+@pytest.mark.parametrize("group", [4, 7, 16])
+@pytest.mark.parametrize("kind", list(SCALES))
+@pytest.mark.parametrize("counts,tails", [([50, 33], [5, 0]), ([300, 131, 2], [0, 17, 3])])
+def test_scales_that_differ_by_page(kind, group, counts, tails):
+    """V's scales from below 2^-10 to above 100 within a sequence, in the order of its pages, so that
+    the weights' range is moved in the first tile, in later ones and behind a correction of the sums;
+    K's scales in another order (with q small enough that a score has no more than about 30)."""
+    H, n = 2, max(counts) + 3
+    k, v = _scaled(H, n, 200, SCALES[kind][::-1]), _scaled(H, n, 201, SCALES[kind], loud=1)
+    g = torch.Generator(device="cuda").manual_seed(202)
+    B, cap = len(counts), max(tails)
+    tab = torch.arange(max(counts), dtype=torch.int32, device="cuda").repeat(B, 1)
+    for dtype in (torch.float16, torch.bfloat16):
+        q = (torch.randn(B, H * group, 1, HD, generator=g, device="cuda") / max(SCALES[kind])).to(dtype)
+        tk, tv = (torch.randn(B, H, cap, HD, generator=g, device="cuda").to(dtype) for _ in range(2))
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+        for w in (None, torch.zeros(B, max(counts), device="cuda")):
+            want, tol, exp, wtol = _reference(k, v, q, tab, counts, tk, tv, tails, rounded=w is not None)
+            got = paged_decode_attention(k, v, q, tab, i32(counts), tk, tv, tail_len=i32(tails), weights=w, decay=0.0)
+            assert bool(((got.double() - want).abs() <= tol).all())
+            if w is not None:
+                on = torch.arange(max(counts), device="cuda") < i32(counts)[:, None]
+                assert bool(((w.double() - exp).abs() <= exp * (wtol + (H * group + 2) * 2.0 ** -24) + 1e-30)[on].all())
+
+
+@pytest.mark.parametrize("group", [1, 5, 16])
+@pytest.mark.parametrize("scale", [2.0 ** -8, 2.0 ** -12, 2.0 ** -14])
+@pytest.mark.parametrize("weights", [False, True])
+def test_light_tokens_of_small_scales(scale, group, weights):
+    """Tokens of 2^-17.5 of the weight of one that every wave meets, with small scales of V: what
+    they give keeps its bits, as with a scale of one.  2 x 8 x 131072 tokens by pages that stand many
+    times; every 32nd page's first token is the heavy one, with V = 0."""
+    H, W, every = 8, 8192, 32
+    k, v = PagedKV(H, 2, device="cuda"), PagedKV(H, 2, device="cuda")
+    one = torch.ones(2, H, device="cuda")
+    x = torch.zeros(2, H, PAGE, HD, device="cuda")
+    x[1, :, 0] = 1.0                                       # the heavy token's K
+    k.write(x, torch.arange(2, device="cuda")[:, None], one / 4, one.half() / 4)
+    x = torch.full_like(x, 15.0) * scale
+    x[1, :, 0] = 0.0
+    v.write(x, torch.arange(2, device="cuda")[:, None], one * scale, one.half() * scale)
+    a = 17.55 * math.log(2.0) / math.sqrt(HD)              # q k / sqrt(128) for the heavy token: 128 a / sqrt(128)
+    q = torch.full((2, H * group, 1, HD), a, device="cuda").bfloat16()
+    tab = (torch.arange(W, device="cuda") % every == 0).int().repeat(2, 1)
+    cnt = torch.tensor([W, W], dtype=torch.int32, device="cuda")
+    acc = torch.zeros(2, W, device="cuda") if weights else None
+    got = paged_decode_attention(k, v, q, tab, cnt, weights=acc)
+    z = float(q[0, 0, 0, 0].double()) * math.sqrt(HD)
+    heavy, light = W // every, W * PAGE - W // every
+    want = 15.0 * scale * light / (light + heavy * math.exp(z))
+    # P rounded once (2^-11) or its sum; a score's 130 x 2^-24 of |q||k| and the bias 4 |q|, twice; exp2
+    # (2^-16); the sums: 34 x 2^-23 of (15 + 32) scales; the output's rounding 2^-8
+    size = 128 * abs(a) * 5 / math.sqrt(HD)
+    tol = want * (2.0 ** -11 + 2 * 130 * 2.0 ** -24 * size + 2.0 ** -16 + 2.0 ** -8) + 34 * 2.0 ** -23 * 47 * scale
+    err = float((got.double() - want).abs().max())
+    assert err <= tol, (err / want, tol / want)
