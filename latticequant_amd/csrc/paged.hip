@@ -1178,7 +1178,8 @@ bool plan(int64_t n_seq, int64_t heads, int64_t group, int64_t width, int64_t ta
         return false;
     const int64_t tiles = (width + 1) / 2 + (tail_cap + 31) / 32;
     if (tiles + kAhead > INT_MAX / (n_seq * heads)) return false;
-    const int64_t most = (n_seq * heads * tiles + kWaves - 1) / kWaves;
+    // (no tile at all: the sequences' zeros are dealt to the workgroups)
+    const int64_t most = tiles ? (n_seq * heads * tiles + kWaves - 1) / kWaves : n_seq;
     p->whole = tiles <= kWhole && n_seq * heads <= kGroups;
     p->grid = (int)(p->whole ? n_seq * heads : most < kGroups ? most : kGroups);
     const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };

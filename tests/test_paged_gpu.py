@@ -650,3 +650,24 @@ def test_light_tokens_of_small_scales(scale, group, weights):
     tol = want * (2.0 ** -11 + 2 * 130 * 2.0 ** -24 * size + 2.0 ** -16 + 2.0 ** -8) + 34 * 2.0 ** -23 * 47 * scale
     err = float((got.double() - want).abs().max())
     assert err <= tol, (err / want, tol / want)
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("B,H", [(64, 8), (65, 8), (130, 8), (700, 1)])
+def test_no_pages_and_no_tail_of_many_units(B, H, weights):
+    """More units than are taken whole, none of which can have a token."""
+    k = _pool(H, 2, 95)
+    q = torch.randn(B, 2 * H, 1, HD, device="cuda").half()
+    none = torch.zeros(B, 0, dtype=torch.int32, device="cuda")
+    cnt = torch.full((B,), 3, dtype=torch.int32, device="cuda")
+    w = torch.zeros(B, 0, device="cuda") if weights else None
+    empty = torch.zeros(B, H, 0, HD, device="cuda").half()
+    for tails in ((None, None), (empty, empty)):
+        out = torch.full_like(q, 7.0)
+        paged_decode_attention(k, k, q, none, cnt, *tails, weights=w, out=out)
+        assert not bool(out.any())
+    cap, wide = torch.zeros(B, H, 9, HD, device="cuda").half(), torch.zeros(B, 3, dtype=torch.int32, device="cuda")
+    w = torch.ones(B, 3, device="cuda") if weights else None
+    out = torch.full_like(q, 7.0)
+    paged_decode_attention(k, k, q, wide, torch.zeros_like(cnt), cap, cap, tail_len=torch.zeros_like(cnt), weights=w, out=out)
+    assert not bool(out.any()) and (w is None or bool((w == 1).all()))

@@ -135,3 +135,10 @@ def test_a_pool_checks_page_numbers_of_64_bits(monkeypatch):
     for bad in (2 ** 32, -2 ** 32, 2 ** 63 - 1):
         with pytest.raises(ValueError, match="outside the pool"):
             p._numbers(torch.tensor([[bad]]), None, False)
+
+
+@pytest.mark.parametrize("weights", [False, True])
+def test_geometry_without_pages_and_tail(weights):
+    """A table of no width and no tail is a call like any other, however many units it has."""
+    for b, h in ((1, 1), (2, 2), (64, 8), (65, 8), (128, 8), (65535, 3)):
+        assert paged_workspace_size(b, h, 4, 0, 0, weights) > 0
