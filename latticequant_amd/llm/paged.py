@@ -45,7 +45,7 @@ class _Pool(ResidentKV):
         self.n_tokens = n_pages * PAGE
         self.room = torch.zeros(n_heads * n_pages, dtype=torch.int32, device=self.a.device)
         self.rec = torch.zeros(exc_cap, dtype=torch.uint8, device=self.a.device)
-        self._pages = None
+        self._pages = self._pages_of = None
 
     def _grow_exc(self, cap: int, keep: int) -> None:
         super()._grow_exc(cap, keep)
@@ -54,9 +54,10 @@ class _Pool(ResidentKV):
         self.rec = grown
 
     def pages(self) -> L.Pages:
-        """The buffers as the C ABI's lq_pages (cached as struct() is)."""
-        if self._st is None or self._pages is None:
-            self._pages = L.Pages(r=self.struct(), room=self.room.data_ptr(), rec=self.rec.data_ptr())
+        """The buffers as the C ABI's lq_pages (cached with the struct() that it holds)."""
+        st = self.struct()
+        if self._pages_of is not st:
+            self._pages, self._pages_of = L.Pages(r=st, room=self.room.data_ptr(), rec=self.rec.data_ptr()), st
         return self._pages
 
 

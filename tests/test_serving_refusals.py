@@ -142,3 +142,16 @@ def test_geometry_without_pages_and_tail(weights):
     """A table of no width and no tail is a call like any other, however many units it has."""
     for b, h in ((1, 1), (2, 2), (64, 8), (65, 8), (128, 8), (65535, 3)):
         assert paged_workspace_size(b, h, 4, 0, 0, weights) > 0
+
+
+def test_the_view_of_a_pool_follows_its_buffers():
+    """A longer exception list is in the next view of the pool, whatever took the resident
+    form's own view in between."""
+    p = PagedKV(2, 4, device="cpu", exc_cap=16)
+    assert p.struct().r.exc_cap == 16 and p.struct() is p.struct()
+    for cap, between in ((40, lambda: None), (90, p.pool.struct)):
+        p.pool._grow_exc(cap, 16)
+        between()
+        st = p.struct()
+        assert (st.r.exc_cap, st.r.exc, st.rec) == (cap, p.pool.exc.data_ptr(), p.pool.rec.data_ptr())
+        assert p.exc_cap == cap and p.pool.rec.numel() == cap
