@@ -48,9 +48,9 @@ class _Pool(ResidentKV):
         self._pages = self._pages_of = None
 
     def _grow_exc(self, cap: int, keep: int) -> None:
-        super()._grow_exc(cap, keep)
         grown = torch.zeros(cap, dtype=torch.uint8, device=self.device)
         grown[:keep] = self.rec[:keep]
+        super()._grow_exc(cap, keep)           # (where memory runs out, both are as they were)
         self.rec = grown
 
     def pages(self) -> L.Pages:

@@ -155,3 +155,19 @@ def test_the_view_of_a_pool_follows_its_buffers():
         st = p.struct()
         assert (st.r.exc_cap, st.r.exc, st.rec) == (cap, p.pool.exc.data_ptr(), p.pool.rec.data_ptr())
         assert p.exc_cap == cap and p.pool.rec.numel() == cap
+
+
+@pytest.mark.parametrize("fails", [torch.int16, torch.uint8])
+def test_a_list_that_cannot_be_lengthened_stays_whole(fails, monkeypatch):
+    """Where there is no memory for a longer list, entries and their records stay as long as each other."""
+    p = PagedKV(2, 4, device="cpu", exc_cap=16)
+    zeros = torch.zeros
+
+    def full(*a, **kw):
+        if kw.get("dtype") is fails:
+            raise torch.OutOfMemoryError("no room")
+        return zeros(*a, **kw)
+    monkeypatch.setattr(torch, "zeros", full)
+    with pytest.raises(torch.OutOfMemoryError):
+        p.pool._grow_exc(40, 16)
+    assert p.struct().r.exc_cap == p.exc_cap == 16 and p.pool.rec.numel() == 16
