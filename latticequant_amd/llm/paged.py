@@ -40,6 +40,8 @@ def _no_grad(what: str, *ts) -> None:
 class _Pool(ResidentKV):
     """The resident form behind a PagedKV: its exception list has the entries' records beside it."""
 
+    _by_number = True
+
     def __init__(self, n_heads: int, n_pages: int, device, exc_cap: int):
         super().__init__(n_heads, n_pages * PAGE, device=device, exc_cap=exc_cap)
         self.n_tokens = n_pages * PAGE

@@ -38,6 +38,8 @@ class ResidentKV:
     being told: given here, or that of the rows appended; None where rows of different
     groupings were."""
 
+    _by_number = False   # a pool of pages: a block keeps its place, and exception entries of its own
+
     def __init__(self, n_heads: int, cap_tokens: int, device=None, exc_cap: Optional[int] = None,
                  n_seq: Optional[int] = None):
         if n_heads <= 0 or cap_tokens <= 0:
@@ -94,6 +96,8 @@ class ResidentKV:
         nb = (cap_tokens + RB - 1) // RB
         if nb <= self.cap_blocks:
             return
+        if self._by_number:
+            raise ValueError("a pool of pages keeps its size")
         H, ob = self.n_heads, self.cap_blocks
         used = (self.n_tokens + RB - 1) // RB
 
@@ -338,6 +342,8 @@ def reorder_sequences(residents: Sequence[ResidentKV], index: torch.Tensor, t_fr
         raise ValueError(f"index must name 1..{MAX_REORDER} sequences that the heads divide into evenly "
                          "(more: ResidentKV.select makes a reordered copy)")
     H, T = r0.n_heads, r0.n_tokens
+    if any(r._by_number for r in residents):
+        raise ValueError("the blocks of a pool of pages keep their places: reorder the tables")
     for r in residents:
         if r.n_heads != H or r.n_tokens != T or r.a.device != dev:
             raise ValueError("the prefixes must have the same heads, tokens and device")

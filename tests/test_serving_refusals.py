@@ -8,6 +8,7 @@ from latticequant_amd import _lib as L
 from latticequant_amd._dev import int32_on
 from latticequant_amd.llm.logprobs import token_logprobs
 from latticequant_amd.llm.paged import PagedKV, evict_pages, paged_decode_attention, paged_workspace_size
+from latticequant_amd.llm.resident import reorder_sequences
 from latticequant_amd.llm.tree import _ints
 
 
@@ -171,3 +172,17 @@ def test_a_list_that_cannot_be_lengthened_stays_whole(fails, monkeypatch):
     with pytest.raises(torch.OutOfMemoryError):
         p.pool._grow_exc(40, 16)
     assert p.struct().r.exc_cap == p.exc_cap == 16 and p.pool.rec.numel() == 16
+
+
+def test_a_pool_keeps_its_size_and_its_blocks():
+    """What the resident form behind a pool would do without the pages' rooms (their array is as
+    long as the pool, and a moved block would write over another's entries)."""
+    p = PagedKV(4, 8, device="cpu")
+    p.pool.reserve(8 * 16)
+    with pytest.raises(ValueError, match="keeps its size"):
+        p.pool.reserve(9 * 16)
+    assert p.struct().r.cap_blocks == 8 and p.pool.room.numel() == 32
+    for move in (lambda: p.pool.reorder(torch.tensor([1, 0])),
+                 lambda: reorder_sequences([p.pool], torch.tensor([1, 0]), 16)):
+        with pytest.raises(ValueError, match="keep their places"):
+            move()
