@@ -12,7 +12,8 @@ together (llm/compressed_kv_cache.py:384-395), here each has its own length.
 * ``evict_pages`` shortens the sequences to the pages of most weight: their numbers leave
   the table, nothing is copied.
 
-None of it waits for the device, except ``write`` of many pages at once.
+None of it waits for the device, except ``write``: of more than 64 blocks (pages times heads), and
+where only the count of exceptions tells whether the list is long enough.
 """
 from __future__ import annotations
 
@@ -67,9 +68,13 @@ class PagedKV:
     """A pool of n_pages pages of n_heads kv heads (K or V of a layer).
 
     exc_cap: room for exceptions (vectors outside the 5-bit range), by default eight a
-    page and head; ``write`` lengthens the list where it is too short, which moves it: a
-    graph captured over the pool holds the list as it was, so give a sufficient exc_cap
-    before capturing, or capture again when ``exc_cap`` has grown."""
+    page and head.  ``write`` lengthens the list, which moves it, where it is too short: where
+    the entries in use and 256 more for each page and head that is written (of which a write
+    of more than 64 counts only those it turns out to need) do not fit.  A page has the next power
+    of two of its largest number of exceptions in use, and under as many again of
+    earlier ones: 512 a page and head and 256 a page and head of a write always suffice.
+    A graph captured over the pool holds the list as it was: capture again when
+    ``exc_cap`` has grown."""
 
     def __init__(self, n_heads: int, n_pages: int, device=None, exc_cap: Optional[int] = None):
         if n_heads < 1 or n_pages < 1:

@@ -163,12 +163,16 @@ class ResidentKV:
     def _with_exceptions(self, n_new: int, launch, anew: bool) -> None:
         """launch(), which may add n_new exception entries, with room for them.  anew: where
         the list was too short and launch runs again, its entries are numbered again (else
-        those that have numbers keep them)."""
+        those that have numbers keep them, and a graph may hold the list: it moves only where
+        the entries in use and n_new do not fit, which the host may have to wait for)."""
         if n_new <= self.ASYNC_MAX_VECTORS:
             if self._exc_read is not None and self._exc_read[1].query():
                 host, _, after = self._exc_read
                 self._exc_known, self._exc_since, self._exc_read = int(host[0]), after, None
             need = self._exc_known + self._exc_since + n_new
+            if need > self.exc_cap >= self._exc_known + n_new and not anew:
+                self._exc_known, self._exc_since, self._exc_read = int(self.n_exc.item()), 0, None
+                need = self._exc_known + n_new
             if need > self.exc_cap:
                 self._grow_exc(max(2 * self.exc_cap, need), self.exc_cap)
             launch()

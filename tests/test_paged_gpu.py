@@ -671,3 +671,48 @@ def test_no_pages_and_no_tail_of_many_units(B, H, weights):
     out = torch.full_like(q, 7.0)
     paged_decode_attention(k, k, q, wide, torch.zeros_like(cnt), cap, cap, tail_len=torch.zeros_like(cnt), weights=w, out=out)
     assert not bool(out.any()) and (w is None or bool((w == 1).all()))
+
+
+# ----------------------------------------------------------- exception lists --
+
+def test_a_list_that_suffices_does_not_move():
+    """Many small writes in a row, each of which might be nothing but exceptions: the list has room
+    for those there are, so a graph captured over it stays right."""
+    H, n = 8, 96
+    k, v = (PagedKV(H, n, device="cuda", exc_cap=4096) for _ in range(2))
+    x, s = _rows(n, H, PAGE, 110, loud=0)
+    x /= 2                                                 # within the range: six deviations
+    x[:, :, 3, 40] = 9.0                                   # an exception a page and head
+    every = torch.arange(n, device="cuda")[:, None]
+    k.write(x, every, s, s.half())
+    v.write(x, every, s, s.half())
+    tab, cnt = every.t().int().contiguous(), torch.tensor([n], dtype=torch.int32, device="cuda")
+    q, out = torch.randn(1, 2 * H, 1, HD, device="cuda").half(), torch.empty(1, 2 * H, 1, HD, device="cuda").half()
+    work = paged_attn_workspace(1, H, 2, n, 0, device="cuda")
+    paged_decode_attention(k, v, q, tab, cnt, work=work, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged_decode_attention(k, v, q, tab, cnt, work=work, out=out)
+    torch.cuda.synchronize()
+    at = [(p.pool.exc.data_ptr(), p.pool.rec.data_ptr()) for p in (k, v)]
+    for i in range(3):
+        x, s = _rows(n, H, PAGE, 111 + i, loud=0)
+        x /= 2
+        x[:, :, 3 + i, 40] = 9.0
+        for j in range(n):
+            for p in (k, v):
+                p.write(x[j:j + 1], every[j:j + 1], s[j:j + 1], s[j:j + 1].half())
+        assert [(p.pool.exc.data_ptr(), p.pool.rec.data_ptr()) for p in (k, v)] == at and k.exc_cap == 4096
+        assert n * H <= int(k.pool.n_exc) <= 4096 - 256 * H and int(k.pool.status) == 0
+        fresh = ResidentKV(n * H, PAGE, device="cuda")
+        fresh.append(x.reshape(1, n * H, PAGE, HD), s.reshape(-1), s.reshape(-1).half())
+        assert torch.equal(k.read(every).reshape(n * H, PAGE, HD), fresh.dequant())
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, paged_decode_attention(k, v, q, tab, cnt))
+    x = torch.randn(1, H, PAGE, HD, device="cuda") * 100   # nothing but exceptions: it has to move now
+    t = torch.full((1, H), 0.25, device="cuda")
+    while k.exc_cap == 4096:
+        k.write(x, every[int(k.pool.n_exc) // 2048:][:1], t, t.half())
+        assert int(k.pool.n_exc) <= k.exc_cap and int(k.pool.status) == 0
