@@ -716,3 +716,40 @@ def test_a_list_that_suffices_does_not_move():
     while k.exc_cap == 4096:
         k.write(x, every[int(k.pool.n_exc) // 2048:][:1], t, t.half())
         assert int(k.pool.n_exc) <= k.exc_cap and int(k.pool.status) == 0
+
+
+@pytest.mark.parametrize("cap", [1, 700, 5000])
+def test_a_large_write_that_overflows_the_list(cap):
+    """More than 16384 vectors at once and a list too short for their exceptions, twice, on top of
+    pages that own entries: it is lengthened and the call repeated, with the rooms already taken."""
+    H, n = 8, 40
+    p = PagedKV(H, n, device="cuda", exc_cap=cap)
+    rows, scales = _rows(n, H, PAGE, 120, loud=3)
+    every = torch.arange(n, device="cuda")[:, None]
+
+    def check():
+        r = ResidentKV(n * H, PAGE, device="cuda")
+        r.append(rows.reshape(1, n * H, PAGE, HD), scales.reshape(-1), scales.reshape(-1).half())
+        assert int(r.status) == 0
+        assert torch.equal(p.read(every).reshape(n * H, PAGE, HD), r.dequant())
+        assert int(p.pool.status) == 0 and int(p.pool.n_exc) <= p.exc_cap == p.pool.rec.numel()
+
+    p.write(rows[:4], every[:4], scales[:4], scales[:4].half())          # within the bound of small writes
+    p.write(rows[4:], every[4:], scales[4:], scales[4:].half())
+    grown = p.exc_cap
+    assert grown > cap
+    check()
+    x, s = _rows(30, H, PAGE, 121, loud=100)                             # nearly all are exceptions now
+    rows[5:35], scales[5:35] = x, s
+    p.write(x, every[5:35], s, s.half())
+    assert p.exc_cap > grown
+    check()
+    q = torch.randn(2, 4 * H, 1, HD, device="cuda").half() / 16
+    tab = torch.stack([every[:, 0], every[:, 0].flip(0)]).int()
+    cnt = torch.tensor([n, 17], dtype=torch.int32, device="cuda")
+    for w in (None, torch.zeros(2, n, device="cuda")):
+        want, tol, exp, wtol = _reference(p, p, q, tab, [n, 17], None, None, [0, 0], rounded=w is not None)
+        got = paged_decode_attention(p, p, q, tab, cnt, weights=w)
+        assert bool(((got.double() - want).abs() <= tol).all())
+        if w is not None:
+            assert bool(((w.double() - exp).abs() <= exp * (wtol + (4 * H + 2) * 2.0 ** -24) + 1e-30).all())
