@@ -323,8 +323,7 @@ def evict_pages(pages: torch.Tensor, n_pages: torch.Tensor, weights: torch.Tenso
         if W == 0:
             out.n_pages.zero_()
             return out
-        big = 2 ** 29                          # beyond any table
-        L.check(lib.lq_evict_pages(tab.data_ptr(), cnt.data_ptr(), w.data_ptr(), B, W, min(keep, 2 * big), min(sink, big),
-                                   min(recent, big), out.pages.data_ptr(), out.n_pages.data_ptr(),
+        L.check(lib.lq_evict_pages(tab.data_ptr(), cnt.data_ptr(), w.data_ptr(), B, W, min(keep, 2 * W), min(sink, W),
+                                   min(recent, W), out.pages.data_ptr(), out.n_pages.data_ptr(),
                                    out.weights.data_ptr(), out.freed.data_ptr(), L.raw_stream(dev)), "lq_evict_pages")
     return out

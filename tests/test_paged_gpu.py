@@ -753,3 +753,13 @@ def test_a_large_write_that_overflows_the_list(cap):
         assert bool(((got.double() - want).abs() <= tol).all())
         if w is not None:
             assert bool(((w.double() - exp).abs() <= exp * (wtol + (4 * H + 2) * 2.0 ** -24) + 1e-30).all())
+
+
+@pytest.mark.parametrize("big", [2 ** 29 - 1, 2 ** 29, 2 ** 30, 2 ** 31 - 1, 2 ** 40])
+def test_eviction_that_protects_more_than_there_is(big):
+    w, n = torch.rand(2, 5, device="cuda"), torch.tensor([5, 3], device="cuda")
+    pages = torch.arange(10, device="cuda").reshape(2, 5)
+    for keep, sink, recent in ((big, big, 0), (big, 0, big), (2 * big, big, big), (big + 1, 1, big), (big, 0, 0)):
+        got = evict_pages(pages, n, w, keep, sink, recent)
+        assert got.n_pages.tolist() == [5, 3] and got.pages.tolist() == [[0, 1, 2, 3, 4], [5, 6, 7, -1, -1]]
+        assert bool((got.freed == -1).all())
