@@ -537,10 +537,16 @@ int lq_token_logprobs(const void *d_logits, int dtype, int64_t stride, int64_t r
     if (!d_logits || dtype < 0 || dtype > 2 || stride < 0 || rows < 1 || rows > INT_MAX || vocab < 1 || vocab > INT_MAX ||
         top < 0 || top > kTop || top > vocab || !d_logprob || !d_entropy || (top && (!d_ids || !d_top)))
         return LQ_ERR_ARG;
-    const LogArgs A = {static_cast<const char*>(d_logits), stride, vocab, d_tokens, top, d_logprob, d_entropy, d_ids, d_top};
-    if (dtype == LQ_F32) launch<LQ_F32>(A, rows, s);
-    else if (dtype == LQ_BF16) launch<LQ_BF16>(A, rows, s);
-    else launch<LQ_F16>(A, rows, s);
+    constexpr int64_t kRows = 1 << 22;         // of a launch: a grid has fewer than 2^32 threads
+    const char* logits = static_cast<const char*>(d_logits);
+    for (int64_t r = 0; r < rows; r += kRows) {
+        const LogArgs A = {logits + r * stride * (dtype == LQ_F32 ? 4 : 2), stride, vocab, d_tokens ? d_tokens + r : nullptr, top,
+                           d_logprob + r, d_entropy + r, top ? d_ids + r * top : nullptr, top ? d_top + r * top : nullptr};
+        const int64_t n = rows - r < kRows ? rows - r : kRows;
+        if (dtype == LQ_F32) launch<LQ_F32>(A, n, s);
+        else if (dtype == LQ_BF16) launch<LQ_BF16>(A, n, s);
+        else launch<LQ_F16>(A, n, s);
+    }
     return launch_status();
 }
 

@@ -209,3 +209,21 @@ def test_logits_of_large_size_and_small_differences(centre, vocab):
     x = torch.randn(4, vocab, device="cuda") * 4 + centre
     tok = torch.randint(0, vocab, (4,), device="cuda")
     _check(x, tok, 20, token_logprobs(x, tok, 20))
+
+
+@pytest.mark.parametrize("top", [0, 2])
+def test_more_rows_than_a_grid_has(top):
+    """2^24 + 3 rows: more than 2^32 threads hold, at a row a workgroup."""
+    n, V = 2 ** 24 + 3, 5
+    x = torch.randn(n, V, device="cuda").half()
+    tok = torch.randint(-1, V, (n,), device="cuda")
+    got = token_logprobs(x, tok, top)
+    for i in (slice(0, 999), slice(2 ** 22 - 500, 2 ** 22 + 500), slice(2 ** 23 - 9, 2 ** 23 + 9), slice(n - 999, n)):
+        part = [None if t is None else t[i] for t in got]
+        assert not bool(part[0][tok[i] < 0].any())
+        part[0] = torch.where(tok[i] < 0, torch.log_softmax(x[i].double(), 1)[:, 0].float(), part[0])
+        _check(x[i], tok[i], top, type(got)(*part))
+    # a sum over all of them says that none was left out
+    p = torch.log_softmax(x.float(), 1)
+    want = torch.where(tok < 0, 0.0, p.gather(1, tok.clamp_min(0)[:, None])[:, 0])
+    assert bool(((got.logprob - want).abs() < 1e-4).all()) and bool((got.entropy > 0).all())
