@@ -267,7 +267,8 @@ __global__ __launch_bounds__(256) void k_res_dequant(lq_resident r, int64_t h0, 
 // records of exceptions; 134 MB written at 3 TB/s).
 struct PageMap {
     const int32_t* pages;
-    uint32_t heads, per;                       // of the pool; blocks of a row
+    uint32_t heads, per, first;                // of the pool; blocks of a row; the launch's first unit
+    __device__ __forceinline__ uint32_t unit() const { return first + blockIdx.x; }
     __device__ __forceinline__ int64_t block(const lq_resident& r, uint32_t hh, uint32_t bb) const {
         const int64_t p = pages[(int64_t)(hh / heads) * per + bb];
         return p >= 0 && p < r.cap_blocks ? (int64_t)(hh % heads) * r.cap_blocks + p : -1;
@@ -277,7 +278,7 @@ struct PageMap {
 __global__ __launch_bounds__(256) void k_page_quant(const void* __restrict__ x, int dtype, PageMap P,
                                                     const float* __restrict__ scale32,
                                                     const uint16_t* __restrict__ scale16, lq_resident r) {
-    const uint32_t hh = blockIdx.x / P.per, bb = blockIdx.x % P.per;
+    const uint32_t hh = P.unit() / P.per, bb = P.unit() % P.per;
     const int64_t rb = P.block(r, hh, bb);
     if (rb >= 0) quant_block<true>(x, dtype, (int64_t)P.per * kRB, scale32, scale16, r, hh, bb, rb);
 }
@@ -290,9 +291,9 @@ __global__ __launch_bounds__(256) void k_page_quant(const void* __restrict__ x, 
 __global__ __launch_bounds__(1024) void k_page_rooms(PageMap P, int64_t units, lq_resident r, int32_t* __restrict__ room) {
     constexpr int U = 4;
     __shared__ uint32_t part[16];
-    __shared__ uint32_t s_run;
+    __shared__ uint64_t s_run;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    uint32_t run = (uint32_t)*r.n_exc;
+    uint64_t run = (uint32_t)*r.n_exc;
     for (int64_t i0 = 0; i0 < units; i0 += U * 1024) {
         int64_t rb[U];
         uint32_t n[U], had[U], need[U], sum = 0;
@@ -320,11 +321,11 @@ __global__ __launch_bounds__(1024) void k_page_rooms(PageMap P, int64_t units, l
         if (lane == 63) part[wave] = upto;
         __syncthreads();
         for (int w = 0; w < wave; w++) upto += part[w];
-        uint32_t at = run + upto - sum;
+        uint64_t at = run + upto - sum;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (!need[u]) continue;
-            r.meta[rb[u] * 4 + 2] = at;
+            r.meta[rb[u] * 4 + 2] = (uint32_t)min(at, (uint64_t)INT_MAX);   // (as far as any list goes)
             room[rb[u]] = (int32_t)need[u];
             at += need[u];
         }
@@ -332,26 +333,26 @@ __global__ __launch_bounds__(1024) void k_page_rooms(PageMap P, int64_t units, l
         __syncthreads();
         run = s_run;
     }
-    if (tid == 0) *r.n_exc = (int32_t)min(run, (uint32_t)INT_MAX);
+    if (tid == 0) *r.n_exc = (int32_t)min(run, (uint64_t)INT_MAX);
 }
 
 __global__ __launch_bounds__(256) void k_page_fill(const void* __restrict__ x, int dtype, PageMap P,
                                                    const float* __restrict__ scale32, lq_resident r,
                                                    const int32_t* __restrict__ room, uint8_t* __restrict__ rec) {
-    const uint32_t hh = blockIdx.x / P.per, bb = blockIdx.x % P.per;
+    const uint32_t hh = P.unit() / P.per, bb = P.unit() % P.per;
     const int64_t rb = P.block(r, hh, bb);
     // (the masks of a page that stands twice may be of both, with more exceptions than either has)
     if (rb >= 0) fill_block(x, dtype, (int64_t)P.per * kRB, scale32, r, hh, bb, rb, room[rb], rec);
 }
 
 __global__ __launch_bounds__(256) void k_page_dequant(lq_resident r, PageMap P, void* __restrict__ out, int out_dtype) {
-    const uint32_t hh = blockIdx.x / P.per, bb = blockIdx.x % P.per;
+    const uint32_t hh = P.unit() / P.per, bb = P.unit() % P.per;
     const int64_t rb = P.block(r, hh, bb);
     if (rb >= 0) {
         dequant_block(r, hh, bb, rb, P.per, out, out_dtype);
     } else {
         const float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        store8(out, out_dtype, (int64_t)blockIdx.x * 256 + threadIdx.x, y);
+        store8(out, out_dtype, (int64_t)P.unit() * 256 + threadIdx.x, y);
     }
 }
 
@@ -1008,6 +1009,16 @@ int64_t n_splits(int64_t n_heads, int group, int64_t t_prefix, int64_t t_tail) {
     return n > 0 ? n : 1;
 }
 
+// f(grid) for all units, a workgroup each: a grid has fewer than 2^32 threads
+template <typename F>
+void each_grid(int64_t units, PageMap* P, F f) {
+    constexpr int64_t kUnits = 1 << 23;
+    for (int64_t u = 0; u < units; u += kUnits) {
+        P->first = (uint32_t)u;
+        f(dim3((unsigned)(units - u < kUnits ? units - u : kUnits)));
+    }
+}
+
 bool res_ok(const lq_resident* r) {
     return r && r->a && r->b && r->mask && r->meta && r->scale && r->n_exc && r->status && r->n_heads > 0 &&
            r->cap_blocks > 0 && r->exc_cap >= 0;
@@ -1105,10 +1116,14 @@ int lq_page_quantize(const void *d_x, int dtype, int64_t n, int64_t t_tokens, co
     const int64_t per = t_tokens / kRB;
     if (n > INT_MAX / per || n * per > INT_MAX / r.n_heads) return LQ_ERR_ARG;
     const int64_t units = n * r.n_heads * per;
-    const PageMap P = {d_pages, (uint32_t)r.n_heads, (uint32_t)per};
-    hipLaunchKernelGGL(k_page_quant, dim3((unsigned)units), dim3(256), 0, s, d_x, dtype, P, d_scale32, d_scale16, r);
+    PageMap P = {d_pages, (uint32_t)r.n_heads, (uint32_t)per, 0};
+    each_grid(units, &P, [&](const dim3& g) {
+        hipLaunchKernelGGL(k_page_quant, g, dim3(256), 0, s, d_x, dtype, P, d_scale32, d_scale16, r);
+    });
     hipLaunchKernelGGL(k_page_rooms, dim3(1), dim3(1024), 0, s, P, units, r, p->room);
-    hipLaunchKernelGGL(k_page_fill, dim3((unsigned)units), dim3(256), 0, s, d_x, dtype, P, d_scale32, r, p->room, p->rec);
+    each_grid(units, &P, [&](const dim3& g) {
+        hipLaunchKernelGGL(k_page_fill, g, dim3(256), 0, s, d_x, dtype, P, d_scale32, r, p->room, p->rec);
+    });
     return launch_status();
 }
 
@@ -1117,8 +1132,10 @@ int lq_page_dequant(const lq_pages *p, const int32_t *d_pages, int64_t n, int64_
     if (!p || !res_ok(&p->r) || !d_pages || !d_out || out_dtype < 0 || out_dtype > 2 || n < 1 || per < 1 ||
         n > INT_MAX / per || n * per > INT_MAX / p->r.n_heads)
         return LQ_ERR_ARG;
-    const PageMap P = {d_pages, (uint32_t)p->r.n_heads, (uint32_t)per};
-    hipLaunchKernelGGL(k_page_dequant, dim3((unsigned)(n * p->r.n_heads * per)), dim3(256), 0, s, p->r, P, d_out, out_dtype);
+    PageMap P = {d_pages, (uint32_t)p->r.n_heads, (uint32_t)per, 0};
+    each_grid(n * p->r.n_heads * per, &P, [&](const dim3& g) {
+        hipLaunchKernelGGL(k_page_dequant, g, dim3(256), 0, s, p->r, P, d_out, out_dtype);
+    });
     return launch_status();
 }
 

@@ -174,7 +174,7 @@ class ResidentKV:
                 self._exc_known, self._exc_since, self._exc_read = int(self.n_exc.item()), 0, None
                 need = self._exc_known + n_new
             if need > self.exc_cap:
-                self._grow_exc(max(2 * self.exc_cap, need), self.exc_cap)
+                self._grow_exc(self._longer(need), self.exc_cap)
             launch()
             self._exc_since += n_new
             if self._exc_read is not None:
@@ -194,11 +194,17 @@ class ResidentKV:
                 if n1 <= self.exc_cap:
                     break
                 # grow the exception list to the exact need and launch again
-                self._grow_exc(max(n1, 2 * self.exc_cap), n0 if anew else self.exc_cap)
+                self._grow_exc(self._longer(n1), n0 if anew else self.exc_cap)
                 if anew:
                     self.n_exc.fill_(n0)
                 self.status.zero_()
             self._exc_known, self._exc_since, self._exc_read = n1, 0, None
+
+    def _longer(self, need: int) -> int:
+        """The length of a list that gets too short for `need` entries."""
+        if need >= 2 ** 31 - 1:
+            raise RuntimeError("an exception list has fewer than 2^31 entries")
+        return min(max(2 * self.exc_cap, need), 2 ** 31 - 2)
 
     def _grow_exc(self, cap: int, keep: int) -> None:
         """A longer exception list holding the first `keep` entries."""

@@ -763,3 +763,47 @@ def test_eviction_that_protects_more_than_there_is(big):
         got = evict_pages(pages, n, w, keep, sink, recent)
         assert got.n_pages.tolist() == [5, 3] and got.pages.tolist() == [[0, 1, 2, 3, 4], [5, 6, 7, -1, -1]]
         assert bool((got.freed == -1).all())
+
+
+def test_more_blocks_than_a_grid_has():
+    """2^24 + 7 blocks in one write and one read: more than 2^32 threads hold, at a workgroup a block.
+    All but a few numbers are outside the pool."""
+    n = 2 ** 24 + 7
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("rows of 69 GB")
+    p = _pool(1, 12, 130)
+    num = torch.full((1, n), -1, dtype=torch.int32, device="cuda")
+    places = [0, 5, 2 ** 23 - 1, 2 ** 23, 2 ** 23 + 1, n - 2, n - 1]
+    for i, j in enumerate(places):
+        num[0, j] = i
+    before = p.read(torch.arange(7, 12, device="cuda")[None])
+    x = torch.zeros(1, 1, n * PAGE, HD, dtype=torch.float16, device="cuda")
+    rows, s = _rows(1, 1, len(places) * PAGE, 131, loud=3)
+    for i, j in enumerate(places):
+        x[:, :, j * PAGE:(j + 1) * PAGE] = rows[:, :, i * PAGE:(i + 1) * PAGE]
+    p.write(x, num, s, s.half())
+    del x
+    fresh = ResidentKV(1, len(places) * PAGE, device="cuda")
+    fresh.append(rows, s, s.half())
+    want = fresh.dequant()
+    assert torch.equal(p.read(torch.arange(7, device="cuda")[None])[0], want)
+    assert torch.equal(p.read(torch.arange(7, 12, device="cuda")[None]), before) and int(p.pool.status) == 0
+    got = p.read(num)[0, 0].view(n, PAGE, HD)
+    assert torch.equal(got[places].reshape(1, -1, HD), want)
+    got[places] = 0.0
+    assert not bool(torch.stack([got[i:i + 2 ** 20].any() for i in range(0, n, 2 ** 20)]).any())
+
+
+def test_numbers_of_entries_end_at_32_bits():
+    """Rooms that would lie past 2^31 entries are in no list: the write fails, what is there stays."""
+    p = _pool(8, 12, 140)
+    every = torch.arange(12, device="cuda")[:, None]
+    before = p.read(every[:2])
+    p.pool.n_exc.fill_(2 ** 31 - 100)
+    y, t = torch.randn(10, 8, PAGE, HD, device="cuda") * 100, torch.full((10, 8), 0.25, device="cuda")
+    cap = p.exc_cap
+    with pytest.raises(RuntimeError, match="fewer than 2\\^31"):
+        p.write(y, every[2:], t, t.half())
+    assert int(p.pool.n_exc) == 2 ** 31 - 1 and p.exc_cap == cap
+    assert torch.equal(p.read(every[:2]), before)
+    assert not bool(p.read(every[2:]).isnan().any())
