@@ -755,7 +755,7 @@ int lq_paged_attention(const lq_pages *k, const lq_pages *v, const lq_rows *q, i
  * `recent` stay, and of the others those of most weight (NaN above all, the lower place of
  * equal ones), in their order.  Tables and weights are [n_seq][max_pages]; those written
  * are others than those read.  d_out_pages / d_out_weights: the d_out_n[b] kept, then -1 and
- * 0; d_freed: the others' numbers in order, then -1. */
+ * 0; d_freed: the others' numbers in order, then -1.  n_seq below 2^22. */
 int lq_evict_pages(const int32_t *d_pages, const int32_t *d_n_pages, const float *d_weights, int64_t n_seq,
                    int64_t max_pages, int64_t keep, int64_t sink, int64_t recent, int32_t *d_out_pages, int32_t *d_out_n,
                    float *d_out_weights, int32_t *d_freed, hipStream_t s);

@@ -1299,7 +1299,7 @@ int lq_evict_pages(const int32_t *d_pages, const int32_t *d_n_pages, const float
                    int64_t max_pages, int64_t keep, int64_t sink, int64_t recent, int32_t *d_out_pages, int32_t *d_out_n,
                    float *d_out_weights, int32_t *d_freed, hipStream_t s) {
     if (!d_pages || !d_n_pages || !d_weights || !d_out_pages || !d_out_n || !d_out_weights || !d_freed || n_seq < 1 ||
-        n_seq > INT_MAX || max_pages < 1 || max_pages > INT_MAX / 2 || sink < 0 || recent < 0 || sink > INT_MAX / 2 ||
+        n_seq > UINT32_MAX / kEvictThreads || max_pages < 1 || max_pages > INT_MAX / 2 || sink < 0 || recent < 0 || sink > INT_MAX / 2 ||
         recent > INT_MAX / 2 || keep < sink + recent || keep > INT_MAX)
         return LQ_ERR_ARG;
     const EvictArgs A = {d_pages, d_n_pages, d_weights, max_pages, (int)keep, (int)sink, (int)recent,

@@ -300,8 +300,8 @@ def evict_pages(pages: torch.Tensor, n_pages: torch.Tensor, weights: torch.Tenso
         raise ValueError("weights must be (B, W) fp32")
     B, W = weights.shape
     dev = weights.device
-    if B < 1:
-        raise ValueError("at least one sequence")
+    if not 1 <= B < 2 ** 22:
+        raise ValueError("at least one sequence, and fewer than 2^22")
     if sink < 0 or recent < 0 or keep < sink + recent:
         raise ValueError("keep must be at least sink + recent, and neither below 0")
     if dev.type != "cuda":

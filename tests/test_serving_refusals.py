@@ -186,3 +186,14 @@ def test_a_pool_keeps_its_size_and_its_blocks():
                  lambda: reorder_sequences([p.pool], torch.tensor([1, 0]), 16)):
         with pytest.raises(ValueError, match="keep their places"):
             move()
+
+
+def test_eviction_of_more_sequences_than_a_grid_has():
+    """2^32 threads of 1024 a sequence."""
+    lib = L.load()
+    for n in (2 ** 22, 2 ** 31 - 1):
+        assert lib.lq_evict_pages(16, 16, 16, n, 4, 2, 1, 1, 16, 16, 16, 16, None) == L.LQ_ERR_ARG
+    n = 2 ** 22
+    with pytest.raises(ValueError, match="fewer than 2\\^22"):
+        evict_pages(torch.zeros(1, 2, dtype=torch.int32).expand(n, 2), torch.zeros(1, dtype=torch.int32).expand(n),
+                    torch.zeros(1, 2).expand(n, 2), 1)
