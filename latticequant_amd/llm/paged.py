@@ -34,7 +34,7 @@ PAGE = RB        # tokens of a page
 def _no_grad(what: str, *ts) -> None:
     if torch.is_grad_enabled():
         for t in ts:
-            if t.requires_grad:
+            if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 
@@ -125,7 +125,7 @@ class PagedKV:
             raise ValueError(f"pages must have shape {(n, T // PAGE)}, not {tuple(pages.shape)}")
         if n * T == 0:
             return
-        _no_grad("a write to pages", x)
+        _no_grad("a write to pages", x, scale32, scale16)
         num = self._numbers(pages, None, True)
         lib, r = L.lib(), self.pool
         with L.on_device(self.device):
@@ -231,7 +231,7 @@ def paged_decode_attention(k: PagedKV, v: PagedKV, q: torch.Tensor, pages: torch
     for t in given:
         if t.dtype is not dt or t.device != dev:
             raise ValueError("q and the tail must be of one type, on the pools' device")
-    _no_grad("paged_decode_attention", *given)
+    _no_grad("paged_decode_attention", *given, weights, out)
     if weights is not None and (weights.shape != (B, W) or weights.dtype is not torch.float32 or weights.device != dev or
                                 not weights.is_contiguous()):
         raise ValueError("weights must be (B, W) fp32, contiguous, on the pools' device")
@@ -304,6 +304,7 @@ def evict_pages(pages: torch.Tensor, n_pages: torch.Tensor, weights: torch.Tenso
         raise ValueError("at least one sequence, and fewer than 2^22")
     if sink < 0 or recent < 0 or keep < sink + recent:
         raise ValueError("keep must be at least sink + recent, and neither below 0")
+    _no_grad("evict_pages", weights)
     if dev.type != "cuda":
         raise ValueError("weights must be on the GPU")
     lib = L.lib()

@@ -197,3 +197,16 @@ def test_eviction_of_more_sequences_than_a_grid_has():
     with pytest.raises(ValueError, match="fewer than 2\\^22"):
         evict_pages(torch.zeros(1, 2, dtype=torch.int32).expand(n, 2), torch.zeros(1, dtype=torch.int32).expand(n),
                     torch.zeros(1, 2).expand(n, 2), 1)
+
+
+def test_nothing_that_wants_a_gradient_is_written_or_passed_by():
+    a = _args()
+    for name, t in (("weights", torch.zeros(2, 3)), ("tail_v", a["tail_v"].clone()), ("out", torch.zeros(2, 8, 1, 128).half())):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            paged_decode_attention(**{**_args(), name: t.requires_grad_()})
+    p, x, at = PagedKV(2, 4, device="cpu"), torch.zeros(1, 2, 16, 128), torch.tensor([[0]])
+    for s32, s16 in ((torch.ones(2, requires_grad=True), torch.ones(2)), (torch.ones(2), torch.ones(2, requires_grad=True))):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            p.write(x, at, s32, s16)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        evict_pages(torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros(2, 3, requires_grad=True), 1)
