@@ -178,6 +178,16 @@ def paged_attn_workspace(n_seq: int, n_heads: int, group: int, max_pages: int, t
                        device=device)
 
 
+def _apart(out: torch.Tensor) -> bool:
+    """Whether the rows of out (B, Hq, 1, 128) share no element."""
+    if out.is_contiguous():
+        return True
+    (a, n), (b, m) = sorted(zip(out.stride()[:2], out.shape[:2]))
+    if n == 1 or m == 1:
+        return n * m == 1 or (b if n == 1 else a) >= HD
+    return a >= HD and b >= (n - 1) * a + HD
+
+
 def paged_decode_attention(k: PagedKV, v: PagedKV, q: torch.Tensor, pages: torch.Tensor, n_pages: torch.Tensor,
                            tail_k: Optional[torch.Tensor] = None, tail_v: Optional[torch.Tensor] = None,
                            tail_len: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
@@ -236,8 +246,7 @@ def paged_decode_attention(k: PagedKV, v: PagedKV, q: torch.Tensor, pages: torch
                                 not weights.is_contiguous()):
         raise ValueError("weights must be (B, W) fp32, contiguous, on the pools' device")
     if out is not None and (out.shape != q.shape or out.dtype is not dt or out.device != dev or out.stride(3) != 1 or
-                            any(s % 8 or (s == 0 and n > 1) for s, n in zip(out.stride()[:2], out.shape)) or
-                            out.data_ptr() % 16):
+                            any(s % 8 for s in out.stride()[:2]) or out.data_ptr() % 16 or not _apart(out)):
         raise ValueError("out must be like q, its rows 16-byte aligned and apart")
     lib = L.lib()
     with L.on_device(dev):

@@ -7,7 +7,7 @@ import torch
 from latticequant_amd import _lib as L
 from latticequant_amd._dev import int32_on
 from latticequant_amd.llm.logprobs import token_logprobs
-from latticequant_amd.llm.paged import PagedKV, evict_pages, paged_decode_attention, paged_workspace_size
+from latticequant_amd.llm.paged import PagedKV, _apart, evict_pages, paged_decode_attention, paged_workspace_size
 from latticequant_amd.llm.resident import reorder_sequences
 from latticequant_amd.llm.tree import _ints
 
@@ -210,3 +210,20 @@ def test_nothing_that_wants_a_gradient_is_written_or_passed_by():
             p.write(x, at, s32, s16)
     with pytest.raises(RuntimeError, match="no gradient"):
         evict_pages(torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros(2, 3, requires_grad=True), 1)
+
+
+def test_rows_of_out_are_apart():
+    """Against a count of every element's place, over strides that rows share elements by and that they do not."""
+    for B in (1, 2, 3):
+        for Hq in (1, 2, 4):
+            for sb in (0, 64, 120, 128, 136, 256, 504, 512, 640):
+                for sh in (0, 8, 128, 136, 256, 384, 1536):
+                    out = torch.zeros(8000).as_strided((B, Hq, 1, 128), (sb, sh, 128, 1))
+                    places = torch.arange(8000).as_strided((B, Hq, 1, 128), (sb, sh, 128, 1))
+                    alone = places.unique().numel() == places.numel()
+                    # (rows that lie between each other's are refused with those that overlap)
+                    assert alone or not _apart(out), (B, Hq, sb, sh)
+                    if _apart(out) != alone:
+                        assert B > 1 and Hq > 1 and min(sb, sh) >= 128, (B, Hq, sb, sh)
+    with pytest.raises(ValueError, match="out must be"):
+        paged_decode_attention(**{**_args(), "out": torch.zeros(6000).half().as_strided((2, 8, 1, 128), (512, 64, 128, 1))})
