@@ -211,7 +211,7 @@ __device__ __forceinline__ void each_entry(const lq_pages& p, const Meta2& m, En
     }
 }
 
-// Without the record's bias: as a pair of fp16 numbers 2^-24 w, w = 2 c + 32, whole and
+// K's records without their bias: as a pair of fp16 numbers 2^-24 w, w = 2 c + 32, whole and
 // below 64 for a record.  What is multiplied by them needs neither the 32 taken off nor the
 // scale: both go into the other operand's sum and into the product (see attend below).
 template <int SH>   // b's byte from bit SH on
@@ -224,26 +224,31 @@ __device__ __forceinline__ void raw_pairs(uint32_t a, uint32_t b, uint32_t p[4])
     const uint32_t par = ((uint32_t)__builtin_popcount(a & kLsbMask) + u6) & 1u;
     p[3] = kc | (u6 << 1) | (((c7h << 1) | par) << 17);
 }
+// V's as coordinates c.  (As 2^-24 w, with 2^-19 sum P taken off the sums, V cost 32 instructions a
+// tile less, 0.5 to 3 us of the cases; but the products' unit drops what lies 2^-24 below its
+// largest term, taking a subnormal number's exponent for 2^-14 where w = 32 is 2^-19: beside
+// a token of nearly all the weight the 31 others lost up to 2^-15 of a scale each, and the taking
+// off is as exact as w, not as c.)
 template <int SH, int K>   // both bytes, from bits SH and SH + 8 on, into each dimension's pair K
-__device__ __forceinline__ void raw_pairs_tok(uint32_t a0, uint32_t a1, uint32_t b, u32x4_t p[8]) {
+__device__ __forceinline__ void pairs_tok(uint32_t a0, uint32_t a1, uint32_t b, u32x4_t p[8]) {
     const uint32_t lo = __builtin_amdgcn_perm(a1, a0, 0x05040100u);
     const uint32_t hi = __builtin_amdgcn_perm(a1, a0, 0x07060302u);
-    const uint32_t kc = lo & 0x00010001u;
-    p[0][K] = (lo & kFieldMask) | kc;
-    p[2][K] = ((lo >> 5) & kFieldMask) | kc;
-    p[4][K] = ((lo >> 10) & kFieldMask) | kc;
-    p[1][K] = (hi & kFieldMask) | kc;
-    p[3][K] = ((hi >> 5) & kFieldMask) | kc;
-    p[5][K] = ((hi >> 10) & kFieldMask) | kc;
+    const uint32_t kc = 0x60006000u | (lo & 0x00010001u);   // 512 and the coset's half
+    p[0][K] = unbias((lo & kFieldMask) | kc);
+    p[2][K] = unbias(((lo >> 5) & kFieldMask) | kc);
+    p[4][K] = unbias(((lo >> 10) & kFieldMask) | kc);
+    p[1][K] = unbias((hi & kFieldMask) | kc);
+    p[3][K] = unbias(((hi >> 5) & kFieldMask) | kc);
+    p[5][K] = unbias(((hi >> 10) & kFieldMask) | kc);
     const uint32_t u0 = (b >> SH) & 31u, u1 = (b >> (SH + 8)) & 31u;
     const uint32_t h0 = ((b >> (SH + 5)) & 7u) | ((a0 >> 13) & 8u);
     const uint32_t h1 = ((b >> (SH + 13)) & 7u) | ((a1 >> 13) & 8u);
     const uint32_t q0 = ((uint32_t)__builtin_popcount(a0 & kLsbMask) + u0) & 1u;
     const uint32_t q1 = ((uint32_t)__builtin_popcount(a1 & kLsbMask) + u1) & 1u;
-    p[6][K] = kc | (u0 << 1) | (u1 << 17);
-    p[7][K] = kc | (((h0 << 1) | q0) << 1) | (((h1 << 1) | q1) << 17);
+    p[6][K] = unbias(kc | (u0 << 1) | (u1 << 17));
+    p[7][K] = unbias(kc | (((h0 << 1) | q0) << 1) | (((h1 << 1) | q1) << 17));
 }
-// an entry's eight values 2c so (beyond 2048 they lose bits, as fp16 does), and as c
+// an entry of K's eight values 2c so (beyond 2048 they lose bits, as fp16 does)
 __device__ __forceinline__ void raw_entry(const uint4& w, uint32_t p[4]) {
     const uint32_t x[4] = {w.x, w.y, w.z, w.w};
     const h2_t tiny = __builtin_bit_cast(h2_t, 0x00010001u), bias = __builtin_bit_cast(h2_t, 0x00200020u);   // 2^-24, 2^-19
@@ -273,17 +278,15 @@ __device__ __forceinline__ float pair_sum(float v) {   // of lane and lane ^ 16
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// State of a row over a unit's pages.  K's and V's values are c times their token's scale,
-// and enter the products as 2^-24 (2 c + 32):
+// State of a row over a unit's pages.  K's and V's values are c times their token's scale; K's
+// enter the products as k_i = 2^-24 (2 c + 32), V's as c:
 //   z   = kScale2 2^23 s_k (sum_i q_i k_i - 2^-19 sum_i q_i)
-//   o   = 2^23 (sum_t P_t v_t - 2^-19 sum_t P_t),   P_t = fp16(2^(z_t - m + shift) s_v)
-// so a record is decoded by bit operations alone.  The correction of z starts the product's
-// accumulator; that of o is taken off every 32 tiles, so that the sums stay near their result
-// (N tokens of like weights: the result falls as sqrt(N) beside them).  ROUND: K's values
-// are rounded to fp16 as the cache's readers see them, for weights that agree with a dense
-// attention's in 32 bits: c's own pairs, times the scale.
+//   o   = sum_t P_t c_t,   P_t = fp16(2^(z_t - m + shift) s_v)
+// so a record of K is decoded by bit operations alone; the correction of z starts the product's
+// accumulator.  ROUND: K's values are rounded to fp16 as the cache's readers see them, for weights
+// that agree with a dense attention's in 32 bits: c's own pairs, times the scale.
 struct PageState {
-    float m, l, sum;                           // reference, sum of 2^(z - m + shift), of P_t since the last correction
+    float m, l;                                // reference, sum of 2^(z - m + shift)
     float shift;                               // kPShift less the exponent of V's largest scale so far: P's range is that of a scale of 1
     float limit;                               // a logarithm of a weight beyond it raises the reference
     f4_t o[8];
@@ -291,7 +294,6 @@ struct PageState {
 constexpr float kUnit = 8388608.0f;            // 2^23
 __device__ __forceinline__ void rescale(PageState& st, float f) {
     st.l *= f;
-    st.sum *= f;
 #pragma unroll
     for (int mm = 0; mm < 8; mm++)
 #pragma unroll
@@ -314,21 +316,10 @@ __device__ __forceinline__ float shares_sum(float v) {   // within a quarter
     return v;
 }
 template <int NR>
-__device__ __forceinline__ float row_sum(float v) { return quarters_sum(shares_sum<NR>(v)); }
-template <int NR>
 __device__ __forceinline__ float row_max(float v) {
     if (NR <= 8) v = fmaxf(v, dppf<0x128>(v));
     if (NR <= 4) v = fmaxf(v, dppf<0x124>(v));
     return quarters_max(v);
-}
-template <int NR>
-__device__ __forceinline__ void correct(PageState& st) {
-    const float c = row_sum<NR>(st.sum) * (-0x1p-19f);
-#pragma unroll
-    for (int mm = 0; mm < 8; mm++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) st.o[mm][i] += c;
-    st.sum = 0.f;
 }
 // the largest of the lane's scales, and the least e with 2^e >= every one of the wave's (fp16's: -24 at least)
 template <int NR>
@@ -345,7 +336,7 @@ __device__ __forceinline__ float scale_log(const uint32_t s[4]) {
 }
 
 // One tile: scores s[y][i] of token 8 (lane / 16) + 2 i + y (without their scales, or with
-// them where ROUND), raw V.  With SUMS the logarithm (base 2) of the sum of the lane's page
+// them where ROUND), V's coordinates.  With SUMS the logarithm (base 2) of the sum of the lane's page
 // (lanes 0..31 hold the first page's tokens, 32..63 the second's).
 template <bool SUMS, bool ROUND, int NR>
 __device__ __forceinline__ float attend(const f4_t s[2], const uint32_t ks[4], const uint32_t vs[4], uint32_t word,
@@ -394,10 +385,9 @@ __device__ __forceinline__ float attend(const f4_t s[2], const uint32_t ks[4], c
 #pragma unroll
     for (int i = 0; i < N / 2; i++) {
         const float u = __builtin_amdgcn_exp2f(z[2 * i]), v = __builtin_amdgcn_exp2f(z[2 * i + 1]);
-        const h2_t sv = __builtin_bit_cast(h2_t, vs[i]), one = {(_Float16)1.f, (_Float16)1.f};
+        const h2_t sv = __builtin_bit_cast(h2_t, vs[i]);
         sum += u + v;
         p[i] = pair_h(u * (float)sv[0], v * (float)sv[1]);   // the product's operand: one rounding, 2^-11 of it at most
-        st.sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, p[i]), one, st.sum, false);
     }
     st.l += sum;
     // back to lane r, which has row r's eight tokens in the product (what the others have goes
@@ -577,7 +567,7 @@ __global__ __launch_bounds__(W * 64, 2) void k_paged(PagedArgs A) {
                 }
                 PageState ps;
                 ps.m = -INFINITY;
-                ps.l = ps.sum = 0.f;
+                ps.l = 0.f;
                 ps.shift = kPShift;
                 ps.limit = -INFINITY;
                 float largest = 0.f;           // no scale has been above it
@@ -661,10 +651,10 @@ __global__ __launch_bounds__(W * 64, 2) void k_paged(PagedArgs A) {
                     {
                         const uint32_t aw[8] = {rd.va[0].x, rd.va[0].y, rd.va[0].z, rd.va[0].w,
                                                 rd.va[1].x, rd.va[1].y, rd.va[1].z, rd.va[1].w};
-                        raw_pairs_tok<0, 0>(aw[0], aw[1], rd.vb.x, vq);
-                        raw_pairs_tok<16, 1>(aw[2], aw[3], rd.vb.x, vq);
-                        raw_pairs_tok<0, 2>(aw[4], aw[5], rd.vb.y, vq);
-                        raw_pairs_tok<16, 3>(aw[6], aw[7], rd.vb.y, vq);
+                        pairs_tok<0, 0>(aw[0], aw[1], rd.vb.x, vq);
+                        pairs_tok<16, 1>(aw[2], aw[3], rd.vb.x, vq);
+                        pairs_tok<0, 2>(aw[4], aw[5], rd.vb.y, vq);
+                        pairs_tok<16, 3>(aw[6], aw[7], rd.vb.y, vq);
                     }
                     if (const uint32_t most = most_of(mv)) {
 #pragma unroll
@@ -672,7 +662,7 @@ __global__ __launch_bounds__(W * 64, 2) void k_paged(PagedArgs A) {
                         wave_lds_sync();
                         each_entry<BIG>(A.v, mv, ev, most, lane, [&](uint32_t rec, const uint4& v) __attribute__((always_inline)) {
                             uint32_t e[4];
-                            raw_entry(v, e);
+                            exc_pairs(v, e);
                             const uint32_t tok = 16 * (lane >> 5) + (rec & 15);
                             uint16_t* w = reinterpret_cast<uint16_t*>(area + 16 * (tok >> 3) + (rec >> 4)) + (tok & 7);
 #pragma unroll
@@ -700,7 +690,6 @@ __global__ __launch_bounds__(W * 64, 2) void k_paged(PagedArgs A) {
                         pg.g++;
                         pg.near = pg.far;
                         pg.far = load_pages(row, L.pages, cap, pg.g + 1, lane);
-                        correct<NR>(ps);           // with the sums of the tiles before this one
                     }
                     blocks(tile + 2);
                     nk = load_meta<BIG>(A.k, x1, y1, lane);
@@ -712,14 +701,13 @@ __global__ __launch_bounds__(W * 64, 2) void k_paged(PagedArgs A) {
                     }
                 }
                 // on as the tail's rows are taken
-                correct<NR>(ps);
                 const float f = __builtin_amdgcn_exp2f(kPShift - ps.shift);
                 st.m = ps.m;
                 st.l = l32 = shares_sum<NR>(ps.l) * f;
 #pragma unroll
                 for (int mm = 0; mm < 8; mm++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) st.o[mm][i] = ps.o[mm][i] * (f * kUnit);
+                    for (int i = 0; i < 4; i++) st.o[mm][i] = ps.o[mm][i] * f;
             }
             // ---- the tail's
             for (int tile = max(t, L.page_tiles); tile < t + n; tile++) {

@@ -807,3 +807,46 @@ def test_numbers_of_entries_end_at_32_bits():
     assert int(p.pool.n_exc) == 2 ** 31 - 1 and p.exc_cap == cap
     assert torch.equal(p.read(every[:2]), before)
     assert not bool(p.read(every[2:]).isnan().any())
+
+
+# -------------------------------------------------------------- light tokens --
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("group", [1, 4, 7, 16])
+@pytest.mark.parametrize("pages", [1, 2, 31, 300])
+def test_light_tokens_beside_a_heavy_one(pages, group, dtype, weights):
+    """A first token that takes nearly all of the weight and has V = 0 (as an attention sink has), so
+    that the output is what the others give: as exact relatively to that as without it.
+
+    P is rounded once and its sum is not (2^-11), V's coordinates are exact. Sums in fp32 of
+    32 tokens of a product, of up to 64 tiles a wave, of waves and workgroups: 2^-23 of the sum of
+    p |v| each, 128 in all (a product of 32 tokens may drop what lies 2^-24 below its largest
+    term, and each of the 32 does). Scores: 130 x 2^-24 of |q| (|k| + 16 scales), twice, 2^-16 for exp2."""
+    H, n = 2, pages * PAGE
+    g = torch.Generator(device="cuda").manual_seed(300 + pages)
+    k, v = PagedKV(H, pages, device="cuda"), PagedKV(H, pages, device="cuda")
+    one = torch.ones(pages, H, device="cuda")
+    x = torch.randn(pages, H, PAGE, HD, generator=g, device="cuda") * 0.25
+    x[0, :, 0] = 4.0                                       # z = 128 a 4 / sqrt(128) for the first, sum of few q k for others
+    k.write(x, torch.arange(pages, device="cuda")[:, None], one / 4, one.half() / 4)
+    x = torch.randn(pages, H, PAGE, HD, generator=g, device="cuda") * 3
+    x[0, :, 0] = 0.0
+    v.write(x, torch.arange(pages, device="cuda")[:, None], one, one.half())
+    a = (math.log(100.0) + math.log(n)) / (4 * math.sqrt(HD))   # a share of 1 % for the others together
+    q = torch.full((1, H * group, 1, HD), a, device="cuda") * (1 + 0.1 * torch.randn(1, H * group, 1, HD, generator=g, device="cuda"))
+    q = q.to(dtype)
+    tab = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    cnt = torch.tensor([pages], dtype=torch.int32, device="cuda")
+    got = paged_decode_attention(k, v, q, tab, cnt, weights=torch.zeros(1, pages, device="cuda") if weights else None)
+    every = tab.long().t()
+    for h in range(H):
+        kk, vv = (p.read(every, torch.float32).double()[:, h].reshape(n, HD) for p in (k, v))
+        qq = q[0, h * group:(h + 1) * group, 0].double()
+        p = torch.softmax(qq @ kk.t().contiguous() / math.sqrt(HD), 1)
+        want, size = p @ vv, p @ vv.abs()
+        es = 130 * 2.0 ** -24 * ((qq.abs() @ kk.abs().t().contiguous()).amax(1) + 4 * qq.abs().sum(1)) / math.sqrt(HD)
+        tol = (size * (2.0 ** -11 + 128 * 2.0 ** -23 + 2 * es[:, None] + 2.0 ** -16) + want.abs() * HALF[dtype] * (1 + 2.0 ** -9) +
+               (2.0 ** -25 if dtype is torch.float16 else 0.0))
+        err = (got[0, h * group:(h + 1) * group, 0].double() - want).abs()
+        assert bool((err <= tol).all()), (float((err / tol).max()), float(p[:, 0].min()), float(err.max()), float(size.max()))
