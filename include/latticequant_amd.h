@@ -719,7 +719,8 @@ typedef struct {
  * number outside the pool moves nothing; one that stands twice leaves its page undefined.
  * A page that needs more exception entries than it owns takes the next power of two at
  * *n_exc.  Where the list is too short (*n_exc > exc_cap, LQ_RES_ST_EXC_OVERFLOW), lengthen it
- * (its first exc_cap entries and their rec kept) and call again: no room is taken twice. */
+ * (its first exc_cap entries and their rec kept) and call again: no room is taken twice.
+ * *n_exc stops at 2^31 - 1, which no list has: entries past it are zero vectors. */
 int lq_page_quantize(const void *d_x, int dtype, int64_t n, int64_t t_tokens, const float *d_scale32,
                      const uint16_t *d_scale16, const lq_pages *p, const int32_t *d_pages, hipStream_t s);
 
@@ -744,7 +745,9 @@ int64_t lq_paged_attn_workspace(int64_t n_seq, int64_t heads, int group, int64_t
  * dtype LQ_F16 or LQ_BF16 of q, the tail and out, products fp16, as lq_resident_tree_attention
  * (bf16 beyond fp16's range becomes infinite, below 2^-14 it loses bits).  A page's value is its
  * lattice coordinate times its scale: V's unrounded, K's rounded to fp16 with d_weights, as
- * lq_page_dequant rounds it, and unrounded without.
+ * lq_page_dequant rounds it, and unrounded without (so d_weights moves out by what that rounding
+ * does).  Coordinates of exceptions beyond 1024, K's without d_weights beyond 1008, have
+ * fp16's 11 bits.
  * group 1..16; stride_t of q and out is not used.  Deterministic. */
 int lq_paged_attention(const lq_pages *k, const lq_pages *v, const lq_rows *q, int64_t n_seq, int group,
                        const int32_t *d_pages, int64_t max_pages, const int32_t *d_n_pages, const lq_rows *tail_k,

@@ -19,13 +19,15 @@
 // device-scope stores, release and acquire took the 4 to 5 us of the second launch with 136
 // tiles, and 9 us more than it with 8200.)
 //
-// Long ones are bound by instructions and memory alike: 480 vector instructions a tile (decode
-// of K and V about 310, K's exceptions through LDS and back 60, softmax of a lane's two
-// tokens and both products' rest 110) at two waves a SIMD, one tile in flight beside the
+// Long ones are bound by instructions and memory alike: 520 vector instructions a tile (decode
+// of K and V about 345, K's exceptions through LDS and back 60, softmax of a lane's two
+// tokens and both products' rest 115) at two waves a SIMD, one tile in flight beside the
 // one that is worked on; 2 sequences of 131072 tokens, 8 heads, 4 rows, 8 % of K's vectors
-// exceptions: 86 us, 4.2 TB/s (three waves a SIMD 105, two tiles in flight 139: both spill).
-// Short ones by latency: lengths, table, records and exceptions are loaded in turn, and a tile
-// takes a lone wave 4200 cycles; 1 sequence of 500 tokens 10.4 us.
+// exceptions: 87 to 92 us, 3.9 to 4.1 TB/s (of a form of 480 instructions, 83 to 87: three waves
+// a SIMD 105, two tiles in flight 139, both spill).
+// Short ones by latency (32 sequences up to 2048 tokens: two fifths of the waves' cycles they
+// wait, a third they issue): lengths, table, records and exceptions are loaded in turn, and a
+// tile takes a lone wave 4200 cycles; 1 sequence of 500 tokens 11.0 us.
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -45,17 +47,17 @@ constexpr int kGroups = 512;                   // workgroups at most
 // Where no (sequence, head) can have more than kWhole tiles and all fit on the chip at once, a
 // workgroup takes one as a whole, of eight waves where each finds a compute unit, and there is
 // no second launch.  1 / 8 / 32 sequences of 8 heads, replayed from a graph, against equal
-// shares: 4 tiles 5.9 / 6.0 / 6.1 us (9.1 / 9.7 / 9.8), 20 tiles 9.5 / 10.0 / 10.2 (11.5 / 13.2 /
-// 18.2), 32 tiles 11.9 / 12.8 / 14.7 (11.5 / 14.0 / 20.7), the host's 3 us for a launch not
-// counted; 48 tiles 17.0 / 17.9 / 19.0 (11.9 / 15.3 / 23.5), and lengths may differ.  64
-// sequences, with four waves so that all are there at once: 2 / 16 / 32 tiles 5.9 / 13.9 / 21.6
-// (shares 8.6 / 18.5 / 25.6, eight waves 9.8 / 18.9 / 26.3).  A kernel of its own, without what
-// finds shares: code that is only branched around cost 0.9 us (11.1 for 10.3 with 17 tiles).
+// shares: 4 tiles 5.9 / 6.1 / 6.2 us (8.9 / 9.8 / 10.0), 20 tiles 9.5 / 10.2 / 10.9 (11.1 / 13.0 /
+// 16.7), 32 tiles 12.6 / 13.6 / 15.1 (11.1 / 14.0 / 20.7), the host's 3 us for a launch not
+// counted; 48 tiles 16.3 / 17.7 / 19.2 (11.5 / 15.4 / 24.2), and lengths may differ.  64
+// sequences, with four waves so that all are there at once: 2 / 16 / 32 tiles 6.0 / 15.0 / 22.8
+// (shares 8.7 / 19.7 / 26.9, eight waves 10.0 / 19.7 / 27.7).  A kernel of its own, without what
+// finds shares: code that is only branched around cost 0.9 us (with 17 tiles).
 constexpr int kWhole = 32;
 // A unit's first tile waits for its page numbers, records and exceptions in turn and its tail
 // for its rows, which took about two tiles' time: the list has two places for that before each
-// unit's tiles.  32 sequences up to 2048 tokens 24.1 -> 21.6 us, 64 up to 8192 with weights
-// 112.7 -> 104.6 (one place: 22.2 and 106.8, four: 21.8 and 106.8).
+// unit's tiles.  32 sequences up to 2048 tokens / 64 up to 8192 with weights, a call: one place
+// 23.2 / 119.0 us, two 23.3 / 116.9, four 24.1 / 117.3 (without any the kernel took 2.5 / 8 more).
 constexpr int kAhead = 2;
 constexpr int kMRow = kHd + 4;                 // floats of a piece's row in LDS: o[128], m, l, l32
 constexpr int kRecF = 4 + kHd;                 // floats of a record's row: m, l, l32, unused, o[128]
@@ -986,7 +988,7 @@ constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64, kBins = 20
 // each wave a part of them.  A sequence of up to 8192 pages is a workgroup's, N of them a
 // lane in registers, read once.  Longer ones (N = 0) are searched by `parts` workgroups each
 // of which looks at all of it and writes its part: the search is repeated on compute units
-// that would idle (4 sequences of 65536 pages: 41 us, one workgroup each 80).  1 / 64 / 256
+// that would idle (4 sequences of 65536 pages: 46 us, one workgroup each 80).  1 / 64 / 256
 // tables of 8192 pages 13.8 / 17.0 / 19.5 us (N = 0: 15.7 / 16.9 / 20.4), of 16384 with 16 a
 // lane 21.2 / 26.0 / 29.6 (20.9 / 23.0 / 31.0).  Bound by latency with few pages (1024: 5.4 us),
 // by instructions with many.

@@ -261,8 +261,8 @@ __global__ __launch_bounds__(256) void k_res_dequant(lq_resident r, int64_t h0, 
 //
 // Blocks by number: unit (i, h, j) of x (n, heads, t_tokens, 128) goes to block
 // pages[i][j] of head h; a number outside the pool moves nothing.  The resident form's
-// work, a workgroup a block.  64 pages of 8 heads at random places: quantized in 5.1 us, room
-// 3.4, entries 5.0, read back 4.1 (latency); 4096 pages with outlier channels: 91, 53, 42 and 44
+// work, a workgroup a block.  64 pages of 8 heads at random places: quantized in 5.2 us, room
+// 3.2, entries 5.0, read back 4.3 (latency); 4096 pages with outlier channels: 91, 52, 43 and 45
 // (the nearest points' instructions; one compute unit's scattered loads; scattered
 // records of exceptions; 134 MB written at 3 TB/s).
 struct PageMap {

@@ -74,7 +74,8 @@ class PagedKV:
     of two of its largest number of exceptions in use, and under as many again of
     earlier ones: 512 a page and head and 256 a page and head of a write always suffice.
     A graph captured over the pool holds the list as it was: capture again when
-    ``exc_cap`` has grown."""
+    ``exc_cap`` has grown.  Calls on one pool from several streams are the caller's to order,
+    whichever pages they name: a write may move the list that the others read."""
 
     def __init__(self, n_heads: int, n_pages: int, device=None, exc_cap: Optional[int] = None):
         if n_heads < 1 or n_pages < 1:
@@ -111,7 +112,8 @@ class PagedKV:
         (n, T / 16), each the next 16 tokens of its row.  scale32 / scale16: the rows'
         scales per head, n * n_heads of each (those of the chunk codec give its points);
         without them they are taken from x at `bits` bits per dimension.  What the pages held
-        is gone; all their numbers are to differ (numbers outside the pool write nothing)."""
+        is gone; all their numbers are to differ.  Numbers on the device that are outside the
+        pool write nothing (from the host such, and equal ones, are refused)."""
         if x.dim() != 4 or x.shape[1] != self.n_heads or x.shape[3] != HD:
             raise ValueError(f"x must be (n, {self.n_heads}, T, 128)")
         n, H, T, _ = x.shape
@@ -210,7 +212,8 @@ def paged_decode_attention(k: PagedKV, v: PagedKV, q: torch.Tensor, pages: torch
     write, of q's shape and type.  Returns (B, Hq, 1, 128).  The products are fp16 as
     resident_tree_attention's are; a page's value is its lattice coordinate times its scale,
     V's unrounded, K's rounded to fp16 (as ``read`` rounds it) with weights and unrounded
-    without.  The same inputs give the same bits."""
+    without (so asking for weights moves the result by what that rounding does); coordinates
+    of exceptions beyond 1024 (K's without weights 1008) have fp16's 11 bits.  The same inputs give the same bits."""
     dev = k.device
     dt, shape = q.dtype, q.shape
     if len(shape) != 4 or dt not in _DTYPES or shape[2] != 1 or shape[3] != HD:
