@@ -194,6 +194,8 @@ class ResidentKV:
                 if n1 <= self.exc_cap:
                     break
                 # grow the exception list to the exact need and launch again
+                if not anew:
+                    self._exc_known, self._exc_since, self._exc_read = n1, 0, None   # if there is no room for it
                 self._grow_exc(self._longer(n1), n0 if anew else self.exc_cap)
                 if anew:
                     self.n_exc.fill_(n0)

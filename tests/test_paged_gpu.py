@@ -850,3 +850,15 @@ def test_light_tokens_beside_a_heavy_one(pages, group, dtype, weights):
                (2.0 ** -25 if dtype is torch.float16 else 0.0))
         err = (got[0, h * group:(h + 1) * group, 0].double() - want).abs()
         assert bool((err <= tol).all()), (float((err / tol).max()), float(p[:, 0].min()), float(err.max()), float(size.max()))
+
+
+def test_a_small_write_after_one_that_found_no_room():
+    """A large write whose entries have no room leaves their number known: a small one then fails
+    too, where it would drop its own, instead of taking the list for long enough."""
+    p = _pool(8, 12, 150)
+    every = torch.arange(12, device="cuda")[:, None]
+    p.pool.n_exc.fill_(2 ** 31 - 100)
+    y, t = torch.randn(10, 8, PAGE, HD, device="cuda") * 100, torch.full((10, 8), 0.25, device="cuda")
+    for n in (10, 1, 2):
+        with pytest.raises(RuntimeError, match="fewer than 2\\^31"):
+            p.write(y[:n], every[:n], t[:n], t[:n].half())
